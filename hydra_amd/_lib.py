@@ -22,6 +22,8 @@ EXPORTS = [
     "hh_expert_gemv", "hh_expert_gemm", "hh_combine",
     "hh_runner_create", "hh_runner_destroy", "hh_runner_set_layer", "hh_runner_reserve",
     "hh_runner_forward", "hh_runner_capture",
+    "hh_attention_tree", "hh_draft_verify", "hh_cache_commit", "hh_attention_weights",
+    "hh_cache_evict", "hh_draft_reserve",
 ]
 
 # int (*hh_layer_hook)(void *user, int32_t layer, void *stream)
@@ -71,6 +73,26 @@ class MatrixC(C.Structure):
 class BlobLayoutC(C.Structure):
     _fields_ = [("slot_count", C.c_int32), ("offset", C.c_size_t * 9), ("bytes", C.c_size_t * 9),
                 ("payload_bytes", C.c_size_t), ("stride_bytes", C.c_size_t)]
+
+
+class TreeDescC(C.Structure):
+    _fields_ = [("sequences", C.c_int32), ("nodes", C.c_int32), ("q_heads", C.c_int32),
+                ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("type", C.c_int32),
+                ("cache_type", C.c_int32), ("window", C.c_int32), ("max_length", C.c_int32),
+                ("sm_scale", C.c_float), ("q_stride", C.c_int64), ("kv_stride", C.c_int64)]
+
+
+class KVCacheC(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("sequence_stride", C.c_int64),
+                ("rows", C.c_int32), ("ring", C.c_int32), ("lengths", C.c_void_p),
+                ("weights", C.c_void_p), ("positions", C.c_void_p), ("next_position", C.c_void_p)]
+
+
+class VerifyDescC(C.Structure):
+    _fields_ = [("sequences", C.c_int32), ("nodes", C.c_int32), ("vocab", C.c_int32),
+                ("type", C.c_int32), ("draft", C.c_int32), ("max_children", C.c_int32),
+                ("temperature", C.c_float), ("target_stride", C.c_int64),
+                ("draft_stride", C.c_int64)]
 
 
 _lib = None
@@ -125,6 +147,14 @@ def lib() -> C.CDLL:
     L.hh_scatter_expert_tensor.argtypes = [vp, C.POINTER(MoEDescC), i32, i32, i32, vp, i64, vp,
                                            C.c_uint64]
     L.hh_ctx_decode_fused.argtypes = [vp, i32]
+    L.hh_attention_tree.argtypes = [vp, C.POINTER(TreeDescC), C.POINTER(KVCacheC)] + [vp] * 8
+    L.hh_attention_weights.argtypes = [vp, C.POINTER(TreeDescC), C.POINTER(KVCacheC)] + [vp] * 4
+    L.hh_draft_verify.argtypes = [vp, C.POINTER(VerifyDescC)] + [vp] * 10
+    L.hh_cache_commit.argtypes = [vp, C.POINTER(TreeDescC), C.POINTER(KVCacheC), i32, C.POINTER(vp),
+                                  C.POINTER(vp), vp, vp]
+    L.hh_cache_evict.argtypes = [vp, C.POINTER(TreeDescC), C.POINTER(KVCacheC), i32, i32, i32]
+    L.hh_draft_reserve.argtypes = [vp, C.POINTER(TreeDescC), C.POINTER(KVCacheC), i32,
+                                   C.POINTER(VerifyDescC)]
     L.hh_ctx_profile_read.argtypes = [vp, C.POINTER(C.c_double), C.POINTER(C.c_int64)]
     for name in EXPORTS:
         if name not in ("hh_last_error", "hh_ctx_stream", "hh_dispatch_count"):

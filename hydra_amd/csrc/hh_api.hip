@@ -11,6 +11,7 @@
 #include <vector>
 
 #include "hh_common.hpp"
+#include "hh_ctx.hpp"
 #include "hydra_hip.h"
 
 namespace hh {
@@ -55,53 +56,25 @@ hipError_t launch_activation(int act, float alpha, float limit, const float *gat
                              const float *up, int64_t n, float *out, hipStream_t s);
 }  // namespace hh
 
-struct hh_ctx {
-  // Flags of the fused decode kernel: allocated and zeroed once, then only ever written with
-  // flag values; `epoch` is the value of the last call.
-  uint32_t *flags = nullptr;
-  uint32_t epoch = 0;
-  uint32_t fused_calls = 0;    // one-launch decode calls so far (the counter region parity)
-  int decode_fused = -1;   // 1 on, 0 off, -1 the environment's choice
-  int device = 0;
-  hipStream_t stream = nullptr;
-  uint8_t *arena = nullptr;
-  size_t arena_bytes = 0;
-  int64_t dispatches = 0;
-  // Profiling: a pool of events, a start/stop pair per phase of each profiled forward call.
-  bool profile = false;
-  std::vector<hipEvent_t> events;
-  size_t events_used = 0;
-  // Graph capture: calls are recorded, not run; dispatches counted while recording are moved
-  // to the graph and added back per launch.
-  bool capturing = false;
-  int64_t capture_base = 0;
-  // Decode attention partials (per query head and chunk), grown on demand.
-  float *attn = nullptr;
-  size_t attn_bytes = 0;
-  // Instantiated graphs of this context that are not yet destroyed: they hold the arena's and
-  // the attention partials' device addresses, so neither may be reallocated while any exist.
-  int live_graphs = 0;
-  // This device's copy of the static scratch array (hh_moe_forward_noalloc), or NULL when its
-  // address could not be resolved (scratch_error then says why).
-  uint8_t *scratch = nullptr;
-  std::string scratch_error;
-};
-
-struct hh_graph {
-  hh_ctx *ctx = nullptr;
-  hipGraph_t graph = nullptr;
-  hipGraphExec_t exec = nullptr;
-  int64_t dispatches = 0;
-};
-
 // Scratch of hh_moe_forward_noalloc: a fixed array in every device's memory, held from module
 // load until the process ends. Host code never uses this name as an address (on the host it is
 // only a stand-in for the symbol); static_scratch() resolves each device's copy once.
 static __device__ __align__(256) uint8_t scratch[HH_NOALLOC_SCRATCH_BYTES];
 
 namespace {
+thread_local std::string g_error;   // hh_last_error's text
+}
 
-thread_local std::string g_error;
+int hh::fail(int code, const std::string &msg) {
+  g_error = msg;
+  return code;
+}
+
+int hh::hip_fail(hipError_t e, const char *what) {
+  return fail(HH_EHIP, std::string(what) + ": " + hipGetErrorString(e));
+}
+
+namespace {
 
 constexpr int kMaxDevices = 64;
 std::mutex g_scratch_mu;
@@ -127,20 +100,8 @@ uint8_t *static_scratch(int device, std::string *err) {
   return g_scratch_ptr[device];
 }
 
-int fail(int code, const std::string &msg) {
-  g_error = msg;
-  return code;
-}
-
-int hip_fail(hipError_t e, const char *what) {
-  return fail(HH_EHIP, std::string(what) + ": " + hipGetErrorString(e));
-}
-
-#define HH_HIP(call)                                  \
-  do {                                                \
-    hipError_t e_ = (call);                           \
-    if (e_ != hipSuccess) return hip_fail(e_, #call); \
-  } while (0)
+using hh::fail;
+using hh::hip_fail;
 
 size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
@@ -709,6 +670,7 @@ int hh_ctx_destroy(hh_ctx *ctx) {
   if (ctx->stream) (void)hipStreamSynchronize(ctx->stream);
   if (ctx->arena) (void)hipFree(ctx->arena);
   if (ctx->attn) (void)hipFree(ctx->attn);
+  if (ctx->draft) (void)hipFree(ctx->draft);
   if (ctx->flags) (void)hipFree(ctx->flags);
   for (hipEvent_t ev : ctx->events) (void)hipEventDestroy(ev);
   if (ctx->stream) (void)hipStreamDestroy(ctx->stream);

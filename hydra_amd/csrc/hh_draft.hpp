@@ -1,0 +1,72 @@
+// hh_draft.hpp — argument blocks of the drafted-token kernels (hh_tree.hip, hh_verify.hip,
+// hh_cache.hip), shared with their C entries (hh_draft.hip).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace hh {
+
+enum Elem { E_F32 = 0, E_F16 = 1, E_BF16 = 2 };
+constexpr int kTreeNodes = 64;    // most nodes of a tree: an ancestor set is one 64-bit mask
+constexpr int kTreeQM = 16;       // most query heads per kv head
+
+struct TreeArgs {
+  const void *q, *dk, *dv;          // [S][N][qh][d] and [S][N][kvh][d], strides below
+  const uint16_t *k, *v;            // [S][rows][kvh][d]
+  const int32_t *lengths, *parents, *counts;
+  const uint16_t *sinks;            // bf16 [qh] or null
+  void *out;                        // [S][N][qh][d]
+  float *lse;                       // [S][N][qh] or null
+  int S, N, qh, kvh, d, rows, ring, window;
+  float scale;
+  int64_t q_stride, kv_stride, seq_stride;   // elements between nodes, nodes, sequences
+  // hh_attention_weights
+  const float *lse_in;
+  const int32_t *path, *accepted;
+  float *weights;                   // [S][kvh][rows]
+};
+
+// One layer of a commit or an eviction.
+struct RowsLayer {
+  uint16_t *k, *v;
+  const uint16_t *dk, *dv;
+  int32_t *lengths;
+  float *weights;
+  int32_t *positions, *next;
+  int64_t seq_stride;
+  int32_t rows, ring;
+  int32_t limit;                    // most rows that `lengths` may count
+  int32_t last;                     // of the call's layers that share `lengths`
+};
+constexpr int kRowsLayers = 32;     // layers per launch: their blocks are kernel arguments
+
+struct RowsArgs {
+  RowsLayer layer[kRowsLayers];
+  const int32_t *path, *accepted;
+  int layers, S, N, kvh, d;
+  int64_t kv_stride;
+  // Eviction.
+  int keep, recent, max_moves;
+  int32_t *moves;                   // [layer][S][kvh]: rows that move
+  int32_t *from, *to;               // [layer][S][kvh][max_moves]
+};
+
+struct VerifyArgs {
+  const void *target, *draft;
+  int64_t t_stride, d_stride;       // elements between nodes
+  const int32_t *tokens, *parents, *counts;
+  const float *u, *u_final;
+  int32_t *path, *accepted, *next;
+  int S, N, V, type, mode, children;
+  double inv_t;                     // 1 / temperature; 0: greedy
+  uint8_t *ws;
+};
+
+size_t verify_workspace(int S, int N, int V, int mode, int children, bool greedy);
+hipError_t launch_tree(const TreeArgs &a, int type, hipStream_t s);
+hipError_t launch_weights(const TreeArgs &a, int type, hipStream_t s);
+hipError_t launch_verify(const VerifyArgs &a, hipStream_t s);
+hipError_t launch_commit(const RowsArgs &a, bool last, hipStream_t s);
+hipError_t launch_evict(const RowsArgs &a, hipStream_t s);
+
+}  // namespace hh

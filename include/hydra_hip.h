@@ -387,6 +387,143 @@ int hh_expert_gemm(hh_ctx *ctx, const hh_matrix *m, const float *x, int32_t toke
 int hh_combine(hh_ctx *ctx, const float *slots, const float *weights, int32_t tokens,
                int32_t count, int32_t size, float *y);
 
+/* ---- decoding with drafted tokens ---------------------------------------------------------
+ * A drafted tree of each of S sequences runs through the layers as one batch of S·N tokens; the
+ * entries below are the steps around it: attention of the tree over the history
+ * (hh_attention_tree), verification against the target's probabilities (hh_draft_verify), the
+ * accepted rows into the histories (hh_cache_commit), and histories of bounded size, whose rows
+ * of least accumulated attention weight go (hh_attention_weights, hh_cache_evict). The reference
+ * decodes one token at a time (ModelRunner.swift:110-230) and has no counterpart of them.
+ *
+ * A tree: parents int32 [S][N], parents[s][i] in 0..i−1, or −1 for a node without one (any other
+ * value counts as −1); node 0 is the pending token, the last one that was sampled. node_counts
+ * int32 [S] (0..N): nodes from the count on are padding; what belongs to them is neither read nor
+ * written, unless stated. Lengths, counts, paths and random numbers are device memory, so that
+ * every call may be recorded in a graph and replayed; what the host cannot check there is bounded
+ * by the kernels (an index out of range is skipped).                                         */
+typedef enum { HH_F32 = 0, HH_F16 = 1, HH_BF16 = 2 } hh_elem;
+
+#define HH_TREE_MAX_NODES 64
+
+/* Types: F32 activations over an F16 history (as hh_attention_decode), or both F16, or both BF16. */
+typedef struct hh_tree_desc {
+  int32_t sequences, nodes;               /* S >= 1, N = 1..64                                  */
+  int32_t q_heads, kv_heads, head_dim;    /* q_heads = kv_heads x 1..16; head_dim 64, 128, 256  */
+  int32_t type;                           /* hh_elem of q and out                               */
+  int32_t cache_type;                     /* hh_elem of the history and the drafted k and v     */
+  int32_t window;                         /* 0, or a node at position p sees positions > p − window */
+  int32_t max_length;                     /* longest expected history, 0 = the cache's rows: it
+                                             sizes the launch; every length is handled          */
+  float   sm_scale;
+  int64_t q_stride, kv_stride;            /* elements between nodes of q, and of the drafted k and
+                                             v; 0 = packed. Multiples of 16 bytes               */
+} hh_tree_desc;
+
+/* One layer's key/value history of S sequences. Without `ring`, row r of a sequence is its r-th
+ * key, lengths[s] rows are in use, and a full history (length = rows) takes no more. With `ring`,
+ * lengths[s] counts every token so far and position p is row p % rows. weights and positions are
+ * what eviction goes by; a ring has none. next_position: the position of the sequence's next token
+ * (its length, until rows are evicted).                                                      */
+typedef struct hh_kv_cache {
+  uint16_t *k, *v;           /* [S][rows][kv_heads][head_dim]                                   */
+  int64_t   sequence_stride; /* elements between sequences, 0 = packed                          */
+  int32_t   rows, ring;
+  int32_t  *lengths;         /* [S]                                                             */
+  float    *weights;         /* [S][kv_heads][rows]: accumulated attention weight, or NULL      */
+  int32_t  *positions;       /* [S][kv_heads][rows]: position of the token behind a row, or NULL */
+  int32_t  *next_position;   /* [S], with positions                                             */
+} hh_kv_cache;
+
+/* Attention of the drafted nodes: node i of sequence s sees the history's keys (positions below
+ * lengths[s]; of a ring the last `rows`) and, of the drafted ones, itself and its ancestors; its
+ * position is lengths[s] + its depth. Semantics of hh_attention_decode otherwise: logits
+ * sm_scale·q·k, an optional sink per head in the denominator only.
+ *   q, out   type [S][N][q_heads][head_dim] (q with q_stride)
+ *   draft_k, draft_v  cache_type [S][N][kv_heads][head_dim] (with kv_stride)
+ *   sinks    bf16 [q_heads] or NULL;  lse  fp32 [S][N][q_heads] or NULL: the log of the denominator
+ * Keys that a node does not see, infinities and NaN among them, have no part in its output.
+ * Sums are held in fp32; with F32 activations queries and probabilities enter the products as pairs of
+ * fp16 (about 2^-22), with F16 and BF16 probabilities are rounded once to the type.            */
+int hh_attention_tree(hh_ctx *ctx, const hh_tree_desc *desc, const hh_kv_cache *cache,
+                      const void *q, const void *draft_k, const void *draft_v,
+                      const int32_t *parents, const int32_t *node_counts, const uint16_t *sinks,
+                      void *out, float *lse);
+
+/* How the tokens of a node's children were drawn from the draft's distribution there. */
+typedef enum {
+  HH_DRAFT_GIVEN = 0,     /* chosen, not drawn: no draft logits                                 */
+  HH_DRAFT_IID = 1,       /* each independently                                                 */
+  HH_DRAFT_DISTINCT = 2   /* one after the other without putting back                           */
+} hh_draft_mode;
+
+typedef struct hh_verify_desc {
+  int32_t sequences, nodes, vocab;        /* S >= 1, N = 1..64, V = 1..2^24                     */
+  int32_t type;                           /* hh_elem of the logits                              */
+  int32_t draft;                          /* hh_draft_mode                                      */
+  int32_t max_children;                   /* a node's children beyond this many are not tried; 0 = N − 1 */
+  float   temperature;                    /* of both distributions; 0: greedy                   */
+  int64_t target_stride, draft_stride;    /* elements between nodes' logits; 0 = packed         */
+} hh_verify_desc;
+
+/* Verification of the drafted tokens, sequence by sequence. p = softmax(target row / temperature)
+ * and q = softmax(draft row / temperature) of the current node, from node 0 on: its children are
+ * tried in the order of their index; a child with token x is accepted if u·q(x) < p(x), u its entry of
+ * `uniforms`, and becomes the current node; otherwise p becomes max(p − q, 0) off the tokens tried at
+ * this node, normalised (with HH_DRAFT_DISTINCT q loses x and is normalised too), and the next child
+ * is tried; with HH_DRAFT_GIVEN q(x) is 1 for each child in turn. When none is accepted the next token
+ * is drawn from what p has become: the smallest v whose cumulative probability exceeds the sequence's
+ * final uniform. The tokens that come out are distributed as the target's. Temperature 0: a child
+ * is accepted if its token is the target's most probable (ties: the lowest), which is the next token
+ * at the last node.
+ *   target, draft  type [S][N][vocab] logits: row i is the distribution behind node i. NaN counts as
+ *                  −inf; entries of +inf share the probability. A row with no finite entry accepts nothing
+ *                  and gives next_token −1. draft is NULL with HH_DRAFT_GIVEN and temperature 0.
+ *   tokens int32 [S][N] (node 0's is not read; one outside the vocabulary is rejected);
+ *   uniforms fp32 [S][N], final_uniforms fp32 [S], in [0, 1)
+ *   path int32 [S][N]: the accepted nodes from node 0 on, −1 behind them; accepted int32 [S]: how many;
+ *   next_token int32 [S]. A sequence of no nodes: 0 accepted, next_token −1.
+ * Probabilities and sums are held in fp64 and added in a fixed order: a call's answer depends on its
+ * inputs alone.                                                                               */
+int hh_draft_verify(hh_ctx *ctx, const hh_verify_desc *desc, const void *target, const void *draft,
+                    const int32_t *tokens, const int32_t *parents, const int32_t *node_counts,
+                    const float *uniforms, const float *final_uniforms, int32_t *path,
+                    int32_t *accepted, int32_t *next_token);
+
+/* The accepted nodes' rows into the histories of `count` layers, and the lengths on:
+ * row lengths[s] + i of sequence s takes the drafted k and v of node path[s][i], i < accepted[s]
+ * (of a ring: row (lengths[s] + i) % rows, the last `rows` of a longer path). New rows have weight 0 and
+ * position next_position[s] + i. Lengths and next_position advance once, however many layers share
+ * them. Rows past a history's last are dropped. desc: sequences, nodes, kv_heads, head_dim, cache_type and
+ * kv_stride.
+ *   draft_k, draft_v: host arrays of `count` device pointers                                  */
+int hh_cache_commit(hh_ctx *ctx, const hh_tree_desc *desc, const hh_kv_cache *caches, int32_t count,
+                    const void *const *draft_k, const void *const *draft_v, const int32_t *path,
+                    const int32_t *accepted);
+
+/* The accepted nodes' attention added to the weight of each key of one layer, after hh_cache_commit:
+ * weights[s][g][r] += Σ over i < accepted[s] and the heads h of group g of
+ * exp(sm_scale·q[s][path[s][i]][h]·k[s][r][g] − lse[s][path[s][i]][h]), r up to the node's own row
+ * lengths[s] − accepted[s] + i. q and lse are hh_attention_tree's of this layer. Not for rings or
+ * windows. Each weight is summed by one wave in a fixed order.                                */
+int hh_attention_weights(hh_ctx *ctx, const hh_tree_desc *desc, const hh_kv_cache *cache, const void *q,
+                         const float *lse, const int32_t *path, const int32_t *accepted);
+
+/* Histories back to `keep` rows a head: of each layer, sequence and kv head whose length exceeds
+ * `keep`, the rows of the `recent` newest positions stay (position >= next_position − recent), then those of
+ * the largest weight (NaN counts as −inf), ties to the lowest row. The i-th freed row below `keep` takes the
+ * i-th kept row from `keep` on, with its weight and position; the other rows stay where they are, and
+ * rows from `keep` on are left as they were. lengths becomes `keep`. Layers that share lengths are
+ * evicted in one call. 0 < keep <= rows, 0 <= recent <= keep. Every cache needs weights, positions and
+ * next_position. desc: sequences, kv_heads, head_dim.                                          */
+int hh_cache_evict(hh_ctx *ctx, const hh_tree_desc *desc, const hh_kv_cache *caches, int32_t count,
+                   int32_t keep, int32_t recent);
+
+/* Pre-sizes the context's workspace of the calls above (each argument NULL where its calls are not
+ * made): hh_attention_tree on `cache`, hh_draft_verify, and hh_cache_evict of `layers` layers like `cache`. A
+ * workspace grows by itself in eager calls, but not while a graph is recorded or lives.       */
+int hh_draft_reserve(hh_ctx *ctx, const hh_tree_desc *tree, const hh_kv_cache *cache, int32_t layers,
+                     const hh_verify_desc *verify);
+
 #ifdef __cplusplus
 }
 #endif
