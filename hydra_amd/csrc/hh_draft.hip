@@ -72,7 +72,7 @@ int check_tree(const hh_tree_desc *d) {
 int check_cache(const hh_tree_desc *d, const hh_kv_cache *c) {
   if (!c) return fail(HH_EINVAL, "cache is NULL");
   if (!c->k || !c->v || !c->lengths) return fail(HH_EINVAL, "a cache needs k, v and lengths");
-  if (c->rows < 1) return fail(HH_EINVAL, "a cache needs rows >= 1");
+  if (c->rows < 1 || c->rows > 1 << 30) return fail(HH_EINVAL, "a cache's rows outside 1..2^30");
   if (!aligned16(c->k) || !aligned16(c->v)) return fail(HH_EALIGN, "the caches must be 16-byte aligned");
   const int64_t all = (int64_t)c->rows * d->kv_heads * d->head_dim;
   if (c->sequence_stride && c->sequence_stride < all) return fail(HH_ESHAPE, "sequence_stride is smaller than a sequence's rows");
@@ -201,8 +201,14 @@ int hh_attention_tree(hh_ctx *ctx, const hh_tree_desc *d, const hh_kv_cache *cac
   a.sinks = sinks;
   a.out = out;
   a.lse = lse;
+  hh::tree_plan(a, d->max_length ? d->max_length : cache->rows);
+  if (int rc = ensure_draft(ctx, hh::tree_workspace(a))) return rc;
+  const size_t slots = (size_t)a.S * a.N * a.qh * a.chunks;
+  a.po = (float *)ctx->draft;
+  a.pm = a.po + slots * a.d;
+  a.pl = a.pm + slots;
   HH_HIP(hh::launch_tree(a, d->type, ctx->stream));
-  ctx->dispatches += 1;
+  ctx->dispatches += a.chunks > 1 ? 2 : 1;
   return HH_OK;
 }
 
@@ -348,6 +354,13 @@ int hh_draft_reserve(hh_ctx *ctx, const hh_tree_desc *tree, const hh_kv_cache *c
     if (int rc = check_cache(tree, cache)) return rc;
     const int per = layers < hh::kRowsLayers ? layers : hh::kRowsLayers;
     if (layers) need = evict_bytes(tree, per, cache->rows);
+    if (tree->nodes) {
+      if (int rc = check_tree(tree)) return rc;
+      hh::TreeArgs a = tree_args(tree, cache, nullptr);
+      hh::tree_plan(a, tree->max_length ? tree->max_length : cache->rows);
+      const size_t b = hh::tree_workspace(a);
+      if (b > need) need = b;
+    }
   }
   if (verify) {
     if (int rc = check_verify(verify)) return rc;

@@ -9,6 +9,8 @@ namespace hh {
 enum Elem { E_F32 = 0, E_F16 = 1, E_BF16 = 2 };
 constexpr int kTreeNodes = 64;    // most nodes of a tree: an ancestor set is one 64-bit mask
 constexpr int kTreeQM = 16;       // most query heads per kv head
+constexpr int kTreeGroups = 512;  // workgroups that a call's keys are split for
+constexpr int kTreeChunks = 256;  // most chunks of a sequence
 
 struct TreeArgs {
   const void *q, *dk, *dv;          // [S][N][qh][d] and [S][N][kvh][d], strides below
@@ -20,6 +22,9 @@ struct TreeArgs {
   int S, N, qh, kvh, d, rows, ring, window;
   float scale;
   int64_t q_stride, kv_stride, seq_stride;   // elements between nodes, nodes, sequences
+  // How a call's keys are split (tree_plan): chunks of per_chunk keys, whole tiles; blocks of rows.
+  int chunks, per_chunk, tile, row_blocks;
+  float *pm, *pl, *po;              // chunk states [S][N][qh][chunks], their sums [..][chunks][d]
   // hh_attention_weights
   const float *lse_in;
   const int32_t *path, *accepted;
@@ -63,6 +68,8 @@ struct VerifyArgs {
 };
 
 size_t verify_workspace(int S, int N, int V, int mode, int children, bool greedy);
+void tree_plan(TreeArgs &a, int64_t length);
+size_t tree_workspace(const TreeArgs &a);
 hipError_t launch_tree(const TreeArgs &a, int type, hipStream_t s);
 hipError_t launch_weights(const TreeArgs &a, int type, hipStream_t s);
 hipError_t launch_verify(const VerifyArgs &a, hipStream_t s);

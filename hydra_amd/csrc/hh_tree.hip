@@ -1,29 +1,65 @@
 // hh_tree.hip — attention of a tree of drafted tokens over the history, and the accumulation of
 // the accepted tokens' attention weights.
+//
+// Attention. A kv head's rows are the (node, query head) pairs of its group, r = node·qm + head; a
+// workgroup takes 32·RT of them and a chunk of the keys (the history's visible rows, behind the last of
+// them the drafted ones), a wave 32 rows and every KS-th run of 32 keys. Keys and values go straight to
+// an LDS ring, NST − 1 tiles of 32·KS keys ahead. One pass with the running maximum M and sum L of
+// each row, everything in the exponent base 2 (y = logit·log2 e):
+//   S^T [32 keys × 32 rows] = K · q^T, keys as the A operand, the rows' queries in registers;
+//   O^T [D × 32 rows] += V^T · P^T, the value tile read by columns (transposing LDS reads), P^T from S^T's own
+//   registers: a lane holds one row's probabilities at 16 keys, and the products' order over the keys is the
+//   lane's. So a row's maximum and sum stay in its two lanes, and rescaling needs no exchange.
+// p = 2^(y − M + 10): small probabilities stay above fp16's smallest step. F32 activations: queries and
+// probabilities as fp16 pairs hi + lo, two products each (exact in fp32 to ~2^-22).
+// A chunk's state (M, L, O) goes to the workspace and tree_merge_kernel joins a row's chunks in order; a call of
+// one chunk writes its outputs at once. The sink enters where the states are joined.
 #include "hh_common.hpp"
 #include "hh_draft.hpp"
 
 namespace hh {
 
-__device__ __forceinline__ float elem_f32(const _Float16 *p) { return (float)*p; }
-__device__ __forceinline__ float elem_f32(const float *p) { return *p; }
-__device__ __forceinline__ float elem_f32(const __bf16 *p) { return (float)*p; }
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ float wsum(float v) {
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  return v;
+// 16 bytes per lane from global memory straight into LDS byte `l` + 16·lane; the kernels wait with wait_vm. In
+// assembly, so that the compiler does not order the wave's LDS reads after its loads in flight.
+__device__ __forceinline__ void dma16(const void *p, uint32_t l) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(l), "v"(p) : "memory", "m0");
 }
-__device__ __forceinline__ float wmax(float v) {
-  for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-  return v;
-}
+template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+// Barrier after the wave's own LDS reads have returned: the next tile may overwrite what they read.
+__device__ __forceinline__ void step_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+typedef __attribute__((address_space(3))) void *lds_ptr_t;
+__device__ __forceinline__ uint32_t lds_addr(const void *l) { return (uint32_t)(uintptr_t)(lds_ptr_t)l; }
 
-// The ancestors-or-self of every node as bit masks, lane i node i (i < N).
+template <bool BF> __device__ __forceinline__ f32x16 mfma32(const u32x4 &a, const u32x4 &b, const f32x16 &c) {
+  if constexpr (BF) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// The value of the other half of the wave (lane ^ 32).
+__device__ __forceinline__ float other_half(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+__device__ __forceinline__ float max_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kOff = 10.f;       // p = 2^(y − M + kOff)
+constexpr float kNone = -1e30f;    // a maximum of nothing: finite, so that no difference of maxima is NaN
+
+// The ancestors-or-self of every node as bit masks, lane i node i (i < N); a parent that is not an
+// earlier node counts as none.
 __device__ __forceinline__ uint64_t ancestors(const int32_t *parents, int N, int lane) {
   int up = lane < N ? parents[lane] : -1;
   if (up < 0 || up >= lane) up = -1;
   uint64_t mask = 1ull << lane;
-  for (int r = 0; r < 6; ++r) {
+  for (int r = 0; r < 6; ++r) {   // lines of up to 64 nodes, by doubling
     const int at = up < 0 ? lane : up;
     const uint32_t lo = __shfl((uint32_t)mask, at), hi = __shfl((uint32_t)(mask >> 32), at);
     const int next = __shfl(up, at);
@@ -34,74 +70,360 @@ __device__ __forceinline__ uint64_t ancestors(const int32_t *parents, int N, int
   }
   return mask;
 }
-
-// One wave per (sequence, node, head).
-template <class Q, class C>
-__global__ __launch_bounds__(64) void tree_kernel(TreeArgs a) {
-  const int lane = threadIdx.x, h = blockIdx.x % a.qh, n = blockIdx.x / a.qh % a.N, s = blockIdx.x / (a.qh * a.N);
-  if (n >= a.counts[s]) return;
-  __shared__ float s_q[256], s_p[64];
-  const int g = h / (a.qh / a.kvh), D = a.d;
-  const Q *q = (const Q *)a.q + ((int64_t)s * a.N + n) * a.q_stride + (int64_t)h * D;
-  for (int i = lane; i < D; i += 64) s_q[i] = elem_f32(q + i) * a.scale;
-  const uint64_t mask = ancestors(a.parents + (int64_t)s * a.N, a.N, lane);
-  const uint64_t own = ((uint64_t)(uint32_t)__shfl((uint32_t)(mask >> 32), n) << 32) | (uint32_t)__shfl((uint32_t)mask, n);
-  const int depth = __popcll(mask) - 1;
-  const int64_t length = a.ring ? max(a.lengths[s], 0) : min(max(a.lengths[s], 0), a.rows);
-  const int64_t pos = length + __popcll(own) - 1;
-  int64_t first = a.ring ? max((int64_t)0, length - a.rows) : 0;
-  if (a.window) first = max(first, pos - a.window + 1);
-  const int64_t keys = max((int64_t)0, length - first);
-  __syncthreads();
-  float M = a.sinks ? bf16_bits_to_f32(a.sinks[h]) : -INFINITY, L = a.sinks ? 1.f : 0.f;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  const int64_t base = (int64_t)s * a.seq_stride + (int64_t)g * D;
-  for (int64_t t = 0; t < keys + a.N; t += 64) {
-    const int64_t j = t + lane;
-    const C *kr = nullptr;
-    if (j < keys) {
-      const int64_t row = a.ring ? (first + j) % a.rows : first + j;
-      kr = (const C *)a.k + base + row * a.kvh * D;
-    } else if (j < keys + a.N) {
-      const int m = (int)(j - keys);
-      const int dm = __popcll(own & ((2ull << m) - 1)) - 1;   // the ancestor's depth
-      if ((own >> m & 1) && (!a.window || dm + length > pos - a.window))
-        kr = (const C *)a.dk + ((int64_t)s * a.N + m) * a.kv_stride + (int64_t)g * D;
-    }
-    float x = -INFINITY;
-    if (kr) {
-      x = 0.f;
-      for (int i = 0; i < D; ++i) x = fmaf(s_q[i], elem_f32(kr + i), x);
-    }
-    const float mn = fmaxf(M, wmax(x));
-    const float p = kr ? __expf(x - mn) : 0.f;
-    const float corr = mn == -INFINITY ? 1.f : __expf(M - mn);
-    L = L * corr + wsum(p);
-    M = mn;
-    s_p[lane] = p;
-    const uint64_t used = __ballot(kr != nullptr);
-    __syncthreads();
-    for (int i = 0; i < 4; ++i) acc[i] *= corr;
-    for (int jj = 0; jj < 64; ++jj) {
-      if (!(used >> jj & 1)) continue;
-      const int64_t j2 = t + jj;
-      const C *vr;
-      if (j2 < keys) {
-        const int64_t row = a.ring ? (first + j2) % a.rows : first + j2;
-        vr = (const C *)a.v + base + row * a.kvh * D;
-      } else {
-        vr = (const C *)a.dv + ((int64_t)s * a.N + (j2 - keys)) * a.kv_stride + (int64_t)g * D;
-      }
-      for (int i = 0; i < 4; ++i)
-        if (lane + 64 * i < D) acc[i] = fmaf(s_p[jj], elem_f32(vr + lane + 64 * i), acc[i]);
-    }
-    __syncthreads();
-  }
-  const int64_t o = (((int64_t)s * a.N + n) * a.qh + h) * D;
-  for (int i = 0; i < 4; ++i)
-    if (lane + 64 * i < D) ((Q *)a.out)[o + lane + 64 * i] = (Q)(acc[i] / L);
-  if (lane == 0 && a.lse) a.lse[((int64_t)s * a.N + n) * a.qh + h] = M + __logf(L);
+__device__ __forceinline__ uint64_t shfl64(uint64_t v, int at) {
+  return ((uint64_t)__shfl((uint32_t)(v >> 32), at) << 32) | __shfl((uint32_t)v, at);
 }
+
+// A sequence's visible history: positions first .. first + keys − 1 (those that its roots see), in `used`
+// chunks of `per` keys. A launch sized for shorter histories has chunks of more keys.
+struct Span {
+  int64_t length, first;
+  int keys, per, used;
+};
+__device__ __forceinline__ Span span_of(const TreeArgs &a, int s) {
+  Span p;
+  p.length = a.ring ? max(a.lengths[s], 0) : min(max(a.lengths[s], 0), a.rows);
+  p.first = a.ring ? max((int64_t)0, p.length - a.rows) : 0;
+  if (a.window) p.first = max(p.first, p.length - a.window + 1);
+  p.keys = (int)(p.length - p.first);
+  const int need = (p.keys + a.chunks - 1) / a.chunks;
+  p.per = max(a.per_chunk, (need + a.tile - 1) / a.tile * a.tile);
+  p.used = max(1, (p.keys + p.per - 1) / p.per);
+  return p;
+}
+
+// A row's four outputs from its joined state: the sink's share of the denominator, the quotient, its rounding.
+template <int QT, int D>
+__device__ __forceinline__ void finish_row(const TreeArgs &a, int64_t row, int head, int q4, float m, float den, f32x4 o) {
+  if (a.sinks) {
+    const float y = bf16_bits_to_f32(a.sinks[head]) * kLog2e, mn = fmaxf(m, y), f = exp2_(m - mn);
+    den = fmaf(den, f, exp2_(y - mn));
+    o *= f;
+    m = mn;
+  }
+  const float inv = 1.f / den;
+  if constexpr (QT == E_F32) {
+    *(f32x4 *)((float *)a.out + row * D + 4 * q4) = o * inv;
+  } else if constexpr (QT == E_F16) {
+    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+    *(f16x4 *)((_Float16 *)a.out + row * D + 4 * q4) = f16x4{(_Float16)(o[0] * inv), (_Float16)(o[1] * inv), (_Float16)(o[2] * inv), (_Float16)(o[3] * inv)};
+  } else {
+    typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+    *(bf16x4 *)((__bf16 *)a.out + row * D + 4 * q4) = bf16x4{(__bf16)(o[0] * inv), (__bf16)(o[1] * inv), (__bf16)(o[2] * inv), (__bf16)(o[3] * inv)};
+  }
+  if (q4 == 0 && a.lse) a.lse[row] = (m + __builtin_amdgcn_logf(den)) * kLn2;
+}
+
+// QT: hh_elem of q. RT row tiles of 32, KS key splits, a ring of NST tiles.
+template <int QT, int D, int RT, int KS, int NST>
+__global__ __launch_bounds__(64 * RT * KS) void tree_split_kernel(TreeArgs a) {
+  constexpr int NW = RT * KS, NT = 64 * NW, KT = 32 * KS, CH = D / 8, NL = D / (8 * RT), STAGE = KT * D * 4;
+  constexpr int ROWS = 32 * RT, NB = D / 32;
+  constexpr bool BF = QT == E_BF16, PAIR = QT == E_F32;
+  constexpr int OUTS = KS * ROWS * D * 4, LDS = NST * STAGE > OUTS ? NST * STAGE : OUTS;
+  __shared__ __align__(1024) uint8_t s_mem[LDS];
+  __shared__ float s_m[KS][ROWS], s_l[KS][ROWS];
+  warm_kernargs<sizeof(TreeArgs)>();
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rt = wave % RT, ks = wave / RT, l32 = lane & 31, hh = lane >> 5;
+  // Row blocks of one (sequence, kv head, chunk) on one XCD: they read the same keys.
+  const int groups = a.S * a.kvh * a.chunks;
+  const int x = blockIdx.x & 7, y = blockIdx.x >> 3, rb = y % a.row_blocks, grp = (y / a.row_blocks) * 8 + x;
+  if (grp >= groups) return;
+  const int chunk = grp / (a.S * a.kvh), sg = grp - chunk * (a.S * a.kvh), s = sg / a.kvh, g = sg - s * a.kvh;
+  const int qm = a.qh / a.kvh;
+  const int count = min(max(a.counts[s], 0), a.N);
+  if (rb * ROWS >= count * qm) return;
+  const Span sp = span_of(a, s);
+  if (chunk >= sp.used) return;
+  const int c0 = chunk * sp.per, nc = min(sp.per, sp.keys - c0);   // cached keys of the chunk
+  const int drafted = chunk == sp.used - 1 ? count : 0;
+  const int tiles = (nc + drafted + KT - 1) / KT;
+
+  // Loads: 16-byte pieces of a row in consecutive lanes, XORed by the row (sw) so that both ways of reading
+  // are free of bank conflicts.
+  const int r0 = (int)(a.ring ? (sp.first + c0) % a.rows : sp.first + c0);
+  const uint16_t *kb = a.k + (int64_t)s * a.seq_stride + (int64_t)g * D, *vb = a.v + (int64_t)s * a.seq_stride + (int64_t)g * D;
+  const int64_t dbase = (int64_t)s * a.N * a.kv_stride + (int64_t)g * D;
+  const uint16_t *dkb = (const uint16_t *)a.dk + dbase, *dvb = (const uint16_t *)a.dv + dbase;
+  const uint32_t lds0 = lds_addr(s_mem);
+  const int rstride = a.kvh * D;
+  auto sw = [](int row) { return ((row & 3) << 1) | ((row >> 2) & 1); };
+  auto load_tile = [&](int t, int slot) {
+#pragma unroll
+    for (int u = 0; u < NL; ++u) {
+      const int p0 = (u * NW + wave) * 64;             // uniform
+      const bool v = p0 >= KT * CH;
+      const int p = (v ? p0 - KT * CH : p0) + lane, row = p / CH, c = (p % CH) ^ sw(row);
+      const int idx = t * KT + row;
+      const uint16_t *src;
+      if (idx < nc) {
+        int r = r0 + idx;
+        if (r >= a.rows) r -= a.rows;                  // a ring's end
+        src = (v ? vb : kb) + (int64_t)r * rstride;
+      } else {
+        const int m = idx - nc;                        // rows past the last node are masked: read node 0's
+        src = (v ? dvb : dkb) + (int64_t)(m < count ? m : 0) * a.kv_stride;
+      }
+      dma16(src + 8 * c, lds0 + slot * STAGE + p0 * 16);
+    }
+  };
+#pragma unroll
+  for (int t = 0; t < NST - 1; ++t)
+    if (t < tiles) load_tile(t, t);
+
+  // The lane's row: its node, what that sees, its queries.
+  const int r = rb * ROWS + rt * 32 + l32, rn = r / qm;
+  const bool real = rn < count;
+  const int node = real ? rn : 0, head = g * qm + (real ? r - rn * qm : 0);
+  uint64_t vis = shfl64(ancestors(a.parents + (int64_t)s * a.N, a.N, lane), node);
+  const int depth = __popcll(vis) - 1;
+  int lo = 0;   // the first cached key of the chunk that the node sees
+  if (a.window) {
+    lo = (int)max((int64_t)0, sp.length + depth - a.window + 1 - sp.first) - c0;
+    while (__popcll(vis) > a.window) vis &= vis - 1;   // the oldest ancestors
+  }
+  int lo_max = lo;
+  if (a.window)
+    for (int o = 16; o; o >>= 1) lo_max = max(lo_max, __shfl_xor(lo_max, o));
+  lo_max = __builtin_amdgcn_readfirstlane(lo_max);
+  const float scale = PAIR ? 1.f : fabsf(a.scale) * kLog2e;   // S -> y
+  u32x4 qf[D / 16], ql[PAIR ? D / 16 : 1];
+  {
+    const int64_t at = ((int64_t)s * a.N + node) * a.q_stride + (int64_t)head * D + 8 * hh;
+#pragma unroll
+    for (int dc = 0; dc < D / 16; ++dc) {
+      if constexpr (PAIR) {
+        const f32x4 *qp = (const f32x4 *)((const float *)a.q + at + 16 * dc);
+        const f32x4 q0 = qp[0], q1 = qp[1];
+        f16x8 h, l;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float v = (e < 4 ? q0[e & 3] : q1[e & 3]) * (a.scale * kLog2e);
+          // Rounded to fp32 before it is split: hi must not come from the product by one mixed-precision
+          // instruction, whose single rounding differs near ties from that of the hi that lo is the rest of.
+          asm volatile("" : "+v"(v));
+          h[e] = (_Float16)v;
+          l[e] = (_Float16)(v - (float)h[e]);
+        }
+        qf[dc] = __builtin_bit_cast(u32x4, h);
+        ql[dc] = __builtin_bit_cast(u32x4, l);
+      } else {
+        qf[dc] = *(const u32x4 *)((const uint16_t *)a.q + at + 16 * dc);
+        if (a.scale < 0.f) qf[dc] ^= 0x80008000u;
+      }
+    }
+  }
+  float M = kNone, L = 0.f;
+  f32x16 acc[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) acc[n] = f32x16{};
+  const int j16 = lane & 15;
+  const int vrow = 4 * hh + (j16 >> 2), vpiece = (2 * ((lane >> 4) & 1) + ((j16 & 3) >> 1)) ^ sw(vrow), vhalf = (j16 & 1) * 8;
+
+  for (int t = 0; t < tiles; ++t) {
+    if (t + NST - 2 < tiles) wait_vm<(NST - 2) * NL>();
+    else wait_vm<0>();
+    step_barrier();
+    if (t + NST - 1 < tiles) load_tile(t + NST - 1, (t + NST - 1) % NST);
+    const uint8_t *kt = s_mem + (t % NST) * STAGE, *vt = kt + KT * D * 2;
+    const int base = t * KT + 32 * ks;   // the wave's first key
+    f32x16 S = f32x16{};
+    const uint8_t *krow = kt + (32 * ks + l32) * (2 * D);
+#pragma unroll
+    for (int dc = 0; dc < D / 16; ++dc) {
+      const u32x4 kf = *(const u32x4 *)(krow + (((2 * dc + hh) ^ sw(l32)) << 4));
+      S = mfma32<BF>(kf, qf[dc], S);
+      if constexpr (PAIR) S = mfma32<BF>(kf, ql[dc], S);
+    }
+    // Key of element i: base + 8 (i / 4) + 4 hh + i % 4.
+    const bool border = base + 32 > nc || base < lo_max;
+    if (border)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int k = base + 8 * (i >> 2) + 4 * hh + (i & 3), m = k - nc;
+        const bool sees = m < 0 ? k >= lo : (m < 64 && (vis >> (m & 63) & 1));
+        S[i] = sees ? S[i] : -INFINITY;
+      }
+    float top = fmaxf(S[0], S[1]);
+#pragma unroll
+    for (int i = 2; i < 16; ++i) top = fmaxf(top, S[i]);
+    top = max_halves(top) * scale;
+    if (__any(top > M)) {
+      const float mn = fmaxf(M, top), corr = exp2_(M - mn);
+      M = mn;
+      L *= corr;
+#pragma unroll
+      for (int n = 0; n < NB; ++n) acc[n] *= corr;
+    }
+    const float sub = kOff - M;
+    float p[16];
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      p[i] = exp2_(fmaf(S[i], scale, sub));
+      sum[i & 3] += p[i];
+    }
+    L += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    // Infinities or NaN in the values of a tile that some row does not see whole: 0 · NaN would carry them into
+    // rows that do not see them. Such a tile's values are added key by key, to the rows that do.
+    bool odd = false;
+    if (border) {
+      const uint32_t em = BF ? 0x7F80u : 0x7C00u;
+#pragma unroll
+      for (int u = 0; u < D / 16; ++u) {
+        const u32x4 w = *(const u32x4 *)(vt + 32 * ks * 2 * D + (u * 64 + lane) * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) odd |= (w[e] & em) == em || (w[e] >> 16 & em) == em;
+      }
+      odd = __any(odd);
+    }
+    if (odd) {
+      for (int k = 0; k < 32; ++k) {
+        const int i = 4 * (k >> 3) + (k & 3);
+        float pk = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) pk = e == i ? p[e] : pk;
+        const float po = other_half(pk);
+        pk = (k >> 2 & 1) == hh ? pk : po;
+        const int kk = base + k, m = kk - nc;
+        const bool sees = m < 0 ? kk >= lo : (m < 64 && (vis >> (m & 63) & 1));
+        const int row = 32 * ks + k;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int d = 32 * n + 8 * (e >> 2) + 4 * hh + (e & 3);
+            const uint16_t w = *(const uint16_t *)(vt + row * 2 * D + (((d >> 3) ^ sw(row)) << 4) + 2 * (d & 7));
+            const float vv = BF ? bf16_bits_to_f32(w) : (float)__builtin_bit_cast(_Float16, w);
+            acc[n][e] = sees ? fmaf(pk, vv, acc[n][e]) : acc[n][e];
+          }
+      }
+      continue;
+    }
+    u32x4 ph[2], pl[PAIR ? 2 : 1];
+#pragma unroll
+    for (int kc = 0; kc < 2; ++kc) {
+      if constexpr (BF) {
+        bf16x8 h;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = (__bf16)p[8 * kc + e];
+        ph[kc] = __builtin_bit_cast(u32x4, h);
+      } else {
+        f16x8 h, l;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          h[e] = (_Float16)p[8 * kc + e];
+          if constexpr (PAIR) l[e] = (_Float16)(p[8 * kc + e] - (float)h[e]);
+        }
+        ph[kc] = __builtin_bit_cast(u32x4, h);
+        if constexpr (PAIR) pl[kc] = __builtin_bit_cast(u32x4, l);
+      }
+    }
+    // V^T: lane (l32, hh) takes dimension 32 n + l32 of keys 16 kc + 8 x + 4 hh .. + 3, the order of P^T.
+    const uint8_t *vcol = vt + (32 * ks + vrow) * (2 * D) + vhalf;
+#pragma unroll
+    for (int kc = 0; kc < 2; ++kc)
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        u32x4 vf;
+#pragma unroll
+        for (int x8 = 0; x8 < 2; ++x8) {
+          const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s16x4 *)(vcol + (16 * kc + 8 * x8) * 2 * D + ((vpiece ^ (4 * n)) << 4)));
+          const u32x2 b = __builtin_bit_cast(u32x2, w);
+          vf[2 * x8] = b[0];
+          vf[2 * x8 + 1] = b[1];
+        }
+        acc[n] = mfma32<BF>(vf, ph[kc], acc[n]);
+        if constexpr (PAIR) acc[n] = mfma32<BF>(vf, pl[kc], acc[n]);
+      }
+  }
+
+  // The splits' states meet in LDS, the sums of a row in 16-byte pieces XORed by the row.
+  L += other_half(L);
+  step_barrier();
+  float *so = (float *)s_mem + (size_t)(ks * ROWS + rt * 32 + l32) * D;
+  if (hh == 0) {
+    s_m[ks][rt * 32 + l32] = M - kOff;   // the exponent that L and O are relative to
+    s_l[ks][rt * 32 + l32] = L;
+  }
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const f32x4 w = {acc[n][4 * e], acc[n][4 * e + 1], acc[n][4 * e + 2], acc[n][4 * e + 3]};
+      *(f32x4 *)(so + 4 * ((8 * n + 2 * e + hh) ^ (l32 & 7))) = w;
+    }
+  __syncthreads();
+  for (int e = tid; e < ROWS * (D / 4); e += NT) {
+    const int row = e / (D / 4), q4 = e % (D / 4), rr = rb * ROWS + row, n = rr / qm;
+    if (n >= count) break;               // rows are in the order of their nodes
+    float m = s_m[0][row];
+#pragma unroll
+    for (int k = 1; k < KS; ++k) m = fmaxf(m, s_m[k][row]);
+    float den = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const float f = exp2_(s_m[k][row] - m);
+      den = fmaf(s_l[k][row], f, den);
+      const f32x4 w = *(const f32x4 *)((const float *)s_mem + (size_t)(k * ROWS + row) * D + 4 * (q4 ^ (row & 7)));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = fmaf(w[i], f, o[i]);
+    }
+    const int hd = g * qm + rr - n * qm;
+    const int64_t out = ((int64_t)s * a.N + n) * a.qh + hd;
+    if (a.chunks > 1) {
+      const int64_t slot = out * a.chunks + chunk;
+      *(f32x4 *)(a.po + slot * D + 4 * q4) = o;
+      if (q4 == 0) {
+        a.pm[slot] = m;
+        a.pl[slot] = den;
+      }
+    } else {
+      finish_row<QT, D>(a, out, hd, q4, m, den, o);
+    }
+  }
+}
+
+// Joins a row's chunks, in order: a wave per row, D / 4 lanes a chunk.
+template <int QT, int D>
+__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
+  warm_kernargs<sizeof(TreeArgs)>();
+  constexpr int LR = D / 4, GR = 64 / LR;    // lanes per chunk, chunks at a time
+  const int lane = threadIdx.x & 63, q4 = lane % LR, cg = lane / LR;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= (int64_t)a.S * a.N * a.qh) return;
+  const int hd = (int)(row % a.qh), n = (int)(row / a.qh % a.N), s = (int)(row / ((int64_t)a.qh * a.N));
+  if (n >= a.counts[s]) return;
+  const int used = span_of(a, s).used;
+  const float *pm = a.pm + row * a.chunks, *pl = a.pl + row * a.chunks, *po = a.po + row * a.chunks * D;
+  float m = kNone;
+  for (int c = lane; c < used; c += 64) m = fmaxf(m, pm[c]);
+  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  float den = 0.f;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int c = cg; c < used; c += GR) {
+    const float f = exp2_(pm[c] - m);
+    den = fmaf(pl[c], f, den);
+    const f32x4 w = *(const f32x4 *)(po + (int64_t)c * D + 4 * q4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] = fmaf(w[i], f, sum[i]);
+  }
+#pragma unroll
+  for (int o = LR; o < 64; o <<= 1) {
+    den += __shfl_xor(den, o);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] += __shfl_xor(sum[i], o);
+  }
+  if (cg == 0) finish_row<QT, D>(a, row, hd, q4, m, den, sum);
+}
+
+__device__ __forceinline__ float elem_f32(const _Float16 *p) { return (float)*p; }
+__device__ __forceinline__ float elem_f32(const float *p) { return *p; }
+__device__ __forceinline__ float elem_f32(const __bf16 *p) { return (float)*p; }
 
 // One wave per (sequence, kv head, 64 rows), a lane per row.
 template <class Q, class C>
@@ -127,12 +449,72 @@ __global__ __launch_bounds__(64) void weights_kernel(TreeArgs a) {
   a.weights[((int64_t)s * a.kvh + g) * a.rows + row] += w;
 }
 
-hipError_t launch_tree(const TreeArgs &a, int type, hipStream_t s) {
-  const dim3 grid(a.S * a.N * a.qh);
-  if (type == E_F32) hipLaunchKernelGGL((tree_kernel<float, _Float16>), grid, dim3(64), 0, s, a);
-  else if (type == E_F16) hipLaunchKernelGGL((tree_kernel<_Float16, _Float16>), grid, dim3(64), 0, s, a);
-  else hipLaunchKernelGGL((tree_kernel<__bf16, __bf16>), grid, dim3(64), 0, s, a);
+// The launch: RT by the rows of a kv head, KS and the ring so that a workgroup's tiles in flight cover the
+// memory's latency and fit LDS.
+struct TreeShape { int rt, ks, nst; };
+static TreeShape tree_shape(int d, int rows) {
+  const int rt = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+  if (d == 64) return {rt, 8 / rt, rt == 4 ? 4 : rt == 2 ? 3 : 2};
+  if (d == 128) return {rt, rt == 1 ? 4 : 8 / rt, rt == 4 ? 4 : 2};
+  return {rt, rt == 4 ? 1 : 2, rt == 4 ? 4 : 2};
+}
+
+// Fills in how the call's keys are split, for histories of up to `length` keys.
+void tree_plan(TreeArgs &a, int64_t length) {
+  const int rows = a.N * (a.qh / a.kvh);
+  const TreeShape t = tree_shape(a.d, rows);
+  a.tile = 32 * t.ks;
+  a.row_blocks = (rows + 32 * t.rt - 1) / (32 * t.rt);
+  int64_t keys = length < a.rows ? length : a.rows;
+  if (a.window && keys > a.window) keys = a.window;
+  const int64_t own = (int64_t)a.S * a.kvh * a.row_blocks;
+  int64_t chunks = kTreeGroups / own, most = (keys + a.tile - 1) / a.tile;
+  if (chunks > most) chunks = most;
+  if (chunks > kTreeChunks) chunks = kTreeChunks;
+  if (chunks < 1) chunks = 1;
+  int64_t per = ((keys + chunks - 1) / chunks + a.tile - 1) / a.tile * a.tile;
+  if (per < a.tile) per = a.tile;
+  a.per_chunk = (int)per;
+  a.chunks = (int)((keys + per - 1) / per);
+  if (a.chunks < 1) a.chunks = 1;
+}
+
+size_t tree_workspace(const TreeArgs &a) {
+  return a.chunks > 1 ? sizeof(float) * (size_t)a.S * a.N * a.qh * a.chunks * (a.d + 2) : 0;
+}
+
+template <int QT, int D> static hipError_t launch_tree_d(const TreeArgs &a, hipStream_t s) {
+  const TreeShape t = tree_shape(D, a.N * (a.qh / a.kvh));
+  const int groups = a.S * a.kvh * a.chunks;
+  const dim3 grid((groups + 7) / 8 * 8 * a.row_blocks), block(64 * t.rt * t.ks);
+  if constexpr (D == 64) {
+    if (t.rt == 1) hipLaunchKernelGGL((tree_split_kernel<QT, 64, 1, 8, 2>), grid, block, 0, s, a);
+    else if (t.rt == 2) hipLaunchKernelGGL((tree_split_kernel<QT, 64, 2, 4, 3>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((tree_split_kernel<QT, 64, 4, 2, 4>), grid, block, 0, s, a);
+  } else if constexpr (D == 128) {
+    if (t.rt == 1) hipLaunchKernelGGL((tree_split_kernel<QT, 128, 1, 4, 2>), grid, block, 0, s, a);
+    else if (t.rt == 2) hipLaunchKernelGGL((tree_split_kernel<QT, 128, 2, 4, 2>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((tree_split_kernel<QT, 128, 4, 2, 4>), grid, block, 0, s, a);
+  } else {
+    if (t.rt == 1) hipLaunchKernelGGL((tree_split_kernel<QT, 256, 1, 2, 2>), grid, block, 0, s, a);
+    else if (t.rt == 2) hipLaunchKernelGGL((tree_split_kernel<QT, 256, 2, 2, 2>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((tree_split_kernel<QT, 256, 4, 1, 4>), grid, block, 0, s, a);
+  }
+  if (a.chunks > 1) {
+    const int64_t rows = (int64_t)a.S * a.N * a.qh;
+    hipLaunchKernelGGL((tree_merge_kernel<QT, D>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, s, a);
+  }
   return hipGetLastError();
+}
+
+template <int QT> static hipError_t launch_tree_q(const TreeArgs &a, hipStream_t s) {
+  if (a.d == 64) return launch_tree_d<QT, 64>(a, s);
+  return a.d == 128 ? launch_tree_d<QT, 128>(a, s) : launch_tree_d<QT, 256>(a, s);
+}
+
+hipError_t launch_tree(const TreeArgs &a, int type, hipStream_t s) {
+  if (type == E_F32) return launch_tree_q<E_F32>(a, s);
+  return type == E_F16 ? launch_tree_q<E_F16>(a, s) : launch_tree_q<E_BF16>(a, s);
 }
 
 hipError_t launch_weights(const TreeArgs &a, int type, hipStream_t s) {

@@ -200,7 +200,10 @@ def test_keys_that_a_node_does_not_see_have_no_part(kind, D, H, G, N, ring):
         hit = np.array([depth[m] == 0 or 2 in line_of(t["parents"][0].tolist(), m) for m in range(N - 1)])
         assert hit.any() and not hit.all()
         assert not torch.isfinite(out2[0, :N - 1][torch.tensor(hit)]).any()
-        assert torch.equal(out2[0, :N - 1][torch.tensor(~hit)], out[0, :N - 1][torch.tensor(~hit)])
+        # The tile that holds such values is added key by key, in other roundings: both results are within TOL of the
+        # exact one, so within twice TOL of each other (plus a second-order term, below TOL^2).
+        a, b = (x[0, :N - 1][torch.tensor(~hit)].double() for x in (out2, out))
+        assert torch.isfinite(a).all() and (a - b).norm() < 2 * TOL[kind] * (1 + TOL[kind]) * b.norm()
         assert torch.equal(out2[1], out[1])
     finally:
         ctx.close()
