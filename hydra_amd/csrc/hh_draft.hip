@@ -40,6 +40,7 @@ int check_rows(const hh_tree_desc *d) {
   if (!d) return fail(HH_EINVAL, "desc is NULL");
   if (d->sequences < 1 || d->sequences > kMaxSequences) return fail(HH_EINVAL, "sequences outside 1..4096");
   if (d->kv_heads < 1 || d->kv_heads > 256) return fail(HH_ESHAPE, "kv_heads outside 1..256");
+  if ((int64_t)d->sequences * d->kv_heads > 1 << 18) return fail(HH_EINVAL, "sequences x kv_heads above 2^18");
   if (d->head_dim != 64 && d->head_dim != 128 && d->head_dim != 256)
     return fail(HH_ESHAPE, "head_dim must be 64, 128 or 256");
   return HH_OK;
@@ -50,6 +51,7 @@ int check_nodes(const hh_tree_desc *d) {
   if (d->nodes < 1 || d->nodes > HH_TREE_MAX_NODES) return fail(HH_EINVAL, "nodes outside 1..64");
   if (d->cache_type != HH_F16 && d->cache_type != HH_BF16) return fail(HH_EINVAL, "cache_type must be F16 or BF16");
   const int64_t row = (int64_t)d->kv_heads * d->head_dim;
+  if (d->kv_stride > 1 << 30) return fail(HH_ESHAPE, "kv_stride above 2^30");
   if (d->kv_stride && d->kv_stride < row) return fail(HH_ESHAPE, "kv_stride is smaller than a node's rows");
   if (d->kv_stride % 8) return fail(HH_EALIGN, "kv_stride must be a multiple of 16 bytes");
   return HH_OK;

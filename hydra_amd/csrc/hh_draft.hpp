@@ -23,7 +23,8 @@ struct TreeArgs {
   float scale;
   int64_t q_stride, kv_stride, seq_stride;   // elements between nodes, nodes, sequences
   // How a call's keys are split (tree_plan): chunks of per_chunk keys, whole tiles; blocks of rows.
-  int chunks, per_chunk, tile, row_blocks;
+  int chunks, per_chunk, tile, row_blocks, qm;
+  float inv_qm;
   float *pm, *pl, *po;              // chunk states [S][N][qh][chunks], their sums [..][chunks][d]
   // hh_attention_weights
   const float *lse_in;

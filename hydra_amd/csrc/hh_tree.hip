@@ -74,21 +74,24 @@ __device__ __forceinline__ uint64_t shfl64(uint64_t v, int at) {
   return ((uint64_t)__shfl((uint32_t)(v >> 32), at) << 32) | __shfl((uint32_t)v, at);
 }
 
-// A sequence's visible history: positions first .. first + keys − 1 (those that its roots see), in `used`
-// chunks of `per` keys. A launch sized for shorter histories has chunks of more keys.
+// A sequence's visible history: positions first .. first + keys − 1 (those that its roots see), in chunks of
+// `per` keys; chunk c is in use if c·per < keys, or c = 0. A launch sized for shorter histories has
+// chunks of more keys.
 struct Span {
-  int64_t length, first;
-  int keys, per, used;
+  int length, first, keys, per;
 };
 __device__ __forceinline__ Span span_of(const TreeArgs &a, int s) {
   Span p;
-  p.length = a.ring ? max(a.lengths[s], 0) : min(max(a.lengths[s], 0), a.rows);
-  p.first = a.ring ? max((int64_t)0, p.length - a.rows) : 0;
-  if (a.window) p.first = max(p.first, p.length - a.window + 1);
-  p.keys = (int)(p.length - p.first);
-  const int need = (p.keys + a.chunks - 1) / a.chunks;
-  p.per = max(a.per_chunk, (need + a.tile - 1) / a.tile * a.tile);
-  p.used = max(1, (p.keys + p.per - 1) / p.per);
+  p.length = max(a.lengths[s], 0);
+  if (!a.ring) p.length = min(p.length, a.rows);
+  p.first = a.ring ? max(0, p.length - a.rows) : 0;
+  if (a.window) p.first = max(p.first, (int)max((int64_t)0, (int64_t)p.length - a.window + 1));
+  p.keys = p.length - p.first;
+  p.per = a.per_chunk;
+  if ((int64_t)p.per * a.chunks < p.keys) {
+    const int need = (int)((uint32_t)p.keys / (uint32_t)a.chunks) + 1;
+    p.per = (int)(((uint32_t)need + a.tile - 1) & ~(uint32_t)(a.tile - 1));
+  }
   return p;
 }
 
@@ -114,58 +117,59 @@ __device__ __forceinline__ void finish_row(const TreeArgs &a, int64_t row, int h
   if (q4 == 0 && a.lse) a.lse[row] = (m + __builtin_amdgcn_logf(den)) * kLn2;
 }
 
-// QT: hh_elem of q. RT row tiles of 32, KS key splits, a ring of NST tiles.
-template <int QT, int D, int RT, int KS, int NST>
-__global__ __launch_bounds__(64 * RT * KS) void tree_split_kernel(TreeArgs a) {
+// QT: hh_elem of q. RT row tiles of 32, KS key splits, a ring of NST tiles, OCC waves per SIMD.
+template <int QT, int D, int RT, int KS, int NST, int OCC>
+__global__ __launch_bounds__(64 * RT * KS, OCC) void tree_split_kernel(TreeArgs a) {
   constexpr int NW = RT * KS, NT = 64 * NW, KT = 32 * KS, CH = D / 8, NL = D / (8 * RT), STAGE = KT * D * 4;
   constexpr int ROWS = 32 * RT, NB = D / 32;
   constexpr bool BF = QT == E_BF16, PAIR = QT == E_F32;
   constexpr int OUTS = KS * ROWS * D * 4, LDS = NST * STAGE > OUTS ? NST * STAGE : OUTS;
   __shared__ __align__(1024) uint8_t s_mem[LDS];
   __shared__ float s_m[KS][ROWS], s_l[KS][ROWS];
+  __shared__ uint64_t s_vis[ROWS];
+  __shared__ int s_lo[ROWS], s_odd;
   warm_kernargs<sizeof(TreeArgs)>();
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rt = wave % RT, ks = wave / RT, l32 = lane & 31, hh = lane >> 5;
-  // Row blocks of one (sequence, kv head, chunk) on one XCD: they read the same keys.
-  const int groups = a.S * a.kvh * a.chunks;
-  const int x = blockIdx.x & 7, y = blockIdx.x >> 3, rb = y % a.row_blocks, grp = (y / a.row_blocks) * 8 + x;
-  if (grp >= groups) return;
-  const int chunk = grp / (a.S * a.kvh), sg = grp - chunk * (a.S * a.kvh), s = sg / a.kvh, g = sg - s * a.kvh;
-  const int qm = a.qh / a.kvh;
+  // Row blocks of one (sequence, kv head, chunk) on one XCD, one after the other: they read the same keys.
+  const uint32_t grp = blockIdx.y * 8 + (blockIdx.x & 7), own = a.S * a.kvh;
+  const int rb = blockIdx.x >> 3, chunk = (int)(grp / own);
+  if (chunk >= a.chunks) return;
+  const int sg = (int)(grp - chunk * own), s = sg / a.kvh, g = sg - s * a.kvh, qm = a.qm;
   const int count = min(max(a.counts[s], 0), a.N);
   if (rb * ROWS >= count * qm) return;
   const Span sp = span_of(a, s);
-  if (chunk >= sp.used) return;
-  const int c0 = chunk * sp.per, nc = min(sp.per, sp.keys - c0);   // cached keys of the chunk
-  const int drafted = chunk == sp.used - 1 ? count : 0;
-  const int tiles = (nc + drafted + KT - 1) / KT;
+  const int64_t c064 = (int64_t)chunk * sp.per;
+  if (chunk && c064 >= sp.keys) return;
+  const int c0 = (int)c064, nc = min(sp.per, sp.keys - c0);   // cached keys of the chunk
+  const bool last = c064 + sp.per >= sp.keys;
+  const int tiles = (nc + (last ? count : 0) + KT - 1) / KT;
 
   // Loads: 16-byte pieces of a row in consecutive lanes, XORed by the row (sw) so that both ways of reading
   // are free of bank conflicts.
-  const int r0 = (int)(a.ring ? (sp.first + c0) % a.rows : sp.first + c0);
-  const uint16_t *kb = a.k + (int64_t)s * a.seq_stride + (int64_t)g * D, *vb = a.v + (int64_t)s * a.seq_stride + (int64_t)g * D;
+  const uint32_t r0 = a.ring ? (uint32_t)(sp.first + c0) % (uint32_t)a.rows : sp.first + c0;
+  const uint64_t kb = (uint64_t)(a.k + (int64_t)s * a.seq_stride + (int64_t)g * D);
+  const uint64_t vb = (uint64_t)(a.v + (int64_t)s * a.seq_stride + (int64_t)g * D);
   const int64_t dbase = (int64_t)s * a.N * a.kv_stride + (int64_t)g * D;
-  const uint16_t *dkb = (const uint16_t *)a.dk + dbase, *dvb = (const uint16_t *)a.dv + dbase;
-  const uint32_t lds0 = lds_addr(s_mem);
-  const int rstride = a.kvh * D;
+  const uint64_t dkb = (uint64_t)((const uint16_t *)a.dk + dbase), dvb = (uint64_t)((const uint16_t *)a.dv + dbase);
+  const uint32_t lds0 = lds_addr(s_mem), rstride = 2 * a.kvh * D, dstride = 2 * (uint32_t)a.kv_stride;
   auto sw = [](int row) { return ((row & 3) << 1) | ((row >> 2) & 1); };
   auto load_tile = [&](int t, int slot) {
 #pragma unroll
-    for (int u = 0; u < NL; ++u) {
-      const int p0 = (u * NW + wave) * 64;             // uniform
-      const bool v = p0 >= KT * CH;
-      const int p = (v ? p0 - KT * CH : p0) + lane, row = p / CH, c = (p % CH) ^ sw(row);
-      const int idx = t * KT + row;
-      const uint16_t *src;
-      if (idx < nc) {
-        int r = r0 + idx;
-        if (r >= a.rows) r -= a.rows;                  // a ring's end
-        src = (v ? vb : kb) + (int64_t)r * rstride;
-      } else {
-        const int m = idx - nc;                        // rows past the last node are masked: read node 0's
-        src = (v ? dvb : dkb) + (int64_t)(m < count ? m : 0) * a.kv_stride;
+    for (int v = 0; v < 2; ++v) {                      // keys, values
+      const uint64_t cached = v ? vb : kb, drafted = v ? dvb : dkb;
+#pragma unroll 4
+      for (int u = 0; u < NL / 2; ++u) {
+        const int p0 = (u * NW + wave) * 64, p = p0 + lane, row = p / CH, c = (p % CH) ^ sw(row);
+        const int idx = t * KT + row, m = idx - nc;
+        uint32_t r = r0 + idx;
+        r = r >= (uint32_t)a.rows ? r - a.rows : r;    // a ring's end
+        // Behind the cached keys the nodes; rows past the last node are masked: they read node 0's.
+        const uint32_t at = m < 0 ? r : m < count ? m : 0, stride = m < 0 ? rstride : dstride;
+        const uint64_t base = (m < 0 ? cached : drafted) + 16 * c;
+        dma16((const void *)(base + (uint64_t)at * stride),
+              __builtin_amdgcn_readfirstlane(lds0 + slot * STAGE + v * (KT * D * 2) + p0 * 16));
       }
-      dma16(src + 8 * c, lds0 + slot * STAGE + p0 * 16);
     }
   };
 #pragma unroll
@@ -173,20 +177,23 @@ __global__ __launch_bounds__(64 * RT * KS) void tree_split_kernel(TreeArgs a) {
     if (t < tiles) load_tile(t, t);
 
   // The lane's row: its node, what that sees, its queries.
-  const int r = rb * ROWS + rt * 32 + l32, rn = r / qm;
+  const int r = rb * ROWS + rt * 32 + l32, rn = (int)(((float)r + 0.5f) * a.inv_qm);   // r / qm: exact below 2^20
   const bool real = rn < count;
   const int node = real ? rn : 0, head = g * qm + (real ? r - rn * qm : 0);
-  uint64_t vis = shfl64(ancestors(a.parents + (int64_t)s * a.N, a.N, lane), node);
-  const int depth = __popcll(vis) - 1;
-  int lo = 0;   // the first cached key of the chunk that the node sees
-  if (a.window) {
-    lo = (int)max((int64_t)0, sp.length + depth - a.window + 1 - sp.first) - c0;
-    while (__popcll(vis) > a.window) vis &= vis - 1;   // the oldest ancestors
+  uint64_t vis = 0;
+  int lo = 0, lo_max = 0;   // the first cached key of the chunk that the node sees, and that every node sees
+  if (last || a.window) {
+    const uint64_t mask = ancestors(a.parents + (int64_t)s * a.N, a.N, lane);
+    vis = shfl64(mask, node);
+    if (a.window) {
+      auto low = [&](int depth) { return (int)max((int64_t)0, (int64_t)sp.length + depth - a.window + 1 - sp.first) - c0; };
+      lo = low(__popcll(vis) - 1);
+      int deepest = lane < count ? __popcll(mask) : 1;
+      for (int o = 32; o; o >>= 1) deepest = max(deepest, __shfl_xor(deepest, o));
+      lo_max = __builtin_amdgcn_readfirstlane(low(deepest - 1));
+      while (__popcll(vis) > a.window) vis &= vis - 1;   // the oldest ancestors
+    }
   }
-  int lo_max = lo;
-  if (a.window)
-    for (int o = 16; o; o >>= 1) lo_max = max(lo_max, __shfl_xor(lo_max, o));
-  lo_max = __builtin_amdgcn_readfirstlane(lo_max);
   const float scale = PAIR ? 1.f : fabsf(a.scale) * kLog2e;   // S -> y
   u32x4 qf[D / 16], ql[PAIR ? D / 16 : 1];
   {
@@ -214,6 +221,12 @@ __global__ __launch_bounds__(64 * RT * KS) void tree_split_kernel(TreeArgs a) {
       }
     }
   }
+  if (ks == 0 && hh == 0) {
+    s_vis[rt * 32 + l32] = vis;
+    s_lo[rt * 32 + l32] = lo;
+  }
+  if (tid == 0) s_odd = 0;
+  auto is_part = [&](int t) { return t * KT < lo_max || (t + 1) * KT > nc; };
   float M = kNone, L = 0.f;
   f32x16 acc[NB];
 #pragma unroll
@@ -226,7 +239,30 @@ __global__ __launch_bounds__(64 * RT * KS) void tree_split_kernel(TreeArgs a) {
     else wait_vm<0>();
     step_barrier();
     if (t + NST - 1 < tiles) load_tile(t + NST - 1, (t + NST - 1) % NST);
-    const uint8_t *kt = s_mem + (t % NST) * STAGE, *vt = kt + KT * D * 2;
+    uint8_t *kt = s_mem + (t % NST) * STAGE, *vt = kt + KT * D * 2;
+    // A tile that some row does not see whole: infinities and NaN among its values are taken out (0 · NaN would
+    // carry them to rows that do not see them) and put back into the rows that do behind the loop.
+    const bool part = is_part(t);
+    if (part) {
+#pragma unroll
+      for (int u = 0; u < D / (16 * RT); ++u) {
+        u32x4 *w = (u32x4 *)vt + u * NT + tid;
+        u32x4 x = *w;
+        bool odd = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t em = BF ? 0x7F80u : 0x7C00u;
+          const bool l = (x[e] & em) == em, h = (x[e] >> 16 & em) == em;
+          x[e] &= (l ? 0u : 0xFFFFu) | (h ? 0u : 0xFFFF0000u);
+          odd |= l || h;
+        }
+        if (odd) {
+          *w = x;
+          s_odd = 1;
+        }
+      }
+      step_barrier();
+    }
     const int base = t * KT + 32 * ks;   // the wave's first key
     f32x16 S = f32x16{};
     const uint8_t *krow = kt + (32 * ks + l32) * (2 * D);
@@ -237,8 +273,7 @@ __global__ __launch_bounds__(64 * RT * KS) void tree_split_kernel(TreeArgs a) {
       if constexpr (PAIR) S = mfma32<BF>(kf, ql[dc], S);
     }
     // Key of element i: base + 8 (i / 4) + 4 hh + i % 4.
-    const bool border = base + 32 > nc || base < lo_max;
-    if (border)
+    if (part)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int k = base + 8 * (i >> 2) + 4 * hh + (i & 3), m = k - nc;
@@ -265,42 +300,6 @@ __global__ __launch_bounds__(64 * RT * KS) void tree_split_kernel(TreeArgs a) {
       sum[i & 3] += p[i];
     }
     L += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    // Infinities or NaN in the values of a tile that some row does not see whole: 0 · NaN would carry them into
-    // rows that do not see them. Such a tile's values are added key by key, to the rows that do.
-    bool odd = false;
-    if (border) {
-      const uint32_t em = BF ? 0x7F80u : 0x7C00u;
-#pragma unroll
-      for (int u = 0; u < D / 16; ++u) {
-        const u32x4 w = *(const u32x4 *)(vt + 32 * ks * 2 * D + (u * 64 + lane) * 16);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) odd |= (w[e] & em) == em || (w[e] >> 16 & em) == em;
-      }
-      odd = __any(odd);
-    }
-    if (odd) {
-      for (int k = 0; k < 32; ++k) {
-        const int i = 4 * (k >> 3) + (k & 3);
-        float pk = 0.f;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) pk = e == i ? p[e] : pk;
-        const float po = other_half(pk);
-        pk = (k >> 2 & 1) == hh ? pk : po;
-        const int kk = base + k, m = kk - nc;
-        const bool sees = m < 0 ? kk >= lo : (m < 64 && (vis >> (m & 63) & 1));
-        const int row = 32 * ks + k;
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int d = 32 * n + 8 * (e >> 2) + 4 * hh + (e & 3);
-            const uint16_t w = *(const uint16_t *)(vt + row * 2 * D + (((d >> 3) ^ sw(row)) << 4) + 2 * (d & 7));
-            const float vv = BF ? bf16_bits_to_f32(w) : (float)__builtin_bit_cast(_Float16, w);
-            acc[n][e] = sees ? fmaf(pk, vv, acc[n][e]) : acc[n][e];
-          }
-      }
-      continue;
-    }
     u32x4 ph[2], pl[PAIR ? 2 : 1];
 #pragma unroll
     for (int kc = 0; kc < 2; ++kc) {
@@ -357,7 +356,7 @@ __global__ __launch_bounds__(64 * RT * KS) void tree_split_kernel(TreeArgs a) {
     }
   __syncthreads();
   for (int e = tid; e < ROWS * (D / 4); e += NT) {
-    const int row = e / (D / 4), q4 = e % (D / 4), rr = rb * ROWS + row, n = rr / qm;
+    const int row = e / (D / 4), q4 = e % (D / 4), rr = rb * ROWS + row, n = (int)(((float)rr + 0.5f) * a.inv_qm);
     if (n >= count) break;               // rows are in the order of their nodes
     float m = s_m[0][row];
 #pragma unroll
@@ -371,6 +370,26 @@ __global__ __launch_bounds__(64 * RT * KS) void tree_split_kernel(TreeArgs a) {
       const f32x4 w = *(const f32x4 *)((const float *)s_mem + (size_t)(k * ROWS + row) * D + 4 * (q4 ^ (row & 7)));
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[i] = fmaf(w[i], f, o[i]);
+    }
+    if (s_odd) {
+      // The infinities and NaN of the tiles that were seen in part, from memory.
+      const uint64_t sees = s_vis[row];
+      for (int t = 0; t < tiles; ++t) {
+        if (!is_part(t)) continue;
+        for (int k = t * KT; k < t * KT + KT && k < nc + count; ++k) {
+          const int m = k - nc;
+          if (m < 0 ? k < s_lo[row] : !(sees >> m & 1)) continue;
+          uint32_t at = r0 + k;
+          at = at >= (uint32_t)a.rows ? at - a.rows : at;
+          const uint64_t src = (m < 0 ? vb + (uint64_t)at * rstride : dvb + (uint64_t)m * dstride) + 8 * q4;
+          const u32x2 w = *(const u32x2 *)src;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t h = w[i >> 1] >> 16 * (i & 1) & 0xFFFFu, em = BF ? 0x7F80u : 0x7C00u;
+            if ((h & em) == em) o[i] += BF ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+          }
+        }
+      }
     }
     const int hd = g * qm + rr - n * qm;
     const int64_t out = ((int64_t)s * a.N + n) * a.qh + hd;
@@ -397,7 +416,8 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
   if (row >= (int64_t)a.S * a.N * a.qh) return;
   const int hd = (int)(row % a.qh), n = (int)(row / a.qh % a.N), s = (int)(row / ((int64_t)a.qh * a.N));
   if (n >= a.counts[s]) return;
-  const int used = span_of(a, s).used;
+  const Span sp = span_of(a, s);
+  const int used = sp.keys <= sp.per ? 1 : (int)(((uint32_t)sp.keys + sp.per - 1) / (uint32_t)sp.per);
   const float *pm = a.pm + row * a.chunks, *pl = a.pl + row * a.chunks, *po = a.po + row * a.chunks * D;
   float m = kNone;
   for (int c = lane; c < used; c += 64) m = fmaxf(m, pm[c]);
@@ -461,7 +481,9 @@ static TreeShape tree_shape(int d, int rows) {
 
 // Fills in how the call's keys are split, for histories of up to `length` keys.
 void tree_plan(TreeArgs &a, int64_t length) {
-  const int rows = a.N * (a.qh / a.kvh);
+  a.qm = a.qh / a.kvh;
+  a.inv_qm = 1.f / (float)a.qm;
+  const int rows = a.N * a.qm;
   const TreeShape t = tree_shape(a.d, rows);
   a.tile = 32 * t.ks;
   a.row_blocks = (rows + 32 * t.rt - 1) / (32 * t.rt);
@@ -485,20 +507,20 @@ size_t tree_workspace(const TreeArgs &a) {
 
 template <int QT, int D> static hipError_t launch_tree_d(const TreeArgs &a, hipStream_t s) {
   const TreeShape t = tree_shape(D, a.N * (a.qh / a.kvh));
-  const int groups = a.S * a.kvh * a.chunks;
-  const dim3 grid((groups + 7) / 8 * 8 * a.row_blocks), block(64 * t.rt * t.ks);
+  const int64_t groups = (int64_t)a.S * a.kvh * a.chunks;
+  const dim3 grid(8 * a.row_blocks, (uint32_t)((groups + 7) / 8)), block(64 * t.rt * t.ks);
   if constexpr (D == 64) {
-    if (t.rt == 1) hipLaunchKernelGGL((tree_split_kernel<QT, 64, 1, 8, 2>), grid, block, 0, s, a);
-    else if (t.rt == 2) hipLaunchKernelGGL((tree_split_kernel<QT, 64, 2, 4, 3>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((tree_split_kernel<QT, 64, 4, 2, 4>), grid, block, 0, s, a);
+    if (t.rt == 1) hipLaunchKernelGGL((tree_split_kernel<QT, 64, 1, 8, 2, 2>), grid, block, 0, s, a);
+    else if (t.rt == 2) hipLaunchKernelGGL((tree_split_kernel<QT, 64, 2, 4, 3, 2>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((tree_split_kernel<QT, 64, 4, 2, 4, 4>), grid, block, 0, s, a);
   } else if constexpr (D == 128) {
-    if (t.rt == 1) hipLaunchKernelGGL((tree_split_kernel<QT, 128, 1, 4, 2>), grid, block, 0, s, a);
-    else if (t.rt == 2) hipLaunchKernelGGL((tree_split_kernel<QT, 128, 2, 4, 2>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((tree_split_kernel<QT, 128, 4, 2, 4>), grid, block, 0, s, a);
+    if (t.rt == 1) hipLaunchKernelGGL((tree_split_kernel<QT, 128, 1, 4, 2, 1>), grid, block, 0, s, a);
+    else if (t.rt == 2) hipLaunchKernelGGL((tree_split_kernel<QT, 128, 2, 4, 2, 2>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((tree_split_kernel<QT, 128, 4, 2, 4, 2>), grid, block, 0, s, a);
   } else {
-    if (t.rt == 1) hipLaunchKernelGGL((tree_split_kernel<QT, 256, 1, 2, 2>), grid, block, 0, s, a);
-    else if (t.rt == 2) hipLaunchKernelGGL((tree_split_kernel<QT, 256, 2, 2, 2>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((tree_split_kernel<QT, 256, 4, 1, 4>), grid, block, 0, s, a);
+    if (t.rt == 1) hipLaunchKernelGGL((tree_split_kernel<QT, 256, 1, 2, 2, 1>), grid, block, 0, s, a);
+    else if (t.rt == 2) hipLaunchKernelGGL((tree_split_kernel<QT, 256, 2, 2, 2, 1>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((tree_split_kernel<QT, 256, 4, 1, 4, 1>), grid, block, 0, s, a);
   }
   if (a.chunks > 1) {
     const int64_t rows = (int64_t)a.S * a.N * a.qh;
