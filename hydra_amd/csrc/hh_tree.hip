@@ -20,6 +20,7 @@
 namespace hh {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
@@ -53,10 +54,9 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kOff = 10.f;       // p = 2^(y − M + kOff)
 constexpr float kNone = -1e30f;    // a maximum of nothing: finite, so that no difference of maxima is NaN
 
-// The ancestors-or-self of every node as bit masks, lane i node i (i < N); a parent that is not an
-// earlier node counts as none.
-__device__ __forceinline__ uint64_t ancestors(const int32_t *parents, int N, int lane) {
-  int up = lane < N ? parents[lane] : -1;
+// The ancestors-or-self of every node as bit masks, lane i node i with parent `up`; a parent that is not
+// an earlier node counts as none.
+__device__ __forceinline__ uint64_t ancestors(int up, int lane) {
   if (up < 0 || up >= lane) up = -1;
   uint64_t mask = 1ull << lane;
   for (int r = 0; r < 6; ++r) {   // lines of up to 64 nodes, by doubling
@@ -133,9 +133,33 @@ __global__ __launch_bounds__(64 * RT * KS, OCC) void tree_split_kernel(TreeArgs 
   const int rt = wave % RT, ks = wave / RT, l32 = lane & 31, hh = lane >> 5;
   // Row blocks of one (sequence, kv head, chunk) on one XCD, one after the other: they read the same keys.
   const uint32_t grp = blockIdx.y * 8 + (blockIdx.x & 7), own = a.S * a.kvh;
-  const int rb = blockIdx.x >> 3, chunk = (int)(grp / own);
-  if (chunk >= a.chunks) return;
-  const int sg = (int)(grp - chunk * own), s = sg / a.kvh, g = sg - s * a.kvh, qm = a.qm;
+  const int rb = blockIdx.x >> 3;
+  // The last chunks first: theirs are the drafted nodes.
+  const uint32_t at_chunk = grp / own;
+  const int chunk = a.chunks - 1 - (int)at_chunk;
+  if (chunk < 0) return;
+  const int sg = (int)(grp - at_chunk * own), s = sg / a.kvh, g = sg - s * a.kvh, qm = a.qm;
+
+  // The lane's row: its node and queries, asked for before anything else (a wait for them behind the tiles' loads
+  // would be one for those too).
+  const int r = rb * ROWS + rt * 32 + l32, rn = (int)(((float)r + 0.5f) * a.inv_qm);   // r / qm: exact below 2^20
+  const bool in = rn < a.N;
+  const int node = in ? rn : 0, head = g * qm + (in ? r - rn * qm : 0);
+  const int up = lane < a.N ? a.parents[(int64_t)s * a.N + lane] : -1;
+  u32x4 qf[D / 16], ql[PAIR ? D / 16 : 1];
+  {
+    const int64_t at = ((int64_t)s * a.N + node) * a.q_stride + (int64_t)head * D + 8 * hh;
+#pragma unroll
+    for (int dc = 0; dc < D / 16; ++dc) {
+      if constexpr (PAIR) {
+        const u32x4 *qp = (const u32x4 *)((const float *)a.q + at + 16 * dc);
+        qf[dc] = qp[0];
+        ql[dc] = qp[1];
+      } else {
+        qf[dc] = *(const u32x4 *)((const uint16_t *)a.q + at + 16 * dc);
+      }
+    }
+  }
   const int count = min(max(a.counts[s], 0), a.N);
   if (rb * ROWS >= count * qm) return;
   const Span sp = span_of(a, s);
@@ -144,46 +168,30 @@ __global__ __launch_bounds__(64 * RT * KS, OCC) void tree_split_kernel(TreeArgs 
   const int c0 = (int)c064, nc = min(sp.per, sp.keys - c0);   // cached keys of the chunk
   const bool last = c064 + sp.per >= sp.keys;
   const int tiles = (nc + (last ? count : 0) + KT - 1) / KT;
-
-  // Loads: 16-byte pieces of a row in consecutive lanes, XORed by the row (sw) so that both ways of reading
-  // are free of bank conflicts.
-  const uint32_t r0 = a.ring ? (uint32_t)(sp.first + c0) % (uint32_t)a.rows : sp.first + c0;
-  const uint64_t kb = (uint64_t)(a.k + (int64_t)s * a.seq_stride + (int64_t)g * D);
-  const uint64_t vb = (uint64_t)(a.v + (int64_t)s * a.seq_stride + (int64_t)g * D);
-  const int64_t dbase = (int64_t)s * a.N * a.kv_stride + (int64_t)g * D;
-  const uint64_t dkb = (uint64_t)((const uint16_t *)a.dk + dbase), dvb = (uint64_t)((const uint16_t *)a.dv + dbase);
-  const uint32_t lds0 = lds_addr(s_mem), rstride = 2 * a.kvh * D, dstride = 2 * (uint32_t)a.kv_stride;
-  auto sw = [](int row) { return ((row & 3) << 1) | ((row >> 2) & 1); };
-  auto load_tile = [&](int t, int slot) {
+  const float scale = PAIR ? 1.f : fabsf(a.scale) * kLog2e;   // S -> y
 #pragma unroll
-    for (int v = 0; v < 2; ++v) {                      // keys, values
-      const uint64_t cached = v ? vb : kb, drafted = v ? dvb : dkb;
-#pragma unroll 4
-      for (int u = 0; u < NL / 2; ++u) {
-        const int p0 = (u * NW + wave) * 64, p = p0 + lane, row = p / CH, c = (p % CH) ^ sw(row);
-        const int idx = t * KT + row, m = idx - nc;
-        uint32_t r = r0 + idx;
-        r = r >= (uint32_t)a.rows ? r - a.rows : r;    // a ring's end
-        // Behind the cached keys the nodes; rows past the last node are masked: they read node 0's.
-        const uint32_t at = m < 0 ? r : m < count ? m : 0, stride = m < 0 ? rstride : dstride;
-        const uint64_t base = (m < 0 ? cached : drafted) + 16 * c;
-        dma16((const void *)(base + (uint64_t)at * stride),
-              __builtin_amdgcn_readfirstlane(lds0 + slot * STAGE + v * (KT * D * 2) + p0 * 16));
+  for (int dc = 0; dc < D / 16; ++dc) {
+    if constexpr (PAIR) {
+      f16x8 h, l;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float v = __uint_as_float(e < 4 ? qf[dc][e & 3] : ql[dc][e & 3]) * (a.scale * kLog2e);
+        // Rounded to fp32 before it is split: hi must not come from the product by one mixed-precision
+        // instruction, whose single rounding differs near ties from that of the hi that lo is the rest of.
+        asm volatile("" : "+v"(v));
+        h[e] = (_Float16)v;
+        l[e] = (_Float16)(v - (float)h[e]);
       }
+      qf[dc] = __builtin_bit_cast(u32x4, h);
+      ql[dc] = __builtin_bit_cast(u32x4, l);
+    } else {
+      if (a.scale < 0.f) qf[dc] ^= 0x80008000u;
     }
-  };
-#pragma unroll
-  for (int t = 0; t < NST - 1; ++t)
-    if (t < tiles) load_tile(t, t);
-
-  // The lane's row: its node, what that sees, its queries.
-  const int r = rb * ROWS + rt * 32 + l32, rn = (int)(((float)r + 0.5f) * a.inv_qm);   // r / qm: exact below 2^20
-  const bool real = rn < count;
-  const int node = real ? rn : 0, head = g * qm + (real ? r - rn * qm : 0);
+  }
   uint64_t vis = 0;
   int lo = 0, lo_max = 0;   // the first cached key of the chunk that the node sees, and that every node sees
   if (last || a.window) {
-    const uint64_t mask = ancestors(a.parents + (int64_t)s * a.N, a.N, lane);
+    const uint64_t mask = ancestors(up, lane);
     vis = shfl64(mask, node);
     if (a.window) {
       auto low = [&](int depth) { return (int)max((int64_t)0, (int64_t)sp.length + depth - a.window + 1 - sp.first) - c0; };
@@ -194,33 +202,59 @@ __global__ __launch_bounds__(64 * RT * KS, OCC) void tree_split_kernel(TreeArgs 
       while (__popcll(vis) > a.window) vis &= vis - 1;   // the oldest ancestors
     }
   }
-  const float scale = PAIR ? 1.f : fabsf(a.scale) * kLog2e;   // S -> y
-  u32x4 qf[D / 16], ql[PAIR ? D / 16 : 1];
-  {
-    const int64_t at = ((int64_t)s * a.N + node) * a.q_stride + (int64_t)head * D + 8 * hh;
+
+  // Loads: 16-byte pieces of a row in consecutive lanes, XORed by the row (sw) so that both ways of reading
+  // are free of bank conflicts. Tiles of cached keys that do not pass a ring's end step one address per lane.
+  const uint32_t r0 = a.ring ? (uint32_t)(sp.first + c0) % (uint32_t)a.rows : sp.first + c0;
+  const uint64_t kb = (uint64_t)(a.k + (int64_t)s * a.seq_stride + (int64_t)g * D);
+  const uint64_t vb = (uint64_t)(a.v + (int64_t)s * a.seq_stride + (int64_t)g * D);
+  const int64_t dbase = (int64_t)s * a.N * a.kv_stride + (int64_t)g * D;
+  const uint64_t dkb = (uint64_t)((const uint16_t *)a.dk + dbase), dvb = (uint64_t)((const uint16_t *)a.dv + dbase);
+  const uint32_t lds0 = lds_addr(s_mem), rstride = 2 * a.kvh * D, dstride = 2 * (uint32_t)a.kv_stride;
+  auto sw = [](int row) { return ((row & 3) << 1) | ((row >> 2) & 1); };
+  constexpr int RPL = NW * 64 / CH;                    // rows that one load of every wave covers
+  constexpr int NPT = RPL % 8 ? 2 : 1;                 // addresses per lane: rows 4 apart differ in their XOR
+  uint64_t step[NPT];
 #pragma unroll
-    for (int dc = 0; dc < D / 16; ++dc) {
-      if constexpr (PAIR) {
-        const f32x4 *qp = (const f32x4 *)((const float *)a.q + at + 16 * dc);
-        const f32x4 q0 = qp[0], q1 = qp[1];
-        f16x8 h, l;
+  for (int i = 0; i < NPT; ++i) {
+    const int p = (i * NW + wave) * 64 + lane, row = p / CH;
+    step[i] = (uint64_t)(r0 + row) * rstride + 16 * ((p % CH) ^ sw(row));
+  }
+  const int plain = min(nc / KT, (int)(((uint32_t)a.rows - r0) / KT));   // tiles 0 .. plain − 1 step so
+  auto load_tile = [&](int t, int slot) {
+    const uint32_t l0 = lds0 + slot * STAGE + wave * 1024;
+    if (t < plain) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float v = (e < 4 ? q0[e & 3] : q1[e & 3]) * (a.scale * kLog2e);
-          // Rounded to fp32 before it is split: hi must not come from the product by one mixed-precision
-          // instruction, whose single rounding differs near ties from that of the hi that lo is the rest of.
-          asm volatile("" : "+v"(v));
-          h[e] = (_Float16)v;
-          l[e] = (_Float16)(v - (float)h[e]);
-        }
-        qf[dc] = __builtin_bit_cast(u32x4, h);
-        ql[dc] = __builtin_bit_cast(u32x4, l);
-      } else {
-        qf[dc] = *(const u32x4 *)((const uint16_t *)a.q + at + 16 * dc);
-        if (a.scale < 0.f) qf[dc] ^= 0x80008000u;
+      for (int v = 0; v < 2; ++v)                      // keys, values
+#pragma unroll
+        for (int u = 0; u < NL / 2; ++u)
+          dma16((const void *)(step[u % NPT] + ((v ? vb : kb) + (uint64_t)(u / NPT * NPT * RPL) * rstride)),
+                __builtin_amdgcn_readfirstlane(l0 + v * (KT * D * 2) + u * NW * 1024));
+#pragma unroll
+      for (int i = 0; i < NPT; ++i) step[i] += (uint64_t)KT * rstride;
+      return;
+    }
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      const uint64_t cached = v ? vb : kb, drafted = v ? dvb : dkb;
+#pragma unroll 4
+      for (int u = 0; u < NL / 2; ++u) {
+        const int p = (u * NW + wave) * 64 + lane, row = p / CH, c = (p % CH) ^ sw(row);
+        const int idx = t * KT + row, m = idx - nc;
+        uint32_t rw = r0 + idx;
+        rw = rw >= (uint32_t)a.rows ? rw - a.rows : rw;    // a ring's end
+        // Behind the cached keys the nodes; rows past the last node are masked: they read node 0's.
+        const uint32_t at = m < 0 ? rw : m < count ? m : 0, stride = m < 0 ? rstride : dstride;
+        const uint64_t base = (m < 0 ? cached : drafted) + 16 * c;
+        dma16((const void *)(base + (uint64_t)at * stride),
+              __builtin_amdgcn_readfirstlane(l0 + v * (KT * D * 2) + u * NW * 1024));
       }
     }
-  }
+  };
+#pragma unroll
+  for (int t = 0; t < NST - 1; ++t)
+    if (t < tiles) load_tile(t, t);
+
   if (ks == 0 && hh == 0) {
     s_vis[rt * 32 + l32] = vis;
     s_lo[rt * 32 + l32] = lo;
@@ -309,14 +343,23 @@ __global__ __launch_bounds__(64 * RT * KS, OCC) void tree_split_kernel(TreeArgs 
         for (int e = 0; e < 8; ++e) h[e] = (__bf16)p[8 * kc + e];
         ph[kc] = __builtin_bit_cast(u32x4, h);
       } else {
-        f16x8 h, l;
+        if constexpr (PAIR) {   // hi cut off, lo the rest
+          f16x8 l;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          h[e] = (_Float16)p[8 * kc + e];
-          if constexpr (PAIR) l[e] = (_Float16)(p[8 * kc + e] - (float)h[e]);
+          for (int e = 0; e < 4; ++e) {
+            const float p0 = p[8 * kc + 2 * e], p1 = p[8 * kc + 2 * e + 1];
+            const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(p0, p1));
+            ph[kc][e] = __builtin_bit_cast(uint32_t, h);
+            l[2 * e] = (_Float16)fmaf((float)h[0], -1.f, p0);
+            l[2 * e + 1] = (_Float16)fmaf((float)h[1], -1.f, p1);
+          }
+          pl[kc] = __builtin_bit_cast(u32x4, l);
+        } else {
+          f16x8 h;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) h[e] = (_Float16)p[8 * kc + e];
+          ph[kc] = __builtin_bit_cast(u32x4, h);
         }
-        ph[kc] = __builtin_bit_cast(u32x4, h);
-        if constexpr (PAIR) pl[kc] = __builtin_bit_cast(u32x4, l);
       }
     }
     // V^T: lane (l32, hh) takes dimension 32 n + l32 of keys 16 kc + 8 x + 4 hh .. + 3, the order of P^T.
