@@ -9,7 +9,7 @@ namespace hh {
 enum Elem { E_F32 = 0, E_F16 = 1, E_BF16 = 2 };
 constexpr int kTreeNodes = 64;    // most nodes of a tree: an ancestor set is one 64-bit mask
 constexpr int kTreeQM = 16;       // most query heads per kv head
-constexpr int kTreeGroups = 512;  // workgroups that a call's keys are split for
+constexpr int kTreeGroups = 256;  // workgroups that a call's keys are split for
 constexpr int kTreeChunks = 256;  // most chunks of a sequence
 
 struct TreeArgs {

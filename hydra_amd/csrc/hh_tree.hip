@@ -29,7 +29,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void dma16(const void *p, uint32_t l) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(l), "v"(p) : "memory", "m0");
 }
-template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N < 63 ? N : 63) : "memory"); }
 // Barrier after the wave's own LDS reads have returned: the next tile may overwrite what they read.
 __device__ __forceinline__ void step_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 typedef __attribute__((address_space(3))) void *lds_ptr_t;
@@ -72,6 +72,19 @@ __device__ __forceinline__ uint64_t ancestors(int up, int lane) {
 }
 __device__ __forceinline__ uint64_t shfl64(uint64_t v, int at) {
   return ((uint64_t)__shfl((uint32_t)(v >> 32), at) << 32) | __shfl((uint32_t)v, at);
+}
+
+// Two probabilities as fp16 pairs: hi cut off, lo the rest of it, rounded. minus1 is −1 in a register: with
+// the constant the compiler makes a conversion and a subtraction of the one mixed-precision instruction.
+__device__ __forceinline__ u32x2 split_pair(float p0, float p1, float minus1) {
+  const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(p0, p1));
+  const f16x2 l = {(_Float16)fmaf((float)h[0], minus1, p0), (_Float16)fmaf((float)h[1], minus1, p1)};
+  return u32x2{__builtin_bit_cast(uint32_t, h), __builtin_bit_cast(uint32_t, l)};
+}
+// Waits for the first of the tiles that were asked for ahead of the loop.
+template <int NL, int NST> __device__ __forceinline__ void wait_first(int tiles) {
+  if (tiles >= NST - 1) wait_vm<(NST - 2) * NL>();
+  else wait_vm<0>();
 }
 
 // A sequence's visible history: positions first .. first + keys − 1 (those that its roots see), in chunks of
@@ -213,7 +226,7 @@ __global__ __launch_bounds__(64 * RT * KS, OCC) void tree_split_kernel(TreeArgs 
   const uint32_t lds0 = lds_addr(s_mem), rstride = 2 * a.kvh * D, dstride = 2 * (uint32_t)a.kv_stride;
   auto sw = [](int row) { return ((row & 3) << 1) | ((row >> 2) & 1); };
   constexpr int RPL = NW * 64 / CH;                    // rows that one load of every wave covers
-  constexpr int NPT = RPL % 8 ? 2 : 1;                 // addresses per lane: rows 4 apart differ in their XOR
+  constexpr int NPT = RPL < 8 ? 8 / RPL : 1;           // addresses per lane: rows not 8 apart differ in their XOR
   uint64_t step[NPT];
 #pragma unroll
   for (int i = 0; i < NPT; ++i) {
@@ -260,64 +273,72 @@ __global__ __launch_bounds__(64 * RT * KS, OCC) void tree_split_kernel(TreeArgs 
     s_lo[rt * 32 + l32] = lo;
   }
   if (tid == 0) s_odd = 0;
+  // A tile that some row does not see whole: infinities and NaN among its values are taken out (0 · NaN would
+  // carry them to rows that do not see them) and put back into the rows that do behind the loop.
   auto is_part = [&](int t) { return t * KT < lo_max || (t + 1) * KT > nc; };
-  float M = kNone, L = 0.f;
+  auto clean = [&](int t) {
+    uint8_t *vt = s_mem + (t % NST) * STAGE + KT * D * 2;
+#pragma unroll
+    for (int u = 0; u < D / (16 * RT); ++u) {
+      u32x4 *w = (u32x4 *)vt + u * NT + tid;
+      u32x4 x = *w;
+      bool odd = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t em = BF ? 0x7F80u : 0x7C00u;
+        const bool l = (x[e] & em) == em, h = (x[e] >> 16 & em) == em;
+        x[e] &= (l ? 0u : 0xFFFFu) | (h ? 0u : 0xFFFF0000u);
+        odd |= l || h;
+      }
+      if (odd) {
+        *w = x;
+        s_odd = 1;
+      }
+    }
+    step_barrier();
+  };
+  float M = kNone, L = 0.f, minus1 = -1.f;
+  asm volatile("" : "+s"(minus1));
   f32x16 acc[NB];
 #pragma unroll
   for (int n = 0; n < NB; ++n) acc[n] = f32x16{};
   const int j16 = lane & 15;
   const int vrow = 4 * hh + (j16 >> 2), vpiece = (2 * ((lane >> 4) & 1) + ((j16 & 3) >> 1)) ^ sw(vrow), vhalf = (j16 & 1) * 8;
-
-  for (int t = 0; t < tiles; ++t) {
-    if (t + NST - 2 < tiles) wait_vm<(NST - 2) * NL>();
-    else wait_vm<0>();
-    step_barrier();
-    if (t + NST - 1 < tiles) load_tile(t + NST - 1, (t + NST - 1) % NST);
-    uint8_t *kt = s_mem + (t % NST) * STAGE, *vt = kt + KT * D * 2;
-    // A tile that some row does not see whole: infinities and NaN among its values are taken out (0 · NaN would
-    // carry them to rows that do not see them) and put back into the rows that do behind the loop.
-    const bool part = is_part(t);
-    if (part) {
-#pragma unroll
-      for (int u = 0; u < D / (16 * RT); ++u) {
-        u32x4 *w = (u32x4 *)vt + u * NT + tid;
-        u32x4 x = *w;
-        bool odd = false;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t em = BF ? 0x7F80u : 0x7C00u;
-          const bool l = (x[e] & em) == em, h = (x[e] >> 16 & em) == em;
-          x[e] &= (l ? 0u : 0xFFFFu) | (h ? 0u : 0xFFFF0000u);
-          odd |= l || h;
-        }
-        if (odd) {
-          *w = x;
-          s_odd = 1;
-        }
-      }
-      step_barrier();
-    }
-    const int base = t * KT + 32 * ks;   // the wave's first key
+  // S^T of the wave's 32 keys of tile t.
+  auto scores = [&](int t) {
+    const uint8_t *krow = s_mem + (t % NST) * STAGE + (32 * ks + l32) * (2 * D);
     f32x16 S = f32x16{};
-    const uint8_t *krow = kt + (32 * ks + l32) * (2 * D);
 #pragma unroll
     for (int dc = 0; dc < D / 16; ++dc) {
       const u32x4 kf = *(const u32x4 *)(krow + (((2 * dc + hh) ^ sw(l32)) << 4));
       S = mfma32<BF>(kf, qf[dc], S);
       if constexpr (PAIR) S = mfma32<BF>(kf, ql[dc], S);
     }
-    // Key of element i: base + 8 (i / 4) + 4 hh + i % 4.
-    if (part)
+    return S;
+  };
+  // Keys that the row does not see, and the row's maximum. Element i is key 8 (i / 4) + 4 hh + i % 4 of the 32.
+  auto masked_top = [&](f32x16 &S, int t, bool part) {
+    if (part) {
+      const int base = t * KT + 32 * ks;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int k = base + 8 * (i >> 2) + 4 * hh + (i & 3), m = k - nc;
         const bool sees = m < 0 ? k >= lo : (m < 64 && (vis >> (m & 63) & 1));
         S[i] = sees ? S[i] : -INFINITY;
       }
+    }
     float top = fmaxf(S[0], S[1]);
 #pragma unroll
     for (int i = 2; i < 16; ++i) top = fmaxf(top, S[i]);
-    top = max_halves(top) * scale;
+    return max_halves(top) * scale;
+  };
+  wait_first<NL, NST>(tiles);
+  step_barrier();
+  bool part = is_part(0);
+  if (part) clean(0);
+  f32x16 S = scores(0);
+  float top = masked_top(S, 0, part);
+  for (int t = 0; t < tiles; ++t) {
     if (__any(top > M)) {
       const float mn = fmaxf(M, top), corr = exp2_(M - mn);
       M = mn;
@@ -325,47 +346,43 @@ __global__ __launch_bounds__(64 * RT * KS, OCC) void tree_split_kernel(TreeArgs 
 #pragma unroll
       for (int n = 0; n < NB; ++n) acc[n] *= corr;
     }
+    // The next tile's scores are formed with this one's probabilities and values: the matrix unit works under the
+    // exponentials. Its keys must be there; the slot that the tile before this one left is loaded again.
+    const bool more = t + 1 < tiles;
+    part = false;
+    if (more) {
+      if (t + NST - 2 < tiles) wait_vm<(NST - 3) * NL>();
+      else wait_vm<0>();
+      step_barrier();
+      if (t + NST - 1 < tiles) load_tile(t + NST - 1, (t + NST - 1) % NST);
+      part = is_part(t + 1);
+      if (part) clean(t + 1);
+    }
+    // Behind the last tile its own scores once more: not used.
+    f32x16 Sn = scores(more ? t + 1 : t);
     const float sub = kOff - M;
-    float p[16];
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      p[i] = exp2_(fmaf(S[i], scale, sub));
-      sum[i & 3] += p[i];
+      S[i] = exp2_(fmaf(S[i], scale, sub));
+      sum[i & 3] += S[i];
     }
     L += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    u32x4 ph[2], pl[PAIR ? 2 : 1];
+    // V^T: lane (l32, hh) takes dimension 32 n + l32 of keys 16 kc + 8 x + 4 hh .. + 3, the order of P^T.
+    const uint8_t *vcol = s_mem + (t % NST) * STAGE + KT * D * 2 + (32 * ks + vrow) * (2 * D) + vhalf;
 #pragma unroll
     for (int kc = 0; kc < 2; ++kc) {
-      if constexpr (BF) {
-        bf16x8 h;
+      u32x4 ph, pl;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] = (__bf16)p[8 * kc + e];
-        ph[kc] = __builtin_bit_cast(u32x4, h);
-      } else {
-        if constexpr (PAIR) {   // hi cut off, lo the rest
-          f16x8 l;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float p0 = p[8 * kc + 2 * e], p1 = p[8 * kc + 2 * e + 1];
-            const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(p0, p1));
-            ph[kc][e] = __builtin_bit_cast(uint32_t, h);
-            l[2 * e] = (_Float16)fmaf((float)h[0], -1.f, p0);
-            l[2 * e + 1] = (_Float16)fmaf((float)h[1], -1.f, p1);
-          }
-          pl[kc] = __builtin_bit_cast(u32x4, l);
-        } else {
-          f16x8 h;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) h[e] = (_Float16)p[8 * kc + e];
-          ph[kc] = __builtin_bit_cast(u32x4, h);
-        }
+      for (int e = 0; e < 4; ++e) {
+        const float p0 = S[8 * kc + 2 * e], p1 = S[8 * kc + 2 * e + 1];
+        if constexpr (PAIR) {
+          const u32x2 w = split_pair(p0, p1, minus1);
+          ph[e] = w[0];
+          pl[e] = w[1];
+        } else if constexpr (BF) ph[e] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)p0, (__bf16)p1});
+        else ph[e] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)p0, (_Float16)p1});
       }
-    }
-    // V^T: lane (l32, hh) takes dimension 32 n + l32 of keys 16 kc + 8 x + 4 hh .. + 3, the order of P^T.
-    const uint8_t *vcol = vt + (32 * ks + vrow) * (2 * D) + vhalf;
-#pragma unroll
-    for (int kc = 0; kc < 2; ++kc)
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
         u32x4 vf;
@@ -373,13 +390,16 @@ __global__ __launch_bounds__(64 * RT * KS, OCC) void tree_split_kernel(TreeArgs 
         for (int x8 = 0; x8 < 2; ++x8) {
           const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
               (__attribute__((address_space(3))) s16x4 *)(vcol + (16 * kc + 8 * x8) * 2 * D + ((vpiece ^ (4 * n)) << 4)));
-          const u32x2 b = __builtin_bit_cast(u32x2, w);
-          vf[2 * x8] = b[0];
-          vf[2 * x8 + 1] = b[1];
+          const u32x2 v = __builtin_bit_cast(u32x2, w);
+          vf[2 * x8] = v[0];
+          vf[2 * x8 + 1] = v[1];
         }
-        acc[n] = mfma32<BF>(vf, ph[kc], acc[n]);
-        if constexpr (PAIR) acc[n] = mfma32<BF>(vf, pl[kc], acc[n]);
+        acc[n] = mfma32<BF>(vf, ph, acc[n]);
+        if constexpr (PAIR) acc[n] = mfma32<BF>(vf, pl, acc[n]);
       }
+    }
+    S = Sn;
+    top = masked_top(S, t + 1, part);
   }
 
   // The splits' states meet in LDS, the sums of a row in 16-byte pieces XORed by the row.
@@ -514,12 +534,11 @@ __global__ __launch_bounds__(64) void weights_kernel(TreeArgs a) {
 
 // The launch: RT by the rows of a kv head, KS and the ring so that a workgroup's tiles in flight cover the
 // memory's latency and fit LDS.
-struct TreeShape { int rt, ks, nst; };
+struct TreeShape { int rt, ks; };
 static TreeShape tree_shape(int d, int rows) {
   const int rt = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
-  if (d == 64) return {rt, 8 / rt, rt == 4 ? 4 : rt == 2 ? 3 : 2};
-  if (d == 128) return {rt, rt == 1 ? 4 : 8 / rt, rt == 4 ? 4 : 2};
-  return {rt, rt == 4 ? 1 : 2, rt == 4 ? 4 : 2};
+  if (d == 64) return {rt, rt == 4 ? 2 : 4};
+  return {rt, d == 128 ? 2 : 1};
 }
 
 // Fills in how the call's keys are split, for histories of up to `length` keys.
@@ -552,19 +571,10 @@ template <int QT, int D> static hipError_t launch_tree_d(const TreeArgs &a, hipS
   const TreeShape t = tree_shape(D, a.N * (a.qh / a.kvh));
   const int64_t groups = (int64_t)a.S * a.kvh * a.chunks;
   const dim3 grid(8 * a.row_blocks, (uint32_t)((groups + 7) / 8)), block(64 * t.rt * t.ks);
-  if constexpr (D == 64) {
-    if (t.rt == 1) hipLaunchKernelGGL((tree_split_kernel<QT, 64, 1, 8, 2, 2>), grid, block, 0, s, a);
-    else if (t.rt == 2) hipLaunchKernelGGL((tree_split_kernel<QT, 64, 2, 4, 3, 2>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((tree_split_kernel<QT, 64, 4, 2, 4, 4>), grid, block, 0, s, a);
-  } else if constexpr (D == 128) {
-    if (t.rt == 1) hipLaunchKernelGGL((tree_split_kernel<QT, 128, 1, 4, 2, 1>), grid, block, 0, s, a);
-    else if (t.rt == 2) hipLaunchKernelGGL((tree_split_kernel<QT, 128, 2, 4, 2, 2>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((tree_split_kernel<QT, 128, 4, 2, 4, 2>), grid, block, 0, s, a);
-  } else {
-    if (t.rt == 1) hipLaunchKernelGGL((tree_split_kernel<QT, 256, 1, 2, 2, 1>), grid, block, 0, s, a);
-    else if (t.rt == 2) hipLaunchKernelGGL((tree_split_kernel<QT, 256, 2, 2, 2, 1>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((tree_split_kernel<QT, 256, 4, 1, 4, 1>), grid, block, 0, s, a);
-  }
+  constexpr int K4 = D == 64 ? 2 : D == 128 ? 2 : 1, K2 = D == 64 ? 4 : K4, NST = 4;
+  if (t.rt == 1) hipLaunchKernelGGL((tree_split_kernel<QT, D, 1, K2, NST, 1>), grid, block, 0, s, a);
+  else if (t.rt == 2) hipLaunchKernelGGL((tree_split_kernel<QT, D, 2, K2, NST, D == 64 ? 2 : 1>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((tree_split_kernel<QT, D, 4, K4, D == 64 ? 6 : NST, D == 256 ? 1 : 2>), grid, block, 0, s, a);
   if (a.chunks > 1) {
     const int64_t rows = (int64_t)a.S * a.N * a.qh;
     hipLaunchKernelGGL((tree_merge_kernel<QT, D>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, s, a);
