@@ -10,6 +10,7 @@ enum Elem { E_F32 = 0, E_F16 = 1, E_BF16 = 2 };
 constexpr int kTreeNodes = 64;    // most nodes of a tree: an ancestor set is one 64-bit mask
 constexpr int kTreeQM = 16;       // most query heads per kv head
 constexpr int kTreeGroups = 256;  // workgroups that a call's keys are split for
+constexpr int kTreeTiles = 4;     // tiles of keys that one workgroup takes without a split
 constexpr int kTreeChunks = 256;  // most chunks of a sequence
 
 struct TreeArgs {

@@ -10,7 +10,7 @@
 //   O^T [D × 32 rows] += V^T · P^T, the value tile read by columns (transposing LDS reads), P^T from S^T's own
 //   registers: a lane holds one row's probabilities at 16 keys, and the products' order over the keys is the
 //   lane's. So a row's maximum and sum stay in its two lanes, and rescaling needs no exchange.
-// p = 2^(y − M + 10): small probabilities stay above fp16's smallest step. F32 activations: queries and
+// F32 activations: queries and
 // probabilities as fp16 pairs hi + lo, two products each (exact in fp32 to ~2^-22).
 // A chunk's state (M, L, O) goes to the workspace and tree_merge_kernel joins a row's chunks in order; a call of
 // one chunk writes its outputs at once. The sink enters where the states are joined.
@@ -51,7 +51,10 @@ __device__ __forceinline__ float max_halves(float v) {
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kOff = 10.f;       // p = 2^(y − M + kOff)
+// M follows a row's maximum by steps of at least kLag: rescaling costs more than what it keeps small, and with
+// M moved at every new maximum some row of 32 moved it at nearly every tile. p = 2^(y − M + kOff) < 2^12 fits
+// fp16, and the largest p of a row is 2^4 or more.
+constexpr float kOff = 4.f, kLag = 8.f;
 constexpr float kNone = -1e30f;    // a maximum of nothing: finite, so that no difference of maxima is NaN
 
 // The ancestors-or-self of every node as bit masks, lane i node i with parent `up`; a parent that is not
@@ -264,9 +267,10 @@ __global__ __launch_bounds__(64 * RT * KS, OCC) void tree_split_kernel(TreeArgs 
       }
     }
   };
-#pragma unroll
-  for (int t = 0; t < NST - 1; ++t)
-    if (t < tiles) load_tile(t, t);
+  // Not unrolled, as little here is: the first workgroup of a compute unit waits for its instructions (about 0.1 us
+  // a 64-byte line).
+#pragma unroll 1
+  for (int t = 0; t < min(NST - 1, tiles); ++t) load_tile(t, t);
 
   if (ks == 0 && hh == 0) {
     s_vis[rt * 32 + l32] = vis;
@@ -319,13 +323,13 @@ __global__ __launch_bounds__(64 * RT * KS, OCC) void tree_split_kernel(TreeArgs 
   // Keys that the row does not see, and the row's maximum. Element i is key 8 (i / 4) + 4 hh + i % 4 of the 32.
   auto masked_top = [&](f32x16 &S, int t, bool part) {
     if (part) {
-      const int base = t * KT + 32 * ks;
+      // Bit j: the row sees key base + j. Cached keys from lo to nc, then the nodes.
+      const int base = t * KT + 32 * ks, from = min(max(lo - base, 0), 32), to = min(max(nc - base, 0), 32), m = base - nc;
+      uint32_t sees = (uint32_t)(((1ull << to) - 1) & ~((1ull << from) - 1));
+      sees |= m >= 0 ? (m < 64 ? (uint32_t)(vis >> m) : 0u) : m > -32 ? (uint32_t)(vis << -m) : 0u;
+      sees >>= 4 * hh;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int k = base + 8 * (i >> 2) + 4 * hh + (i & 3), m = k - nc;
-        const bool sees = m < 0 ? k >= lo : (m < 64 && (vis >> (m & 63) & 1));
-        S[i] = sees ? S[i] : -INFINITY;
-      }
+      for (int i = 0; i < 16; ++i) S[i] = sees >> (8 * (i >> 2) + (i & 3)) & 1 ? S[i] : -INFINITY;
     }
     float top = fmaxf(S[0], S[1]);
 #pragma unroll
@@ -338,8 +342,8 @@ __global__ __launch_bounds__(64 * RT * KS, OCC) void tree_split_kernel(TreeArgs 
   if (part) clean(0);
   f32x16 S = scores(0);
   float top = masked_top(S, 0, part);
-  for (int t = 0; t < tiles; ++t) {
-    if (__any(top > M)) {
+  auto step_tile = [&](f32x16 &S, f32x16 &Sn, int t) {
+    if (__any(top > M + kLag)) {
       const float mn = fmaxf(M, top), corr = exp2_(M - mn);
       M = mn;
       L *= corr;
@@ -359,7 +363,7 @@ __global__ __launch_bounds__(64 * RT * KS, OCC) void tree_split_kernel(TreeArgs 
       if (part) clean(t + 1);
     }
     // Behind the last tile its own scores once more: not used.
-    f32x16 Sn = scores(more ? t + 1 : t);
+    Sn = scores(more ? t + 1 : t);
     const float sub = kOff - M;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -398,8 +402,15 @@ __global__ __launch_bounds__(64 * RT * KS, OCC) void tree_split_kernel(TreeArgs 
         if constexpr (PAIR) acc[n] = mfma32<BF>(vf, pl, acc[n]);
       }
     }
-    S = Sn;
-    top = masked_top(S, t + 1, part);
+    top = masked_top(Sn, t + 1, part);
+  };
+  // Two tiles a round: the scores of one and of the next in registers of their own, with no copies between.
+  f32x16 Sn;
+  for (int t = 0;;) {
+    step_tile(S, Sn, t);
+    if (++t >= tiles) break;
+    step_tile(Sn, S, t);
+    if (++t >= tiles) break;
   }
 
   // The splits' states meet in LDS, the sums of a row in 16-byte pieces XORed by the row.
@@ -418,6 +429,7 @@ __global__ __launch_bounds__(64 * RT * KS, OCC) void tree_split_kernel(TreeArgs 
       *(f32x4 *)(so + 4 * ((8 * n + 2 * e + hh) ^ (l32 & 7))) = w;
     }
   __syncthreads();
+#pragma unroll 1
   for (int e = tid; e < ROWS * (D / 4); e += NT) {
     const int row = e / (D / 4), q4 = e % (D / 4), rr = rb * ROWS + row, n = (int)(((float)rr + 0.5f) * a.inv_qm);
     if (n >= count) break;               // rows are in the order of their nodes
@@ -437,14 +449,16 @@ __global__ __launch_bounds__(64 * RT * KS, OCC) void tree_split_kernel(TreeArgs 
     if (s_odd) {
       // The infinities and NaN of the tiles that were seen in part, from memory.
       const uint64_t sees = s_vis[row];
+#pragma unroll 1
       for (int t = 0; t < tiles; ++t) {
         if (!is_part(t)) continue;
-        for (int k = t * KT; k < t * KT + KT && k < nc + count; ++k) {
-          const int m = k - nc;
-          if (m < 0 ? k < s_lo[row] : !(sees >> m & 1)) continue;
+#pragma unroll 1
+        for (int k = t * KT; k < min(t * KT + KT, nc + count); ++k) {
+          const int m2 = k - nc;
+          if (m2 < 0 ? k < s_lo[row] : !(sees >> m2 & 1)) continue;
           uint32_t at = r0 + k;
           at = at >= (uint32_t)a.rows ? at - a.rows : at;
-          const uint64_t src = (m < 0 ? vb + (uint64_t)at * rstride : dvb + (uint64_t)m * dstride) + 8 * q4;
+          const uint64_t src = (m2 < 0 ? vb + (uint64_t)at * rstride : dvb + (uint64_t)m2 * dstride) + 8 * q4;
           const u32x2 w = *(const u32x2 *)src;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -553,7 +567,8 @@ void tree_plan(TreeArgs &a, int64_t length) {
   if (a.window && keys > a.window) keys = a.window;
   const int64_t own = (int64_t)a.S * a.kvh * a.row_blocks;
   int64_t chunks = kTreeGroups / own, most = (keys + a.tile - 1) / a.tile;
-  if (chunks > most) chunks = most;
+  // A few tiles one after the other take less than a second launch that joins them (4 to 6 us).
+  if (chunks > most || most <= kTreeTiles) chunks = most <= kTreeTiles ? 1 : most;
   if (chunks > kTreeChunks) chunks = kTreeChunks;
   if (chunks < 1) chunks = 1;
   int64_t per = ((keys + chunks - 1) / chunks + a.tile - 1) / a.tile * a.tile;
