@@ -163,6 +163,7 @@ int check_verify(const hh_verify_desc *d) {
   if (d->type < HH_F32 || d->type > HH_BF16) return fail(HH_EINVAL, "unknown type");
   if (d->draft < HH_DRAFT_GIVEN || d->draft > HH_DRAFT_DISTINCT) return fail(HH_EINVAL, "unknown draft mode");
   if (d->max_children < 0 || d->max_children >= HH_TREE_MAX_NODES) return fail(HH_EINVAL, "max_children outside 0..63");
+  if (!hh::verify_fits(d->sequences, d->nodes, d->vocab)) return fail(HH_EINVAL, "more than 2^23 chunks of logits: split the batch");
   if (!(d->temperature >= 0.f) || !std::isfinite(d->temperature)) return fail(HH_EINVAL, "temperature must be finite and >= 0");
   if (d->temperature != 0.f && d->temperature < 1e-6f)
     return fail(HH_EINVAL, "temperature below 1e-6: 0 is greedy");
@@ -172,13 +173,8 @@ int check_verify(const hh_verify_desc *d) {
 }
 
 int verify_children(const hh_verify_desc *d) {
-  const int most = d->nodes > 1 ? d->nodes - 1 : 1;
+  const int most = d->nodes - 1;
   return d->max_children && d->max_children < most ? d->max_children : most;
-}
-
-size_t verify_bytes(const hh_verify_desc *d) {
-  const bool greedy = d->temperature == 0.f;
-  return hh::verify_workspace(d->sequences, d->nodes, d->vocab, greedy ? HH_DRAFT_GIVEN : d->draft, verify_children(d), greedy);
 }
 
 }  // namespace
@@ -246,7 +242,7 @@ int hh_draft_verify(hh_ctx *ctx, const hh_verify_desc *d, const void *target, co
   if (!greedy && (!uniforms || !final_uniforms)) return fail(HH_EINVAL, "sampling needs uniforms and final_uniforms");
   if (mode != HH_DRAFT_GIVEN && !draft) return fail(HH_EINVAL, "draws from a distribution need the draft's logits");
   HH_HIP(hipSetDevice(ctx->device));
-  if (int rc = ensure_draft(ctx, verify_bytes(d))) return rc;
+  if (int rc = ensure_draft(ctx, hh::verify_workspace(d->sequences, d->nodes, d->vocab))) return rc;
   hh::VerifyArgs a{};
   a.target = target;
   a.draft = draft;
@@ -268,8 +264,10 @@ int hh_draft_verify(hh_ctx *ctx, const hh_verify_desc *d, const void *target, co
   a.children = verify_children(d);
   a.inv_t = greedy ? 0.0 : 1.0 / (double)d->temperature;
   a.ws = ctx->draft;
-  HH_HIP(hh::launch_verify(a, ctx->stream));
-  ctx->dispatches += 2;
+  a.k64 = 64 * 1.4426950408889634074 * a.inv_t;
+  int launches = 0;
+  HH_HIP(hh::launch_verify(a, ctx->stream, &launches));
+  ctx->dispatches += launches;
   return HH_OK;
 }
 
@@ -366,7 +364,7 @@ int hh_draft_reserve(hh_ctx *ctx, const hh_tree_desc *tree, const hh_kv_cache *c
   }
   if (verify) {
     if (int rc = check_verify(verify)) return rc;
-    const size_t b = verify_bytes(verify);
+    const size_t b = hh::verify_workspace(verify->sequences, verify->nodes, verify->vocab);
     if (b > need) need = b;
   }
   HH_HIP(hipSetDevice(ctx->device));

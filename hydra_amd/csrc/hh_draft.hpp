@@ -65,16 +65,17 @@ struct VerifyArgs {
   const float *u, *u_final;
   int32_t *path, *accepted, *next;
   int S, N, V, type, mode, children;
-  double inv_t;                     // 1 / temperature; 0: greedy
+  double inv_t, k64;                // 1 / temperature (0: greedy), 64 log2(e) / temperature
   uint8_t *ws;
 };
 
-size_t verify_workspace(int S, int N, int V, int mode, int children, bool greedy);
+size_t verify_workspace(int S, int N, int V);
+bool verify_fits(int S, int N, int V);   // launches' block counts
 void tree_plan(TreeArgs &a, int64_t length);
 size_t tree_workspace(const TreeArgs &a);
 hipError_t launch_tree(const TreeArgs &a, int type, hipStream_t s);
 hipError_t launch_weights(const TreeArgs &a, int type, hipStream_t s);
-hipError_t launch_verify(const VerifyArgs &a, hipStream_t s);
+hipError_t launch_verify(const VerifyArgs &a, hipStream_t s, int *launches);
 hipError_t launch_commit(const RowsArgs &a, bool last, hipStream_t s);
 hipError_t launch_evict(const RowsArgs &a, hipStream_t s);
 

@@ -7,255 +7,556 @@
 // tokens are not put back (q_j = q / R_j, R_j the mass of q off them), and c = 0 for given tokens. A
 // child with token x is accepted if r_j(x) > u W_j q_j(x). That needs no normalised copy of a row, and does
 // not depend on what happens at other nodes: every node's tests are made at once, and the walk follows.
+//
+// A row of logits is cut into chunks, a workgroup each, so that one sequence's rows fill the chip:
+//   stats    every row's maximum and sum of exponentials by chunk (greedy: its largest entry);
+//   round j  of the nodes with at least j children: the j-th child's test, then W_j and R_j by chunk (given
+//            tokens: all tests and the last residual in one round);
+//   walk     a workgroup per sequence follows the accepted children and finds the next token: its chunk by the
+//            chunks' sums, its place by a scan of that chunk.
+// Bound by the launches' dependent chain for a few rows, and by the exponentials in 64 bits for many: the next token
+// is where a sum of up to V terms passes a random bound, and with errors of 1e-7 in it one in twenty draws from
+// the tail of 250000 tokens would differ. exp goes by a table of 2^(i / 64) and five terms of a series (relative error
+// below 1e-15 beside the argument's): 13 instructions in fp64.
+#include <climits>
+
 #include "hh_common.hpp"
 #include "hh_draft.hpp"
 
 namespace hh {
 
-template <class T> __device__ __forceinline__ float logit(const void *row, int v) {
-  const float x = (float)((const T *)row)[v];
-  return x != x ? -INFINITY : x;
+constexpr int kVT = 256;              // threads of stats and rounds
+constexpr int kWalkT = 1024;
+
+__device__ __forceinline__ float finite_or_less(float x) { return x != x ? -INFINITY : x; }
+
+// exp((x − top) / temperature) with tab[i] = 2^(i / 64) in LDS, k64 = 64 log2(e) / temperature.
+__device__ __forceinline__ double exp_of(float x, double top, double k64, const double *tab) {
+  const double y = fmax(((double)x - top) * k64, -64.0 * 1100), n = rint(y), f = y - n;
+  constexpr double c = 0.010830424696249145;   // ln 2 / 64
+  double s = fma(f, c * c * c * c * c / 120, c * c * c * c / 24);
+  s = fma(f, s, c * c * c / 6);
+  s = fma(f, s, c * c / 2);
+  s = fma(f, s, c);
+  s = fma(f, s, 1.0);
+  const int i = (int)n;
+  return ldexp(s * tab[i & 63], i >> 6);
+}
+// The same for a row whose largest entry is infinite: its +inf entries share the probability, a row of −inf has none.
+__device__ __forceinline__ double exp_any(float x, float top, double k64, const double *tab) {
+  if (fabsf(top) == INFINITY) return top > 0.f && x == top ? 1.0 : 0.0;
+  return exp_of(x, top, k64, tab);
+}
+// exp_any as a call: where each of a kernel's few uses is run once, its instructions are fetched once (a cold
+// 64-byte line of instructions costs about 0.1 us).
+__device__ __noinline__ double exp_call(float x, float top, double k64, const double *tab) {
+  return exp_any(x, top, k64, tab);
+}
+__device__ __forceinline__ void fill_table(double *tab) {
+  if (threadIdx.x < 64) tab[threadIdx.x] = exp2((double)threadIdx.x / 64);
 }
 
-// exp((x − top) / temperature): entries equal to the largest are 1 also where that is infinite.
-__device__ __forceinline__ double scaled_exp(float x, float top, double inv_t) {
-  if (x == -INFINITY) return 0.0;
-  return x == top ? 1.0 : exp(((double)x - (double)top) * inv_t);
-}
-
-constexpr int kVT = 1024;
-
-template <class F> __device__ __forceinline__ double block_sum(double v, double *s_d) {
+// Sum and maximum over a workgroup, in a fixed order, in every thread. s_d: T / 64 doubles of its own per call site.
+template <int T> __device__ __forceinline__ double block_sum(double v, double *s_d) {
   for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  __syncthreads();
   if ((threadIdx.x & 63) == 0) s_d[threadIdx.x >> 6] = v;
   __syncthreads();
-  double t = 0.0;
-  for (int w = 0; w < kVT / 64; ++w) t += s_d[w];
+  double t = s_d[0];
+  for (int w = 1; w < T / 64; ++w) t += s_d[w];
   return t;
 }
-__device__ __forceinline__ float block_max(float v, double *s_d) {
+template <int T> __device__ __forceinline__ float block_max(float v, float *s_f) {
   for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  if ((threadIdx.x & 63) == 0) s_f[threadIdx.x >> 6] = v;
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) s_d[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float t = -INFINITY;
-  for (int w = 0; w < kVT / 64; ++w) t = fmaxf(t, (float)s_d[w]);
+  float t = s_f[0];
+  for (int w = 1; w < T / 64; ++w) t = fmaxf(t, s_f[w]);
   return t;
 }
 
+// Logits v0 + 4 (256 i + thread) + e of a row, −inf past its end and for NaN.
+template <class T, int EPT> __device__ __forceinline__ void load_chunk(const T *row, int v0, int V, float (&x)[EPT]) {
+  typedef T vec4 __attribute__((ext_vector_type(4)));
+  const bool aligned = ((uintptr_t)row & (4 * sizeof(T) - 1)) == 0;
+#pragma unroll
+  for (int i = 0; i < EPT / 4; ++i) {
+    const int v = v0 + 4 * (kVT * i + (int)threadIdx.x);
+    if (aligned && v + 4 <= V) {
+      const vec4 w = *(const vec4 *)(row + v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * i + e] = finite_or_less((float)w[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * i + e] = v + e < V ? finite_or_less((float)row[v + e]) : -INFINITY;
+    }
+  }
+}
+
+// What rounds leave of a node: reciprocals of its rows' sums, their maxima, and c of the round.
 struct NodeState {
-  double zp, zq, c, w, rest;
+  double ip, iq, c;
   float mp, mq;
-  int tried;
 };
 
-__device__ __forceinline__ bool is_tried(const int *s_tok, int n, int v) {
-  for (int i = 0; i < n; ++i)
-    if (s_tok[i] == v) return true;
-  return false;
+// The workspace. Chunk arrays are [row][chunks], row = s·N + n; part, state: of odd and even rounds.
+struct VerifyPlan {
+  int chunk, chunks;
+  size_t max_of[2], sum_of[2], part[2], rest[2], state[2], accept, best, total;
+};
+__host__ __device__ inline VerifyPlan verify_plan(int S, int N, int V) {
+  VerifyPlan p{};
+  const size_t rows = (size_t)S * N;
+  // 4096 logits a workgroup where that makes 512 of them, else 1024 (16 or 4 a thread): one row of 32000, six nodes 28 us
+  // with 1024, 37 with 4096.
+  p.chunk = rows * V >= (size_t)512 * 4096 ? 4096 : 1024;
+  p.chunks = (V + p.chunk - 1) / p.chunk;
+  size_t c = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = c;
+    c += (bytes + 255) / 256 * 256;
+    return o;
+  };
+  const size_t n = rows * p.chunks;
+  for (int i = 0; i < 2; ++i) {
+    p.max_of[i] = take(4 * n);
+    p.sum_of[i] = take(8 * n);
+    p.part[i] = take(8 * n);
+    p.rest[i] = take(8 * n);
+    p.state[i] = take(sizeof(NodeState) * rows);
+  }
+  p.accept = take(4 * rows);
+  p.best = take(4 * n);
+  p.total = c;
+  return p;
 }
 
-// Children of a node in order, at most `most`: their indices into s_child; returns how many.
-__device__ __forceinline__ int children_of(const VerifyArgs &a, int s, int n, int count, int most, int *s_child) {
-  int k = 0;
-  for (int m = n + 1; m < count && k < most; ++m)
-    if (a.parents[(int64_t)s * a.N + m] == n) s_child[k++] = m;
-  return k;
+// The children of node n as a mask, the first `most`; every lane of the wave takes part.
+__device__ __forceinline__ uint64_t children_of(const VerifyArgs &a, int s, int n, int count, int most) {
+  const int lane = threadIdx.x & 63;
+  uint64_t m = __ballot(lane > n && lane < count && a.parents[(int64_t)s * a.N + min(lane, a.N - 1)] == n);
+  if (__popcll(m) > most) {
+    uint64_t left = m;
+    for (int i = 0; i < most; ++i) left &= left - 1;
+    m &= ~left;
+  }
+  return m;
 }
 
-template <class T>
-__global__ __launch_bounds__(kVT) void node_kernel(VerifyArgs a) {
-  __shared__ double s_d[kVT / 64];
-  __shared__ int s_child[kTreeNodes], s_tok[kTreeNodes], s_k;
-  const int n = blockIdx.x % a.N, s = blockIdx.x / a.N, tid = threadIdx.x;
+template <class T, int EPT, bool GREEDY>
+__global__ __launch_bounds__(kVT) void stats_kernel(VerifyArgs a, VerifyPlan w) {
+  __shared__ double s_tab[64], s_d[kVT / 64];
+  __shared__ float s_f[kVT / 64];
+  __shared__ int s_i[kVT / 64];
+  const int chunk = blockIdx.x % w.chunks, row = blockIdx.x / w.chunks, s = row / a.N, n = row - s * a.N, tid = threadIdx.x;
+  const int count = min(max(a.counts[s], 0), a.N), of = blockIdx.y;
+  if (n >= count) return;
+  if (of && children_of(a, s, n, count, a.children) == 0) return;   // the draft's row of a node that has no children
+  if (!GREEDY) fill_table(s_tab);
+  const T *base = (const T *)(of ? a.draft : a.target) + (int64_t)row * (of ? a.d_stride : a.t_stride);
+  float x[EPT];
+  load_chunk<T, EPT>(base, chunk * w.chunk, a.V, x);
+  float top = x[0];
+#pragma unroll
+  for (int i = 1; i < EPT; ++i) top = fmaxf(top, x[i]);
+  const float all = block_max<kVT>(top, s_f);
+  const size_t at = (size_t)row * w.chunks + chunk;
+  if (GREEDY) {
+    int best = a.V;
+#pragma unroll
+    for (int i = EPT - 1; i >= 0; --i)
+      if (x[i] == all) best = chunk * w.chunk + 4 * (kVT * (i / 4) + tid) + i % 4;
+    for (int o = 32; o; o >>= 1) best = min(best, __shfl_xor(best, o));
+    if ((tid & 63) == 0) s_i[tid >> 6] = best;
+    __syncthreads();
+    if (tid == 0) {
+      for (int k = 1; k < kVT / 64; ++k) best = min(best, s_i[k]);
+      ((float *)(a.ws + w.max_of[0]))[at] = all;
+      ((int32_t *)(a.ws + w.best))[at] = best;
+    }
+    return;
+  }
+  double sum = 0.0;
+  if (fabsf(all) == INFINITY) {
+    const bool one = all > 0.f;
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) sum += one && x[i] == all ? 1.0 : 0.0;
+  } else {
+    const double top64 = all;
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) sum += exp_of(x[i], top64, a.k64, s_tab);   // −inf: 0
+  }
+  sum = block_sum<kVT>(sum, s_d);
+  if (tid == 0) {
+    ((float *)(a.ws + w.max_of[of]))[at] = all;
+    ((double *)(a.ws + w.sum_of[of]))[at] = sum;
+    if (!of && chunk == 0) ((int32_t *)(a.ws + w.accept))[row] = 0;
+  }
+}
+
+// A row's maximum and sum from its chunks'.
+template <int T>
+__device__ __forceinline__ double joined(const float *mx, const double *sm, int chunks, double k64, const double *tab, float *s_f,
+                                         double *s_d, float &top) {
+  float m = -INFINITY;
+  for (int c = threadIdx.x; c < chunks; c += T) m = fmaxf(m, mx[c]);
+  top = block_max<T>(m, s_f);
+  double z = 0.0;
+#pragma unroll 1
+  for (int c = threadIdx.x; c < chunks; c += T) z += sm[c] * exp_call(mx[c], top, k64, tab);
+  return block_sum<T>(z, s_d);
+}
+
+template <class T, int EPT, int MODE>
+__global__ __launch_bounds__(kVT) void round_kernel(VerifyArgs a, VerifyPlan w, int round) {
+  __shared__ double s_tab[64], s_d[6][kVT / 64];
+  __shared__ float s_f[2][kVT / 64];
+  __shared__ int s_tok[kTreeNodes];
+  constexpr bool DRAWN = MODE != 0;
+  const int chunk = blockIdx.x % w.chunks, row = blockIdx.x / w.chunks, s = row / a.N, n = row - s * a.N, tid = threadIdx.x;
+  const int lane = tid & 63;
   const int count = min(max(a.counts[s], 0), a.N);
   if (n >= count) return;
-  NodeState *st = (NodeState *)a.ws + blockIdx.x;
-  int *accept = (int *)((NodeState *)a.ws + a.S * a.N) + s * a.N;
-  if (tid == 0) s_k = children_of(a, s, n, count, a.children, s_child);
+  const uint64_t kids = children_of(a, s, n, count, a.children);
+  const int k = __popcll(kids);
+  if (k < round) return;
+  const int tried = DRAWN ? round : k;       // given tokens: what is left when all are rejected
+  const T *tr = (const T *)a.target + (int64_t)row * a.t_stride;
+  const T *dr = (const T *)a.draft + (int64_t)row * a.d_stride;
+  const int v0 = chunk * w.chunk;
+  float x[EPT], y[DRAWN ? EPT : 1];
+  load_chunk<T, EPT>(tr, v0, a.V, x);
+  if constexpr (DRAWN) load_chunk<T, EPT>(dr, v0, a.V, y);
+  fill_table(s_tab);
+  if (tid < 64 && (kids >> lane & 1)) {      // the tokens in the order of their trial
+    const int at = __popcll(kids & ((1ull << lane) - 1));
+    s_tok[at] = a.tokens[(int64_t)s * a.N + lane];
+  }
   __syncthreads();
-  const int k = s_k;
-  const T *tr = (const T *)a.target + ((int64_t)s * a.N + n) * a.t_stride;
-  const T *dr = (const T *)a.draft + ((int64_t)s * a.N + n) * a.d_stride;
-  const bool q_on = a.mode != 0 && k > 0;
-  float mp = -INFINITY, mq = -INFINITY;
-  for (int v = tid; v < a.V; v += kVT) {
-    mp = fmaxf(mp, logit<T>(tr, v));
-    if (q_on) mq = fmaxf(mq, logit<T>(dr, v));
+  const size_t at = (size_t)row * w.chunks;
+  NodeState st{};
+  double mass = 1.0, rest = 1.0;
+  if (round == 1) {
+    float m;
+    const double zp = joined<kVT>((const float *)(a.ws + w.max_of[0]) + at, (const double *)(a.ws + w.sum_of[0]) + at, w.chunks,
+                                  a.k64, s_tab, s_f[0], s_d[0], m);
+    st.mp = m;
+    st.ip = zp > 0 ? 1.0 / zp : 0.0;
+    if constexpr (DRAWN) {
+      const double zq = joined<kVT>((const float *)(a.ws + w.max_of[1]) + at, (const double *)(a.ws + w.sum_of[1]) + at, w.chunks,
+                                    a.k64, s_tab, s_f[1], s_d[1], m);
+      st.mq = m;
+      st.iq = zq > 0 ? 1.0 / zq : 0.0;
+    }
+  } else {
+    st = ((const NodeState *)(a.ws + w.state[(round - 1) & 1]))[row];
+    const double *pw = (const double *)(a.ws + w.part[(round - 1) & 1]) + at, *pr = (const double *)(a.ws + w.rest[(round - 1) & 1]) + at;
+    double sw = 0.0, sr = 0.0;
+    for (int c = tid; c < w.chunks; c += kVT) {
+      sw += pw[c];
+      if constexpr (MODE == 2) sr += pr[c];
+    }
+    mass = block_sum<kVT>(sw, s_d[2]);
+    if constexpr (MODE == 2) rest = block_sum<kVT>(sr, s_d[3]);
   }
-  mp = block_max(mp, s_d);
-  mq = block_max(mq, s_d);
-  if (a.inv_t == 0.0) {   // greedy: the lowest of the largest
-    int best = a.V;
-    for (int v = tid; v < a.V; v += kVT)
-      if (logit<T>(tr, v) == mp) { best = v; break; }
-    for (int o = 32; o; o >>= 1) best = min(best, __shfl_xor(best, o));
-    __shared__ int s_best[kVT / 64];
-    if ((tid & 63) == 0) s_best[tid >> 6] = best;
-    __syncthreads();
-    if (tid == 0) {
-      for (int w = 0; w < kVT / 64; ++w) best = min(best, s_best[w]);
-      if (mp == -INFINITY) best = -1;
-      st->tried = best;
-      for (int j = 0; j < k; ++j) {
-        const int x = a.tokens[(int64_t)s * a.N + s_child[j]];
-        accept[s_child[j]] = x >= 0 && x == best;
+  const double left = MODE == 2 ? fmax(rest, 0x1p-52) : 1.0;
+  if (chunk == 0 && tid < 64) {
+    int32_t *accept = (int32_t *)(a.ws + w.accept) + (int64_t)s * a.N;
+    if constexpr (DRAWN) {
+      uint64_t m = kids;
+      for (int i = 1; i < round; ++i) m &= m - 1;
+      const int child = __ffsll((unsigned long long)m) - 1, t = s_tok[round - 1];
+      bool again = false;
+      for (int i = 0; i < round - 1; ++i) again |= s_tok[i] == t;
+      if (lane == 0 && t >= 0 && t < a.V && !again) {
+        const double p = exp_call(finite_or_less((float)tr[t]), st.mp, a.k64, s_tab) * st.ip;
+        const double q = exp_call(finite_or_less((float)dr[t]), st.mq, a.k64, s_tab) * st.iq;
+        accept[child] = fmax(p - st.c * q, 0.0) > (double)a.u[(int64_t)s * a.N + child] * mass * (q / left);
+      }
+    } else if (kids >> lane & 1) {
+      // Every child at once, in its own lane: the mass left at its turn is what the distinct tokens before it have not.
+      const int mine = __popcll(kids & ((1ull << lane) - 1)), t = s_tok[mine];
+      double before = 0.0;
+      bool again = false;
+      for (int i = 0; i < mine; ++i) {
+        const int o = s_tok[i];
+        again |= o == t;
+        bool first = o >= 0 && o < a.V;
+        for (int e = 0; e < i; ++e) first &= s_tok[e] != o;
+        if (first) before += exp_call(finite_or_less((float)tr[o]), st.mp, a.k64, s_tab) * st.ip;
+      }
+      if (t >= 0 && t < a.V && !again)
+        accept[lane] = exp_call(finite_or_less((float)tr[t]), st.mp, a.k64, s_tab) * st.ip >
+                       (double)a.u[(int64_t)s * a.N + lane] * fmax(1.0 - before, 0.0);
+    }
+  }
+  st.c = DRAWN ? st.c + mass / left : 0.0;
+  if (chunk == 0 && tid == 0) ((NodeState *)(a.ws + w.state[round & 1]))[row] = st;
+  // The residual off the tokens tried, of which few chunks hold one.
+  bool here = false;
+  for (int i = 0; i < tried; ++i) here |= s_tok[i] >= v0 && s_tok[i] < v0 + w.chunk;
+  if (here) {
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {
+      const int v = v0 + 4 * (kVT * (i / 4) + tid) + i % 4;
+      for (int e = 0; e < tried; ++e)
+        if (s_tok[e] == v) {
+          x[i] = -INFINITY;
+          if constexpr (DRAWN) y[i] = -INFINITY;
+        }
+    }
+  }
+  double sw = 0.0, sr = 0.0;
+  if (fabsf(st.mp) == INFINITY || (DRAWN && fabsf(st.mq) == INFINITY)) {
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {
+      const double p = exp_call(x[i], st.mp, a.k64, s_tab) * st.ip;
+      double q = 0.0;
+      if constexpr (DRAWN) q = exp_call(y[i], st.mq, a.k64, s_tab) * st.iq;
+      sw += fmax(p - st.c * q, 0.0);
+      sr += q;
+    }
+  } else {
+    const double mp = st.mp, mq = st.mq, cq = st.c * st.iq;
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {
+      const double p = exp_of(x[i], mp, a.k64, s_tab);
+      if constexpr (DRAWN) {
+        const double q = exp_of(y[i], mq, a.k64, s_tab);
+        sw += fmax(p * st.ip - cq * q, 0.0);
+        if constexpr (MODE == 2) sr += q * st.iq;
+      } else {
+        sw += p * st.ip;
       }
     }
-    return;
   }
-  double zp = 0.0, zq = 0.0;
-  for (int v = tid; v < a.V; v += kVT) {
-    zp += scaled_exp(logit<T>(tr, v), mp, a.inv_t);
-    if (q_on) zq += scaled_exp(logit<T>(dr, v), mq, a.inv_t);
+  sw = block_sum<kVT>(sw, s_d[4]);
+  if constexpr (MODE == 2) sr = block_sum<kVT>(sr, s_d[5]);
+  if (tid == 0) {
+    ((double *)(a.ws + w.part[round & 1]))[at + chunk] = sw;
+    if constexpr (MODE == 2) ((double *)(a.ws + w.rest[round & 1]))[at + chunk] = sr;
   }
-  zp = block_sum<T>(zp, s_d);
-  zq = block_sum<T>(zq, s_d);
-  const double ip = zp > 0 ? 1.0 / zp : 0.0, iq = zq > 0 ? 1.0 / zq : 0.0;
-  double c = 0.0, w = 1.0, rest = 1.0;
-  int tried = 0;
-  for (int j = 0; j < k; ++j) {
-    const int m = s_child[j], x = a.tokens[(int64_t)s * a.N + m];
-    const bool in = x >= 0 && x < a.V, again = in && is_tried(s_tok, tried, x);
-    if (tid == 0) {
-      int yes = 0;
-      if (in && !again) {
-        const double p = scaled_exp(logit<T>(tr, x), mp, a.inv_t) * ip;
-        const double q0 = q_on ? scaled_exp(logit<T>(dr, x), mq, a.inv_t) * iq : 1.0;
-        const double q = a.mode == 2 ? q0 / fmax(rest, 0x1p-52) : q0;
-        const double r = q_on ? fmax(p - c * q0, 0.0) : p;
-        yes = r > (double)a.u[(int64_t)s * a.N + m] * w * q;
-      }
-      accept[m] = yes;
-    }
-    __syncthreads();
-    if (in && !again) {
-      if (tid == 0) s_tok[tried] = x;
-      ++tried;
-    }
-    __syncthreads();
-    if (q_on) c += a.mode == 2 ? w / fmax(rest, 0x1p-52) : w;
-    double ws = 0.0, rs = 0.0;
-    for (int v = tid; v < a.V; v += kVT) {
-      if (is_tried(s_tok, tried, v)) continue;
-      const double p = scaled_exp(logit<T>(tr, v), mp, a.inv_t) * ip;
-      if (!q_on) { ws += p; continue; }
-      const double q = scaled_exp(logit<T>(dr, v), mq, a.inv_t) * iq;
-      ws += fmax(p - c * q, 0.0);
-      rs += q;
-    }
-    w = block_sum<T>(ws, s_d);
-    rest = block_sum<T>(rs, s_d);
-  }
-  if (tid == 0) *st = NodeState{zp, zq, c, w, rest, mp, mq, tried};
 }
 
 template <class T>
-__global__ __launch_bounds__(kVT) void walk_kernel(VerifyArgs a) {
-  __shared__ int s_cur, s_k, s_child[kTreeNodes], s_tok[kTreeNodes], s_hit, s_last;
-  __shared__ double s_sum[kVT];
-  const int s = blockIdx.x, tid = threadIdx.x;
+__global__ __launch_bounds__(kWalkT) void walk_kernel(VerifyArgs a, VerifyPlan w) {
+  __shared__ double s_tab[64], s_d[kWalkT / 64], s_scan[kWalkT / 64], s_goal;
+  __shared__ float s_f[kWalkT / 64];
+  __shared__ int s_best[kTreeNodes], s_tok[kTreeNodes], s_cur, s_hit[2];
+  const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int count = min(max(a.counts[s], 0), a.N);
-  const int *accept = (const int *)((NodeState *)a.ws + a.S * a.N) + s * a.N;
-  if (tid == 0) {
-    int cur = 0, len = count > 0 ? 1 : 0;
-    if (len) a.path[(int64_t)s * a.N] = 0;
-    // Children come behind their parent, in the order of their trial.
-    for (int m = 1; m < count; ++m) {
-      const int up = a.parents[(int64_t)s * a.N + m];
-      if (up != cur) continue;
-      int before = 0;   // children past the most that are tried carry no flag
-      for (int i = up + 1; i < m; ++i) before += a.parents[(int64_t)s * a.N + i] == up;
-      if (before < a.children && accept[m]) {
-        cur = m;
-        a.path[(int64_t)s * a.N + len++] = m;
+  const bool greedy = a.inv_t == 0.0;
+  if (greedy) {
+    for (int n = wave; n < count; n += kWalkT / 64) {   // the rows' largest entries, the lowest of equals
+      const size_t at = ((size_t)s * a.N + n) * w.chunks;
+      const float *mx = (const float *)(a.ws + w.max_of[0]) + at;
+      const int32_t *bx = (const int32_t *)(a.ws + w.best) + at;
+      float m = -INFINITY;
+      int b = a.V;
+      for (int c = lane; c < w.chunks; c += 64)
+        if (mx[c] > m) m = mx[c], b = bx[c];
+      for (int o = 32; o; o >>= 1) {
+        const float om = __shfl_xor(m, o);
+        const int ob = __shfl_xor(b, o);
+        if (om > m || (om == m && ob < b)) m = om, b = ob;
       }
+      if (lane == 0) s_best[n] = m > -INFINITY ? b : -1;
     }
-    for (int i = len; i < a.N; ++i) a.path[(int64_t)s * a.N + i] = -1;
-    a.accepted[s] = len;
-    s_cur = cur;
-    s_hit = a.V;
-    s_last = -1;
-    s_k = children_of(a, s, cur, count, a.children, s_child);
+    __syncthreads();
+  } else {
+    fill_table(s_tab);
+  }
+  if (wave == 0) {
+    const int64_t at = (int64_t)s * a.N;
+    const bool real = lane < count;
+    const int up = real ? a.parents[at + lane] : -1, token = real ? a.tokens[at + lane] : -1;
+    bool yes = real && up >= 0 && up < lane;
+    if (greedy) {
+      yes = yes && token >= 0 && token == s_best[yes ? up : 0];
+      // Children past the most that are tried.
+      int before = 0;
+      for (int i = 0; i < 64; ++i) before += i < lane && __shfl(up, i) == up;
+      yes = yes && before < a.children;
+    } else if (yes) {
+      yes = ((const int32_t *)(a.ws + w.accept))[at + lane] != 0;
+    }
+    int cur = 0, len = count > 0 ? 1 : 0, place = lane == 0 && len ? 0 : -1;
+    if (count > 0)
+      for (;;) {   // a child comes behind its parent: at most N steps
+        const uint64_t m = __ballot(yes && up == cur);
+        if (!m) break;
+        cur = __ffsll((unsigned long long)m) - 1;
+        if (lane == len) place = cur;
+        ++len;
+      }
+    if (lane < a.N) a.path[at + lane] = place;
+    if (lane == 0) {
+      a.accepted[s] = len;
+      s_cur = cur;
+    }
   }
   __syncthreads();
-  const int n = s_cur;
-  if (count == 0) {
-    if (tid == 0) a.next[s] = -1;
+  const int n = s_cur, row = s * a.N + n;
+  if (count == 0 || greedy) {
+    if (tid == 0) a.next[s] = count == 0 ? -1 : s_best[n];
     return;
   }
-  const NodeState st = ((NodeState *)a.ws)[s * a.N + n];
-  if (a.inv_t == 0.0) {
-    if (tid == 0) a.next[s] = st.tried;
-    return;
-  }
-  if (!(st.zp > 0)) {
-    if (tid == 0) a.next[s] = -1;
-    return;
-  }
-  // A residual without mass: the target's own probabilities.
-  const bool left = s_k == 0 || st.w > 0;
-  const bool q_on = a.mode != 0 && s_k > 0 && left;
-  if (tid < s_k) s_tok[tid] = a.tokens[(int64_t)s * a.N + s_child[tid]];
-  __syncthreads();
-  const int tried = left ? s_k : 0;
-  const T *tr = (const T *)a.target + ((int64_t)s * a.N + n) * a.t_stride;
-  const T *dr = (const T *)a.draft + ((int64_t)s * a.N + n) * a.d_stride;
-  const double ip = 1.0 / st.zp, iq = st.zq > 0 ? 1.0 / st.zq : 0.0;
-  auto r = [&](int v) -> double {
-    if (is_tried(s_tok, tried, v)) return 0.0;
-    const double p = scaled_exp(logit<T>(tr, v), st.mp, a.inv_t) * ip;
-    return q_on ? fmax(p - st.c * (scaled_exp(logit<T>(dr, v), st.mq, a.inv_t) * iq), 0.0) : p;
+  const size_t at = (size_t)row * w.chunks;
+  const uint64_t kids = children_of(a, s, n, count, a.children);
+  const int k = __popcll(kids);
+  if (tid < 64 && (kids >> lane & 1)) s_tok[__popcll(kids & ((1ull << lane) - 1))] = a.tokens[(int64_t)s * a.N + lane];
+  const float *mx = (const float *)(a.ws + w.max_of[0]) + at;
+  const double *sm = (const double *)(a.ws + w.sum_of[0]) + at;
+  const int parity = a.mode ? k & 1 : 1;
+  const double *pw = (const double *)(a.ws + w.part[parity]) + at;
+  // Runs of chunks per thread; the running sum over them, first of the residual.
+  const int per = (w.chunks + kWalkT - 1) / kWalkT, c0 = min(tid * per, w.chunks), c1 = min(c0 + per, w.chunks);
+  auto scan = [&](double v, double &whole) {   // exclusive prefix over the threads
+    double p = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double q = __shfl_up(p, o);
+      if (lane >= o) p += q;
+    }
+    __syncthreads();
+    if (lane == 63) s_scan[wave] = p;
+    __syncthreads();
+    double before = 0.0;
+    whole = 0.0;
+    for (int i = 0; i < kWalkT / 64; ++i) {
+      if (i < wave) before += s_scan[i];
+      whole += s_scan[i];
+    }
+    const double e = __shfl_up(p, 1);
+    return before + (lane ? e : 0.0);
   };
-  const int per = (a.V + kVT - 1) / kVT, v0 = min(tid * per, a.V), v1 = min(v0 + per, a.V);
-  double own = 0.0;
-  for (int v = v0; v < v1; ++v) own += r(v);
-  s_sum[tid] = own;
-  __syncthreads();
-  if (tid == 0) {
-    double run = 0.0;
-    for (int i = 0; i < kVT; ++i) {
-      const double t = run + s_sum[i];
-      s_sum[i] = run;
-      run = t;
-    }
-    const double goal = (double)fmaxf(a.u_final[s], 0.f) * run;
-    int at = -1, last = -1;
-    for (int i = 0; i < kVT; ++i) {
-      const double end = i + 1 < kVT ? s_sum[i + 1] : run;
-      if (end > s_sum[i]) {
-        last = i;
-        if (at < 0 && end > goal) at = i;
-      }
-    }
-    if (at < 0) at = last;
-    double sum = s_sum[at < 0 ? 0 : at];
-    int token = -1;
-    for (int v = at * per; at >= 0 && v < min(at * per + per, a.V); ++v) {
-      const double x = r(v);
-      if (x <= 0.0) continue;
-      token = v;
-      sum += x;
-      if (sum > goal) break;
-    }
-    a.next[s] = token;
+  NodeState st{};
+  double own = 0.0, whole = 0.0, run = 0.0;
+  if (k) {
+    st = ((const NodeState *)(a.ws + w.state[parity]))[row];
+    for (int c = c0; c < c1; ++c) own += pw[c];
+    run = scan(own, whole);
   }
+  // A leaf, or a residual without mass: the target's own probabilities.
+  const bool resid = whole > 0;
+  if (!resid) {
+    const double zp = joined<kWalkT>(mx, sm, w.chunks, a.k64, s_tab, s_f, s_d, st.mp);
+    if (!(zp > 0)) {
+      if (tid == 0) a.next[s] = -1;
+      return;
+    }
+    st.ip = 1.0 / zp;
+    own = 0.0;
+#pragma unroll 1
+    for (int c = c0; c < c1; ++c) own += sm[c] * exp_call(mx[c], st.mp, a.k64, s_tab) * st.ip;
+    run = scan(own, whole);
+  }
+  // s_hit[0]: the first chunk past the goal, s_hit[1]: the last with any mass (for a goal that rounding puts at the whole).
+  const double goal = (double)fmaxf(a.u_final[s], 0.f) * whole;
+  if (tid < 2) s_hit[tid] = tid ? -1 : w.chunks;
+  __syncthreads();
+  // (One atomic a wave: the same address from every lane would be 64 of them in turn.)
+  auto meet = [&](int first, int last) {
+    const uint64_t f = __ballot(first < INT_MAX), l = __ballot(last >= 0);
+    if (f && lane == __ffsll((unsigned long long)f) - 1) atomicMin(&s_hit[0], first);
+    if (l && lane == 63 - __clzll((long long)l)) atomicMax(&s_hit[1], last);
+  };
+  double upto = run;
+  int first = INT_MAX, last = -1;
+#pragma unroll 1
+  for (int c = c0; c < c1; ++c) {
+    const double v = resid ? pw[c] : sm[c] * exp_call(mx[c], st.mp, a.k64, s_tab) * st.ip;
+    if (v > 0) {
+      last = c;
+      if (upto + v > goal) first = min(first, c);
+    }
+    upto += v;
+  }
+  meet(first, last);
+  __syncthreads();
+  const int chunk = s_hit[0] < w.chunks ? s_hit[0] : s_hit[1];
+  __syncthreads();
+  if (chunk >= c0 && chunk < c1) {   // the thread that holds it: what is left of the goal there
+    upto = run;
+#pragma unroll 1
+    for (int c = c0; c < chunk; ++c) upto += resid ? pw[c] : sm[c] * exp_call(mx[c], st.mp, a.k64, s_tab) * st.ip;
+    s_goal = goal - upto;
+  }
+  if (tid < 2) s_hit[tid] = tid ? -1 : a.V;
+  __syncthreads();
+  // The place in the chunk: one or four logits a thread.
+  const T *tr = (const T *)a.target + (int64_t)row * a.t_stride;
+  const T *dr = (const T *)a.draft + (int64_t)row * a.d_stride;
+  const int ept = w.chunk / kWalkT, v0 = chunk * w.chunk + tid * ept;
+  float x[4], y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool in = i < ept && v0 + i < a.V;
+    x[i] = in ? finite_or_less((float)tr[v0 + i]) : -INFINITY;
+    y[i] = in && resid && a.mode ? finite_or_less((float)dr[v0 + i]) : -INFINITY;
+  }
+  bool here = false;
+  if (resid)
+    for (int e = 0; e < k; ++e) here |= s_tok[e] >= v0 && s_tok[e] < v0 + ept;
+  double r[4], mine = 0.0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    r[i] = 0.0;
+    if (i >= ept) break;
+    r[i] = exp_call(x[i], st.mp, a.k64, s_tab) * st.ip;
+    if (resid && a.mode) r[i] = fmax(r[i] - st.c * st.iq * exp_call(y[i], st.mq, a.k64, s_tab), 0.0);
+    if (here)
+      for (int e = 0; e < k; ++e) r[i] = s_tok[e] == v0 + i ? 0.0 : r[i];
+    mine += r[i];
+  }
+  const double want = s_goal;
+  double end, sum = scan(mine, end);
+  first = INT_MAX, last = -1;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (r[i] > 0) {
+      last = v0 + i;
+      if (sum + r[i] > want) first = min(first, v0 + i);
+    }
+    sum += r[i];
+  }
+  meet(first, last);
+  __syncthreads();
+  if (tid == 0) a.next[s] = s_hit[0] < a.V ? s_hit[0] : s_hit[1];
 }
 
-size_t verify_workspace(int S, int N, int V, int mode, int children, bool greedy) {
-  return (sizeof(NodeState) + sizeof(int)) * (size_t)S * N;
+bool verify_fits(int S, int N, int V) {
+  const VerifyPlan p = verify_plan(S, N, V);
+  return (size_t)S * N * p.chunks <= (size_t)1 << 23;
 }
 
-hipError_t launch_verify(const VerifyArgs &a, hipStream_t s) {
+size_t verify_workspace(int S, int N, int V) { return verify_plan(S, N, V).total; }
+
+template <class T, int EPT> static int launch_verify_t(const VerifyArgs &a, const VerifyPlan &w, hipStream_t s) {
+  const uint32_t blocks = (uint32_t)((size_t)a.S * a.N * w.chunks);
+  int launches = 2;
+  if (a.inv_t == 0.0) {
+    hipLaunchKernelGGL((stats_kernel<T, EPT, true>), dim3(blocks), dim3(kVT), 0, s, a, w);
+  } else {
+    hipLaunchKernelGGL((stats_kernel<T, EPT, false>), dim3(blocks, a.mode && a.children ? 2 : 1), dim3(kVT), 0, s, a, w);
+    const int rounds = a.mode ? a.children : a.children ? 1 : 0;
+    for (int j = 1; j <= rounds; ++j) {
+      if (a.mode == 0) hipLaunchKernelGGL((round_kernel<T, EPT, 0>), dim3(blocks), dim3(kVT), 0, s, a, w, j);
+      else if (a.mode == 1) hipLaunchKernelGGL((round_kernel<T, EPT, 1>), dim3(blocks), dim3(kVT), 0, s, a, w, j);
+      else hipLaunchKernelGGL((round_kernel<T, EPT, 2>), dim3(blocks), dim3(kVT), 0, s, a, w, j);
+    }
+    launches += rounds;
+  }
+  hipLaunchKernelGGL((walk_kernel<T>), dim3(a.S), dim3(kWalkT), 0, s, a, w);
+  return launches;
+}
+
+hipError_t launch_verify(const VerifyArgs &a, hipStream_t s, int *launches) {
+  const VerifyPlan w = verify_plan(a.S, a.N, a.V);
   auto go = [&](auto t) {
     using T = decltype(t);
-    hipLaunchKernelGGL(node_kernel<T>, dim3(a.S * a.N), dim3(kVT), 0, s, a);
-    hipLaunchKernelGGL(walk_kernel<T>, dim3(a.S), dim3(kVT), 0, s, a);
+    return w.chunk == 4096 ? launch_verify_t<T, 16>(a, w, s) : launch_verify_t<T, 4>(a, w, s);
   };
-  if (a.type == E_F32) go(float{});
-  else if (a.type == E_F16) go(_Float16{});
-  else go(__bf16{});
+  *launches = a.type == E_F32 ? go(float{}) : a.type == E_F16 ? go(_Float16{}) : go(__bf16{});
   return hipGetLastError();
 }
 
