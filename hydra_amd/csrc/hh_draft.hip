@@ -107,6 +107,8 @@ hh::TreeArgs tree_args(const hh_tree_desc *d, const hh_kv_cache *c, const void *
   a.q_stride = d->q_stride ? d->q_stride : (int64_t)d->q_heads * d->head_dim;
   a.kv_stride = d->kv_stride ? d->kv_stride : (int64_t)d->kv_heads * d->head_dim;
   a.seq_stride = seq_stride(d, c);
+  a.qm = d->q_heads / d->kv_heads;
+  a.inv_qm = 1.f / (float)a.qm;
   return a;
 }
 

@@ -11,6 +11,7 @@ constexpr int kTreeNodes = 64;    // most nodes of a tree: an ancestor set is on
 constexpr int kTreeQM = 16;       // most query heads per kv head
 constexpr int kTreeGroups = 256;  // workgroups that a call's keys are split for
 constexpr int kTreeTiles = 4;     // tiles of keys that one workgroup takes without a split
+constexpr int kWeightGroups = 1024; // workgroups of the accumulation
 constexpr int kTreeChunks = 256;  // most chunks of a sequence
 
 struct TreeArgs {
@@ -74,7 +75,7 @@ bool verify_fits(int S, int N, int V);   // launches' block counts
 void tree_plan(TreeArgs &a, int64_t length);
 size_t tree_workspace(const TreeArgs &a);
 hipError_t launch_tree(const TreeArgs &a, int type, hipStream_t s);
-hipError_t launch_weights(const TreeArgs &a, int type, hipStream_t s);
+hipError_t launch_weights(TreeArgs a, int type, hipStream_t s);
 hipError_t launch_verify(const VerifyArgs &a, hipStream_t s, int *launches);
 hipError_t launch_commit(const RowsArgs &a, bool last, hipStream_t s);
 hipError_t launch_evict(const RowsArgs &a, hipStream_t s);

@@ -518,32 +518,93 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
   if (cg == 0) finish_row<QT, D>(a, row, hd, q4, m, den, sum);
 }
 
-__device__ __forceinline__ float elem_f32(const _Float16 *p) { return (float)*p; }
-__device__ __forceinline__ float elem_f32(const float *p) { return *p; }
-__device__ __forceinline__ float elem_f32(const __bf16 *p) { return (float)*p; }
-
-// One wave per (sequence, kv head, 64 rows), a lane per row.
-template <class Q, class C>
-__global__ __launch_bounds__(64) void weights_kernel(TreeArgs a) {
-  const int tiles = (a.rows + 63) / 64;
-  const int t = blockIdx.x % tiles, g = blockIdx.x / tiles % a.kvh, s = blockIdx.x / (tiles * a.kvh);
-  const int row = t * 64 + threadIdx.x, D = a.d, qm = a.qh / a.kvh;
+// Accumulated weights. A wave takes 32 keys of a kv head and holds them as the B operand; the accepted tokens'
+// queries pass as A tiles of 32 rows, S [32 rows × 32 keys], and a lane adds up one key's column. Every weight is
+// read and written once by one lane, in a fixed order. The queries of a (sequence, kv head), scaled and as pairs for
+// F32, are laid out in LDS once per workgroup of four waves, with the rows' lse; a row that does not see a key
+// (rows of the path behind it) adds nothing. Bound by the keys' bytes; a workgroup walks several runs of keys so that
+// the queries' layout is paid for.
+constexpr int kWTiles = 4;    // row tiles of 32 that LDS holds at a time
+template <int QT, int D>
+__global__ __launch_bounds__(256) void weights_kernel(TreeArgs a) {
+  constexpr bool BF = QT == E_BF16, PAIR = QT == E_F32;
+  constexpr int TERMS = PAIR ? 2 : 1, FR = D / 16;                    // fragments of 16 dimensions
+  __shared__ __align__(16) u32x4 s_q[kWTiles][TERMS][FR][64];         // A operand: lane (l32, hh) of each fragment
+  __shared__ float s_lse[kWTiles * 32];
+  __shared__ int s_row[kWTiles * 32];                                 // the last key that the row sees, −1: none
+  warm_kernargs<sizeof(TreeArgs)>();
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l32 = lane & 31, hh = lane >> 5;
+  const int first = blockIdx.x % a.chunks, sg = blockIdx.x / a.chunks, s = sg / a.kvh, g = sg - s * a.kvh, qm = a.qm;
   const int length = min(max(a.lengths[s], 0), a.rows);
   const int acc = min(max(a.accepted[s], 0), min(a.N, length));
-  if (row >= length) return;
-  const C *kr = (const C *)a.k + (int64_t)s * a.seq_stride + ((int64_t)row * a.kvh + g) * D;
-  float w = 0.f;
-  for (int i = 0; i < acc; ++i) {
-    const int n = a.path[(int64_t)s * a.N + i];
-    if (n < 0 || n >= a.N || row > length - acc + i) continue;
-    for (int h = g * qm; h < (g + 1) * qm; ++h) {
-      const Q *q = (const Q *)a.q + ((int64_t)s * a.N + n) * a.q_stride + (int64_t)h * D;
-      float x = 0.f;
-      for (int e = 0; e < D; ++e) x = fmaf(elem_f32(q + e), elem_f32(kr + e), x);
-      w += __expf(x * a.scale - a.lse_in[((int64_t)s * a.N + n) * a.qh + h]);
+  const int runs = (length + 127) / 128;                              // of 128 keys, 32 a wave
+  if (acc == 0 || first >= runs) return;
+  const int rows = acc * qm, tiles = (rows + 31) / 32;
+  const int rstride = a.kvh * D;
+  const uint16_t *kb = a.k + (int64_t)s * a.seq_stride + (int64_t)g * D;
+  float *w = a.weights + (int64_t)sg * a.rows;
+  for (int t0 = 0; t0 < tiles; t0 += kWTiles) {
+    const int nt = min(kWTiles, tiles - t0);
+    if (t0) __syncthreads();
+    for (int e = tid; e < nt * FR * 64; e += 256) {
+      const int t = e / (FR * 64), dc = e / 64 % FR, l = e & 63;
+      const int r = (t0 + t) * 32 + (l & 31), i = (int)(((float)r + 0.5f) * a.inv_qm);
+      const int n = i < acc ? a.path[(int64_t)s * a.N + i] : -1;
+      const bool ok = n >= 0 && n < a.N;
+      const int64_t row = (int64_t)s * a.N + (ok ? n : 0), head = g * qm + (ok ? r - i * qm : 0);
+      const int64_t at = row * a.q_stride + head * D + 16 * dc + 8 * (l >> 5);
+      if constexpr (PAIR) {
+        const f32x4 *qp = (const f32x4 *)((const float *)a.q + at);
+        const f32x4 q0 = qp[0], q1 = qp[1];
+        f16x8 h, lo;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          float v = (k < 4 ? q0[k & 3] : q1[k & 3]) * (a.scale * kLog2e);
+          asm volatile("" : "+v"(v));                                 // rounded before it is split, as above
+          h[k] = (_Float16)v;
+          lo[k] = (_Float16)(v - (float)h[k]);
+        }
+        s_q[t][0][dc][l] = __builtin_bit_cast(u32x4, h);
+        s_q[t][TERMS - 1][dc][l] = __builtin_bit_cast(u32x4, lo);
+      } else {
+        s_q[t][0][dc][l] = *(const u32x4 *)((const uint16_t *)a.q + at);
+      }
+      if (dc == 0 && l < 32) {
+        s_lse[t * 32 + l] = ok ? a.lse_in[row * a.qh + head] * kLog2e : 0.f;
+        s_row[t * 32 + l] = ok ? length - acc + i : -1;
+      }
+    }
+    __syncthreads();
+    const float scale = PAIR ? 1.f : a.scale * kLog2e;
+    for (int run = first; run < runs; run += a.chunks) {
+      const int key = run * 128 + wave * 32 + l32;
+      if (run * 128 + wave * 32 >= length) continue;
+      const u32x4 *kp = (const u32x4 *)(kb + (int64_t)min(key, length - 1) * rstride) + hh;
+      u32x4 kf[FR];
+#pragma unroll
+      for (int dc = 0; dc < FR; ++dc) kf[dc] = kp[2 * dc];
+      float sum = 0.f;
+      for (int t = 0; t < nt; ++t) {
+        f32x16 S = f32x16{};
+#pragma unroll
+        for (int dc = 0; dc < FR; ++dc) {
+          S = mfma32<BF>(s_q[t][0][dc][lane], kf[dc], S);
+          if constexpr (PAIR) S = mfma32<BF>(s_q[t][TERMS - 1][dc][lane], kf[dc], S);
+        }
+        // Element i is row 8 (i / 4) + 4 hh + i % 4 of the tile.
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int r = 32 * t + 8 * (i >> 2) + 4 * hh + (i & 3);
+          const float p = exp2_(fmaf(S[i], scale, -s_lse[r]));
+          part[i & 3] += key <= s_row[r] ? p : 0.f;
+        }
+        sum += (part[0] + part[1]) + (part[2] + part[3]);
+      }
+      sum += other_half(sum);
+      if (hh == 0 && key < length) w[key] += sum;
     }
   }
-  a.weights[((int64_t)s * a.kvh + g) * a.rows + row] += w;
 }
 
 // The launch: RT by the rows of a kv head, KS and the ring so that a workgroup's tiles in flight cover the
@@ -557,8 +618,6 @@ static TreeShape tree_shape(int d, int rows) {
 
 // Fills in how the call's keys are split, for histories of up to `length` keys.
 void tree_plan(TreeArgs &a, int64_t length) {
-  a.qm = a.qh / a.kvh;
-  a.inv_qm = 1.f / (float)a.qm;
   const int rows = a.N * a.qm;
   const TreeShape t = tree_shape(a.d, rows);
   a.tile = 32 * t.ks;
@@ -607,11 +666,22 @@ hipError_t launch_tree(const TreeArgs &a, int type, hipStream_t s) {
   return type == E_F16 ? launch_tree_q<E_F16>(a, s) : launch_tree_q<E_BF16>(a, s);
 }
 
-hipError_t launch_weights(const TreeArgs &a, int type, hipStream_t s) {
-  const dim3 grid(a.S * a.kvh * ((a.rows + 63) / 64));
-  if (type == E_F32) hipLaunchKernelGGL((weights_kernel<float, _Float16>), grid, dim3(64), 0, s, a);
-  else if (type == E_F16) hipLaunchKernelGGL((weights_kernel<_Float16, _Float16>), grid, dim3(64), 0, s, a);
-  else hipLaunchKernelGGL((weights_kernel<__bf16, __bf16>), grid, dim3(64), 0, s, a);
+template <int QT> static void launch_weights_q(const TreeArgs &a, dim3 grid, hipStream_t s) {
+  if (a.d == 64) hipLaunchKernelGGL((weights_kernel<QT, 64>), grid, dim3(256), 0, s, a);
+  else if (a.d == 128) hipLaunchKernelGGL((weights_kernel<QT, 128>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((weights_kernel<QT, 256>), grid, dim3(256), 0, s, a);
+}
+
+hipError_t launch_weights(TreeArgs a, int type, hipStream_t s) {
+  const int64_t own = (int64_t)a.S * a.kvh, runs = ((int64_t)a.rows + 127) / 128;
+  int64_t x = kWeightGroups / own;
+  if (x > runs) x = runs;
+  if (x < 1) x = 1;
+  a.chunks = (int)x;   // workgroups of a (sequence, kv head)
+  const dim3 grid((uint32_t)(x * own));
+  if (type == E_F32) launch_weights_q<E_F32>(a, grid, s);
+  else if (type == E_F16) launch_weights_q<E_F16>(a, grid, s);
+  else launch_weights_q<E_BF16>(a, grid, s);
   return hipGetLastError();
 }
 
