@@ -56,31 +56,24 @@ __device__ __forceinline__ uint32_t rank_key(float w, int pos, int64_t oldest) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelT = 1024;
-
-// Exclusive prefix of `flag` over the workgroup in thread order, and its total.
-__device__ __forceinline__ int block_rank(bool flag, int *s_w, int &total) {
-  const uint64_t b = __ballot(flag);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  if (lane == 0) s_w[wave] = __popcll(b);
-  __syncthreads();
-  int before = 0;
-  total = 0;
-  for (int w = 0; w < kSelT / 64; ++w) {
-    if (w < wave) before += s_w[w];
-    total += s_w[w];
-  }
-  __syncthreads();
-  return before + __popcll(b & ((1ull << lane) - 1));
-}
-
-// One workgroup per (layer, sequence, kv head): the key of the keep-th row by radix selection, eight
-// bits a pass, then the rows below `keep` that go and those from `keep` on that stay, in order.
+// One workgroup per (layer, sequence, kv head) finds the key of the keep-th row and lists the rows that move.
+// A wave owns runs of 64 consecutive rows, a lane per row of a run, their keys in LDS (CAP = 0: more rows than that, read
+// again from memory at each step). The key is built from its highest bit, eleven bits a step, by a histogram of the rows
+// that share what is known of it; the bits that all keys share are skipped, which spreads the rest over many bins (LDS
+// adds to one address go one after the other); a step whose bin is taken whole ends it. Then a lane holds the
+// masks of a run's rows above and at the key, ranks the rows that go from below `keep` and those that stay from
+// `keep` on by scans over the runs, and the rows are listed in order.
+// 12 heads of 4112 rows: the key two bits a step by counting, then the lists by two walks over the rows, 24 us; by
+// histograms of eight bits with a serial scan 46.
+constexpr int kSelT = 1024, kSelW = kSelT / 64, kBits = 11;
+template <int CAP>
 __global__ __launch_bounds__(kSelT) void select_kernel(RowsArgs a) {
-  __shared__ int s_hist[256], s_w[kSelT / 64], s_bin, s_left;
+  __shared__ uint32_t s_key[CAP ? CAP : 1];
+  __shared__ int s_hist[1 << kBits], s_sum[kSelW], s_n[kSelW][2], s_found[3];
+  __shared__ uint32_t s_and[kSelW], s_or[kSelW];
   const int head = blockIdx.x, g = head % a.kvh, s = head / a.kvh % a.S;
   const RowsLayer &y = a.layer[head / (a.kvh * a.S)];
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int n = min(max(y.lengths[s], 0), y.rows);
   if (n <= a.keep) {
     if (tid == 0) a.moves[head] = 0;
@@ -90,69 +83,197 @@ __global__ __launch_bounds__(kSelT) void select_kernel(RowsArgs a) {
   const int64_t base = ((int64_t)s * a.kvh + g) * y.rows;
   const float *w = y.weights + base;
   const int *pos = y.positions + base;
-  uint32_t prefix = 0;
-  int left = a.keep;   // rows still to take among those that share the prefix
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) s_hist[tid] = 0;
-    __syncthreads();
-    for (int r = tid; r < n; r += kSelT) {
-      const uint32_t key = rank_key(w[r], pos[r], oldest);
-      if (shift == 24 || key >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&s_hist[key >> shift & 255], 1);
+  // Rows first .. first + 64 · runs − 1; four runs at a time (rows past n have key 0, which no row has).
+  const int runs = ((n + kSelT - 1) / kSelT + 3) & ~3, first = wave * runs * 64;
+  uint32_t all = 0xFFFFFFFFu, any = 0;
+  for (int i0 = 0; i0 < runs; i0 += 4) {
+    float wv[4];
+    int pv[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int at = min(first + 64 * (i0 + u) + lane, n - 1);
+      wv[u] = w[at];
+      pv[u] = pos[at];
     }
-    __syncthreads();
-    if (tid == 0) {
-      int bin = 255, need = left;
-      while (bin > 0 && s_hist[bin] < need) need -= s_hist[bin--];
-      s_bin = bin;
-      s_left = need;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int r = first + 64 * (i0 + u) + lane;
+      const uint32_t k = rank_key(wv[u], pv[u], oldest);
+      if (r < n) all &= k, any |= k;
+      if constexpr (CAP > 0) s_key[r] = r < n ? k : 0;   // r < 1024 · runs <= CAP
     }
-    __syncthreads();
-    prefix |= (uint32_t)s_bin << shift;
-    left = s_left;
   }
-  // Rows above `prefix` stay, and the first `left` of those equal to it.
-  int equal = 0, holes = 0, from = 0;
+  auto key_of = [&](int i) -> uint32_t {
+    const int r = first + 64 * i + lane;
+    if constexpr (CAP > 0) return s_key[r];
+    return r < n ? rank_key(w[r], pos[r], oldest) : 0;
+  };
+  for (int o = 32; o; o >>= 1) all &= __shfl_xor(all, o), any |= __shfl_xor(any, o);
+  if (lane == 0) s_and[wave] = all, s_or[wave] = any;
+  s_hist[2 * tid] = s_hist[2 * tid + 1] = 0;
+  __syncthreads();
+  for (int i = 0; i < kSelW; ++i) all &= s_and[i], any |= s_or[i];
+  // Of the rows that agree with t above `bit`, the `need` first in the order are among those that stay, as are all rows
+  // above them. At the end t is the key of the last that stays.
+  int bit = 32 - __builtin_clz((all ^ any) | 1), need = a.keep;
+  uint32_t t = bit == 32 ? 0u : all >> bit << bit;
+  while (bit > 0) {
+    const int shift = max(bit - kBits, 0), bins = 1 << (bit - shift);
+    const uint32_t known = bit == 32 ? 0u : ~0u << bit;
+    for (int i0 = 0; i0 < runs; i0 += 4) {
+      uint32_t k[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) k[u] = key_of(i0 + u);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (k[u] && (k[u] & known) == t) atomicAdd(&s_hist[(k[u] & ~known) >> shift], 1);
+    }
+    __syncthreads();
+    // Rows in this thread's two bins and in all above them.
+    const int h0 = s_hist[2 * tid], h1 = s_hist[2 * tid + 1];
+    int sum = h0 + h1;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_down(sum, o);
+      if (lane + o < 64) sum += v;
+    }
+    if (lane == 0) s_sum[wave] = sum;
+    __syncthreads();
+    for (int i = wave + 1; i < kSelW; ++i) sum += s_sum[i];
+    s_hist[2 * tid] = s_hist[2 * tid + 1] = 0;
+    // The bin in which the count from the top reaches `need`.
+    const int over = sum - h0 - h1;
+    if (over < need && sum >= need) {
+      const bool upper = over + h1 >= need;
+      s_found[0] = 2 * tid + upper;
+      s_found[1] = need - (upper ? over : over + h1);
+      s_found[2] = upper ? h1 : h0;
+    }
+    __syncthreads();
+    t |= (uint32_t)s_found[0] << shift;
+    need = s_found[1];
+    bit = shift;
+    if (need == s_found[2]) break;   // the whole bin stays: every row of at least t
+  }
+  // Rows above t stay, and of those equal to it the first: as many as are left (all of them, if t splits exactly).
+  const uint64_t below = (1ull << lane) - 1;
+  uint64_t above = 0, equal = 0;     // of the rows of run `from` + lane
+  auto masks = [&](int from) {
+    above = equal = 0;
+    for (int i0 = from; i0 < min(runs, from + 64); i0 += 4) {
+      uint32_t k[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) k[u] = key_of(i0 + u);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint64_t m = __ballot(k[u] > t), e = __ballot(k[u] == t);
+        if (lane == i0 + u - from) above = m, equal = e;
+      }
+    }
+  };
+  auto wave_total = [](int v) {
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+  };
+  auto before_lane = [&](int v) {    // exclusive prefix over the lanes
+    int p = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int q = __shfl_up(p, o);
+      if (lane >= o) p += q;
+    }
+    return p - v;
+  };
+  int n_above = 0, n_equal = 0;
+  for (int from = 0; from < runs; from += 64) {
+    masks(from);
+    n_above += wave_total(__popcll(above));
+    n_equal += wave_total(__popcll(equal));
+  }
+  if (lane == 0) s_n[wave][0] = n_above, s_n[wave][1] = n_equal;
+  __syncthreads();
+  int rank = 0, left = a.keep;       // equal rows of the waves before this one, and those that stay of all
+  for (int i = 0; i < kSelW; ++i) {
+    left -= s_n[i][0];
+    if (i < wave) rank += s_n[i][1];
+  }
+  __syncthreads();
   int32_t *src = a.from + (int64_t)head * a.max_moves, *dst = a.to + (int64_t)head * a.max_moves;
-  for (int t = 0; t < n; t += kSelT) {
-    const int r = t + tid;
-    const uint32_t key = r < n ? rank_key(w[r], pos[r], oldest) : 0;
-    int total;
-    const bool eq = r < n && key == prefix;
-    const int e = equal + block_rank(eq, s_w, total);
-    equal += total;
-    const bool stay = r < n && (key > prefix || (eq && e < left));
-    const bool hole = r < n && r < a.keep && !stay, move = r >= a.keep && stay;
-    const int i = holes + block_rank(hole, s_w, total);
-    if (hole && i < a.max_moves) dst[i] = r;
-    holes += total;
-    const int j = from + block_rank(move, s_w, total);
-    if (move && j < a.max_moves) src[j] = r;
-    from += total;
+  int hole_at = 0, move_at = 0, total = 0;
+  for (int pass = 0; pass < 2; ++pass) {
+    int eq_rank = rank, holes = 0, moves = 0;
+    for (int from = 0; from < runs; from += 64) {
+      if (runs > 64) masks(from);
+      // This lane's run: its rows that stay, then those that leave a hole below `keep` and those that fill one.
+      const int mine = __popcll(equal), had = eq_rank + before_lane(mine);
+      uint64_t stay = equal;
+      for (int drop = mine - max(0, min(mine, left - had)); drop > 0; --drop) stay &= ~(1ull << (63 - __clzll((long long)stay)));
+      stay |= above;
+      const int64_t r0 = first + 64 * (int64_t)(from + lane);
+      const bool run = from + lane < runs;
+      auto rows_below = [&](int64_t end) { return end <= r0 ? 0ull : end - r0 >= 64 ? ~0ull : (1ull << (end - r0)) - 1; };
+      const uint64_t h = run ? rows_below(min(a.keep, n)) & ~stay : 0, m = run ? stay & ~rows_below(a.keep) : 0;
+      const int nh = __popcll(h), nm = __popcll(m);
+      if (pass) {
+        int hi = hole_at + holes + before_lane(nh), mi = move_at + moves + before_lane(nm);
+        for (uint64_t left_h = h; left_h; left_h &= left_h - 1, ++hi)
+          if (hi < a.max_moves) dst[hi] = (int)r0 + __ffsll((unsigned long long)left_h) - 1;
+        for (uint64_t left_m = m; left_m; left_m &= left_m - 1, ++mi)
+          if (mi < a.max_moves) src[mi] = (int)r0 + __ffsll((unsigned long long)left_m) - 1;
+      }
+      eq_rank += wave_total(mine);
+      holes += wave_total(nh);
+      moves += wave_total(nm);
+    }
+    if (pass) break;
+    if (lane == 0) s_n[wave][0] = holes, s_n[wave][1] = moves;
+    __syncthreads();
+    for (int i = 0; i < kSelW; ++i) {
+      if (i < wave) hole_at += s_n[i][0], move_at += s_n[i][1];
+      total += s_n[i][1];
+    }
   }
-  if (tid == 0) a.moves[head] = min(min(holes, from), a.max_moves);
+  if (tid == 0) a.moves[head] = min(total, a.max_moves);
 }
 
-// Moves the rows of a head, a group of lanes per row; the sources, at `keep` and above, and the
-// destinations, below it, do not overlap. One workgroup of the last layer that shares them shortens the lengths.
+// Moves the rows of a head, a group of lanes per row and four rows in flight; the sources, at `keep` and above,
+// and the destinations, below it, do not overlap. One workgroup of the last layer that shares them shortens the
+// lengths.
 __global__ __launch_bounds__(256) void move_kernel(RowsArgs a, int parts) {
   const int head = blockIdx.x / parts, part = blockIdx.x % parts;
   const int g = head % a.kvh, s = head / a.kvh % a.S;
   const RowsLayer &y = a.layer[head / (a.kvh * a.S)];
+  if (y.last && g == 0 && part == 0 && threadIdx.x == 0) y.lengths[s] = min(y.lengths[s], a.keep);
   const int moves = a.moves[head];
   const int32_t *src = a.from + (int64_t)head * a.max_moves, *dst = a.to + (int64_t)head * a.max_moves;
   const int lanes = a.d / 8, per = 256 / lanes, lane = threadIdx.x % lanes;
   const int64_t base = (int64_t)s * y.seq_stride + (int64_t)g * a.d + 8 * lane, meta = ((int64_t)s * a.kvh + g) * y.rows;
-  for (int i = part * per + threadIdx.x / lanes; i < moves; i += parts * per) {
-    const int f = src[i], t = dst[i];
-    const int64_t fo = base + (int64_t)f * a.kvh * a.d, to = base + (int64_t)t * a.kvh * a.d;
-    *(u32x4 *)(y.k + to) = *(const u32x4 *)(y.k + fo);
-    *(u32x4 *)(y.v + to) = *(const u32x4 *)(y.v + fo);
-    if (lane == 0) {
-      y.weights[meta + t] = y.weights[meta + f];
-      y.positions[meta + t] = y.positions[meta + f];
+  const int64_t row = (int64_t)a.kvh * a.d;
+  for (int i0 = part * 4 * per + threadIdx.x / lanes; i0 < moves; i0 += parts * 4 * per) {
+    int f[4], t[4];
+    u32x4 k[4], v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = min(i0 + u * per, moves - 1);
+      f[u] = src[i];
+      t[u] = dst[i];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      k[u] = *(const u32x4 *)(y.k + base + f[u] * row);
+      v[u] = *(const u32x4 *)(y.v + base + f[u] * row);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (i0 + u * per >= moves) break;
+      *(u32x4 *)(y.k + base + t[u] * row) = k[u];
+      *(u32x4 *)(y.v + base + t[u] * row) = v[u];
+      if (lane == 0) {
+        y.weights[meta + t[u]] = y.weights[meta + f[u]];
+        y.positions[meta + t[u]] = y.positions[meta + f[u]];
+      }
     }
   }
-  if (y.last && g == 0 && part == 0 && threadIdx.x == 0) y.lengths[s] = min(y.lengths[s], a.keep);
 }
 
 hipError_t launch_commit(const RowsArgs &a, bool last, hipStream_t s) {
@@ -163,8 +284,16 @@ hipError_t launch_commit(const RowsArgs &a, bool last, hipStream_t s) {
 
 hipError_t launch_evict(const RowsArgs &a, hipStream_t s) {
   const int heads = a.layers * a.S * a.kvh;
-  hipLaunchKernelGGL(select_kernel, dim3(heads), dim3(kSelT), 0, s, a);
-  const int parts = 8;
+  int rows = 0;
+  for (int i = 0; i < a.layers; ++i) rows = a.layer[i].rows > rows ? a.layer[i].rows : rows;
+  if (rows <= 8192) hipLaunchKernelGGL(select_kernel<8192>, dim3(heads), dim3(kSelT), 0, s, a);
+  else if (rows <= 36864) hipLaunchKernelGGL(select_kernel<36864>, dim3(heads), dim3(kSelT), 0, s, a);
+  else hipLaunchKernelGGL(select_kernel<0>, dim3(heads), dim3(kSelT), 0, s, a);
+  // Workgroups enough to fill the chip with rows in flight, of at least four rounds' rows each.
+  const int per = 4 * 256 / (a.d / 8);
+  int parts = 4096 / heads, most = (a.max_moves + per - 1) / per;
+  if (parts > most) parts = most;
+  if (parts < 1) parts = 1;
   hipLaunchKernelGGL(move_kernel, dim3(heads * parts), dim3(256), 0, s, a, parts);
   return hipGetLastError();
 }
