@@ -374,7 +374,10 @@ __global__ __launch_bounds__(kWalkT) void walk_kernel(VerifyArgs a, VerifyPlan w
       yes = yes && token >= 0 && token == s_best[yes ? up : 0];
       // Children past the most that are tried.
       int before = 0;
-      for (int i = 0; i < 64; ++i) before += i < lane && __shfl(up, i) == up;
+      for (int i = 0; i < 64; ++i) {
+        const int other = __shfl(up, i);   // by every lane: lane i among them
+        before += i < lane && other == up;
+      }
       yes = yes && before < a.children;
     } else if (yes) {
       yes = ((const int32_t *)(a.ws + w.accept))[at + lane] != 0;

@@ -153,7 +153,12 @@ def test_greedy(kind):
             t["tokens"][4, 1:] = -1
             best = torch.where(t["target"].isnan(), float("-inf"), t["target"].float()).argmax(-1)
             t["tokens"][5, 1:] = best[5][t["parents"][5, 1:].long()].int()
-            check(t, "given", call(torch, ctx, t, "given", 0.0), 0.0)
+            for most in (0, 1, 2):
+                check(t, "given", call(torch, ctx, t, "given", 0.0, most), 0.0, most)
+            chain = dict(t, parents=torch.arange(-1, 9, dtype=torch.int32).expand(6, 10).contiguous())
+            chain["tokens"] = torch.cat([t["tokens"][:, :1], best[:, :-1].int()], 1).contiguous()
+            chain["tokens"][1, 5] += 1
+            check(chain, "given", call(torch, ctx, chain, "given", 0.0, 1), 0.0, 1)
             without = dict(t, u=None, uf=None)
             assert all(torch.equal(a, b) for a, b in zip(call(torch, ctx, without, "given", 0.0), call(torch, ctx, t, "given", 0.0)))
     finally:
