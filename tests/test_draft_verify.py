@@ -120,6 +120,8 @@ def check(t, mode, got, temperature=1.0, most=0):
     (3, 13, 2049, "bf16", 3, 1.0),
     (2, 9, 12345, "f32", 2, 0.9),
     (1, 5, 100003, "f16", 4, 1.0),
+    (2, 9, 131073, "f32", 2, 0.9),       # chunks of 4096, a tail of one
+    (3, 6, 140001, "bf16", 5, 1.1),
 ])
 def test_verify(mode, S, N, V, kind, branch, temperature):
     import torch
@@ -127,7 +129,7 @@ def test_verify(mode, S, N, V, kind, branch, temperature):
     print(f"[gpu] verify {mode} S={S} N={N} V={V} {kind} branch={branch}", flush=True)
     ctx = Context(0)
     try:
-        for seed in range(3):
+        for seed in range(3 if V < 50000 else 1):
             t = inputs(torch, S, N, V, kind, mode, branch, seed * 7 + V)
             check(t, mode, call(torch, ctx, t, mode, temperature), temperature)
             for most in (1, 2):
@@ -144,7 +146,7 @@ def test_greedy(kind):
     from hydra_amd.layer import Context
     ctx = Context(0)
     try:
-        for V in (1, 5, 1000, 4097):
+        for V in (1, 5, 1000, 4097, 50001):
             t = inputs(torch, 6, 10, V, kind, "given", 3, V)
             t["target"][0, :, : V // 2] = t["target"][0].amax()      # ties
             t["target"][1, 0] = float("-inf")

@@ -123,6 +123,9 @@ CASES = [
     (1, 6, 8, 2, 64, "f32", 33, [100], 0, True, None),           # a ring without a window: its rows
     (2, 3, 8, 2, 64, "f32", 300, [290, 290], 1, False, CHAIN),   # a window of one: every node alone
     (1, 16, 64, 8, 64, "f32", 5000, [4987], 0, False, None),     # many chunks
+    (1, 2, 2, 1, 64, "f32", 70000, [69990], 0, False, None),     # the most chunks of a sequence
+    (2, 40, 16, 1, 64, "bf16", 700, [650, 699], 0, False, None), # five blocks of rows
+    (1, 33, 4, 1, 256, "f32", 1500, [1500], 0, False, None),
     (9, 4, 8, 2, 64, "f16", 2500, [2400, 1, 0, 77, 2500, 1024, 1025, 640, 2000], 0, False, None),
 ]
 
