@@ -266,7 +266,7 @@ int hh_draft_verify(hh_ctx *ctx, const hh_verify_desc *d, const void *target, co
   a.children = verify_children(d);
   a.inv_t = greedy ? 0.0 : 1.0 / (double)d->temperature;
   a.ws = ctx->draft;
-  a.k64 = 64 * 1.4426950408889634074 * a.inv_t;
+  a.k = 256 * 1.4426950408889634074 * a.inv_t;
   int launches = 0;
   HH_HIP(hh::launch_verify(a, ctx->stream, &launches));
   ctx->dispatches += launches;

@@ -66,7 +66,7 @@ struct VerifyArgs {
   const float *u, *u_final;
   int32_t *path, *accepted, *next;
   int S, N, V, type, mode, children;
-  double inv_t, k64;                // 1 / temperature (0: greedy), 64 log2(e) / temperature
+  double inv_t, k;                  // 1 / temperature (0: greedy), 256 log2(e) / temperature
   uint8_t *ws;
 };
 

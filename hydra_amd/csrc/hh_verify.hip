@@ -16,8 +16,8 @@
 //            chunks' sums, its place by a scan of that chunk.
 // Bound by the launches' dependent chain for a few rows, and by the exponentials in 64 bits for many: the next token
 // is where a sum of up to V terms passes a random bound, and with errors of 1e-7 in it one in twenty draws from
-// the tail of 250000 tokens would differ. exp goes by a table of 2^(i / 64) and five terms of a series (relative error
-// below 1e-15 beside the argument's): 13 instructions in fp64.
+// the tail of 250000 tokens would differ. exp goes by a table of 2^(i / 256) and four terms of a series behind the 1 (relative
+// error below 1e-15 beside the argument's), twelve instructions in fp64.
 #include <climits>
 
 #include "hh_common.hpp"
@@ -30,30 +30,33 @@ constexpr int kWalkT = 1024;
 
 __device__ __forceinline__ float finite_or_less(float x) { return x != x ? -INFINITY : x; }
 
-// exp((x − top) / temperature) with tab[i] = 2^(i / 64) in LDS, k64 = 64 log2(e) / temperature.
-__device__ __forceinline__ double exp_of(float x, double top, double k64, const double *tab) {
-  const double y = fmax(((double)x - top) * k64, -64.0 * 1100), n = rint(y), f = y - n;
-  constexpr double c = 0.010830424696249145;   // ln 2 / 64
-  double s = fma(f, c * c * c * c * c / 120, c * c * c * c / 24);
-  s = fma(f, s, c * c * c / 6);
+// exp((x − top) / temperature) = 2^(y / 256), y = x·k + b, with tab[i] = 2^(i / 256) in LDS, k = 256 log2(e) / temperature and
+// b = −top·k: the rounding of b is one factor of a row's every term. y is split by adding 1.5·2^52, whose low word is
+// then the nearest integer, and the power of two goes into the exponent's bits. Below 2^−1000: 0.
+__device__ __forceinline__ double exp_of(float x, double k, double b, const double *tab) {
+  constexpr double magic = 6755399441055744.0, c = 0.0027076061740622863;   // ln 2 / 256
+  const double y = fmax(fma((double)x, k, b), -256.0 * 1001), m = y + magic, f = y - (m - magic);
+  const int i = (int)(uint32_t)__builtin_bit_cast(uint64_t, m);
+  double s = fma(f, c * c * c * c / 24, c * c * c / 6);
   s = fma(f, s, c * c / 2);
   s = fma(f, s, c);
   s = fma(f, s, 1.0);
-  const int i = (int)n;
-  return ldexp(s * tab[i & 63], i >> 6);
+  const uint64_t v = __builtin_bit_cast(uint64_t, s * tab[i & 255]);
+  const uint32_t hi = (uint32_t)(v >> 32) + ((uint32_t)(i >> 8) << 20);
+  return i >= -256 * 1000 ? __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)v) : 0.0;
 }
 // The same for a row whose largest entry is infinite: its +inf entries share the probability, a row of −inf has none.
-__device__ __forceinline__ double exp_any(float x, float top, double k64, const double *tab) {
+__device__ __forceinline__ double exp_any(float x, float top, double k, const double *tab) {
   if (fabsf(top) == INFINITY) return top > 0.f && x == top ? 1.0 : 0.0;
-  return exp_of(x, top, k64, tab);
+  return exp_of(x, k, -(double)top * k, tab);
 }
 // exp_any as a call: where each of a kernel's few uses is run once, its instructions are fetched once (a cold
 // 64-byte line of instructions costs about 0.1 us).
-__device__ __noinline__ double exp_call(float x, float top, double k64, const double *tab) {
-  return exp_any(x, top, k64, tab);
+__device__ __noinline__ double exp_call(float x, float top, double k, const double *tab) {
+  return exp_any(x, top, k, tab);
 }
 __device__ __forceinline__ void fill_table(double *tab) {
-  if (threadIdx.x < 64) tab[threadIdx.x] = exp2((double)threadIdx.x / 64);
+  if (threadIdx.x < 256) tab[threadIdx.x] = exp2((double)threadIdx.x / 256);
 }
 
 // Sum and maximum over a workgroup, in a fixed order, in every thread. s_d: T / 64 doubles of its own per call site.
@@ -144,7 +147,7 @@ __device__ __forceinline__ uint64_t children_of(const VerifyArgs &a, int s, int 
 
 template <class T, int EPT, bool GREEDY>
 __global__ __launch_bounds__(kVT) void stats_kernel(VerifyArgs a, VerifyPlan w) {
-  __shared__ double s_tab[64], s_d[kVT / 64];
+  __shared__ double s_tab[256], s_d[kVT / 64];
   __shared__ float s_f[kVT / 64];
   __shared__ int s_i[kVT / 64];
   const int chunk = blockIdx.x % w.chunks, row = blockIdx.x / w.chunks, s = row / a.N, n = row - s * a.N, tid = threadIdx.x;
@@ -181,9 +184,9 @@ __global__ __launch_bounds__(kVT) void stats_kernel(VerifyArgs a, VerifyPlan w) 
 #pragma unroll
     for (int i = 0; i < EPT; ++i) sum += one && x[i] == all ? 1.0 : 0.0;
   } else {
-    const double top64 = all;
+    const double b = -(double)all * a.k;
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) sum += exp_of(x[i], top64, a.k64, s_tab);   // −inf: 0
+    for (int i = 0; i < EPT; ++i) sum += exp_of(x[i], a.k, b, s_tab);   // −inf: 0
   }
   sum = block_sum<kVT>(sum, s_d);
   if (tid == 0) {
@@ -195,20 +198,20 @@ __global__ __launch_bounds__(kVT) void stats_kernel(VerifyArgs a, VerifyPlan w) 
 
 // A row's maximum and sum from its chunks'.
 template <int T>
-__device__ __forceinline__ double joined(const float *mx, const double *sm, int chunks, double k64, const double *tab, float *s_f,
+__device__ __forceinline__ double joined(const float *mx, const double *sm, int chunks, double k, const double *tab, float *s_f,
                                          double *s_d, float &top) {
   float m = -INFINITY;
   for (int c = threadIdx.x; c < chunks; c += T) m = fmaxf(m, mx[c]);
   top = block_max<T>(m, s_f);
   double z = 0.0;
 #pragma unroll 1
-  for (int c = threadIdx.x; c < chunks; c += T) z += sm[c] * exp_call(mx[c], top, k64, tab);
+  for (int c = threadIdx.x; c < chunks; c += T) z += sm[c] * exp_call(mx[c], top, k, tab);
   return block_sum<T>(z, s_d);
 }
 
 template <class T, int EPT, int MODE>
 __global__ __launch_bounds__(kVT) void round_kernel(VerifyArgs a, VerifyPlan w, int round) {
-  __shared__ double s_tab[64], s_d[6][kVT / 64];
+  __shared__ double s_tab[256], s_d[6][kVT / 64];
   __shared__ float s_f[2][kVT / 64];
   __shared__ int s_tok[kTreeNodes];
   constexpr bool DRAWN = MODE != 0;
@@ -238,12 +241,12 @@ __global__ __launch_bounds__(kVT) void round_kernel(VerifyArgs a, VerifyPlan w, 
   if (round == 1) {
     float m;
     const double zp = joined<kVT>((const float *)(a.ws + w.max_of[0]) + at, (const double *)(a.ws + w.sum_of[0]) + at, w.chunks,
-                                  a.k64, s_tab, s_f[0], s_d[0], m);
+                                  a.k, s_tab, s_f[0], s_d[0], m);
     st.mp = m;
     st.ip = zp > 0 ? 1.0 / zp : 0.0;
     if constexpr (DRAWN) {
       const double zq = joined<kVT>((const float *)(a.ws + w.max_of[1]) + at, (const double *)(a.ws + w.sum_of[1]) + at, w.chunks,
-                                    a.k64, s_tab, s_f[1], s_d[1], m);
+                                    a.k, s_tab, s_f[1], s_d[1], m);
       st.mq = m;
       st.iq = zq > 0 ? 1.0 / zq : 0.0;
     }
@@ -268,8 +271,8 @@ __global__ __launch_bounds__(kVT) void round_kernel(VerifyArgs a, VerifyPlan w, 
       bool again = false;
       for (int i = 0; i < round - 1; ++i) again |= s_tok[i] == t;
       if (lane == 0 && t >= 0 && t < a.V && !again) {
-        const double p = exp_call(finite_or_less((float)tr[t]), st.mp, a.k64, s_tab) * st.ip;
-        const double q = exp_call(finite_or_less((float)dr[t]), st.mq, a.k64, s_tab) * st.iq;
+        const double p = exp_call(finite_or_less((float)tr[t]), st.mp, a.k, s_tab) * st.ip;
+        const double q = exp_call(finite_or_less((float)dr[t]), st.mq, a.k, s_tab) * st.iq;
         accept[child] = fmax(p - st.c * q, 0.0) > (double)a.u[(int64_t)s * a.N + child] * mass * (q / left);
       }
     } else if (kids >> lane & 1) {
@@ -282,10 +285,10 @@ __global__ __launch_bounds__(kVT) void round_kernel(VerifyArgs a, VerifyPlan w, 
         again |= o == t;
         bool first = o >= 0 && o < a.V;
         for (int e = 0; e < i; ++e) first &= s_tok[e] != o;
-        if (first) before += exp_call(finite_or_less((float)tr[o]), st.mp, a.k64, s_tab) * st.ip;
+        if (first) before += exp_call(finite_or_less((float)tr[o]), st.mp, a.k, s_tab) * st.ip;
       }
       if (t >= 0 && t < a.V && !again)
-        accept[lane] = exp_call(finite_or_less((float)tr[t]), st.mp, a.k64, s_tab) * st.ip >
+        accept[lane] = exp_call(finite_or_less((float)tr[t]), st.mp, a.k, s_tab) * st.ip >
                        (double)a.u[(int64_t)s * a.N + lane] * fmax(1.0 - before, 0.0);
     }
   }
@@ -309,19 +312,19 @@ __global__ __launch_bounds__(kVT) void round_kernel(VerifyArgs a, VerifyPlan w, 
   if (fabsf(st.mp) == INFINITY || (DRAWN && fabsf(st.mq) == INFINITY)) {
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
-      const double p = exp_call(x[i], st.mp, a.k64, s_tab) * st.ip;
+      const double p = exp_call(x[i], st.mp, a.k, s_tab) * st.ip;
       double q = 0.0;
-      if constexpr (DRAWN) q = exp_call(y[i], st.mq, a.k64, s_tab) * st.iq;
+      if constexpr (DRAWN) q = exp_call(y[i], st.mq, a.k, s_tab) * st.iq;
       sw += fmax(p - st.c * q, 0.0);
       sr += q;
     }
   } else {
-    const double mp = st.mp, mq = st.mq, cq = st.c * st.iq;
+    const double bp = -(double)st.mp * a.k, bq = -(double)st.mq * a.k, cq = st.c * st.iq;
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
-      const double p = exp_of(x[i], mp, a.k64, s_tab);
+      const double p = exp_of(x[i], a.k, bp, s_tab);
       if constexpr (DRAWN) {
-        const double q = exp_of(y[i], mq, a.k64, s_tab);
+        const double q = exp_of(y[i], a.k, bq, s_tab);
         sw += fmax(p * st.ip - cq * q, 0.0);
         if constexpr (MODE == 2) sr += q * st.iq;
       } else {
@@ -339,7 +342,7 @@ __global__ __launch_bounds__(kVT) void round_kernel(VerifyArgs a, VerifyPlan w, 
 
 template <class T>
 __global__ __launch_bounds__(kWalkT) void walk_kernel(VerifyArgs a, VerifyPlan w) {
-  __shared__ double s_tab[64], s_d[kWalkT / 64], s_scan[kWalkT / 64], s_goal;
+  __shared__ double s_tab[256], s_d[kWalkT / 64], s_scan[kWalkT / 64], s_goal;
   __shared__ float s_f[kWalkT / 64];
   __shared__ int s_best[kTreeNodes], s_tok[kTreeNodes], s_cur, s_hit[2];
   const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -442,7 +445,7 @@ __global__ __launch_bounds__(kWalkT) void walk_kernel(VerifyArgs a, VerifyPlan w
   // A leaf, or a residual without mass: the target's own probabilities.
   const bool resid = whole > 0;
   if (!resid) {
-    const double zp = joined<kWalkT>(mx, sm, w.chunks, a.k64, s_tab, s_f, s_d, st.mp);
+    const double zp = joined<kWalkT>(mx, sm, w.chunks, a.k, s_tab, s_f, s_d, st.mp);
     if (!(zp > 0)) {
       if (tid == 0) a.next[s] = -1;
       return;
@@ -450,7 +453,7 @@ __global__ __launch_bounds__(kWalkT) void walk_kernel(VerifyArgs a, VerifyPlan w
     st.ip = 1.0 / zp;
     own = 0.0;
 #pragma unroll 1
-    for (int c = c0; c < c1; ++c) own += sm[c] * exp_call(mx[c], st.mp, a.k64, s_tab) * st.ip;
+    for (int c = c0; c < c1; ++c) own += sm[c] * exp_call(mx[c], st.mp, a.k, s_tab) * st.ip;
     run = scan(own, whole);
   }
   // s_hit[0]: the first chunk past the goal, s_hit[1]: the last with any mass (for a goal that rounding puts at the whole).
@@ -467,7 +470,7 @@ __global__ __launch_bounds__(kWalkT) void walk_kernel(VerifyArgs a, VerifyPlan w
   int first = INT_MAX, last = -1;
 #pragma unroll 1
   for (int c = c0; c < c1; ++c) {
-    const double v = resid ? pw[c] : sm[c] * exp_call(mx[c], st.mp, a.k64, s_tab) * st.ip;
+    const double v = resid ? pw[c] : sm[c] * exp_call(mx[c], st.mp, a.k, s_tab) * st.ip;
     if (v > 0) {
       last = c;
       if (upto + v > goal) first = min(first, c);
@@ -481,7 +484,7 @@ __global__ __launch_bounds__(kWalkT) void walk_kernel(VerifyArgs a, VerifyPlan w
   if (chunk >= c0 && chunk < c1) {   // the thread that holds it: what is left of the goal there
     upto = run;
 #pragma unroll 1
-    for (int c = c0; c < chunk; ++c) upto += resid ? pw[c] : sm[c] * exp_call(mx[c], st.mp, a.k64, s_tab) * st.ip;
+    for (int c = c0; c < chunk; ++c) upto += resid ? pw[c] : sm[c] * exp_call(mx[c], st.mp, a.k, s_tab) * st.ip;
     s_goal = goal - upto;
   }
   if (tid < 2) s_hit[tid] = tid ? -1 : a.V;
@@ -505,8 +508,8 @@ __global__ __launch_bounds__(kWalkT) void walk_kernel(VerifyArgs a, VerifyPlan w
   for (int i = 0; i < 4; ++i) {
     r[i] = 0.0;
     if (i >= ept) break;
-    r[i] = exp_call(x[i], st.mp, a.k64, s_tab) * st.ip;
-    if (resid && a.mode) r[i] = fmax(r[i] - st.c * st.iq * exp_call(y[i], st.mq, a.k64, s_tab), 0.0);
+    r[i] = exp_call(x[i], st.mp, a.k, s_tab) * st.ip;
+    if (resid && a.mode) r[i] = fmax(r[i] - st.c * st.iq * exp_call(y[i], st.mq, a.k, s_tab), 0.0);
     if (here)
       for (int e = 0; e < k; ++e) r[i] = s_tok[e] == v0 + i ? 0.0 : r[i];
     mine += r[i];

@@ -40,17 +40,20 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _node_stride(t, name, shape, dtype, device):
-    """The elements between nodes of a [S][N][heads][d] tensor whose heads are packed and whose nodes
-    are equally spaced: a slice of a wider product's output, or the packed tensor."""
-    s = t.stride()
-    if t.shape != shape or t.dtype is not dtype or t.device != device or s[3] != 1 or \
+def _spaced(t, name, got, s, shape, dtype, device):
+    """The elements between nodes of a [S][N][heads][d] tensor (shape `got`, strides `s`) whose heads are packed and
+    whose nodes are equally spaced: a slice of a wider product's output, or the packed tensor."""
+    if got != shape or t.dtype is not dtype or t.device != device or s[3] != 1 or \
             (s[2] != shape[3] and shape[2] > 1) or (s[0] != shape[1] * s[1] and shape[0] > 1):
         raise ValueError(f"{name} must be a {dtype} tensor {tuple(shape)} on {device} with packed heads and equally spaced "
-                         f"nodes, not {t.dtype} {tuple(t.shape)} on {t.device} with strides {s}")
+                         f"nodes, not {t.dtype} {tuple(got)} on {t.device} with strides {s}")
     if shape[1] > 1:
         return s[1]
     return s[0] if shape[0] > 1 else shape[2] * shape[3]
+
+
+def _node_stride(t, name, shape, dtype, device):
+    return _spaced(t, name, t.shape, t.stride(), shape, dtype, device)
 
 
 class KVCache:
@@ -91,6 +94,7 @@ class CacheSet:
             if (b.shape[0], b.shape[2:], b.dtype, b.device) != (a.shape[0], a.shape[2:], a.dtype, a.device):
                 raise ValueError("the caches of a set must agree in sequences, kv_heads, head_dim, type and device")
         self.c = (KVCacheC * len(self.caches))(*[x.c for x in self.caches])
+        self.pointers = C.c_void_p * len(self.caches)
 
     def __len__(self):
         return len(self.caches)
@@ -155,18 +159,22 @@ def attention_weights_into(ctx: Context, cache: KVCache, q, lse, path, accepted,
     return cache.weights
 
 
-def _layers(t, name, layers, shape, dtype, device):
+def _layers(t, name, caches, shape, dtype, device):
     """(host array of the layers' addresses, node stride) of one tensor [layers][S][N][heads][d] or a list."""
+    layers = len(caches)
+    if torch.is_tensor(t):
+        if t.dim() != 5 or t.shape[0] != layers:
+            raise ValueError(f"{name} must hold {layers} layers, not {tuple(t.shape)}")
+        s = t.stride()
+        stride = _spaced(t, name, t.shape[1:], s[1:], shape, dtype, device)
+        p, step = t.data_ptr(), s[0] * t.element_size()
+        return caches.pointers(*range(p, p + layers * step, step) if step else [p] * layers), stride
     if len(t) != layers:
         raise ValueError(f"{name} must hold {layers} layers, not {len(t)}")
-    if torch.is_tensor(t):
-        stride = _node_stride(t[0], name, shape, dtype, device)
-        p, step = t.data_ptr(), t.stride(0) * t.element_size()
-        return (C.c_void_p * layers)(*range(p, p + layers * step, step) if step else [p] * layers), stride
     strides = {_node_stride(x, name, shape, dtype, device) for x in t}
     if len(strides) != 1:
         raise ValueError(f"{name}: the layers' nodes must be spaced alike")
-    return (C.c_void_p * layers)(*[x.data_ptr() for x in t]), strides.pop()
+    return caches.pointers(*[x.data_ptr() for x in t]), strides.pop()
 
 
 def cache_commit(ctx: Context, caches: CacheSet, draft_k, draft_v, path, accepted):
@@ -177,8 +185,8 @@ def cache_commit(ctx: Context, caches: CacheSet, draft_k, draft_v, path, accepte
     _cuda(ctx, dev)
     _same(path, "path", (S, N), _I32, dev)
     _same(accepted, "accepted", (S,), _I32, dev)
-    kp, ks = _layers(draft_k, "draft_k", L, (S, N, G, D), dtype, dev)
-    vp, vs = _layers(draft_v, "draft_v", L, (S, N, G, D), dtype, dev)
+    kp, ks = _layers(draft_k, "draft_k", caches, (S, N, G, D), dtype, dev)
+    vp, vs = _layers(draft_v, "draft_v", caches, (S, N, G, D), dtype, dev)
     if ks != vs:
         raise ValueError("draft_k and draft_v must be spaced alike")
     d = TreeDescC(S, N, G, G, D, ELEM[dtype], ELEM[dtype], 0, 0, 1.0, 0, ks)
