@@ -106,7 +106,7 @@ __device__ __forceinline__ Span span_of(const TreeArgs &a, int s) {
   p.per = a.per_chunk;
   if ((int64_t)p.per * a.chunks < p.keys) {
     const int need = (int)((uint32_t)p.keys / (uint32_t)a.chunks) + 1;
-    p.per = (int)(((uint32_t)need + a.tile - 1) & ~(uint32_t)(a.tile - 1));
+    p.per = (int)(((uint32_t)need + a.tile - 1) / (uint32_t)a.tile * (uint32_t)a.tile);
   }
   return p;
 }
@@ -607,8 +607,12 @@ __global__ __launch_bounds__(256) void weights_kernel(TreeArgs a) {
   }
 }
 
-// The launch: RT by the rows of a kv head, KS and the ring so that a workgroup's tiles in flight cover the
-// memory's latency and fit LDS.
+// The launch: RT by the rows of a kv head; KS so that a workgroup fills its compute unit's LDS and registers by itself
+// (two waves per SIMD, heads of 256 one) with four tiles, 64 KB or more, in flight or in use. Whole call, 16 nodes of
+// 64 / 8 heads of 64 at 32768 keys (F32, RT 4): KS 2 with a ring of four tiles 31.5 us, of six 33.0, KS 3 (twelve waves) 32.6;
+// before the next tile's scores were formed under the exponentials: two workgroups of KS 2 per unit 36.5, one of KS 4 40.
+// RT 4 is at the matrix unit's and the VALU's time one after the other (16 products of 32 cycles and about 100
+// instructions a tile and wave), smaller RT and heads of 128 at HBM (3 to 3.6 TB/s).
 struct TreeShape { int rt, ks; };
 static TreeShape tree_shape(int d, int rows) {
   const int rt = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
@@ -645,10 +649,10 @@ template <int QT, int D> static hipError_t launch_tree_d(const TreeArgs &a, hipS
   const TreeShape t = tree_shape(D, a.N * (a.qh / a.kvh));
   const int64_t groups = (int64_t)a.S * a.kvh * a.chunks;
   const dim3 grid(8 * a.row_blocks, (uint32_t)((groups + 7) / 8)), block(64 * t.rt * t.ks);
-  constexpr int K4 = D == 64 ? 2 : D == 128 ? 2 : 1, K2 = D == 64 ? 4 : K4, NST = 4;
+  constexpr int K4 = D == 256 ? 1 : 2, K2 = D == 64 ? 4 : K4, NST = 4;
   if (t.rt == 1) hipLaunchKernelGGL((tree_split_kernel<QT, D, 1, K2, NST, 1>), grid, block, 0, s, a);
   else if (t.rt == 2) hipLaunchKernelGGL((tree_split_kernel<QT, D, 2, K2, NST, D == 64 ? 2 : 1>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((tree_split_kernel<QT, D, 4, K4, D == 64 ? 6 : NST, D == 256 ? 1 : 2>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((tree_split_kernel<QT, D, 4, K4, NST, D == 256 ? 1 : 2>), grid, block, 0, s, a);
   if (a.chunks > 1) {
     const int64_t rows = (int64_t)a.S * a.N * a.qh;
     hipLaunchKernelGGL((tree_merge_kernel<QT, D>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, s, a);
