@@ -64,7 +64,7 @@ int check_tree(const hh_tree_desc *d) {
   if (!((d->type == HH_F32 && d->cache_type == HH_F16) || (d->type != HH_F32 && d->type == d->cache_type)))
     return fail(HH_EINVAL, "types must be F32 over F16, F16 over F16 or BF16 over BF16");
   if (d->window < 0 || d->max_length < 0) return fail(HH_EINVAL, "window and max_length must be >= 0");
-  if (!std::isfinite(d->sm_scale)) return fail(HH_EINVAL, "sm_scale must be finite");
+  if (!std::isfinite(d->sm_scale) || d->sm_scale == 0.f) return fail(HH_EINVAL, "sm_scale must be finite and not 0");
   const int64_t row = (int64_t)d->q_heads * d->head_dim;
   if (d->q_stride && d->q_stride < row) return fail(HH_ESHAPE, "q_stride is smaller than a node's heads");
   if (d->q_stride % (d->type == HH_F32 ? 4 : 8)) return fail(HH_EALIGN, "q_stride must be a multiple of 16 bytes");
@@ -116,6 +116,8 @@ hh::TreeArgs tree_args(const hh_tree_desc *d, const hh_kv_cache *c, const void *
 int check_layers(const hh_tree_desc *d, const hh_kv_cache *caches, int32_t count) {
   if (count < 1 || count > kMaxLayers) return fail(HH_EINVAL, "count outside 1..256");
   if (!caches) return fail(HH_EINVAL, "caches is NULL");
+  if ((int64_t)(count < hh::kRowsLayers ? count : hh::kRowsLayers) * d->sequences * d->kv_heads > 1 << 21)
+    return fail(HH_EINVAL, "more than 2^21 heads a launch: split the batch");
   for (int i = 0; i < count; ++i) {
     if (int rc = check_cache(d, caches + i)) return rc;
     for (int j = 0; j < i; ++j) {
@@ -165,7 +167,7 @@ int check_verify(const hh_verify_desc *d) {
   if (d->type < HH_F32 || d->type > HH_BF16) return fail(HH_EINVAL, "unknown type");
   if (d->draft < HH_DRAFT_GIVEN || d->draft > HH_DRAFT_DISTINCT) return fail(HH_EINVAL, "unknown draft mode");
   if (d->max_children < 0 || d->max_children >= HH_TREE_MAX_NODES) return fail(HH_EINVAL, "max_children outside 0..63");
-  if (!hh::verify_fits(d->sequences, d->nodes, d->vocab)) return fail(HH_EINVAL, "more than 2^23 chunks of logits: split the batch");
+  if (!hh::verify_fits(d->sequences, d->nodes, d->vocab)) return fail(HH_EINVAL, "more than 2^22 chunks of logits: split the batch");
   if (!(d->temperature >= 0.f) || !std::isfinite(d->temperature)) return fail(HH_EINVAL, "temperature must be finite and >= 0");
   if (d->temperature != 0.f && d->temperature < 1e-6f)
     return fail(HH_EINVAL, "temperature below 1e-6: 0 is greedy");

@@ -17,7 +17,7 @@
 // Bound by the launches' dependent chain for a few rows, and by the exponentials in 64 bits for many: the next token
 // is where a sum of up to V terms passes a random bound, and with errors of 1e-7 in it one in twenty draws from
 // the tail of 250000 tokens would differ. exp goes by a table of 2^(i / 256) and four terms of a series behind the 1 (relative
-// error below 1e-15 beside the argument's), twelve instructions in fp64.
+// error below 1e-15 beside the argument's), thirteen instructions in fp64.
 #include <climits>
 
 #include "hh_common.hpp"
@@ -30,12 +30,13 @@ constexpr int kWalkT = 1024;
 
 __device__ __forceinline__ float finite_or_less(float x) { return x != x ? -INFINITY : x; }
 
-// exp((x − top) / temperature) = 2^(y / 256), y = x·k + b, with tab[i] = 2^(i / 256) in LDS, k = 256 log2(e) / temperature and
-// b = −top·k: the rounding of b is one factor of a row's every term. y is split by adding 1.5·2^52, whose low word is
-// then the nearest integer, and the power of two goes into the exponent's bits. Below 2^−1000: 0.
-__device__ __forceinline__ double exp_of(float x, double k, double b, const double *tab) {
+// exp((x − top) / temperature) = 2^(y / 256), y = (x − top)·k <= 0, with tab[i] = 2^(i / 256) in LDS and k = 256 log2(e) /
+// temperature. (The difference first: x·k − top·k is wrong for rows of a type's lowest value.) y is split by adding
+// 1.5·2^52, whose low word is then the nearest integer, and the power of two goes into the exponent's bits. Below
+// 2^−1000: 0.
+__device__ __forceinline__ double exp_of(float x, double top, double k, const double *tab) {
   constexpr double magic = 6755399441055744.0, c = 0.0027076061740622863;   // ln 2 / 256
-  const double y = fmax(fma((double)x, k, b), -256.0 * 1001), m = y + magic, f = y - (m - magic);
+  const double y = fmax(((double)x - top) * k, -256.0 * 1001), m = y + magic, f = y - (m - magic);
   const int i = (int)(uint32_t)__builtin_bit_cast(uint64_t, m);
   double s = fma(f, c * c * c * c / 24, c * c * c / 6);
   s = fma(f, s, c * c / 2);
@@ -48,7 +49,7 @@ __device__ __forceinline__ double exp_of(float x, double k, double b, const doub
 // The same for a row whose largest entry is infinite: its +inf entries share the probability, a row of −inf has none.
 __device__ __forceinline__ double exp_any(float x, float top, double k, const double *tab) {
   if (fabsf(top) == INFINITY) return top > 0.f && x == top ? 1.0 : 0.0;
-  return exp_of(x, k, -(double)top * k, tab);
+  return exp_of(x, top, k, tab);
 }
 // exp_any as a call: where each of a kernel's few uses is run once, its instructions are fetched once (a cold
 // 64-byte line of instructions costs about 0.1 us).
@@ -184,9 +185,9 @@ __global__ __launch_bounds__(kVT) void stats_kernel(VerifyArgs a, VerifyPlan w) 
 #pragma unroll
     for (int i = 0; i < EPT; ++i) sum += one && x[i] == all ? 1.0 : 0.0;
   } else {
-    const double b = -(double)all * a.k;
+    const double top64 = all;
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) sum += exp_of(x[i], a.k, b, s_tab);   // −inf: 0
+    for (int i = 0; i < EPT; ++i) sum += exp_of(x[i], top64, a.k, s_tab);   // −inf: 0
   }
   sum = block_sum<kVT>(sum, s_d);
   if (tid == 0) {
@@ -319,12 +320,12 @@ __global__ __launch_bounds__(kVT) void round_kernel(VerifyArgs a, VerifyPlan w, 
       sr += q;
     }
   } else {
-    const double bp = -(double)st.mp * a.k, bq = -(double)st.mq * a.k, cq = st.c * st.iq;
+    const double mp = st.mp, mq = st.mq, cq = st.c * st.iq;
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
-      const double p = exp_of(x[i], a.k, bp, s_tab);
+      const double p = exp_of(x[i], mp, a.k, s_tab);
       if constexpr (DRAWN) {
-        const double q = exp_of(y[i], a.k, bq, s_tab);
+        const double q = exp_of(y[i], mq, a.k, s_tab);
         sw += fmax(p * st.ip - cq * q, 0.0);
         if constexpr (MODE == 2) sr += q * st.iq;
       } else {
@@ -532,7 +533,7 @@ __global__ __launch_bounds__(kWalkT) void walk_kernel(VerifyArgs a, VerifyPlan w
 
 bool verify_fits(int S, int N, int V) {
   const VerifyPlan p = verify_plan(S, N, V);
-  return (size_t)S * N * p.chunks <= (size_t)1 << 23;
+  return (size_t)S * N * p.chunks <= (size_t)1 << 22;
 }
 
 size_t verify_workspace(int S, int N, int V) { return verify_plan(S, N, V).total; }

@@ -397,8 +397,8 @@ int hh_combine(hh_ctx *ctx, const float *slots, const float *weights, int32_t to
  *
  * A tree: parents int32 [S][N], parents[s][i] in 0..i−1, or −1 for a node without one (any other
  * value counts as −1); node 0 is the pending token, the last one that was sampled. node_counts
- * int32 [S] (0..N): nodes from the count on are padding; what belongs to them is neither read nor
- * written, unless stated. Lengths, counts, paths and random numbers are device memory, so that
+ * int32 [S] (0..N): nodes from the count on are padding; what belongs to them has no part in any
+ * result and is not written, unless stated. Lengths, counts, paths and random numbers are device memory, so that
  * every call may be recorded in a graph and replayed; what the host cannot check there is bounded
  * by the kernels (an index out of range is skipped).                                         */
 typedef enum { HH_F32 = 0, HH_F16 = 1, HH_BF16 = 2 } hh_elem;
@@ -414,7 +414,7 @@ typedef struct hh_tree_desc {
   int32_t window;                         /* 0, or a node at position p sees positions > p − window */
   int32_t max_length;                     /* longest expected history, 0 = the cache's rows: it
                                              sizes the launch; every length is handled          */
-  float   sm_scale;
+  float   sm_scale;                       /* finite, not 0; F32: |q·sm_scale| below 4·10^4       */
   int64_t q_stride, kv_stride;            /* elements between nodes of q, and of the drafted k and
                                              v; 0 = packed. Multiples of 16 bytes               */
 } hh_tree_desc;
@@ -460,8 +460,9 @@ typedef struct hh_verify_desc {
   int32_t sequences, nodes, vocab;        /* S >= 1, N = 1..64, V = 1..2^24                     */
   int32_t type;                           /* hh_elem of the logits                              */
   int32_t draft;                          /* hh_draft_mode                                      */
-  int32_t max_children;                   /* a node's children beyond this many are not tried; 0 = N − 1 */
-  float   temperature;                    /* of both distributions; 0: greedy                   */
+  int32_t max_children;                   /* a node's children beyond this many are not tried; 0 = N − 1.
+                                             Drawn tokens take a launch for each: pass the tree's own */
+  float   temperature;                    /* of both distributions, 1e-6 or more; 0: greedy     */
   int64_t target_stride, draft_stride;    /* elements between nodes' logits; 0 = packed         */
 } hh_verify_desc;
 
@@ -503,8 +504,8 @@ int hh_cache_commit(hh_ctx *ctx, const hh_tree_desc *desc, const hh_kv_cache *ca
 /* The accepted nodes' attention added to the weight of each key of one layer, after hh_cache_commit:
  * weights[s][g][r] += Σ over i < accepted[s] and the heads h of group g of
  * exp(sm_scale·q[s][path[s][i]][h]·k[s][r][g] − lse[s][path[s][i]][h]), r up to the node's own row
- * lengths[s] − accepted[s] + i. q and lse are hh_attention_tree's of this layer. Not for rings or
- * windows. Each weight is summed by one wave in a fixed order.                                */
+ * lengths[s] − accepted[s] + i (all of them must have found room in the commit). q and lse are
+ * hh_attention_tree's of this layer. Not for rings or windows. Each weight is summed by one wave in a fixed order.                                */
 int hh_attention_weights(hh_ctx *ctx, const hh_tree_desc *desc, const hh_kv_cache *cache, const void *q,
                          const float *lse, const int32_t *path, const int32_t *accepted);
 

@@ -194,6 +194,10 @@ def test_odd_rows_and_tokens(mode):
                 D[4, :, :700] = -inf                         # no token in common
                 D[10] = T[10]
                 D[11, 0] = nan
+            T[8, 0] = torch.finfo(torch.float32).min    # rows masked by the lowest value: all of it, and but for two
+            T[8, 1:] = torch.finfo(torch.float32).min
+            T[8, 1:, [77, 901]] = torch.tensor([1.0, 2.0])
+            T[5, 3:] *= 1e30                                # far apart
             t["u"][10] = 1 - 2.0 ** -24
             t["uf"][0], t["uf"][1] = 0.0, 1 - 2.0 ** -24
             check(t, mode, call(torch, ctx, t, mode))
@@ -292,6 +296,7 @@ def _call(desc=None, **kw):
     (dict(desc=dict(type=3)), -1), (dict(desc=dict(draft=3)), -1), (dict(desc=dict(max_children=64)), -1),
     (dict(desc=dict(max_children=-1)), -1), (dict(desc=dict(temperature=-1.0)), -1), (dict(desc=dict(temperature=float("inf"))), -1),
     (dict(desc=dict(temperature=float("nan"))), -1), (dict(desc=dict(temperature=1e-9)), -1), (dict(desc=dict(target_stride=99)), -6),
+    (dict(desc=dict(sequences=4096, nodes=64, vocab=1 << 24)), -1),
     (dict(desc=dict(draft_stride=99)), -6), (dict(target=None), -1), (dict(draft=None), -1), (dict(tokens=None), -1), (dict(parents=None), -1),
     (dict(counts=None), -1), (dict(u=None), -1), (dict(uf=None), -1), (dict(path=None), -1), (dict(accepted=None), -1), (dict(nxt=None), -1),
 ])

@@ -161,7 +161,12 @@ def test_padding_odd_parents_and_lengths_out_of_range():
         # The launch is sized for shorter histories than there are, and without lse.
         out2, _ = call(torch, ctx, t, max_length=10, lse=False)
         check(torch, t, "f32", out2, None)
-        # Another scale.
+        # Another scale, and a negative one.
+        outn, lsen = call(torch, ctx, t, scale=-0.2)
+        check(torch, t, "f32", outn, lsen, scale=-0.2)
+        b = make(torch, 2, 5, 8, 2, 64, "bf16", 100, [90, 3], seed=6)
+        outb, lseb = call(torch, ctx, b, scale=-0.2)
+        check(torch, b, "bf16", outb, lseb, scale=-0.2)
         out3, lse3 = call(torch, ctx, t, scale=0.5)
         check(torch, t, "f32", out3, lse3, scale=0.5)
     finally:
@@ -408,7 +413,8 @@ def _call(fn="hh_attention_tree", desc=None, cache=None, **kw):
     (dict(desc=dict(head_dim=96)), -6), (dict(desc=dict(q_heads=7)), -6), (dict(desc=dict(q_heads=34)), -6),
     (dict(desc=dict(kv_heads=0)), -6), (dict(desc=dict(type=1, cache_type=2)), -1), (dict(desc=dict(type=0, cache_type=2)), -1),
     (dict(desc=dict(cache_type=0)), -1), (dict(desc=dict(type=3)), -1), (dict(desc=dict(window=-1)), -1),
-    (dict(desc=dict(max_length=-1)), -1), (dict(desc=dict(sm_scale=float("nan"))), -1), (dict(desc=dict(q_stride=100)), -6),
+    (dict(desc=dict(max_length=-1)), -1), (dict(desc=dict(sm_scale=float("nan"))), -1), (dict(desc=dict(sm_scale=0.0)), -1),
+    (dict(desc=dict(sequences=4096, kv_heads=128, q_heads=128)), -1), (dict(cache=dict(rows=(1 << 30) + 1)), -1), (dict(desc=dict(q_stride=100)), -6),
     (dict(desc=dict(q_stride=514)), -2), (dict(desc=dict(kv_stride=64)), -6), (dict(desc=dict(kv_stride=132)), -2),
     (dict(cache=dict(k=None)), -1), (dict(cache=dict(v=8200)), -2), (dict(cache=dict(rows=0)), -1),
     (dict(cache=dict(sequence_stride=100)), -6), (dict(cache=dict(sequence_stride=2052)), -2), (dict(cache=dict(lengths=None)), -1),
