@@ -40,6 +40,14 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _step(name, s, shape, row):
+    """The elements between nodes of [S][N] nodes of `row` elements, which may not overlap (0 is the C entries' packed)."""
+    step = s[1] if shape[1] > 1 else s[0] if shape[0] > 1 else row
+    if step < row:
+        raise ValueError(f"{name}: nodes {step} elements apart overlap")
+    return step
+
+
 def _spaced(t, name, got, s, shape, dtype, device):
     """The elements between nodes of a [S][N][heads][d] tensor (shape `got`, strides `s`) whose heads are packed and
     whose nodes are equally spaced: a slice of a wider product's output, or the packed tensor."""
@@ -47,9 +55,7 @@ def _spaced(t, name, got, s, shape, dtype, device):
             (s[2] != shape[3] and shape[2] > 1) or (s[0] != shape[1] * s[1] and shape[0] > 1):
         raise ValueError(f"{name} must be a {dtype} tensor {tuple(shape)} on {device} with packed heads and equally spaced "
                          f"nodes, not {t.dtype} {tuple(got)} on {t.device} with strides {s}")
-    if shape[1] > 1:
-        return s[1]
-    return s[0] if shape[0] > 1 else shape[2] * shape[3]
+    return _step(name, s, shape, shape[2] * shape[3])
 
 
 def _node_stride(t, name, shape, dtype, device):
@@ -68,6 +74,8 @@ class KVCache:
         if k.dtype not in (torch.float16, torch.bfloat16) or v.dtype is not k.dtype or v.shape != k.shape or \
                 v.device != dev or v.stride() != k.stride() or k.stride()[1:] != (heads * d, d, 1):
             raise ValueError("k and v must be alike, fp16 or bf16 [S][rows][kv_heads][d] with a sequence's rows packed")
+        if S > 1 and k.stride(0) < rows * heads * d:
+            raise ValueError("the sequences' histories overlap")
         _same(lengths, "lengths", (S,), _I32, dev)
         if weights is not None:
             _same(weights, "weights", (S, heads, rows), _F32, dev)
@@ -209,9 +217,7 @@ def _row_stride(t, name, shape, dtype, device):
             (s[0] != shape[1] * s[1] and shape[0] > 1 and shape[1] > 1):
         raise ValueError(f"{name} must be a {dtype} tensor {tuple(shape)} on {device} with equally spaced rows, not "
                          f"{t.dtype} {tuple(t.shape)} on {t.device} with strides {s}")
-    if shape[1] > 1:
-        return s[1]
-    return s[0] if shape[0] > 1 else shape[2]
+    return _step(name, s, shape, shape[2])
 
 
 def draft_verify_into(ctx: Context, target, tokens, parents, node_counts, uniforms, final_uniforms, path, accepted,

@@ -454,3 +454,26 @@ def test_python_refuses_tensors_that_do_not_fit():
         device, handle = 0, None
     with pytest.raises(ValueError):        # another device than the context's
         sp.attention_tree_into(Ctx, sp.KVCache(k, k.clone(), lengths), torch.zeros((2, 3, 4, 64)), None, None, None, None, None)
+
+
+def test_python_refuses_expanded_tensors():
+    """A step of 0 between nodes or sequences would be taken for the packed one, and memory behind the tensor read."""
+    import torch
+    from hydra_amd import speculative as sp
+    f16 = torch.float16
+    for shape, base in (((2, 3, 4, 64), (1, 1, 4, 64)), ((2, 1, 4, 64), (1, 1, 4, 64)), ((1, 3, 4, 64), (1, 1, 4, 64))):
+        t = torch.zeros(base, dtype=f16).expand(shape)
+        with pytest.raises(ValueError):
+            sp._node_stride(t, "q", shape, f16, t.device)
+        row = torch.zeros((1, 1, 64)).expand(shape[:2] + (64,))
+        with pytest.raises(ValueError):
+            sp._row_stride(row, "target", row.shape, row.dtype, row.device)
+    one = torch.zeros((1, 1, 4, 64), dtype=f16)
+    assert sp._node_stride(one, "q", one.shape, f16, one.device) == 256
+    wide = torch.zeros((2, 3, 12, 64), dtype=f16)[:, :, 4:8]
+    assert sp._node_stride(wide, "q", wide.shape, f16, wide.device) == 768
+    k = torch.zeros((1, 8, 2, 64), dtype=f16)
+    lengths = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        sp.KVCache(k.expand(2, 8, 2, 64), k.expand(2, 8, 2, 64), lengths)
+    sp.KVCache(k, k.clone(), lengths[:1])
