@@ -120,9 +120,16 @@ int check_layers(const hh_tree_desc *d, const hh_kv_cache *caches, int32_t count
     return fail(HH_EINVAL, "more than 2^21 heads a launch: split the batch");
   for (int i = 0; i < count; ++i) {
     if (int rc = check_cache(d, caches + i)) return rc;
-    for (int j = 0; j < i; ++j) {
-      const hh_kv_cache &x = caches[i], &y = caches[j];
+    const hh_kv_cache &x = caches[i];
+    if (x.k == x.v) return fail(HH_EINVAL, "k and v are the same memory");
+    for (int j = 0; j <= i; ++j) {
+      const hh_kv_cache &y = caches[j];
+      if (x.next_position == y.lengths || y.next_position == x.lengths)   // lengths are never NULL
+        return fail(HH_EINVAL, "lengths and next_position are the same memory");
+      if (j == i) break;
       if (x.k == y.k || x.v == y.v || x.k == y.v || x.v == y.k) return fail(HH_EINVAL, "two layers share a cache");
+      if ((x.weights && x.weights == y.weights) || (x.positions && x.positions == y.positions))
+        return fail(HH_EINVAL, "two layers share weights or positions");
       if (x.next_position && y.next_position && (x.lengths == y.lengths) != (x.next_position == y.next_position))
         return fail(HH_EINVAL, "caches share both lengths and next_position, or neither");
     }

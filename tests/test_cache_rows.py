@@ -265,18 +265,18 @@ def _call(fn, desc=None, caches=None, count=2, **kw):
     d = dict(sequences=1, nodes=4, q_heads=8, kv_heads=2, head_dim=64, type=1, cache_type=1, window=0, max_length=0, sm_scale=0.1,
              q_stride=0, kv_stride=0)
     d.update(desc or {})
-    base = dict(sequence_stride=0, rows=16, ring=0, lengths=64, weights=64, positions=64, next_position=128)
-    both = [dict(base, k=4096, v=8192), dict(base, k=16384, v=32768)]
+    base = dict(sequence_stride=0, rows=16, ring=0, lengths=64, next_position=128)
+    layers = [dict(base, k=4096 << 2 * i, v=8192 << 2 * i, weights=1024 + 16 * i, positions=2048 + 16 * i) for i in range(9)]
     for i, c in (caches or {}).items():
-        both[i].update(c)
-    arr = (_lib.KVCacheC * 2)(*[_lib.KVCacheC(**c) for c in both])
+        layers[i].update(c)
+    arr = (_lib.KVCacheC * 9)(*[_lib.KVCacheC(**c) for c in layers])
     ctx = C.create_string_buffer(4096)      # zeros: never used, the checks come first
     dc = _lib.TreeDescC(**d)
     if fn == "evict":
         a = dict(keep=8, recent=2)
         a.update(kw)
         return L.hh_cache_evict(ctx, C.byref(dc), arr, count, a["keep"], a["recent"])
-    p = (C.c_void_p * 2)(kw.get("dk", 16), 16)
+    p = (C.c_void_p * 9)(kw.get("dk", 16), *[16] * 8)
     return L.hh_cache_commit(ctx, C.byref(dc), arr, count, p, kw.get("dv", p), kw.get("path", 16), 16)
 
 
@@ -286,6 +286,8 @@ def _call(fn, desc=None, caches=None, count=2, **kw):
     (dict(caches={0: dict(positions=None, next_position=None)}), -1), (dict(caches={1: dict(next_position=None)}), -1),
     (dict(caches={1: dict(next_position=256)}), -1), (dict(caches={1: dict(lengths=256)}), -1), (dict(caches={1: dict(k=4096)}), -1),
     (dict(caches={1: dict(rows=4)}), -1), (dict(desc=dict(head_dim=32)), -6), (dict(desc=dict(sequences=0)), -1),
+    (dict(caches={1: dict(weights=1024)}), -1), (dict(caches={1: dict(positions=2048)}), -1),
+    (dict(desc=dict(sequences=4096, kv_heads=64), count=9), -1),
 ])
 def test_evict_refusals(kw, code):
     assert _call("evict", **kw) == code
@@ -294,7 +296,9 @@ def test_evict_refusals(kw, code):
 @pytest.mark.parametrize("kw,code", [
     (dict(desc=dict(nodes=0)), -1), (dict(desc=dict(cache_type=0)), -1), (dict(desc=dict(kv_stride=64)), -6), (dict(dk=None), -1),
     (dict(dk=8), -2), (dict(dv=None), -1), (dict(path=None), -1), (dict(caches={0: dict(v=8194)}), -2), (dict(caches={1: dict(v=4096)}), -1),
-    (dict(count=0), -1),
+    (dict(count=0), -1), (dict(caches={0: dict(v=4096)}), -1), (dict(caches={0: dict(next_position=64)}), -1),
+    (dict(caches={1: dict(lengths=128, next_position=256)}), -1), (dict(caches={1: dict(lengths=256, next_position=64)}), -1),
+    (dict(caches={1: dict(lengths=128, weights=None, positions=None, next_position=None)}), -1),
 ])
 def test_commit_refusals(kw, code):
     assert _call("commit", **kw) == code
