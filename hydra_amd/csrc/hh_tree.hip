@@ -609,8 +609,8 @@ __global__ __launch_bounds__(256) void weights_kernel(TreeArgs a) {
 
 // The launch: RT by the rows of a kv head; KS so that a workgroup fills its compute unit's LDS and registers by itself
 // (two waves per SIMD, heads of 256 one) with four tiles, 64 KB or more, in flight or in use. Whole call, 16 nodes of
-// 64 / 8 heads of 64 at 32768 keys (F32, RT 4): KS 2 with a ring of four tiles 31.5 us, of six 33.0, KS 3 (twelve waves) 32.6;
-// before the next tile's scores were formed under the exponentials: two workgroups of KS 2 per unit 36.5, one of KS 4 40.
+// 64 / 8 heads of 64 at 32768 keys (F32, RT 4): KS 2 with a ring of four tiles 31.6 us, of six 32.9, KS 3 (twelve waves) 31.3;
+// before the next tile's scores were formed under the exponentials: two workgroups of KS 2 per unit 36.5, one of KS 4 41.
 // RT 4 is at the matrix unit's and the VALU's time one after the other (16 products of 32 cycles and about 100
 // instructions a tile and wave), smaller RT and heads of 128 at HBM (3 to 3.6 TB/s).
 struct TreeShape { int rt, ks; };
