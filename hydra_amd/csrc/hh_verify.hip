@@ -135,16 +135,20 @@ __host__ __device__ inline VerifyPlan verify_plan(int S, int N, int V) {
   return p;
 }
 
-// The children of node n as a mask, the first `most`; every lane of the wave takes part.
-__device__ __forceinline__ uint64_t children_of(const VerifyArgs &a, int s, int n, int count, int most) {
+// The children of node n as a mask, the first `most`, from every node's parent in its lane of the wave.
+__device__ __forceinline__ uint64_t children_in(int parent, int n, int count, int most) {
   const int lane = threadIdx.x & 63;
-  uint64_t m = __ballot(lane > n && lane < count && a.parents[(int64_t)s * a.N + min(lane, a.N - 1)] == n);
+  uint64_t m = __ballot(lane > n && lane < count && parent == n);
   if (__popcll(m) > most) {
     uint64_t left = m;
     for (int i = 0; i < most; ++i) left &= left - 1;
     m &= ~left;
   }
   return m;
+}
+
+__device__ __forceinline__ uint64_t children_of(const VerifyArgs &a, int s, int n, int count, int most) {
+  return children_in(a.parents[(int64_t)s * a.N + min((int)threadIdx.x & 63, a.N - 1)], n, count, most);
 }
 
 template <class T, int EPT, bool GREEDY>
@@ -221,9 +225,20 @@ __global__ __launch_bounds__(kVT) void round_kernel(VerifyArgs a, VerifyPlan w, 
   const int lane = tid & 63;
   const int count = min(max(a.counts[s], 0), a.N);
   if (n >= count) return;
-  const uint64_t kids = children_of(a, s, n, count, a.children);
+  const int parent = a.parents[(int64_t)s * a.N + min(lane, a.N - 1)];
+  const uint64_t kids = children_in(parent, n, count, a.children);
   const int k = __popcll(kids);
   if (k < round) return;
+  if (DRAWN && round > 1) {
+    // Rows that no path ends at any more: with a child accepted, or rejected themselves, or with a sibling accepted.
+    const uint64_t taken = __ballot(lane < count && ((const int32_t *)(a.ws + w.accept))[(int64_t)s * a.N + min(lane, a.N - 1)]);
+    if (kids & taken) return;
+    if (n > 0) {
+      const uint64_t sib = children_in(parent, __shfl(parent, n), count, a.children), me = 1ull << n;
+      const bool told = __popcll(sib & (me - 1)) < round - 1;
+      if (!(sib & me) || (sib & taken & ~me) || (told && !(taken & me))) return;
+    }
+  }
   const int tried = DRAWN ? round : k;       // given tokens: what is left when all are rejected
   const T *tr = (const T *)a.target + (int64_t)row * a.t_stride;
   const T *dr = (const T *)a.draft + (int64_t)row * a.d_stride;
