@@ -66,6 +66,7 @@ struct VerifyArgs {
   const float *u, *u_final;
   int32_t *path, *accepted, *next;
   int S, N, V, type, mode, children;
+  bool late_leaves;                 // the statistics of leaves after the rounds
   double inv_t, k;                  // 1 / temperature (0: greedy), 256 log2(e) / temperature
   uint8_t *ws;
 };
@@ -76,7 +77,7 @@ void tree_plan(TreeArgs &a, int64_t length);
 size_t tree_workspace(const TreeArgs &a);
 hipError_t launch_tree(const TreeArgs &a, int type, hipStream_t s);
 hipError_t launch_weights(TreeArgs a, int type, hipStream_t s);
-hipError_t launch_verify(const VerifyArgs &a, hipStream_t s, int *launches);
+hipError_t launch_verify(VerifyArgs a, hipStream_t s, int *launches);
 hipError_t launch_commit(const RowsArgs &a, bool last, hipStream_t s);
 hipError_t launch_evict(const RowsArgs &a, hipStream_t s);
 

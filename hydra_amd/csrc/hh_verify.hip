@@ -10,8 +10,9 @@
 //
 // A row of logits is cut into chunks, a workgroup each, so that one sequence's rows fill the chip:
 //   stats    every row's maximum and sum of exponentials by chunk (greedy: its largest entry);
-//   round j  of the nodes with at least j children: the j-th child's test, then W_j and R_j by chunk (given
-//            tokens: all tests and the last residual in one round);
+//   round j  of the nodes with at least j children that a path may still end at: the j-th child's test, then W_j and
+//            R_j by chunk (given tokens: all tests and the last residual in one round);
+//   leaf     (where leaves' logits are many) the statistics of the leaf that a path ends at;
 //   walk     a workgroup per sequence follows the accepted children and finds the next token: its chunk by the
 //            chunks' sums, its place by a scan of that chunk.
 // Bound by the launches' dependent chain for a few rows, and by the exponentials in 64 bits for many: the next token
@@ -27,6 +28,9 @@ namespace hh {
 
 constexpr int kVT = 256;              // threads of stats and rounds
 constexpr int kWalkT = 1024;
+// Leaves' statistics are left for behind the rounds, when one a sequence is left, from this many bytes of logits on: trees of 21
+// nodes, four children a node: 83 MB 72 us with, 85 without; 42 MB 68 and 57 (a launch more, and fewer workgroups).
+constexpr size_t kLateLeaves = (size_t)64 << 20;
 
 __device__ __forceinline__ float finite_or_less(float x) { return x != x ? -INFINITY : x; }
 
@@ -151,6 +155,39 @@ __device__ __forceinline__ uint64_t children_of(const VerifyArgs &a, int s, int 
   return children_in(a.parents[(int64_t)s * a.N + min((int)threadIdx.x & 63, a.N - 1)], n, count, most);
 }
 
+// The node that a path ends at, in every lane of the wave: yes, up: a node accepted at its parent, in its lane. len: nodes of
+// the path; place: the path's entry of this lane.
+__device__ __forceinline__ int path_end(bool yes, int up, int count, int &len, int &place) {
+  const int lane = threadIdx.x & 63;
+  int cur = 0;
+  len = count > 0 ? 1 : 0, place = lane == 0 && len ? 0 : -1;
+  if (count > 0)
+    for (;;) {   // a child comes behind its parent: at most N steps
+      const uint64_t m = __ballot(yes && up == cur);
+      if (!m) break;
+      cur = __ffsll((unsigned long long)m) - 1;
+      if (lane == len) place = cur;
+      ++len;
+    }
+  return cur;
+}
+
+// Sum of a chunk's exponentials below its largest entry, in every thread of the workgroup.
+template <int EPT>
+__device__ __forceinline__ double chunk_sum(const float (&x)[EPT], float all, double k, const double *tab, double *s_d) {
+  double sum = 0.0;
+  if (fabsf(all) == INFINITY) {
+    const bool one = all > 0.f;
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) sum += one && x[i] == all ? 1.0 : 0.0;
+  } else {
+    const double top = all;
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) sum += exp_of(x[i], top, k, tab);   // −inf: 0
+  }
+  return block_sum<kVT>(sum, s_d);
+}
+
 template <class T, int EPT, bool GREEDY>
 __global__ __launch_bounds__(kVT) void stats_kernel(VerifyArgs a, VerifyPlan w) {
   __shared__ double s_tab[256], s_d[kVT / 64];
@@ -159,7 +196,9 @@ __global__ __launch_bounds__(kVT) void stats_kernel(VerifyArgs a, VerifyPlan w) 
   const int chunk = blockIdx.x % w.chunks, row = blockIdx.x / w.chunks, s = row / a.N, n = row - s * a.N, tid = threadIdx.x;
   const int count = min(max(a.counts[s], 0), a.N), of = blockIdx.y;
   if (n >= count) return;
-  if (of && children_of(a, s, n, count, a.children) == 0) return;   // the draft's row of a node that has no children
+  if (!GREEDY && !of && chunk == 0 && tid == 0) ((int32_t *)(a.ws + w.accept))[row] = 0;
+  // The draft's row of a node that has no children is not used; of the target's one of a sequence's at most.
+  if ((of || (!GREEDY && a.late_leaves)) && children_of(a, s, n, count, a.children) == 0) return;
   if (!GREEDY) fill_table(s_tab);
   const T *base = (const T *)(of ? a.draft : a.target) + (int64_t)row * (of ? a.d_stride : a.t_stride);
   float x[EPT];
@@ -184,21 +223,38 @@ __global__ __launch_bounds__(kVT) void stats_kernel(VerifyArgs a, VerifyPlan w) 
     }
     return;
   }
-  double sum = 0.0;
-  if (fabsf(all) == INFINITY) {
-    const bool one = all > 0.f;
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) sum += one && x[i] == all ? 1.0 : 0.0;
-  } else {
-    const double top64 = all;
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) sum += exp_of(x[i], top64, a.k, s_tab);   // −inf: 0
-  }
-  sum = block_sum<kVT>(sum, s_d);
+  const double sum = chunk_sum<EPT>(x, all, a.k, s_tab, s_d);
   if (tid == 0) {
     ((float *)(a.ws + w.max_of[of]))[at] = all;
     ((double *)(a.ws + w.sum_of[of]))[at] = sum;
-    if (!of && chunk == 0) ((int32_t *)(a.ws + w.accept))[row] = 0;
+  }
+}
+
+// With late_leaves: the statistics of the one leaf that a sequence's path ends at, if it ends at one.
+template <class T, int EPT>
+__global__ __launch_bounds__(kVT) void leaf_kernel(VerifyArgs a, VerifyPlan w) {
+  __shared__ double s_tab[256], s_d[kVT / 64];
+  __shared__ float s_f[kVT / 64];
+  const int chunk = blockIdx.x % w.chunks, s = blockIdx.x / w.chunks, tid = threadIdx.x, lane = tid & 63;
+  const int count = min(max(a.counts[s], 0), a.N);
+  if (count == 0) return;
+  const int64_t node = (int64_t)s * a.N + min(lane, a.N - 1);
+  const int up = a.parents[node], took = ((const int32_t *)(a.ws + w.accept))[node];
+  int len, place;
+  const int n = path_end(lane < count && up >= 0 && up < lane && took, up, count, len, place);
+  if (children_in(up, n, count, a.children)) return;
+  fill_table(s_tab);
+  const int64_t row = (int64_t)s * a.N + n;
+  float x[EPT];
+  load_chunk<T, EPT>((const T *)a.target + row * a.t_stride, chunk * w.chunk, a.V, x);
+  float top = x[0];
+#pragma unroll
+  for (int i = 1; i < EPT; ++i) top = fmaxf(top, x[i]);
+  const float all = block_max<kVT>(top, s_f);
+  const double sum = chunk_sum<EPT>(x, all, a.k, s_tab, s_d);
+  if (tid == 0) {
+    ((float *)(a.ws + w.max_of[0]))[(size_t)row * w.chunks + chunk] = all;
+    ((double *)(a.ws + w.sum_of[0]))[(size_t)row * w.chunks + chunk] = sum;
   }
 }
 
@@ -402,15 +458,8 @@ __global__ __launch_bounds__(kWalkT) void walk_kernel(VerifyArgs a, VerifyPlan w
     } else if (yes) {
       yes = ((const int32_t *)(a.ws + w.accept))[at + lane] != 0;
     }
-    int cur = 0, len = count > 0 ? 1 : 0, place = lane == 0 && len ? 0 : -1;
-    if (count > 0)
-      for (;;) {   // a child comes behind its parent: at most N steps
-        const uint64_t m = __ballot(yes && up == cur);
-        if (!m) break;
-        cur = __ffsll((unsigned long long)m) - 1;
-        if (lane == len) place = cur;
-        ++len;
-      }
+    int len, place;
+    const int cur = path_end(yes, up, count, len, place);
     if (lane < a.N) a.path[at + lane] = place;
     if (lane == 0) {
       a.accepted[s] = len;
@@ -568,13 +617,18 @@ template <class T, int EPT> static int launch_verify_t(const VerifyArgs &a, cons
       else hipLaunchKernelGGL((round_kernel<T, EPT, 2>), dim3(blocks), dim3(kVT), 0, s, a, w, j);
     }
     launches += rounds;
+    if (a.late_leaves) {
+      hipLaunchKernelGGL((leaf_kernel<T, EPT>), dim3((uint32_t)(a.S * w.chunks)), dim3(kVT), 0, s, a, w);
+      ++launches;
+    }
   }
   hipLaunchKernelGGL((walk_kernel<T>), dim3(a.S), dim3(kWalkT), 0, s, a, w);
   return launches;
 }
 
-hipError_t launch_verify(const VerifyArgs &a, hipStream_t s, int *launches) {
+hipError_t launch_verify(VerifyArgs a, hipStream_t s, int *launches) {
   const VerifyPlan w = verify_plan(a.S, a.N, a.V);
+  a.late_leaves = a.inv_t != 0.0 && (size_t)a.S * (a.N - 1) * a.V * (a.type == E_F32 ? 4 : 2) >= kLateLeaves;
   auto go = [&](auto t) {
     using T = decltype(t);
     return w.chunk == 4096 ? launch_verify_t<T, 16>(a, w, s) : launch_verify_t<T, 4>(a, w, s);

@@ -139,6 +139,37 @@ def test_verify(mode, S, N, V, kind, branch, temperature):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("mode", MODES)
+def test_many_leaves(mode):
+    """Logits enough (71 MB) that the leaves' statistics wait for the rounds: paths that end at leaves and at nodes with
+    children, counts from none on, leaves of nothing, NaN and +inf, nodes without a parent, more children than are tried."""
+    import torch
+    from hydra_amd.layer import Context
+    ctx = Context(0)
+    try:
+        S, N, V = 72, 63, 4003
+        print(f"[gpu] verify many leaves {mode}", flush=True)
+        t = inputs(torch, S, N, V, "f32", mode, 3, 5)
+        t["counts"][:8] = torch.tensor([0, 1, 2, 5, 40, 64, -3, 62], dtype=torch.int32)
+        for s in range(8, 24):                                   # every leaf of these, one way each
+            T, way = t["target"][s, 21:], s % 4
+            if way == 0:
+                T[:] = float("-inf")
+            elif way == 1:
+                T[:, ::3] = float("nan")
+            elif way == 2:
+                T[:, [5, 4002]] = float("inf")
+            else:
+                T[:, 1:] = float("-inf")
+        t["parents"][24, 3::5] = torch.tensor([-7, 80, 62, -1, 63, -1, -1, 99, 60, 61, -1, 0][:len(range(3, 63, 5))], dtype=torch.int32)
+        t["u"][8:24] *= 0.2                                      # mostly accepted: paths down to the leaves
+        for most in (0, 2):
+            check(t, mode, call(torch, ctx, t, mode, 0.9, most), 0.9, most)
+    finally:
+        ctx.close()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 def test_greedy(kind):
     """Ties go to the lowest token; the random numbers are not needed."""
