@@ -82,20 +82,25 @@ template <int T> __device__ __forceinline__ float block_max(float v, float *s_f)
   return t;
 }
 
-// Logits v0 + 4 (256 i + thread) + e of a row, −inf past its end and for NaN.
+// Chunks begin at a multiple of four elements in memory, up to three before the row's first: rows of any length load whole
+// vectors (16 trees of five rows of 131071 bf16, greedy: 13.2 us, single elements 15.4).
+template <class T> __device__ __forceinline__ int first_of(const T *row, int chunk, int size) {
+  return chunk * size - (int)((uintptr_t)row / sizeof(T) & 3);
+}
+// Logits v0 + 4 (256 i + thread) + e of a row, −inf outside it and for NaN.
 template <class T, int EPT> __device__ __forceinline__ void load_chunk(const T *row, int v0, int V, float (&x)[EPT]) {
   typedef T vec4 __attribute__((ext_vector_type(4)));
-  const bool aligned = ((uintptr_t)row & (4 * sizeof(T) - 1)) == 0;
+  const bool aligned = (((uintptr_t)row + v0 * (intptr_t)sizeof(T)) & (4 * sizeof(T) - 1)) == 0;
 #pragma unroll
   for (int i = 0; i < EPT / 4; ++i) {
     const int v = v0 + 4 * (kVT * i + (int)threadIdx.x);
-    if (aligned && v + 4 <= V) {
+    if (aligned && v >= 0 && v + 4 <= V) {
       const vec4 w = *(const vec4 *)(row + v);
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[4 * i + e] = finite_or_less((float)w[e]);
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[4 * i + e] = v + e < V ? finite_or_less((float)row[v + e]) : -INFINITY;
+      for (int e = 0; e < 4; ++e) x[4 * i + e] = v + e >= 0 && v + e < V ? finite_or_less((float)row[v + e]) : -INFINITY;
     }
   }
 }
@@ -111,14 +116,14 @@ struct VerifyPlan {
   int chunk, chunks;
   size_t max_of[2], sum_of[2], part[2], rest[2], state[2], accept, best, total;
 };
-__host__ __device__ inline VerifyPlan verify_plan(int S, int N, int V) {
+__host__ __device__ inline VerifyPlan verify_plan(int S, int N, int V, bool aligned) {
   VerifyPlan p{};
   const size_t rows = (size_t)S * N;
   // 4096 logits a workgroup where that makes 512 of them, else 1024 (16 or 4 a thread). Six nodes of 32000 fp32 logits:
   // 20 us with 1024, 28 with 4096; four trees of 21 nodes of 248320, up to four children a node: 138 and 105; 16 trees of five
   // nodes of 131071 bf16 logits, greedy: 18 and 15.
   p.chunk = rows * V >= (size_t)512 * 4096 ? 4096 : 1024;
-  p.chunks = (V + p.chunk - 1) / p.chunk;
+  p.chunks = (V + (aligned ? 0 : 3) + p.chunk - 1) / p.chunk;
   size_t c = 0;
   auto take = [&](size_t bytes) {
     const size_t o = c;
@@ -202,7 +207,8 @@ __global__ __launch_bounds__(kVT) void stats_kernel(VerifyArgs a, VerifyPlan w) 
   if (!GREEDY) fill_table(s_tab);
   const T *base = (const T *)(of ? a.draft : a.target) + (int64_t)row * (of ? a.d_stride : a.t_stride);
   float x[EPT];
-  load_chunk<T, EPT>(base, chunk * w.chunk, a.V, x);
+  const int v0 = first_of(base, chunk, w.chunk);
+  load_chunk<T, EPT>(base, v0, a.V, x);
   float top = x[0];
 #pragma unroll
   for (int i = 1; i < EPT; ++i) top = fmaxf(top, x[i]);
@@ -212,7 +218,7 @@ __global__ __launch_bounds__(kVT) void stats_kernel(VerifyArgs a, VerifyPlan w) 
     int best = a.V;
 #pragma unroll
     for (int i = EPT - 1; i >= 0; --i)
-      if (x[i] == all) best = chunk * w.chunk + 4 * (kVT * (i / 4) + tid) + i % 4;
+      if (x[i] == all) best = v0 + 4 * (kVT * (i / 4) + tid) + i % 4;
     for (int o = 32; o; o >>= 1) best = min(best, __shfl_xor(best, o));
     if ((tid & 63) == 0) s_i[tid >> 6] = best;
     __syncthreads();
@@ -246,7 +252,8 @@ __global__ __launch_bounds__(kVT) void leaf_kernel(VerifyArgs a, VerifyPlan w) {
   fill_table(s_tab);
   const int64_t row = (int64_t)s * a.N + n;
   float x[EPT];
-  load_chunk<T, EPT>((const T *)a.target + row * a.t_stride, chunk * w.chunk, a.V, x);
+  const T *base = (const T *)a.target + row * a.t_stride;
+  load_chunk<T, EPT>(base, first_of(base, chunk, w.chunk), a.V, x);
   float top = x[0];
 #pragma unroll
   for (int i = 1; i < EPT; ++i) top = fmaxf(top, x[i]);
@@ -298,7 +305,7 @@ __global__ __launch_bounds__(kVT) void round_kernel(VerifyArgs a, VerifyPlan w, 
   const int tried = DRAWN ? round : k;       // given tokens: what is left when all are rejected
   const T *tr = (const T *)a.target + (int64_t)row * a.t_stride;
   const T *dr = (const T *)a.draft + (int64_t)row * a.d_stride;
-  const int v0 = chunk * w.chunk;
+  const int v0 = first_of(tr, chunk, w.chunk);
   float x[EPT], y[DRAWN ? EPT : 1];
   load_chunk<T, EPT>(tr, v0, a.V, x);
   if constexpr (DRAWN) load_chunk<T, EPT>(dr, v0, a.V, y);
@@ -558,11 +565,11 @@ __global__ __launch_bounds__(kWalkT) void walk_kernel(VerifyArgs a, VerifyPlan w
   // The place in the chunk: one or four logits a thread.
   const T *tr = (const T *)a.target + (int64_t)row * a.t_stride;
   const T *dr = (const T *)a.draft + (int64_t)row * a.d_stride;
-  const int ept = w.chunk / kWalkT, v0 = chunk * w.chunk + tid * ept;
+  const int ept = w.chunk / kWalkT, v0 = first_of(tr, chunk, w.chunk) + tid * ept;
   float x[4], y[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const bool in = i < ept && v0 + i < a.V;
+    const bool in = i < ept && v0 + i >= 0 && v0 + i < a.V;
     x[i] = in ? finite_or_less((float)tr[v0 + i]) : -INFINITY;
     y[i] = in && resid && a.mode ? finite_or_less((float)dr[v0 + i]) : -INFINITY;
   }
@@ -597,11 +604,11 @@ __global__ __launch_bounds__(kWalkT) void walk_kernel(VerifyArgs a, VerifyPlan w
 }
 
 bool verify_fits(int S, int N, int V) {
-  const VerifyPlan p = verify_plan(S, N, V);
+  const VerifyPlan p = verify_plan(S, N, V, false);
   return (size_t)S * N * p.chunks <= (size_t)1 << 22;
 }
 
-size_t verify_workspace(int S, int N, int V) { return verify_plan(S, N, V).total; }
+size_t verify_workspace(int S, int N, int V) { return verify_plan(S, N, V, false).total; }
 
 template <class T, int EPT> static int launch_verify_t(const VerifyArgs &a, const VerifyPlan &w, hipStream_t s) {
   const uint32_t blocks = (uint32_t)((size_t)a.S * a.N * w.chunks);
@@ -627,7 +634,10 @@ template <class T, int EPT> static int launch_verify_t(const VerifyArgs &a, cons
 }
 
 hipError_t launch_verify(VerifyArgs a, hipStream_t s, int *launches) {
-  const VerifyPlan w = verify_plan(a.S, a.N, a.V);
+  const size_t vec = a.type == E_F32 ? 16 : 8;
+  const bool drafted = a.mode != 0;
+  const VerifyPlan w = verify_plan(a.S, a.N, a.V, ((uintptr_t)a.target | (drafted ? (uintptr_t)a.draft : 0)) % vec == 0 &&
+                                                      (a.t_stride | (drafted ? a.d_stride : 0)) % 4 == 0);
   a.late_leaves = a.inv_t != 0.0 && (size_t)a.S * (a.N - 1) * a.V * (a.type == E_F32 ? 4 : 2) >= kLateLeaves;
   auto go = [&](auto t) {
     using T = decltype(t);

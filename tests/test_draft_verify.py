@@ -269,6 +269,34 @@ def test_tokens_are_distributed_as_the_target(mode, branch):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("mode,temperature", [("given", 0.0), ("given", 1.0), ("iid", 1.0), ("distinct", 1.0)])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_rows_that_begin_anywhere(kind, mode, temperature):
+    """Rows at every offset within a vector, the draft's at others than the target's, about whole chunks; what lies between
+    the rows is NaN and +inf."""
+    import torch
+    from hydra_amd.layer import Context
+    ctx = Context(0)
+    try:
+        for V in (1, 3, 1021, 1024, 2048):
+            print(f"[gpu] verify offsets {mode} {kind} V={V}", flush=True)
+            t = inputs(torch, 3, 7, V, kind, mode, 2, V)
+            for off, gap in ((0, 1), (1, 4), (2, 3), (3, 2), (1, 0)):
+                def view(x, off, gap):
+                    if x is None:
+                        return None
+                    wide = torch.full((off + 21 * (V + gap),), float("inf"), dtype=x.dtype, device="cuda:0")
+                    wide[::2] = float("nan")
+                    v = wide[off:].view(3, 7, V + gap)[:, :, :V]
+                    v.copy_(x)
+                    return v
+                check(t, mode, call(torch, ctx, t, mode, temperature, target=view(t["target"], off, gap),
+                                    draft=view(t["draft"], 3 - off, gap + 1)), temperature)
+    finally:
+        ctx.close()
+
+
+@pytest.mark.gpu
 def test_strided_rows_and_replays():
     """Logits that are slices of padded rows, recorded and replayed on new inputs beside eager calls of another shape."""
     import torch
