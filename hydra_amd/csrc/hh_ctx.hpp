@@ -45,6 +45,7 @@ struct hh_ctx {
   // Workspace of the drafted-token entries (hh_draft.hip), grown on demand.
   uint8_t *draft = nullptr;
   size_t draft_bytes = 0;
+  uint32_t *arrivals = nullptr;   // hh_cache_commit's counters, zero between its launches
   // Instantiated graphs of this context that are not yet destroyed: they hold the arena's,
   // the attention partials' and the draft workspace's device addresses, so none may be reallocated while any exist.
   int live_graphs = 0;

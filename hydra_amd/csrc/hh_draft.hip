@@ -35,6 +35,23 @@ int ensure_draft(hh_ctx *ctx, size_t bytes) {
   return HH_OK;
 }
 
+// The commit's counters, if they are there or can be made now (not while a graph is recorded).
+int ensure_arrivals(hh_ctx *ctx) {
+  if (ctx->arrivals || ctx->capturing) return HH_OK;
+  void *p = nullptr;
+  if (hipMalloc(&p, sizeof(uint32_t) * kMaxSequences) != hipSuccess) {
+    (void)hipGetLastError();
+    return fail(HH_ENOMEM, "commit counters allocation failed");
+  }
+  const hipError_t e = hipMemsetAsync(p, 0, sizeof(uint32_t) * kMaxSequences, ctx->stream);
+  if (e != hipSuccess) {
+    (void)hipFree(p);
+    return hh::hip_fail(e, "hipMemsetAsync");
+  }
+  ctx->arrivals = (uint32_t *)p;
+  return HH_OK;
+}
+
 // Sizes that every call with a tree description goes by.
 int check_rows(const hh_tree_desc *d) {
   if (!d) return fail(HH_EINVAL, "desc is NULL");
@@ -302,8 +319,10 @@ int hh_cache_commit(hh_ctx *ctx, const hh_tree_desc *d, const hh_kv_cache *cache
   a.kvh = d->kv_heads;
   a.d = d->head_dim;
   a.kv_stride = d->kv_stride ? d->kv_stride : (int64_t)d->kv_heads * d->head_dim;
-  // The rows of every layer first: they go by the lengths that the second round advances.
-  for (int round = 0; round < 2; ++round)
+  if (int rc = ensure_arrivals(ctx)) return rc;
+  if (count <= hh::kRowsLayers) a.arrivals = ctx->arrivals;
+  // Otherwise the rows of every layer first: they go by the lengths that the second round advances.
+  for (int round = 0; round < (a.arrivals ? 1 : 2); ++round)
     for (int l = 0; l < count; l += hh::kRowsLayers) {
       a.layers = count - l < hh::kRowsLayers ? count - l : hh::kRowsLayers;
       for (int i = 0; i < a.layers; ++i) {
@@ -379,6 +398,8 @@ int hh_draft_reserve(hh_ctx *ctx, const hh_tree_desc *tree, const hh_kv_cache *c
     if (b > need) need = b;
   }
   HH_HIP(hipSetDevice(ctx->device));
+  if (cache)
+    if (int rc = ensure_arrivals(ctx)) return rc;
   return ensure_draft(ctx, need);
 }
 

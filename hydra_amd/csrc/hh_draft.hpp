@@ -53,6 +53,7 @@ struct RowsArgs {
   const int32_t *path, *accepted;
   int layers, S, N, kvh, d;
   int64_t kv_stride;
+  uint32_t *arrivals;               // a commit's workgroups by sequence, zero between launches; NULL: lengths advance later
   // Eviction.
   int keep, recent, max_moves;
   int32_t *moves;                   // [layer][S][kvh]: rows that move

@@ -257,6 +257,53 @@ def test_recorded_cycles():
         ctx.close()
 
 
+@pytest.mark.gpu
+def test_commits_one_after_the_other():
+    """Many sequences, layers with two sets of lengths, four commits in a row: eager, and recorded by a context that has
+    run nothing before."""
+    import torch
+    from hydra_amd import speculative as sp
+    from hydra_amd.layer import Context
+    rng = np.random.default_rng(12)
+    S, N, G, D, rows, L = 150, 20, 1, 64, 60, 5
+    for captured in (False, True):
+        print(f"[gpu] commits in a row, captured={captured}", flush=True)
+        ctx = Context(0)
+        try:
+            host = [layer(rng, S, rows, G, D, torch.float16, False, i % 2 == 0) for i in range(L)]
+            l0 = [rng.integers(0, 30, S), rng.integers(0, 30, S)]
+            ln = [torch.tensor(x, dtype=torch.int32, device="cuda:0") for x in l0]
+            nx = ln[0] + 7
+            n0 = l0[0] + 7
+            for i, c in enumerate(host):
+                c["lengths"], c["next"] = l0[i % 2], n0
+            dev = [to_gpu(torch, c, ln[i % 2], nx) for i, c in enumerate(host)]
+            dk, dv = (rng.integers(0, 1 << 15, (L, S, N, G, D)).astype(np.int16) for _ in range(2))
+            k, v = (torch.from_numpy(x).to("cuda:0").view(torch.float16) for x in (dk, dv))
+            path = np.tile(np.arange(N, dtype=np.int32), (S, 1))
+            acc = rng.integers(0, N + 1, S).astype(np.int32)
+            p, a = torch.from_numpy(path).to("cuda:0"), torch.from_numpy(acc).to("cuda:0")
+            caches = sp.CacheSet(dev)
+            torch.cuda.synchronize()
+            call = lambda: sp.cache_commit(ctx, caches, k, v, p, a)
+            graph = ctx.capture(call) if captured else None
+            for rep in range(4):
+                graph.launch() if captured and rep != 2 else call()
+                for i, c in enumerate(host):
+                    c["lengths"], c["next"] = l0[i % 2], n0
+                    commit_ref(c, path, acc, dk[i], dv[i], rows)
+                taken = [np.minimum(acc, rows - x) for x in l0]
+                l0, n0 = [x + t for x, t in zip(l0, taken)], n0 + taken[0]
+            ctx.synchronize()
+            for x, y in zip(dev, host):
+                same(torch, x, y)
+            assert [x.tolist() for x in ln] == [x.tolist() for x in l0] and nx.tolist() == n0.tolist()
+            if captured:
+                graph.close()
+        finally:
+            ctx.close()
+
+
 # ---- refusals (no GPU) ------------------------------------------------------------------------------
 
 def _call(fn, desc=None, caches=None, count=2, **kw):
