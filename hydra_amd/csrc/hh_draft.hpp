@@ -46,7 +46,7 @@ struct RowsLayer {
   int32_t limit;                    // most rows that `lengths` may count
   int32_t last;                     // of the call's layers that share `lengths`
 };
-constexpr int kRowsLayers = 32;     // layers per launch: their blocks are kernel arguments
+constexpr int kRowsLayers = 44;     // layers per launch: their blocks are kernel arguments (4 KB)
 
 struct RowsArgs {
   RowsLayer layer[kRowsLayers];
@@ -59,6 +59,8 @@ struct RowsArgs {
   int32_t *moves;                   // [layer][S][kvh]: rows that move
   int32_t *from, *to;               // [layer][S][kvh][max_moves]
 };
+
+static_assert(sizeof(RowsArgs) <= 4096, "kernel arguments");
 
 struct VerifyArgs {
   const void *target, *draft;

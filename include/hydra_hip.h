@@ -424,7 +424,7 @@ typedef struct hh_tree_desc {
  * lengths[s] counts every token so far and position p is row p % rows. weights and positions are
  * what eviction goes by; a ring has none. next_position: the position of the sequence's next token
  * (its length, until rows are evicted). Layers may share lengths, and then next_position, but nothing
- * else. S x kv_heads is at most 2^18, and times the layers of a commit or an eviction (of 32, if there
+ * else. S x kv_heads is at most 2^18, and times the layers of a commit or an eviction (of 44, if there
  * are more) 2^21.                                                                            */
 typedef struct hh_kv_cache {
   uint16_t *k, *v;           /* [S][rows][kv_heads][head_dim]                                   */
