@@ -11,11 +11,16 @@ __device__ __forceinline__ int committed(const RowsLayer &y, const RowsArgs &a, 
   return min(acc, max(0, y.limit - max(y.lengths[s], 0)));
 }
 
-// One workgroup per (layer, sequence, eight places on the path). With `arrivals` (a launch of all layers), the last one
-// of a sequence also does what advance_kernel does: the others have read the lengths by then. Bound by
-// the launch and the chain length, node, row: 12 layers of eight sequences, 16 nodes, 10.9 us a call, 6.4 of it on the
-// GPU; a workgroup a place (4.1) and a second launch for the lengths (1.9) took 13.9.
+// One workgroup per (layer, sequence, up to eight places on the path: 16 KB of rows). With `arrivals` (a launch of all
+// layers), the last one of a sequence also does what advance_kernel does: the others have read the lengths by then. Bound
+// by the launch and the chain length, node, row: 12 layers of eight sequences, 16 nodes, 10.9 us a call, 6.4 of it on the
+// GPU; a workgroup a place (4.1) and a second launch for the lengths (1.9) took 13.9. 36 layers of one sequence, 28 nodes of
+// 8 KB: 14 us by eight places a workgroup, 10 by two.
 constexpr int kPlaces = 8;
+__host__ __device__ inline int places(int kvh, int d) {   // 16 KB of a sequence's rows
+  const int p = 16384 / (4 * kvh * d);
+  return p < 1 ? 1 : p > kPlaces ? kPlaces : p;
+}
 __device__ __forceinline__ void advance(const RowsLayer &y, const RowsArgs &a, int s) {
   if (!y.last) return;
   const int c = committed(y, a, s);
@@ -25,9 +30,9 @@ __device__ __forceinline__ void advance(const RowsLayer &y, const RowsArgs &a, i
 __global__ __launch_bounds__(256) void commit_kernel(RowsArgs a) {
   __shared__ int64_t s_src[kPlaces], s_dst[kPlaces];   // elements; s_src −1: nothing to do
   __shared__ int s_last;
-  const int parts = (a.N + kPlaces - 1) / kPlaces, i0 = blockIdx.x % parts * kPlaces, s = blockIdx.x / parts % a.S;
+  const int each = places(a.kvh, a.d), parts = (a.N + each - 1) / each, i0 = blockIdx.x % parts * each, s = blockIdx.x / parts % a.S;
   const RowsLayer &y = a.layer[blockIdx.x / (parts * a.S)];
-  const int tid = threadIdx.x, c = committed(y, a, s), n = min(kPlaces, c - i0), start = max(y.lengths[s], 0);
+  const int tid = threadIdx.x, c = committed(y, a, s), n = min(each, c - i0), start = max(y.lengths[s], 0);
   if (n > 0) {
     if (tid < n) {
       const int i = i0 + tid, node = a.path[(int64_t)s * a.N + i];
@@ -95,14 +100,15 @@ __device__ __forceinline__ uint32_t rank_key(float w, int pos, int64_t oldest) {
 // adds to one address go one after the other); a step whose bin is taken whole ends it. Then a lane holds the
 // masks of a run's rows above and at the key, ranks the rows that go from below `keep` and those that stay from
 // `keep` on by scans over the runs, and the rows are listed in order.
-// 96 heads of 4112 rows: 16 us; the key two bits a step by counting, then the lists by two walks over the rows, 24; by
-// histograms of eight bits with a serial scan 46.
-constexpr int kSelT = 1024, kSelW = kSelT / 64, kBits = 11;
-template <int CAP>
-__global__ __launch_bounds__(kSelT) void select_kernel(RowsArgs a) {
+// 96 heads of 4112 rows: 13.6 us; the key two bits a step by counting, then the lists by two walks over the rows, 24; by
+// histograms of eight bits with a serial scan 46 (both with 1024 threads).
+template <int CAP, int T>
+__global__ __launch_bounds__(T) void select_kernel(RowsArgs a) {
+  constexpr int W = T / 64, kBits = T == 1024 ? 11 : T == 512 ? 10 : 9;   // 2·T bins
+  static_assert(1 << kBits == 2 * T, "two bins a thread");
   __shared__ uint32_t s_key[CAP ? CAP : 1];
-  __shared__ int s_hist[1 << kBits], s_sum[kSelW], s_n[kSelW][2], s_found[3];
-  __shared__ uint32_t s_and[kSelW], s_or[kSelW];
+  __shared__ int s_hist[1 << kBits], s_sum[W], s_n[W][2], s_found[3];
+  __shared__ uint32_t s_and[W], s_or[W];
   const int head = blockIdx.x, g = head % a.kvh, s = head / a.kvh % a.S;
   const RowsLayer &y = a.layer[head / (a.kvh * a.S)];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -116,7 +122,7 @@ __global__ __launch_bounds__(kSelT) void select_kernel(RowsArgs a) {
   const float *w = y.weights + base;
   const int *pos = y.positions + base;
   // Rows first .. first + 64 · runs − 1; four runs at a time (rows past n have key 0, which no row has).
-  const int runs = ((n + kSelT - 1) / kSelT + 3) & ~3, first = wave * runs * 64;
+  const int runs = ((n + T - 1) / T + 3) & ~3, first = wave * runs * 64;
   uint32_t all = 0xFFFFFFFFu, any = 0;
   for (int i0 = 0; i0 < runs; i0 += 4) {
     float wv[4];
@@ -132,7 +138,7 @@ __global__ __launch_bounds__(kSelT) void select_kernel(RowsArgs a) {
       const int r = first + 64 * (i0 + u) + lane;
       const uint32_t k = rank_key(wv[u], pv[u], oldest);
       if (r < n) all &= k, any |= k;
-      if constexpr (CAP > 0) s_key[r] = r < n ? k : 0;   // r < 1024 · runs <= CAP
+      if constexpr (CAP > 0) s_key[r] = r < n ? k : 0;   // r < T · runs <= CAP
     }
   }
   auto key_of = [&](int i) -> uint32_t {
@@ -144,7 +150,7 @@ __global__ __launch_bounds__(kSelT) void select_kernel(RowsArgs a) {
   if (lane == 0) s_and[wave] = all, s_or[wave] = any;
   s_hist[2 * tid] = s_hist[2 * tid + 1] = 0;
   __syncthreads();
-  for (int i = 0; i < kSelW; ++i) all &= s_and[i], any |= s_or[i];
+  for (int i = 0; i < W; ++i) all &= s_and[i], any |= s_or[i];
   // Of the rows that agree with t above `bit`, the `need` first in the order are among those that stay, as are all rows
   // above them. At the end t is the key of the last that stays.
   int bit = 32 - __builtin_clz((all ^ any) | 1), need = a.keep;
@@ -171,7 +177,7 @@ __global__ __launch_bounds__(kSelT) void select_kernel(RowsArgs a) {
     }
     if (lane == 0) s_sum[wave] = sum;
     __syncthreads();
-    for (int i = wave + 1; i < kSelW; ++i) sum += s_sum[i];
+    for (int i = wave + 1; i < W; ++i) sum += s_sum[i];
     s_hist[2 * tid] = s_hist[2 * tid + 1] = 0;
     // The bin in which the count from the top reaches `need`.
     const int over = sum - h0 - h1;
@@ -225,7 +231,7 @@ __global__ __launch_bounds__(kSelT) void select_kernel(RowsArgs a) {
   if (lane == 0) s_n[wave][0] = n_above, s_n[wave][1] = n_equal;
   __syncthreads();
   int rank = 0, left = a.keep;       // equal rows of the waves before this one, and those that stay of all
-  for (int i = 0; i < kSelW; ++i) {
+  for (int i = 0; i < W; ++i) {
     left -= s_n[i][0];
     if (i < wave) rank += s_n[i][1];
   }
@@ -260,7 +266,7 @@ __global__ __launch_bounds__(kSelT) void select_kernel(RowsArgs a) {
     if (pass) break;
     if (lane == 0) s_n[wave][0] = holes, s_n[wave][1] = moves;
     __syncthreads();
-    for (int i = 0; i < kSelW; ++i) {
+    for (int i = 0; i < W; ++i) {
       if (i < wave) hole_at += s_n[i][0], move_at += s_n[i][1];
       total += s_n[i][1];
     }
@@ -309,8 +315,9 @@ __global__ __launch_bounds__(256) void move_kernel(RowsArgs a, int parts) {
 }
 
 hipError_t launch_commit(const RowsArgs &a, bool last, hipStream_t s) {
+  const int each = places(a.kvh, a.d);
   if (last) hipLaunchKernelGGL(advance_kernel, dim3(a.layers), dim3(64), 0, s, a);
-  else hipLaunchKernelGGL(commit_kernel, dim3(a.layers * a.S * ((a.N + kPlaces - 1) / kPlaces)), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(commit_kernel, dim3(a.layers * a.S * ((a.N + each - 1) / each)), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
@@ -318,9 +325,13 @@ hipError_t launch_evict(const RowsArgs &a, hipStream_t s) {
   const int heads = a.layers * a.S * a.kvh;
   int rows = 0;
   for (int i = 0; i < a.layers; ++i) rows = a.layer[i].rows > rows ? a.layer[i].rows : rows;
-  if (rows <= 8192) hipLaunchKernelGGL(select_kernel<8192>, dim3(heads), dim3(kSelT), 0, s, a);
-  else if (rows <= 36864) hipLaunchKernelGGL(select_kernel<36864>, dim3(heads), dim3(kSelT), 0, s, a);
-  else hipLaunchKernelGGL(select_kernel<0>, dim3(heads), dim3(kSelT), 0, s, a);
+  // Waves by the rows: barriers cost more the more of them wait, and workgroups share a compute unit. 288 heads of 156
+  // rows 20.4 us with 1024 threads, 12.5 with 256; 96 of 4112 15.8 with 1024, 13.6 with 512; a whole cycle with 384 heads
+  // of 7016 34.8 and 27.8.
+  if (rows <= 2048) hipLaunchKernelGGL((select_kernel<2048, 256>), dim3(heads), dim3(256), 0, s, a);
+  else if (rows <= 8192) hipLaunchKernelGGL((select_kernel<8192, 512>), dim3(heads), dim3(512), 0, s, a);
+  else if (rows <= 36864) hipLaunchKernelGGL((select_kernel<36864, 1024>), dim3(heads), dim3(1024), 0, s, a);
+  else hipLaunchKernelGGL((select_kernel<0, 1024>), dim3(heads), dim3(1024), 0, s, a);
   // Workgroups enough to fill the chip with rows in flight, of at least four rounds' rows each.
   const int per = 4 * 256 / (a.d / 8);
   int parts = 4096 / heads, most = (a.max_moves + per - 1) / per;
