@@ -10,8 +10,9 @@
 //   O^T [D × 32 rows] += V^T · P^T, the value tile read by columns (transposing LDS reads), P^T from S^T's own
 //   registers: a lane holds one row's probabilities at 16 keys, and the products' order over the keys is the
 //   lane's. So a row's maximum and sum stay in its two lanes, and rescaling needs no exchange.
-// F32 activations: queries and
-// probabilities as fp16 pairs hi + lo, two products each (exact in fp32 to ~2^-22).
+// Probabilities enter as pairs hi + lo of the values' type, two products each (a single rounding of them would be as large
+// as that of the outputs; eight BF16 sequences of up to 8191 keys: 60 us, 58.6 with a single one), and so do the queries of
+// F32 activations, of fp16.
 // A chunk's state (M, L, O) goes to the workspace and tree_merge_kernel joins a row's chunks in order; a call of
 // one chunk writes its outputs at once. The sink enters where the states are joined.
 #include "hh_common.hpp"
@@ -83,6 +84,12 @@ __device__ __forceinline__ u32x2 split_pair(float p0, float p1, float minus1) {
   const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(p0, p1));
   const f16x2 l = {(_Float16)fmaf((float)h[0], minus1, p0), (_Float16)fmaf((float)h[1], minus1, p1)};
   return u32x2{__builtin_bit_cast(uint32_t, h), __builtin_bit_cast(uint32_t, l)};
+}
+// The same in bf16: to 2^-15 of each.
+__device__ __forceinline__ u32x2 split_pair_bf16(float p0, float p1) {
+  const uint32_t u0 = __float_as_uint(p0), u1 = __float_as_uint(p1);
+  const bf16x2 l = {(__bf16)(p0 - __uint_as_float(u0 & 0xFFFF0000u)), (__bf16)(p1 - __uint_as_float(u1 & 0xFFFF0000u))};
+  return u32x2{__builtin_amdgcn_perm(u1, u0, 0x07060302u), __builtin_bit_cast(uint32_t, l)};
 }
 // Waits for the first of the tiles that were asked for ahead of the loop.
 template <int NL, int NST> __device__ __forceinline__ void wait_first(int tiles) {
@@ -380,12 +387,9 @@ __global__ __launch_bounds__(64 * RT * KS, OCC) void tree_split_kernel(TreeArgs 
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float p0 = S[8 * kc + 2 * e], p1 = S[8 * kc + 2 * e + 1];
-        if constexpr (PAIR) {
-          const u32x2 w = split_pair(p0, p1, minus1);
-          ph[e] = w[0];
-          pl[e] = w[1];
-        } else if constexpr (BF) ph[e] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)p0, (__bf16)p1});
-        else ph[e] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)p0, (_Float16)p1});
+        const u32x2 w = BF ? split_pair_bf16(p0, p1) : split_pair(p0, p1, minus1);
+        ph[e] = w[0];
+        pl[e] = w[1];
       }
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
@@ -399,7 +403,7 @@ __global__ __launch_bounds__(64 * RT * KS, OCC) void tree_split_kernel(TreeArgs 
           vf[2 * x8 + 1] = v[1];
         }
         acc[n] = mfma32<BF>(vf, ph, acc[n]);
-        if constexpr (PAIR) acc[n] = mfma32<BF>(vf, pl, acc[n]);
+        acc[n] = mfma32<BF>(vf, pl, acc[n]);
       }
     }
     top = masked_top(Sn, t + 1, part);

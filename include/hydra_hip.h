@@ -444,8 +444,8 @@ typedef struct hh_kv_cache {
  *   draft_k, draft_v  cache_type [S][N][kv_heads][head_dim] (with kv_stride)
  *   sinks    bf16 [q_heads] or NULL;  lse  fp32 [S][N][q_heads] or NULL: the log of the denominator
  * Keys that a node does not see, infinities and NaN among them, have no part in its output.
- * Sums are held in fp32; with F32 activations queries and probabilities enter the products as pairs of
- * fp16 (about 2^-22), with F16 and BF16 probabilities are rounded once to the type.            */
+ * Sums are held in fp32. Probabilities, and the queries of F32 activations, enter the products as pairs of the
+ * cache's type: to about 2^-21 (F16) and 2^-15 (BF16). Outputs are rounded once.              */
 int hh_attention_tree(hh_ctx *ctx, const hh_tree_desc *desc, const hh_kv_cache *cache,
                       const void *q, const void *draft_k, const void *draft_v,
                       const int32_t *parents, const int32_t *node_counts, const uint16_t *sinks,

@@ -1,0 +1,53 @@
+"""Roundings of the tree attention (hh_attention_tree) with 16-bit activations, output by output against 64 bits on the
+same inputs. An output is rounded once: half a step of its type, 2^-11 (fp16, 2^-25 below its normal range) and 2^-8 (bf16) of its
+value. What comes before that is in fp32 or as good, and its errors go by sum(p |v|), not by the output, which may be
+small beside it: a probability's two parts (2^-21 fp16, 2^-15 bf16), and 1e-5 twice for the logits' fp32 sums (at most 16 + 4
+roundings of 2^-24 of partial sums below 8) in the exponential and in the denominator."""
+import numpy as np
+import pytest
+
+from test_tree_attention import call, make, reference
+
+HALF = {"f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+PARTS = {"f16": 2.0 ** -21, "bf16": 2.0 ** -15}
+LEAST = {"f16": 2.0 ** -25, "bf16": 0.0}
+
+
+def outputs_of(t, got, window=0, ring=False, scale=None):
+    """(got, exact, sum of p |v|) of every real node's outputs, in 64 bits."""
+    num = lambda x: None if x is None else x.double().numpy()
+    scale = t["q"].shape[3] ** -0.5 if scale is None else scale
+    args = lambda v, dv: (num(t["q"]), num(t["k"]), v, num(t["dk"]), dv, t["lengths"].numpy(), t["parents"].numpy(),
+                          t["counts"].numpy(), num(t["sinks"]), window, ring, scale)
+    want, _ = reference(*args(num(t["v"]), num(t["dv"])))
+    size, _ = reference(*args(np.abs(num(t["v"])), np.abs(num(t["dv"]))))
+    g = got.double().cpu().numpy()
+    return np.stack([g[i] for i in want]), np.stack([want[i] for i in want]), np.stack([size[i] for i in want])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S,N,H,G,D,kind,rows,lengths,window,ring", [
+    (1, 1, 8, 2, 64, "f16", 40, [3], 0, False),               # few keys: large probabilities
+    (1, 1, 8, 2, 64, "bf16", 40, [3], 0, False),
+    (2, 5, 8, 2, 128, "bf16", 90, [9, 80], 0, False),
+    (4, 12, 16, 2, 64, "f16", 192, [5000, 191, 3000, 40], 128, True),
+    (2, 25, 8, 2, 128, "bf16", 700, [690, 351], 0, False),    # four tiles of rows, chunks
+    (1, 40, 16, 2, 128, "f16", 1500, [1477], 0, False),
+    (1, 7, 4, 1, 256, "bf16", 1200, [1111], 0, False),
+    (2, 9, 16, 1, 256, "f16", 300, [290, 31], 60, False),
+    (1, 33, 4, 4, 64, "bf16", 600, [577], 0, False),
+])
+def test_outputs_are_rounded_once(S, N, H, G, D, kind, rows, lengths, window, ring):
+    import torch
+    from hydra_amd.layer import Context
+    print(f"[gpu] tree rounding S={S} N={N} H={H} G={G} D={D} {kind} {lengths} w={window}", flush=True)
+    t = make(torch, S, N, H, G, D, kind, rows, lengths, seed=N + D)
+    ctx = Context(0)
+    try:
+        out, _ = call(torch, ctx, t, ring, window)
+    finally:
+        ctx.close()
+    got, want, size = outputs_of(t, out, window, ring)
+    before = (PARTS[kind] + 2e-5) * size
+    off = np.abs(got - want) / (HALF[kind] * (np.abs(want) + before) + LEAST[kind] + before)
+    assert off.max() <= 1.0, (off.max(), (off > 1).mean())
