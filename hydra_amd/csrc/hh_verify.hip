@@ -112,6 +112,7 @@ struct NodeState {
 };
 
 // The workspace. Chunk arrays are [row][chunks], row = s·N + n; part, state: of odd and even rounds.
+// accept: the round in which a node was accepted, 0 if in none.
 struct VerifyPlan {
   int chunk, chunks;
   size_t max_of[2], sum_of[2], part[2], rest[2], state[2], accept, best, total;
@@ -158,6 +159,16 @@ __device__ __forceinline__ uint64_t children_in(int parent, int n, int count, in
 
 __device__ __forceinline__ uint64_t children_of(const VerifyArgs &a, int s, int n, int count, int most) {
   return children_in(a.parents[(int64_t)s * a.N + min((int)threadIdx.x & 63, a.N - 1)], n, count, most);
+}
+
+// Flags of `accept` in a launch that also writes them: only what earlier rounds wrote may count, so that what a workgroup does
+// is the same for all its waves, whenever they look.
+__device__ __forceinline__ bool accepted_before(const int32_t *flag, int round) {
+  const int at = __hip_atomic_load(flag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return at != 0 && at < round;
+}
+__device__ __forceinline__ void accept_in(int32_t *flag, int round) {
+  __hip_atomic_store(flag, round, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // The node that a path ends at, in every lane of the wave: yes, up: a node accepted at its parent, in its lane. len: nodes of
@@ -293,8 +304,10 @@ __global__ __launch_bounds__(kVT) void round_kernel(VerifyArgs a, VerifyPlan w, 
   const int k = __popcll(kids);
   if (k < round) return;
   if (DRAWN && round > 1) {
-    // Rows that no path ends at any more: with a child accepted, or rejected themselves, or with a sibling accepted.
-    const uint64_t taken = __ballot(lane < count && ((const int32_t *)(a.ws + w.accept))[(int64_t)s * a.N + min(lane, a.N - 1)]);
+    // Rows that no path ends at any more by the rounds before: with a child accepted, or rejected themselves, or with a
+    // sibling accepted.
+    const int32_t *flag = (const int32_t *)(a.ws + w.accept) + (int64_t)s * a.N + min(lane, a.N - 1);
+    const uint64_t taken = __ballot(lane < count && accepted_before(flag, round));
     if (kids & taken) return;
     if (n > 0) {
       const uint64_t sib = children_in(parent, __shfl(parent, n), count, a.children), me = 1ull << n;
@@ -353,7 +366,7 @@ __global__ __launch_bounds__(kVT) void round_kernel(VerifyArgs a, VerifyPlan w, 
       if (lane == 0 && t >= 0 && t < a.V && !again) {
         const double p = exp_call(finite_or_less((float)tr[t]), st.mp, a.k, s_tab) * st.ip;
         const double q = exp_call(finite_or_less((float)dr[t]), st.mq, a.k, s_tab) * st.iq;
-        accept[child] = fmax(p - st.c * q, 0.0) > (double)a.u[(int64_t)s * a.N + child] * mass * (q / left);
+        if (fmax(p - st.c * q, 0.0) > (double)a.u[(int64_t)s * a.N + child] * mass * (q / left)) accept_in(accept + child, round);
       }
     } else if (kids >> lane & 1) {
       // Every child at once, in its own lane: the mass left at its turn is what the distinct tokens before it have not.
@@ -367,9 +380,9 @@ __global__ __launch_bounds__(kVT) void round_kernel(VerifyArgs a, VerifyPlan w, 
         for (int e = 0; e < i; ++e) first &= s_tok[e] != o;
         if (first) before += exp_call(finite_or_less((float)tr[o]), st.mp, a.k, s_tab) * st.ip;
       }
-      if (t >= 0 && t < a.V && !again)
-        accept[lane] = exp_call(finite_or_less((float)tr[t]), st.mp, a.k, s_tab) * st.ip >
-                       (double)a.u[(int64_t)s * a.N + lane] * fmax(1.0 - before, 0.0);
+      if (t >= 0 && t < a.V && !again &&
+          exp_call(finite_or_less((float)tr[t]), st.mp, a.k, s_tab) * st.ip > (double)a.u[(int64_t)s * a.N + lane] * fmax(1.0 - before, 0.0))
+        accept_in(accept + lane, round);
     }
   }
   st.c = DRAWN ? st.c + mass / left : 0.0;
