@@ -1,17 +1,19 @@
 // hh_verify.hip — verification of drafted tokens against the target's probabilities.
 //
 // With p and q the target's and the draft's probabilities at a node, the residual after its first j
-// children were rejected is, before it is normalised, r_j(v) = max(p(v) − c_j q(v), 0) off the tokens
+// children were rejected is, before it is normalised, r_j(v) = max(p(v) − c_j q_j(v), 0) off the tokens
 // tried, of mass W_j: r_0 = p, c_0 = 0, W_0 = 1. Rejecting a child subtracts its distribution q_j from
-// r_j / W_j, so c_{j+1} = c_j + W_j for independent draws (q_j = q), c_j + W_j / R_j where the tried
-// tokens are not put back (q_j = q / R_j, R_j the mass of q off them), and c = 0 for given tokens. A
+// r_j / W_j. For independent draws q_j = q and c_{j+1} = c_j + W_j; where the tried tokens are not put back q_j is
+// q off them, normalised, and c_{j+1} = (c_j + W_j) R_j, R_j the mass of q_j off the j-th; c = 0 for given tokens. A
 // child with token x is accepted if r_j(x) > u W_j q_j(x). That needs no normalised copy of a row, and does
 // not depend on what happens at other nodes: every node's tests are made at once, and the walk follows.
+// q_j goes by the maximum and the sum of the tokens off those tried, which the chunks keep from round to round: what is
+// left of a sharp draft may be any number of times smaller than what was tried.
 //
 // A row of logits is cut into chunks, a workgroup each, so that one sequence's rows fill the chip:
 //   stats    every row's maximum and sum of exponentials by chunk (greedy: its largest entry);
 //   round j  of the nodes with at least j children that a path may still end at: the j-th child's test, then W_j and
-//            R_j by chunk (given tokens: all tests and the last residual in one round);
+//            the draft's maxima and sums off it by chunk (given tokens: all tests and the last residual in one round);
 //   leaf     (where leaves' logits are many) the statistics of the leaf that a path ends at;
 //   walk     a workgroup per sequence follows the accepted children and finds the next token: its chunk by the
 //            chunks' sums, its place by a scan of that chunk.
@@ -105,17 +107,19 @@ template <class T, int EPT> __device__ __forceinline__ void load_chunk(const T *
   }
 }
 
-// What rounds leave of a node: reciprocals of its rows' sums, their maxima, and c of the round.
+// What rounds leave of a node: reciprocals of its rows' sums, their maxima (the draft's off the tokens tried before), and the
+// factor of the draft in the round's residual.
 struct NodeState {
   double ip, iq, c;
   float mp, mq;
 };
 
-// The workspace. Chunk arrays are [row][chunks], row = s·N + n; part, state: of odd and even rounds.
+// The workspace. Chunk arrays are [row][chunks], row = s·N + n; part, state: of odd and even rounds; max_of, sum_of: of the
+// target, and of the draft behind even (0: no token tried yet) and odd rounds.
 // accept: the round in which a node was accepted, 0 if in none.
 struct VerifyPlan {
   int chunk, chunks;
-  size_t max_of[2], sum_of[2], part[2], rest[2], state[2], accept, best, total;
+  size_t max_of[3], sum_of[3], part[2], state[2], accept, best, total;
 };
 __host__ __device__ inline VerifyPlan verify_plan(int S, int N, int V, bool aligned) {
   VerifyPlan p{};
@@ -132,11 +136,12 @@ __host__ __device__ inline VerifyPlan verify_plan(int S, int N, int V, bool alig
     return o;
   };
   const size_t n = rows * p.chunks;
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < 3; ++i) {
     p.max_of[i] = take(4 * n);
     p.sum_of[i] = take(8 * n);
+  }
+  for (int i = 0; i < 2; ++i) {
     p.part[i] = take(8 * n);
-    p.rest[i] = take(8 * n);
     p.state[i] = take(sizeof(NodeState) * rows);
   }
   p.accept = take(4 * rows);
@@ -218,7 +223,8 @@ __global__ __launch_bounds__(kVT) void stats_kernel(VerifyArgs a, VerifyPlan w) 
   if (!GREEDY) fill_table(s_tab);
   const T *base = (const T *)(of ? a.draft : a.target) + (int64_t)row * (of ? a.d_stride : a.t_stride);
   float x[EPT];
-  const int v0 = first_of(base, chunk, w.chunk);
+  // Both rows in the target's chunks, as the rounds: equal rows have equal sums.
+  const int v0 = first_of((const T *)a.target + (int64_t)row * a.t_stride, chunk, w.chunk);
   load_chunk<T, EPT>(base, v0, a.V, x);
   float top = x[0];
 #pragma unroll
@@ -291,8 +297,8 @@ __device__ __forceinline__ double joined(const float *mx, const double *sm, int 
 
 template <class T, int EPT, int MODE>
 __global__ __launch_bounds__(kVT) void round_kernel(VerifyArgs a, VerifyPlan w, int round) {
-  __shared__ double s_tab[256], s_d[6][kVT / 64];
-  __shared__ float s_f[2][kVT / 64];
+  __shared__ double s_tab[256], s_d[5][kVT / 64];
+  __shared__ float s_f[3][kVT / 64];
   __shared__ int s_tok[kTreeNodes];
   constexpr bool DRAWN = MODE != 0;
   const int chunk = blockIdx.x % w.chunks, row = blockIdx.x / w.chunks, s = row / a.N, n = row - s * a.N, tid = threadIdx.x;
@@ -330,31 +336,30 @@ __global__ __launch_bounds__(kVT) void round_kernel(VerifyArgs a, VerifyPlan w, 
   __syncthreads();
   const size_t at = (size_t)row * w.chunks;
   NodeState st{};
-  double mass = 1.0, rest = 1.0;
+  double mass = 1.0;
   if (round == 1) {
     float m;
     const double zp = joined<kVT>((const float *)(a.ws + w.max_of[0]) + at, (const double *)(a.ws + w.sum_of[0]) + at, w.chunks,
                                   a.k, s_tab, s_f[0], s_d[0], m);
     st.mp = m;
     st.ip = zp > 0 ? 1.0 / zp : 0.0;
-    if constexpr (DRAWN) {
-      const double zq = joined<kVT>((const float *)(a.ws + w.max_of[1]) + at, (const double *)(a.ws + w.sum_of[1]) + at, w.chunks,
-                                    a.k, s_tab, s_f[1], s_d[1], m);
-      st.mq = m;
-      st.iq = zq > 0 ? 1.0 / zq : 0.0;
-    }
   } else {
     st = ((const NodeState *)(a.ws + w.state[(round - 1) & 1]))[row];
-    const double *pw = (const double *)(a.ws + w.part[(round - 1) & 1]) + at, *pr = (const double *)(a.ws + w.rest[(round - 1) & 1]) + at;
-    double sw = 0.0, sr = 0.0;
-    for (int c = tid; c < w.chunks; c += kVT) {
-      sw += pw[c];
-      if constexpr (MODE == 2) sr += pr[c];
-    }
+    const double *pw = (const double *)(a.ws + w.part[(round - 1) & 1]) + at;
+    double sw = 0.0;
+    for (int c = tid; c < w.chunks; c += kVT) sw += pw[c];
     mass = block_sum<kVT>(sw, s_d[2]);
-    if constexpr (MODE == 2) rest = block_sum<kVT>(sr, s_d[3]);
   }
-  const double left = MODE == 2 ? fmax(rest, 0x1p-52) : 1.0;
+  const int before = 1 + ((round - 1) & 1);   // the draft's maxima and sums off the tokens tried before this round
+  const float *mx_q = (const float *)(a.ws + w.max_of[before]) + at;
+  const double *sm_q = (const double *)(a.ws + w.sum_of[before]) + at;
+  if (DRAWN && (round == 1 || MODE == 2)) {
+    float m;
+    const double zq = joined<kVT>(mx_q, sm_q, w.chunks, a.k, s_tab, s_f[1], s_d[1], m);
+    if (round > 1) st.c *= zq * exp_call(m, st.mq, a.k, s_tab) * st.iq;   // the mass off the last token
+    st.mq = m;
+    st.iq = zq > 0 ? 1.0 / zq : 0.0;
+  }
   if (chunk == 0 && tid < 64) {
     int32_t *accept = (int32_t *)(a.ws + w.accept) + (int64_t)s * a.N;
     if constexpr (DRAWN) {
@@ -363,10 +368,10 @@ __global__ __launch_bounds__(kVT) void round_kernel(VerifyArgs a, VerifyPlan w, 
       const int child = __ffsll((unsigned long long)m) - 1, t = s_tok[round - 1];
       bool again = false;
       for (int i = 0; i < round - 1; ++i) again |= s_tok[i] == t;
-      if (lane == 0 && t >= 0 && t < a.V && !again) {
+      if (lane == 0 && mass > 0 && t >= 0 && t < a.V && !again) {
         const double p = exp_call(finite_or_less((float)tr[t]), st.mp, a.k, s_tab) * st.ip;
         const double q = exp_call(finite_or_less((float)dr[t]), st.mq, a.k, s_tab) * st.iq;
-        if (fmax(p - st.c * q, 0.0) > (double)a.u[(int64_t)s * a.N + child] * mass * (q / left)) accept_in(accept + child, round);
+        if (fmax(p - st.c * q, 0.0) > (double)a.u[(int64_t)s * a.N + child] * mass * q) accept_in(accept + child, round);
       }
     } else if (kids >> lane & 1) {
       // Every child at once, in its own lane: the mass left at its turn is what the distinct tokens before it have not.
@@ -385,7 +390,7 @@ __global__ __launch_bounds__(kVT) void round_kernel(VerifyArgs a, VerifyPlan w, 
         accept_in(accept + lane, round);
     }
   }
-  st.c = DRAWN ? st.c + mass / left : 0.0;
+  st.c = DRAWN ? st.c + mass : 0.0;
   if (chunk == 0 && tid == 0) ((NodeState *)(a.ws + w.state[round & 1]))[row] = st;
   // The residual off the tokens tried, of which few chunks hold one.
   bool here = false;
@@ -401,15 +406,16 @@ __global__ __launch_bounds__(kVT) void round_kernel(VerifyArgs a, VerifyPlan w, 
         }
     }
   }
-  double sw = 0.0, sr = 0.0;
-  if (fabsf(st.mp) == INFINITY || (DRAWN && fabsf(st.mq) == INFINITY)) {
+  double sw = 0.0;
+  if (!(mass > 0)) {
+    // Nothing was left before: p and the draft normalised anew would differ by a rounding.
+  } else if (fabsf(st.mp) == INFINITY || (DRAWN && fabsf(st.mq) == INFINITY)) {
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
       const double p = exp_call(x[i], st.mp, a.k, s_tab) * st.ip;
       double q = 0.0;
       if constexpr (DRAWN) q = exp_call(y[i], st.mq, a.k, s_tab) * st.iq;
       sw += fmax(p - st.c * q, 0.0);
-      sr += q;
     }
   } else {
     const double mp = st.mp, mq = st.mq, cq = st.c * st.iq;
@@ -419,17 +425,28 @@ __global__ __launch_bounds__(kVT) void round_kernel(VerifyArgs a, VerifyPlan w, 
       if constexpr (DRAWN) {
         const double q = exp_of(y[i], mq, a.k, s_tab);
         sw += fmax(p * st.ip - cq * q, 0.0);
-        if constexpr (MODE == 2) sr += q * st.iq;
       } else {
         sw += p * st.ip;
       }
     }
   }
   sw = block_sum<kVT>(sw, s_d[4]);
-  if constexpr (MODE == 2) sr = block_sum<kVT>(sr, s_d[5]);
-  if (tid == 0) {
-    ((double *)(a.ws + w.part[round & 1]))[at + chunk] = sw;
-    if constexpr (MODE == 2) ((double *)(a.ws + w.rest[round & 1]))[at + chunk] = sr;
+  if (tid == 0) ((double *)(a.ws + w.part[round & 1]))[at + chunk] = sw;
+  if constexpr (MODE == 2) {
+    // The draft off this round's token too: new where it is this chunk's.
+    float top = mx_q[chunk];
+    double sum = sm_q[chunk];
+    if (s_tok[round - 1] >= v0 && s_tok[round - 1] < v0 + w.chunk) {
+      float most = y[0];
+#pragma unroll
+      for (int i = 1; i < EPT; ++i) most = fmaxf(most, y[i]);
+      top = block_max<kVT>(most, s_f[2]);
+      sum = chunk_sum<EPT>(y, top, a.k, s_tab, s_d[3]);
+    }
+    if (tid == 0) {
+      ((float *)(a.ws + w.max_of[1 + (round & 1)]))[at + chunk] = top;
+      ((double *)(a.ws + w.sum_of[1 + (round & 1)]))[at + chunk] = sum;
+    }
   }
 }
 
