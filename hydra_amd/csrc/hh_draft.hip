@@ -386,15 +386,13 @@ int hh_draft_reserve(hh_ctx *ctx, const hh_tree_desc *tree, const hh_kv_cache *c
     if (layers) need = evict_bytes(tree, per, cache->rows);
     if (tree->nodes) {
       if (int rc = check_tree(tree)) return rc;
-      hh::TreeArgs a = tree_args(tree, cache, nullptr);
-      hh::tree_plan(a, tree->max_length ? tree->max_length : cache->rows);
-      const size_t b = hh::tree_workspace(a);
+      const size_t b = hh::tree_reserve(tree_args(tree, cache, nullptr), tree->max_length ? tree->max_length : cache->rows);
       if (b > need) need = b;
     }
   }
   if (verify) {
     if (int rc = check_verify(verify)) return rc;
-    const size_t b = hh::verify_workspace(verify->sequences, verify->nodes, verify->vocab);
+    const size_t b = hh::verify_reserve(verify->sequences, verify->nodes, verify->vocab);
     if (b > need) need = b;
   }
   HH_HIP(hipSetDevice(ctx->device));

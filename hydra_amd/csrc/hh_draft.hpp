@@ -75,9 +75,11 @@ struct VerifyArgs {
 };
 
 size_t verify_workspace(int S, int N, int V);
+size_t verify_reserve(int S, int N, int V);   // of every call up to these sizes
 bool verify_fits(int S, int N, int V);   // launches' block counts
 void tree_plan(TreeArgs &a, int64_t length);
 size_t tree_workspace(const TreeArgs &a);
+size_t tree_reserve(const TreeArgs &a, int64_t length);   // of every call up to these sizes
 hipError_t launch_tree(const TreeArgs &a, int type, hipStream_t s);
 hipError_t launch_weights(TreeArgs a, int type, hipStream_t s);
 hipError_t launch_verify(VerifyArgs a, hipStream_t s, int *launches);

@@ -649,6 +649,24 @@ size_t tree_workspace(const TreeArgs &a) {
   return a.chunks > 1 ? sizeof(float) * (size_t)a.S * a.N * a.qh * a.chunks * (a.d + 2) : 0;
 }
 
+// The most that tree_workspace asks for with up to a.S sequences, a.N nodes and `length` keys, whatever the windows. Fewer keys or
+// nodes may take more chunks: chunks are whole tiles, and wider ones where a head has few rows.
+size_t tree_reserve(const TreeArgs &a, int64_t length) {
+  const int64_t keys = length < a.rows ? length : a.rows;
+  size_t most = 0;
+  for (int n = 1; n <= a.N; ++n) {
+    const int rows = n * a.qm;
+    const TreeShape t = tree_shape(a.d, rows);
+    const int64_t own = (int64_t)a.kvh * ((rows + 32 * t.rt - 1) / (32 * t.rt)), tiles = (keys + 32 * t.ks - 1) / (32 * t.ks);
+    int64_t chunks = kTreeGroups / own;                       // of all sequences
+    if (chunks < 2 || tiles <= kTreeTiles) continue;          // one a sequence
+    if (chunks > a.S * tiles) chunks = a.S * tiles;
+    const size_t b = sizeof(float) * (size_t)n * a.qh * chunks * (a.d + 2);
+    if (b > most) most = b;
+  }
+  return most;
+}
+
 template <int QT, int D> static hipError_t launch_tree_d(const TreeArgs &a, hipStream_t s) {
   const TreeShape t = tree_shape(D, a.N * (a.qh / a.kvh));
   const int64_t groups = (int64_t)a.S * a.kvh * a.chunks;

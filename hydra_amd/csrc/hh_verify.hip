@@ -121,21 +121,27 @@ struct VerifyPlan {
   int chunk, chunks;
   size_t max_of[3], sum_of[3], part[2], state[2], accept, best, total;
 };
+constexpr size_t kWideChunks = (size_t)512 * 4096;   // logits from which on chunks are of 4096
+__host__ __device__ inline void place_arrays(VerifyPlan &p, size_t rows, size_t n);
 __host__ __device__ inline VerifyPlan verify_plan(int S, int N, int V, bool aligned) {
   VerifyPlan p{};
   const size_t rows = (size_t)S * N;
   // 4096 logits a workgroup where that makes 512 of them, else 1024 (16 or 4 a thread). Six nodes of 32000 fp32 logits:
   // 20 us with 1024, 28 with 4096; four trees of 21 nodes of 248320, up to four children a node: 138 and 105; 16 trees of five
   // nodes of 131071 bf16 logits, greedy: 18 and 15.
-  p.chunk = rows * V >= (size_t)512 * 4096 ? 4096 : 1024;
+  p.chunk = rows * V >= kWideChunks ? 4096 : 1024;
   p.chunks = (V + (aligned ? 0 : 3) + p.chunk - 1) / p.chunk;
+  place_arrays(p, rows, rows * p.chunks);
+  return p;
+}
+// Where the arrays of `rows` rows and `n` chunks lie.
+__host__ __device__ inline void place_arrays(VerifyPlan &p, size_t rows, size_t n) {
   size_t c = 0;
   auto take = [&](size_t bytes) {
     const size_t o = c;
     c += (bytes + 255) / 256 * 256;
     return o;
   };
-  const size_t n = rows * p.chunks;
   for (int i = 0; i < 3; ++i) {
     p.max_of[i] = take(4 * n);
     p.sum_of[i] = take(8 * n);
@@ -147,7 +153,6 @@ __host__ __device__ inline VerifyPlan verify_plan(int S, int N, int V, bool alig
   p.accept = take(4 * rows);
   p.best = take(4 * n);
   p.total = c;
-  return p;
 }
 
 // The children of node n as a mask, the first `most`, from every node's parent in its lane of the wave.
@@ -639,6 +644,20 @@ bool verify_fits(int S, int N, int V) {
 }
 
 size_t verify_workspace(int S, int N, int V) { return verify_plan(S, N, V, false).total; }
+
+// Fewer logits may make more chunks, of 1024: each begun one of a row, and all of fewer than kWideChunks logits.
+size_t verify_reserve(int S, int N, int V) {
+  VerifyPlan p = verify_plan(S, N, V, false);
+  const size_t rows = (size_t)S * N;
+  size_t n = rows * p.chunks;
+  if (p.chunk == 4096) {
+    const size_t some = kWideChunks / 1024 + rows * (1024 + 2) / 1024 + 1, all = rows * ((V + 3 + 1023) / 1024);
+    const size_t narrow = some < all ? some : all;
+    if (narrow > n) n = narrow;
+  }
+  place_arrays(p, rows, n);
+  return p.total;
+}
 
 template <class T, int EPT> static int launch_verify_t(const VerifyArgs &a, const VerifyPlan &w, hipStream_t s) {
   const uint32_t blocks = (uint32_t)((size_t)a.S * a.N * w.chunks);

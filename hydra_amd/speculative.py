@@ -256,8 +256,8 @@ def reserve(ctx: Context, cache: KVCache | None = None, nodes: int = 1, q_heads:
             max_length: int = 0, verify: tuple | None = None, verify_dtype=torch.float32, distinct: bool = False,
             drawn: bool = True, temperature: float = 1.0, max_children: int = 0):
     """Pre-sizes the context's workspace (hh_draft_reserve), for calls that a graph will record: tree attention
-    of `nodes` nodes and q_heads heads on `cache`, eviction of `layers` layers like it, and verification of logits
-    of the shape `verify` = (S, N, V)."""
+    of up to `nodes` nodes and q_heads heads on `cache` (histories up to max_length, 0: its rows; any window), eviction of
+    `layers` layers like it, and verification of logits up to the shape `verify` = (S, N, V)."""
     t, v = None, None
     if cache is not None:
         S, _, G, D = cache.shape
