@@ -443,7 +443,8 @@ typedef struct hh_kv_cache {
  *   q, out   type [S][N][q_heads][head_dim] (q with q_stride)
  *   draft_k, draft_v  cache_type [S][N][kv_heads][head_dim] (with kv_stride)
  *   sinks    bf16 [q_heads] or NULL;  lse  fp32 [S][N][q_heads] or NULL: the log of the denominator
- * Keys that a node does not see, infinities and NaN among them, have no part in its output.
+ * Keys that a node does not see, infinities and NaN among them, have no part in its output. Logits may be of any
+ * size that fp32 holds, times log2(e).
  * Sums are held in fp32. Probabilities, and the queries of F32 activations, enter the products as pairs of the
  * cache's type: to about 2^-21 (F16) and 2^-15 (BF16). Outputs are rounded once.              */
 int hh_attention_tree(hh_ctx *ctx, const hh_tree_desc *desc, const hh_kv_cache *cache,

@@ -51,3 +51,36 @@ def test_outputs_are_rounded_once(S, N, H, G, D, kind, rows, lengths, window, ri
     before = (PARTS[kind] + 2e-5) * size
     off = np.abs(got - want) / (HALF[kind] * (np.abs(want) + before) + LEAST[kind] + before)
     assert off.max() <= 1.0, (off.max(), (off > 1).mean())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,D,size", [("bf16", 64, 1e16), ("bf16", 128, 3e18), ("bf16", 256, 1e5), ("f16", 64, 4e4), ("f16", 128, 6e3),
+                                         ("f16", 256, 1e4)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_logits_of_any_size(kind, D, size, sign):
+    """Logits far from zero, all of one sign (to 10^36 in bf16, 10^8 in fp16). One dimension counts, so that every logit is a product:
+    the keys that hold the largest tie, the others are lost by more than fp32 tells apart. The outputs are the winners' mean; lse is
+    the largest logit to eight roundings of fp32."""
+    import torch
+    from hydra_amd.layer import Context
+    S, N, H, G, n = 2, 6, 16, 2, 300
+    t = make(torch, S, N, H, G, D, kind, n, [n, 37], seed=3, sinks=False)
+    for x in ("q", "k", "dk"):
+        t[x].zero_()
+    t["q"][..., 0] = size * (1 + torch.arange(N * H).view(1, N, H) / (N * H)) / 2
+    t["k"][..., 0], t["dk"][..., 0] = sign * size, sign * size
+    loser = torch.arange(n) % 3 == 1
+    t["k"][:, loser, :, 0] *= 0.5 if sign > 0 else 1.5
+    print(f"[gpu] tree logits {kind} D={D} {sign * size}", flush=True)
+    ctx = Context(0)
+    try:
+        for scale, most in ((None, 0), (None, 64), (0.3, 0)):
+            out, lse = call(torch, ctx, t, scale=scale, max_length=most)
+            got, want, mean = outputs_of(t, out, scale=scale)
+            assert np.isfinite(got).all()
+            before = (PARTS[kind] + 2e-5) * mean
+            assert (np.abs(got - want) <= HALF[kind] * (np.abs(want) + before) + LEAST[kind] + before).all()
+            top = (t["q"][..., 0].double() * sign * t["k"][0, 0, 0, 0].double().abs() * (D ** -0.5 if scale is None else scale)).numpy()
+            assert (np.abs(lse.double().cpu().numpy() - top) <= 8 * 2.0 ** -24 * np.abs(top) + 7).all()
+    finally:
+        ctx.close()
