@@ -53,9 +53,10 @@ __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // M follows a row's maximum by steps of at least kLag: rescaling costs more than what it keeps small, and with
-// M moved at every new maximum some row of 32 moved it at nearly every tile. p = 2^(y − M + kOff) < 2^12 fits
-// fp16, and the largest p of a row is 2^4 or more.
-constexpr float kOff = 4.f, kLag = 8.f;
+// M moved at every new maximum some row of 32 moved it at nearly every tile. p = 2^(y − M + kOff) fits fp16: at most 2^14.5, and
+// no more where the two are rounded to what fp32 holds beside M. The largest p of a row is 2^7 or more, so that fp16's smallest
+// step holds each to 2^-32 of it.
+constexpr float kOff = 7.f, kLag = 7.5f;
 constexpr float kNone = -3.402823466e38f;    // a maximum of nothing: finite, so that no difference of maxima is NaN, and below none
 
 // The ancestors-or-self of every node as bit masks, lane i node i with parent `up`; a parent that is not

@@ -446,7 +446,8 @@ typedef struct hh_kv_cache {
  * Keys that a node does not see, infinities and NaN among them, have no part in its output. Logits may be of any
  * size that fp32 holds, times log2(e).
  * Sums are held in fp32. Probabilities, and the queries of F32 activations, enter the products as pairs of the
- * cache's type: to about 2^-21 (F16) and 2^-15 (BF16). Outputs are rounded once.              */
+ * cache's type: to about 2^-21 (F16; a probability to 2^-32 of the row's largest and a query's sm_scale·log2(e)·q to 2^-25 where
+ * that is more) and 2^-15 (BF16). Outputs are rounded once.                                   */
 int hh_attention_tree(hh_ctx *ctx, const hh_tree_desc *desc, const hh_kv_cache *cache,
                       const void *q, const void *draft_k, const void *draft_v,
                       const int32_t *parents, const int32_t *node_counts, const uint16_t *sinks,

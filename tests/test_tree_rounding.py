@@ -3,6 +3,8 @@ same inputs. An output is rounded once: half a step of its type, 2^-11 (fp16, 2^
 value. What comes before that is in fp32 or as good, and its errors go by sum(p |v|), not by the output, which may be
 small beside it: a probability's two parts (2^-21 fp16, 2^-15 bf16), and 1e-5 twice for the logits' fp32 sums (at most 16 + 4
 roundings of 2^-24 of partial sums below 8) in the exponential and in the denominator."""
+import math
+
 import numpy as np
 import pytest
 
@@ -84,3 +86,28 @@ def test_logits_of_any_size(kind, D, size, sign):
             assert (np.abs(lse.double().cpu().numpy() - top) <= 8 * 2.0 ** -24 * np.abs(top) + 7).all()
     finally:
         ctx.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_a_long_tail_behind_one_key(kind):
+    """One key takes nearly all, 32767 alike share the rest, each 2^-28.5 of the largest. A probability below fp16's normal
+    range is held to 2^-32 of the row's largest, so the tail is off by at most that a key, and by 2e-5 of itself."""
+    import torch
+    from hydra_amd.layer import Context
+    n, D = 32768, 256                          # heads of 256: one wave walks all the keys of a chunk
+    t = make(torch, 1, 1, 1, 1, D, kind, n, [n], sinks=False)
+    for x in ("q", "k", "dk", "dv"):
+        t[x].zero_()
+    t["v"].fill_(1.0)
+    t["q"][..., 0], t["k"][0, 5, 0, 0], t["v"][0, 5] = 1.0, 28.5, 0.0
+    print(f"[gpu] tree tail {kind}", flush=True)
+    ctx = Context(0)
+    try:
+        out, _ = call(torch, ctx, t, scale=math.log(2.0), max_length=64)     # one chunk
+    finally:
+        ctx.close()
+    tail = (n - 1) * 2.0 ** -28.5
+    want = tail / (1 + tail + 2.0 ** -28.5)
+    off = (out.double().cpu() - want).abs().max()
+    assert off < n * 2.0 ** -32 + 2e-5 * want + (2.0 ** -11 * want if kind == "f16" else 0.0), (float(off), want)
