@@ -215,6 +215,7 @@ int hh_attention_tree(hh_ctx *ctx, const hh_tree_desc *d, const hh_kv_cache *cac
   if (!ctx) return fail(HH_EINVAL, "ctx is NULL");
   if (int rc = check_tree(d)) return rc;
   if (int rc = check_cache(d, cache)) return rc;
+  if (d->window && cache->positions) return fail(HH_EINVAL, "a window goes by the rows' order, which eviction does not keep: none with positions");
   if (!q || !draft_k || !draft_v || !parents || !node_counts || !out) return fail(HH_EINVAL, "NULL argument");
   if (!aligned16(q) || !aligned16(draft_k) || !aligned16(draft_v) || !aligned16(out))
     return fail(HH_EALIGN, "q, draft_k, draft_v and out must be 16-byte aligned");

@@ -118,7 +118,7 @@ def attention_tree_into(ctx: Context, cache: KVCache, q, draft_k, draft_v, paren
     """Attention of the drafted nodes (hh_attention_tree). q, out [S][N][q_heads][d]; draft_k, draft_v
     [S][N][kv_heads][d] of the cache's type; parents int32 [S][N], node_counts int32 [S]; sinks bf16
     (or int16 bits) [q_heads]; lse fp32 [S][N][q_heads]. q and the drafted rows may be slices with equally
-    spaced nodes. Returns `out`."""
+    spaced nodes. No window over a cache with positions. Returns `out`."""
     S, N, H, D = q.shape
     dev = cache.device
     _cuda(ctx, dev)

@@ -411,7 +411,8 @@ typedef struct hh_tree_desc {
   int32_t q_heads, kv_heads, head_dim;    /* q_heads = kv_heads x 1..16; head_dim 64, 128, 256  */
   int32_t type;                           /* hh_elem of q and out                               */
   int32_t cache_type;                     /* hh_elem of the history and the drafted k and v     */
-  int32_t window;                         /* 0, or a node at position p sees positions > p − window */
+  int32_t window;                         /* 0, or a node at position p sees positions > p − window;
+                                             not for a history with positions, whose rows have no order */
   int32_t max_length;                     /* longest expected history, 0 = the cache's rows: it
                                              sizes the launch; every length is handled          */
   float   sm_scale;                       /* finite, not 0; F32: |q·sm_scale| below 4·10^4       */
