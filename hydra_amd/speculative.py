@@ -52,7 +52,7 @@ def _spaced(t, name, got, s, shape, dtype, device):
     """The elements between nodes of a [S][N][heads][d] tensor (shape `got`, strides `s`) whose heads are packed and
     whose nodes are equally spaced: a slice of a wider product's output, or the packed tensor."""
     if got != shape or t.dtype is not dtype or t.device != device or s[3] != 1 or \
-            (s[2] != shape[3] and shape[2] > 1) or (s[0] != shape[1] * s[1] and shape[0] > 1):
+            (s[2] != shape[3] and shape[2] > 1) or (s[0] != shape[1] * s[1] and shape[0] > 1 and shape[1] > 1):
         raise ValueError(f"{name} must be a {dtype} tensor {tuple(shape)} on {device} with packed heads and equally spaced "
                          f"nodes, not {t.dtype} {tuple(got)} on {t.device} with strides {s}")
     return _step(name, s, shape, shape[2] * shape[3])
