@@ -147,8 +147,9 @@ def attention_tree_into(ctx: Context, cache: KVCache, q, draft_k, draft_v, paren
 
 
 def attention_weights_into(ctx: Context, cache: KVCache, q, lse, path, accepted, sm_scale: float | None = None):
-    """Adds the accepted nodes' attention to cache.weights (hh_attention_weights), after the commit: q and lse as
-    attention_tree_into had and gave them, path int32 [S][N], accepted int32 [S]. Returns cache.weights."""
+    """Adds the accepted nodes' attention to cache.weights (hh_attention_weights), after the commit, which must have found
+    room for all of them (rows for N nodes behind the longest length): q and lse as attention_tree_into had and gave
+    them, path int32 [S][N], accepted int32 [S]. Returns cache.weights."""
     S, N, H, D = q.shape
     dev = cache.device
     _cuda(ctx, dev)

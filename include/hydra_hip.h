@@ -392,8 +392,7 @@ int hh_combine(hh_ctx *ctx, const float *slots, const float *weights, int32_t to
  * entries below are the steps around it: attention of the tree over the history
  * (hh_attention_tree), verification against the target's probabilities (hh_draft_verify), the
  * accepted rows into the histories (hh_cache_commit), and histories of bounded size, whose rows
- * of least accumulated attention weight go (hh_attention_weights, hh_cache_evict). The reference
- * decodes one token at a time (ModelRunner.swift:110-230) and has no counterpart of them.
+ * of least accumulated attention weight go (hh_attention_weights, hh_cache_evict).
  *
  * A tree: parents int32 [S][N], parents[s][i] in 0..i−1, or −1 for a node without one (any other
  * value counts as −1); node 0 is the pending token, the last one that was sampled. node_counts
@@ -499,7 +498,8 @@ int hh_draft_verify(hh_ctx *ctx, const hh_verify_desc *desc, const void *target,
  * row lengths[s] + i of sequence s takes the drafted k and v of node path[s][i], i < accepted[s]
  * (of a ring: row (lengths[s] + i) % rows, the last `rows` of a longer path). New rows have weight 0 and
  * position next_position[s] + i. Lengths and next_position advance once, however many layers share
- * them. Rows past a history's last are dropped. desc: sequences, nodes, kv_heads, head_dim, cache_type and
+ * them. Rows past a history's last are dropped, and lengths do not say how many: keep room for N rows, by evicting in
+ * time. A path entry that names no node writes nothing, but counts: its row holds what it held. desc: sequences, nodes, kv_heads, head_dim, cache_type and
  * kv_stride.
  *   draft_k, draft_v: host arrays of `count` device pointers                                  */
 int hh_cache_commit(hh_ctx *ctx, const hh_tree_desc *desc, const hh_kv_cache *caches, int32_t count,
@@ -510,7 +510,8 @@ int hh_cache_commit(hh_ctx *ctx, const hh_tree_desc *desc, const hh_kv_cache *ca
  * weights[s][g][r] += Σ over i < accepted[s] and the heads h of group g of
  * exp(sm_scale·q[s][path[s][i]][h]·k[s][r][g] − lse[s][path[s][i]][h]), r up to the node's own row
  * lengths[s] − accepted[s] + i (all of them must have found room in the commit). q and lse are
- * hh_attention_tree's of this layer. Not for rings or windows. Each weight is summed by one wave in a fixed order.                                */
+ * hh_attention_tree's of this layer. Not for rings or windows. Where the commit dropped rows the others are taken for later ones
+ * than they are; nothing on the device tells. Each weight is summed by one wave in a fixed order.  */
 int hh_attention_weights(hh_ctx *ctx, const hh_tree_desc *desc, const hh_kv_cache *cache, const void *q,
                          const float *lse, const int32_t *path, const int32_t *accepted);
 
