@@ -621,7 +621,7 @@ __global__ __launch_bounds__(256) void weights_kernel(TreeArgs a) {
 // 64 / 8 heads of 64 at 32768 keys (F32, RT 4): KS 2 with a ring of four tiles 31.6 us, of six 32.9, KS 3 (twelve waves) 31.3;
 // before the next tile's scores were formed under the exponentials: two workgroups of KS 2 per unit 36.5, one of KS 4 41.
 // RT 4 is at the matrix unit's and the VALU's time one after the other (16 products of 32 cycles and about 100
-// instructions a tile and wave), smaller RT and heads of 128 at HBM (3 to 3.6 TB/s).
+// instructions a tile and wave; eight ragged sequences with heads of 128: 39 and 45 percent of the busy cycles at 3.3 TB/s), smaller RT at HBM.
 struct TreeShape { int rt, ks; };
 static TreeShape tree_shape(int d, int rows) {
   const int rt = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;

@@ -30,8 +30,9 @@ namespace hh {
 
 constexpr int kVT = 256;              // threads of stats and rounds
 constexpr int kWalkT = 1024;
-// Leaves' statistics are left for behind the rounds, when one a sequence is left, from this many bytes of logits on: trees of 21
-// nodes, four children a node: 83 MB 72 us with, 85 without; 42 MB 68 and 57 (a launch more, and fewer workgroups).
+// Leaves' statistics are left for behind the rounds, when one a sequence is left, from this many bytes of logits on (a launch more). Four
+// trees of V 248320, four children a node, both ways in turn on three sets of inputs: 31 nodes (119 MB) 97 to 99 us and without 110 to 113,
+// 21 nodes (79 MB) 82 to 87 and 89 to 95, 16 (60 MB) 77 to 79 and 80 to 83, 11 (40 MB) 62 to 65 and 63 to 66; 21 given nodes 40 and 45.
 constexpr size_t kLateLeaves = (size_t)64 << 20;
 
 __device__ __forceinline__ float finite_or_less(float x) { return x != x ? -INFINITY : x; }
@@ -127,8 +128,8 @@ __host__ __device__ inline VerifyPlan verify_plan(int S, int N, int V, bool alig
   VerifyPlan p{};
   const size_t rows = (size_t)S * N;
   // 4096 logits a workgroup where that makes 512 of them, else 1024 (16 or 4 a thread). Six nodes of 32000 fp32 logits:
-  // 20 us with 1024, 28 with 4096; four trees of 21 nodes of 248320, up to four children a node: 138 and 105; 16 trees of five
-  // nodes of 131071 bf16 logits, greedy: 18 and 15.
+  // 21 us with 1024, 28 with 4096; four trees of 21 nodes of 248320, up to four children a node: 100 to 103 and 82 to 87; 16 trees of
+  // five nodes of 131071 bf16 logits, greedy: 16.5 and 13.5.
   p.chunk = rows * V >= kWideChunks ? 4096 : 1024;
   p.chunks = (V + (aligned ? 0 : 3) + p.chunk - 1) / p.chunk;
   place_arrays(p, rows, rows * p.chunks);
