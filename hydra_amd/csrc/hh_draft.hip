@@ -379,6 +379,8 @@ int hh_draft_reserve(hh_ctx *ctx, const hh_tree_desc *tree, const hh_kv_cache *c
   if (!ctx) return fail(HH_EINVAL, "ctx is NULL");
   if (layers < 0 || layers > kMaxLayers) return fail(HH_EINVAL, "layers outside 0..256");
   if ((layers > 0 || cache) && (!tree || !cache)) return fail(HH_EINVAL, "a cache needs its tree description, and layers a cache");
+  // Where the workspace may not grow, the calls of these sizes themselves.
+  const bool fixed = ctx->capturing || ctx->live_graphs > 0;
   size_t need = 0;
   if (cache) {
     if (int rc = check_rows(tree)) return rc;
@@ -387,13 +389,16 @@ int hh_draft_reserve(hh_ctx *ctx, const hh_tree_desc *tree, const hh_kv_cache *c
     if (layers) need = evict_bytes(tree, per, cache->rows);
     if (tree->nodes) {
       if (int rc = check_tree(tree)) return rc;
-      const size_t b = hh::tree_reserve(tree_args(tree, cache, nullptr), tree->max_length ? tree->max_length : cache->rows);
+      hh::TreeArgs a = tree_args(tree, cache, nullptr);
+      const int64_t length = tree->max_length ? tree->max_length : cache->rows;
+      hh::tree_plan(a, length);
+      const size_t b = fixed ? hh::tree_workspace(a) : hh::tree_reserve(a, length);
       if (b > need) need = b;
     }
   }
   if (verify) {
     if (int rc = check_verify(verify)) return rc;
-    const size_t b = hh::verify_reserve(verify->sequences, verify->nodes, verify->vocab);
+    const size_t b = (fixed ? hh::verify_workspace : hh::verify_reserve)(verify->sequences, verify->nodes, verify->vocab);
     if (b > need) need = b;
   }
   HH_HIP(hipSetDevice(ctx->device));

@@ -529,7 +529,7 @@ int hh_cache_evict(hh_ctx *ctx, const hh_tree_desc *desc, const hh_kv_cache *cac
  * made): hh_attention_tree on `cache`, hh_draft_verify, and hh_cache_evict of `layers` layers like `cache`, for every
  * call with the same heads and head_dim and with sequences, nodes, rows, max_length, vocab and layers up to these, any window and
  * any `keep`. (max_length 0 counts as the cache's rows, here and in a call.) A workspace grows by itself in
- * eager calls, but not while a graph is recorded or lives.                                    */
+ * eager calls, but not while a graph is recorded or lives: then this succeeds where calls of just these sizes fit.  */
 int hh_draft_reserve(hh_ctx *ctx, const hh_tree_desc *tree, const hh_kv_cache *cache, int32_t layers,
                      const hh_verify_desc *verify);
 

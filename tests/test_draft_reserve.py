@@ -73,3 +73,27 @@ def test_verification_up_to_the_reserved_sizes(most, sizes):
     finally:
         eager.close()
         ctx.close()
+
+
+@pytest.mark.gpu
+def test_reserving_again_while_a_graph_lives():
+    """What eager calls have grown the workspace to is enough for the same calls, also where it may not grow any more."""
+    import torch
+    from hydra_amd import speculative as sp
+    from hydra_amd._lib import HydraHIPError
+    from hydra_amd.layer import Context
+    ctx = Context(0)
+    try:
+        t, v = make(torch, 1, 8, 64, 8, 64, "f32", 4160, [4160], seed=1), inputs(torch, 2, 5, 900, "f32", "iid", 2, 3)
+        tree_call(torch, ctx, t)
+        verify_call(torch, ctx, v, "iid")
+        hold = ctx.capture(lambda: None)
+        cache = sp.KVCache(t["k"].to("cuda:0"), t["v"].to("cuda:0"), t["lengths"].to("cuda:0"))
+        sp.reserve(ctx, cache, nodes=8, q_heads=64, q_dtype=torch.float32)
+        sp.reserve(ctx, verify=(2, 5, 900))
+        with pytest.raises(HydraHIPError):
+            sp.reserve(ctx, cache, nodes=64, q_heads=64, q_dtype=torch.float32)
+        hold.close()
+        sp.reserve(ctx, cache, nodes=64, q_heads=64, q_dtype=torch.float32)
+    finally:
+        ctx.close()
