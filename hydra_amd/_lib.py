@@ -24,6 +24,8 @@ EXPORTS = [
     "hh_runner_forward", "hh_runner_capture",
     "hh_attention_tree", "hh_draft_verify", "hh_cache_commit", "hh_attention_weights",
     "hh_cache_evict", "hh_draft_reserve",
+    "hh_rotary_table", "hh_rotary", "hh_history_write", "hh_history_read", "hh_history_advance",
+    "hh_history_attention", "hh_history_reserve",
 ]
 
 # int (*hh_layer_hook)(void *user, int32_t layer, void *stream)
@@ -95,6 +97,31 @@ class VerifyDescC(C.Structure):
                 ("draft_stride", C.c_int64)]
 
 
+class RotaryDescC(C.Structure):
+    _fields_ = [("head_dim", C.c_int32), ("rotated", C.c_int32), ("span", C.c_int32), ("interleaved", C.c_int32),
+                ("scaling", C.c_int32), ("original_length", C.c_int32), ("truncate", C.c_int32),
+                ("factor", C.c_float), ("beta_fast", C.c_float), ("beta_slow", C.c_float),
+                ("base", C.c_double)]
+
+
+class RotaryRowsC(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("y", C.c_void_p), ("heads", C.c_int32), ("x_stride", C.c_int64),
+                ("y_stride", C.c_int64)]
+
+
+class HistoryC(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
+                ("lengths", C.c_void_p), ("sequences", C.c_int32), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("format", C.c_int32), ("rows", C.c_int32), ("ring", C.c_int32),
+                ("pinned", C.c_int32)]
+
+
+class HistoryDescC(C.Structure):
+    _fields_ = [("tokens", C.c_int32), ("q_heads", C.c_int32), ("type", C.c_int32), ("window", C.c_int32),
+                ("first", C.c_int32), ("max_length", C.c_int32), ("sm_scale", C.c_float),
+                ("q_stride", C.c_int64)]
+
+
 _lib = None
 
 
@@ -155,6 +182,13 @@ def lib() -> C.CDLL:
     L.hh_cache_evict.argtypes = [vp, C.POINTER(TreeDescC), C.POINTER(KVCacheC), i32, i32, i32]
     L.hh_draft_reserve.argtypes = [vp, C.POINTER(TreeDescC), C.POINTER(KVCacheC), i32,
                                    C.POINTER(VerifyDescC)]
+    L.hh_rotary_table.argtypes = [C.POINTER(RotaryDescC), C.POINTER(C.c_double), C.POINTER(C.c_float)]
+    L.hh_rotary.argtypes = [vp, C.POINTER(RotaryDescC), vp, C.c_float, i32, i32, vp, C.POINTER(RotaryRowsC), i32]
+    L.hh_history_write.argtypes = [vp, C.POINTER(HistoryC), i32, vp, vp, i64, i32, vp]
+    L.hh_history_read.argtypes = [vp, C.POINTER(HistoryC), i32, vp, i32, vp, vp, vp]
+    L.hh_history_advance.argtypes = [vp, C.POINTER(HistoryC), i32, vp]
+    L.hh_history_attention.argtypes = [vp, C.POINTER(HistoryDescC), C.POINTER(HistoryC), C.POINTER(HistoryC)] + [vp] * 5
+    L.hh_history_reserve.argtypes = [vp, C.POINTER(HistoryDescC), C.POINTER(HistoryC), C.POINTER(HistoryC)]
     L.hh_ctx_profile_read.argtypes = [vp, C.POINTER(C.c_double), C.POINTER(C.c_int64)]
     for name in EXPORTS:
         if name not in ("hh_last_error", "hh_ctx_stream", "hh_dispatch_count"):

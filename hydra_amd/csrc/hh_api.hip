@@ -671,6 +671,7 @@ int hh_ctx_destroy(hh_ctx *ctx) {
   if (ctx->arena) (void)hipFree(ctx->arena);
   if (ctx->attn) (void)hipFree(ctx->attn);
   if (ctx->draft) (void)hipFree(ctx->draft);
+  if (ctx->hist) (void)hipFree(ctx->hist);
   if (ctx->arrivals) (void)hipFree(ctx->arrivals);
   if (ctx->flags) (void)hipFree(ctx->flags);
   for (hipEvent_t ev : ctx->events) (void)hipEventDestroy(ev);

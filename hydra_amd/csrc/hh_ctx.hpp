@@ -46,8 +46,11 @@ struct hh_ctx {
   uint8_t *draft = nullptr;
   size_t draft_bytes = 0;
   uint32_t *arrivals = nullptr;   // hh_cache_commit's counters, zero between its launches
+  // Workspace of hh_history_attention (hh_history.hip), grown on demand.
+  uint8_t *hist = nullptr;
+  size_t hist_bytes = 0;
   // Instantiated graphs of this context that are not yet destroyed: they hold the arena's,
-  // the attention partials' and the draft workspace's device addresses, so none may be reallocated while any exist.
+  // the attention partials' and the draft and history workspaces' device addresses, so none may be reallocated while any exist.
   int live_graphs = 0;
   // This device's copy of the static scratch array (hh_moe_forward_noalloc), or NULL when its
   // address could not be resolved (scratch_error then says why).

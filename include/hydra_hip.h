@@ -533,6 +533,122 @@ int hh_cache_evict(hh_ctx *ctx, const hh_tree_desc *desc, const hh_kv_cache *cac
 int hh_draft_reserve(hh_ctx *ctx, const hh_tree_desc *tree, const hh_kv_cache *cache, int32_t layers,
                      const hh_verify_desc *verify);
 
+/* ---- rotary positions -----------------------------------------------------------------------
+ * The step before every attention: pairs of a head's columns turn by the token's position times the pair's frequency.
+ * Pair i, i < rotated / 2, is columns i and i + span / 2, or with `interleaved` 2i and 2i + 1; its frequency is
+ * base^(−2i / span) radians a position; columns of no pair stay as they are.                     */
+typedef enum {
+  HH_ROTARY_PLAIN = 0,
+  HH_ROTARY_LINEAR = 1,   /* frequencies / factor                                               */
+  HH_ROTARY_YARN = 2      /* pairs that turn at least beta_fast times in original_length positions keep their frequency, those that turn
+                             at most beta_slow times have it divided by factor, a ramp over the pairs between; the outputs times
+                             0.1·ln(factor) + 1                                                 */
+} hh_rotary_scaling;
+
+typedef struct hh_rotary_desc {
+  int32_t head_dim;            /* a multiple of 8, 8..1024                                      */
+  int32_t rotated, span;       /* even, 2 <= rotated <= span <= head_dim; span 0 = rotated       */
+  int32_t interleaved;
+  int32_t scaling;             /* hh_rotary_scaling                                             */
+  int32_t original_length;     /* YARN                                                          */
+  int32_t truncate;            /* YARN: the ramp's ends at whole pairs                          */
+  float   factor;              /* LINEAR, YARN: 1 or more                                       */
+  float   beta_fast, beta_slow;/* YARN (32 and 1)                                               */
+  double  base;                /* above 1                                                       */
+} hh_rotary_desc;
+
+/* One tensor of a call: [tokens][heads][head_dim] with its heads packed and equally spaced tokens. `y` is x, with the
+ * same stride, or does not overlap it. 16-byte aligned; strides in elements, 0 = packed, multiples of 16 bytes. */
+typedef struct hh_rotary_rows {
+  const void *x;
+  void   *y;
+  int32_t heads;               /* 1..1024                                                       */
+  int64_t x_stride, y_stride;
+} hh_rotary_rows;
+
+/* The pairs' frequencies in turns a position (host memory, rotated / 2 numbers) and the outputs' factor: what a program keeps
+ * for a model, `turns` copied to the device. Runs on the host.                                  */
+int hh_rotary_table(const hh_rotary_desc *desc, double *turns, float *magnitude);
+
+/* Rotates `count` (1 or 2: queries, keys) tensors of `tokens` tokens (0..2^22) in one launch.
+ *   turns      device memory, hh_rotary_table's (or any other) rotated / 2 frequencies in turns a position
+ *   positions  int32 [tokens], device memory: any values
+ * Angles are formed in fp64, their sines and products in fp32, outputs rounded once to `type` (hh_elem).   */
+int hh_rotary(hh_ctx *ctx, const hh_rotary_desc *desc, const double *turns, float magnitude, int32_t type,
+              int32_t tokens, const int32_t *positions, const hh_rotary_rows *rows, int32_t count);
+
+/* ---- histories in 16, 8 and 4 bits -----------------------------------------------------------
+ * Keys and values of S sequences, heads outermost: [S][kv_heads][rows][head_dim], so that a head's rows are one
+ * stretch of memory. MXFP8 (e4m3 codes) and MXFP4 (e2m1, low nibble = even column) hold 32 columns with one e8m0 scale byte,
+ * [S][kv_heads][rows][head_dim / 32]: the least power of two, 2^-126 or more, under which no number passes the format's largest (448, 6). Numbers
+ * are rounded to the nearest, ties to even; 32 columns that hold an infinity or a NaN have scale byte 255 and are NaN.
+ *
+ * A step brings up to `tokens` new tokens a sequence, counts[s] of them real; token i has position lengths[s] + i. Lengths
+ * are what was held before the step: the calls of every layer of a step take the same, and hh_history_advance moves them on
+ * behind the last. Lengths and counts are device memory, so that a step may be recorded and replayed; values out of range
+ * count as the nearest in it (lengths 0..2^30). */
+typedef enum { HH_HISTORY_F16 = 1, HH_HISTORY_BF16 = 2, HH_HISTORY_MXFP8 = 3, HH_HISTORY_MXFP4 = 4 } hh_history_format;
+
+/* Without `ring` position p is row p, and positions from `rows` on are not held. With `ring` rows below `pinned` hold the first
+ * positions for good, and position p >= pinned is row pinned + (p − pinned) % (rows − pinned).            */
+typedef struct hh_history {
+  void    *k, *v;              /* 16-byte aligned                                               */
+  uint8_t *k_scales, *v_scales;/* MXFP8 and MXFP4, 8-byte aligned; NULL otherwise               */
+  const int32_t *lengths;      /* [S]                                                           */
+  int32_t sequences, kv_heads; /* 1..4096, 1..256                                               */
+  int32_t head_dim;            /* 64, 128, 256                                                  */
+  int32_t format;              /* hh_history_format                                             */
+  int32_t rows;                /* 1..2^28                                                       */
+  int32_t ring, pinned;        /* 0 <= pinned < rows; 0 without ring                             */
+} hh_history;
+
+/* A step's rows into the history, quantised.
+ *   k, v  type (hh_elem) [S][tokens][kv_heads][head_dim], kv_stride elements between tokens (0 = packed, a multiple of 16
+ *         bytes), 16-byte aligned. tokens 1..65536, S·tokens at most 2^22.
+ * Of a step longer than a ring its last rows. Positions that are not held are dropped.           */
+int hh_history_write(hh_ctx *ctx, const hh_history *h, int32_t type, const void *k, const void *v, int64_t kv_stride,
+                     int32_t tokens, const int32_t *counts);
+
+/* Rows back as numbers: positions starts[s] + i, i < counts[s], of sequence s to k and v (type, [S][tokens][kv_heads][head_dim],
+ * packed). Which position a ring's row holds is the caller's to know; positions below 0 and, without ring, from `rows` on
+ * leave their places as they were, as do tokens from counts[s] on.                                */
+int hh_history_read(hh_ctx *ctx, const hh_history *h, int32_t type, const int32_t *starts, int32_t tokens,
+                    const int32_t *counts, void *k, void *v);
+
+/* lengths[s] += counts[s] (0..tokens) for each of h's sequences: the end of a step.               */
+int hh_history_advance(hh_ctx *ctx, const hh_history *h, int32_t tokens, const int32_t *counts);
+
+typedef struct hh_history_desc {
+  int32_t tokens;              /* N of the step: 1..65536; S·N at most 2^22                      */
+  int32_t q_heads;             /* kv_heads x 1..16                                              */
+  int32_t type;                /* hh_elem of q and out: F32 and F16 over F16, MXFP8, MXFP4; BF16 over BF16, MXFP8, MXFP4 */
+  int32_t window, first;       /* 0: every position up to the token's own. Otherwise those above its own − window, and those below
+                                  `first`                                                       */
+  int32_t max_length;          /* the longest expected history with the step's tokens, 0 = the history's rows: it sizes the
+                                  launch; every length is handled                                */
+  float   sm_scale;            /* finite, not 0                                                 */
+  int64_t q_stride;            /* elements between tokens of q, 0 = packed; a multiple of 16 bytes */
+} hh_history_desc;
+
+/* Attention of a step's tokens, one a sequence or a whole prompt, over the history that they have been written to
+ * (hh_history_write before this): token i of sequence s sees positions up to its own, by window and first. A ring needs
+ * a window of its own: window + tokens − 1 <= rows − pinned, first <= pinned.
+ *   q, out  type [S][N][q_heads][head_dim] (q with q_stride), 16-byte aligned
+ *   sinks   bf16 [q_heads] or NULL: a logit in the denominator only
+ *   lse     fp32 [S][N][q_heads] or NULL: the log of the denominator
+ *   prefix  NULL, or a history of one sequence (same heads, head_dim and format; no ring; window 0): its lengths[0] rows come before
+ *           every sequence's own and are seen by each token. They are read once for the batch.
+ * Tokens from counts[s] on are not written. A token that sees nothing (its own position not held) gets 0 and lse −inf, or with a sink the
+ * sink. Keys that a token does not see, infinities and NaN among them, have no part in its output. Logits may be of any size that
+ * fp32 holds, times log2(e).                                                                      */
+int hh_history_attention(hh_ctx *ctx, const hh_history_desc *desc, const hh_history *h, const hh_history *prefix,
+                         const void *q, const int32_t *counts, const uint16_t *sinks, void *out, float *lse);
+
+/* Pre-sizes the context's workspace of hh_history_attention for every call with these heads, head_dim, type and format, and with
+ * sequences, tokens, rows, max_length and prefix rows up to these, any window. It grows by itself in eager calls, but not while a graph is
+ * recorded or lives: then this succeeds where a call of just these sizes fits.                    */
+int hh_history_reserve(hh_ctx *ctx, const hh_history_desc *desc, const hh_history *h, const hh_history *prefix);
+
 #ifdef __cplusplus
 }
 #endif
