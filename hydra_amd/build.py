@@ -20,7 +20,8 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libhydra_hip.so")
 SOURCES = ["hh_api.hip", "hh_route.hip", "hh_gemm.hip", "hh_gemm_block.hip", "hh_prefill.hip", "hh_ops.hip", "hh_attn.hip", "hh_block.hip", "hh_proj.hip",
            "hh_tree.hip", "hh_verify.hip", "hh_cache.hip", "hh_draft.hip",
-           "hh_history.hip", "hh_rotary.hip", "hh_hist_rows.hip", "hh_hist_attn.hip"]
+           "hh_history.hip", "hh_rotary.hip", "hh_hist_rows.hip", "hh_hist_attn.hip",
+           "hh_hist_attn_64.hip", "hh_hist_attn_128.hip", "hh_hist_attn_256.hip"]
 
 
 def hipcc() -> str:

@@ -38,6 +38,14 @@ struct HistAttnArgs {
   int S, N, qh, kvh, d, qm, window, first, format;
   float scale;
   int64_t q_stride;
+  // How the work is split (history_plan). A pass is over the sequences' own histories or over the prefix, whose rows are those of
+  // all sequences' tokens; its keys are cut into chunks of `per` keys, whole tiles.
+  struct Pass {
+    int chunks, per, tile, block_rows, row_blocks;
+  } own, pre;
+  int chunks;                          // of a row, the prefix's first
+  int shared;                          // the kernel's pass
+  float *pm, *pl, *po;                 // chunk states [S][N][qh][chunks], their sums [..][chunks][d]
 };
 
 struct RotaryRows {
@@ -69,7 +77,11 @@ __device__ __forceinline__ float hist_scale(uint32_t b) { return b == 255 ? __ui
 hipError_t launch_history_write(const HistRowsArgs &a, hipStream_t s);
 hipError_t launch_history_read(const HistRowsArgs &a, hipStream_t s);
 hipError_t launch_history_advance(int32_t *lengths, const int32_t *counts, int S, int N, hipStream_t s);
-hipError_t launch_history_attention(const HistAttnArgs &a, int type, hipStream_t s, int *launches);
+void history_plan(HistAttnArgs &a, int64_t length, int64_t prefix_rows);
+size_t history_workspace(const HistAttnArgs &a);
+size_t history_reserve(const HistAttnArgs &a, int64_t length, int64_t prefix_rows);   // of every call up to these sizes
+hipError_t launch_history_attention(HistAttnArgs a, int type, hipStream_t s, int *launches);
+template <int D> hipError_t launch_history_attention_d(HistAttnArgs a, int type, hipStream_t s, int *launches);
 hipError_t launch_rotary(RotaryArgs a, hipStream_t s);
 
 }  // namespace hh

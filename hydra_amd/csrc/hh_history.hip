@@ -13,6 +13,28 @@ constexpr int kMaxSequences = 4096, kMaxTokens = 65536, kMaxRows = 1 << 28, kMax
 bool aligned(const void *p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 bool elem(int32_t type) { return type >= HH_F32 && type <= HH_BF16; }
 
+// The workspace grows in eager calls; recorded graphs hold its address.
+int ensure_history(hh_ctx *ctx, size_t bytes) {
+  if (ctx->hist_bytes >= bytes) return HH_OK;
+  if (ctx->capturing || ctx->live_graphs > 0)
+    return fail(HH_EINVAL, "the call needs a larger history workspace, which may not grow while a graph of this context is recorded "
+                           "or lives (hh_history_reserve before capture)");
+  if (ctx->hist) {
+    HH_HIP(hipStreamSynchronize(ctx->stream));
+    HH_HIP(hipFree(ctx->hist));
+    ctx->hist = nullptr;
+    ctx->hist_bytes = 0;
+  }
+  void *p = nullptr;
+  if (hipMalloc(&p, bytes) != hipSuccess) {
+    (void)hipGetLastError();
+    return fail(HH_ENOMEM, "history workspace allocation failed");
+  }
+  ctx->hist = (uint8_t *)p;
+  ctx->hist_bytes = bytes;
+  return HH_OK;
+}
+
 int check_rotary(const hh_rotary_desc *d) {
   if (!d) return fail(HH_EINVAL, "desc is NULL");
   if (d->head_dim < 8 || d->head_dim > 1024 || d->head_dim % 8) return fail(HH_ESHAPE, "head_dim must be a multiple of 8, 8..1024");
@@ -268,6 +290,12 @@ int hh_history_attention(hh_ctx *ctx, const hh_history_desc *d, const hh_history
   a.out = out;
   a.lse = lse;
   HH_HIP(hipSetDevice(ctx->device));
+  hh::history_plan(a, d->max_length ? d->max_length : h->rows, prefix ? prefix->rows : 0);
+  if (int rc = ensure_history(ctx, hh::history_workspace(a))) return rc;
+  const size_t slots = (size_t)a.S * a.N * a.qh * a.chunks;
+  a.po = (float *)ctx->hist;
+  a.pm = a.po + slots * a.d;
+  a.pl = a.pm + slots;
   int launches = 0;
   HH_HIP(hh::launch_history_attention(a, d->type, ctx->stream, &launches));
   ctx->dispatches += launches;
@@ -276,7 +304,18 @@ int hh_history_attention(hh_ctx *ctx, const hh_history_desc *d, const hh_history
 
 int hh_history_reserve(hh_ctx *ctx, const hh_history_desc *d, const hh_history *h, const hh_history *prefix) {
   if (!ctx) return fail(HH_EINVAL, "ctx is NULL");
-  return check_attention(d, h, prefix);
+  if (int rc = check_attention(d, h, prefix)) return rc;
+  hh::HistAttnArgs a = attention_args(d, h, prefix);
+  const int64_t length = d->max_length ? d->max_length : h->rows;
+  size_t need;
+  if (ctx->capturing || ctx->live_graphs > 0) {   // where the workspace may not grow, a call of these sizes itself
+    hh::history_plan(a, length, prefix ? prefix->rows : 0);
+    need = hh::history_workspace(a);
+  } else {
+    need = hh::history_reserve(a, length, prefix ? prefix->rows : 0);
+  }
+  HH_HIP(hipSetDevice(ctx->device));
+  return ensure_history(ctx, need);
 }
 
 }  // extern "C"
