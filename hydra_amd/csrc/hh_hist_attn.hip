@@ -10,7 +10,7 @@ constexpr int kHistChunks = 256;             // most chunks of a pass
 static HistAttnArgs::Pass plan_pass(const HistAttnArgs &a, int64_t rows, int64_t heads, int64_t keys) {
   HistAttnArgs::Pass p{};
   const bool few = rows <= kFewRows;
-  p.block_rows = few ? kFewRows : 128;
+  p.block_rows = rows <= 16 ? 16 : few ? kFewRows : 128;
   p.row_blocks = (int)((rows + p.block_rows - 1) / p.block_rows);
   p.tile = few ? 128 : a.d == 256 ? 32 : 64;
   const int64_t most = (keys + p.tile - 1) / p.tile;

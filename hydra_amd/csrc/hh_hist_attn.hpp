@@ -17,7 +17,7 @@
 
 namespace hh {
 
-constexpr int kFewRows = 32;                 // rows of a kv head up to which a wave takes all of them
+constexpr int kFewRows = 32;                 // rows of a kv head up to which a wave takes all of them, 16 or 32
 
 template <int QT, int FMT> struct HistTypes {
   static constexpr bool BF = FMT != H_F16, MX = FMT >= H_MXFP8;
@@ -26,15 +26,20 @@ template <int QT, int FMT> struct HistTypes {
   static constexpr int NP = QT == E_F32 && BF ? 3 : 2;                                          // of a probability
 };
 
-// 16 bytes of a row and their scale byte as MFMA operands of eight numbers. Scale byte 0 (2^-127) gives 0 or what it stands for; 255 is the
-// caller's to see to.
-template <int FMT> __device__ __forceinline__ void widen(const u32x4 &raw, uint32_t scale, u32x4 (&out)[HistTypes<0, FMT>::E / 8]) {
+// Memory that is read as the device's own: a load that could be of LDS too would wait with LDS's.
+typedef const uint8_t __attribute__((address_space(1))) *gptr_t;
+template <typename V> __device__ __forceinline__ V load_global(gptr_t p) { return *(const V __attribute__((address_space(1))) *)p; }
+
+// N bytes of a row (16, or 8 of MXFP4) and their scale byte as MFMA operands of eight numbers. Scale byte 0 gives 0 or 2^-127; 255 is
+// the caller's to see to.
+constexpr uint32_t kNan2 = 0x7FC07FC0u;
+template <int FMT, int N> __device__ __forceinline__ void widen(const uint32_t (&raw)[N / 4], uint32_t scale, u32x4 (&out)[HistTypes<0, FMT>::E * N / 128]) {
   if constexpr (FMT == H_F16 || FMT == H_BF16) {
-    out[0] = raw;
+    out[0] = u32x4{raw[0], raw[1], raw[2], raw[3]};
   } else {
     const float by = __uint_as_float(scale << 23);
 #pragma unroll
-    for (int x = 0; x < HistTypes<0, FMT>::E / 8; ++x) {
+    for (int x = 0; x < HistTypes<0, FMT>::E * N / 128; ++x) {
       if constexpr (FMT == H_MXFP8) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -93,7 +98,7 @@ struct Block {
   int s, g, r0, count, chunk, c0, nc;       // keys c0 .. c0 + nc − 1
   Visible v;
   int first_low, last_low, first_high;      // of the first and the last row
-  uint64_t k, v_, ks, vs;                   // the head's rows
+  gptr_t k, v_, ks, vs;                     // the head's rows
   int rows, span, pinned, delta;            // position -> row
 };
 __device__ __forceinline__ int row_low(const HistAttnArgs &a, const Visible &v, int i) {
@@ -130,10 +135,10 @@ template <int FMT, int D> __device__ __forceinline__ bool block_of(const HistAtt
   b.c0 = (int)c0;
   b.nc = min(per, b.v.n - b.c0);
   const int64_t base = (int64_t)sg * h.rows;                 // sg counts the prefix's heads too
-  b.k = (uint64_t)(h.k + base * hist_row_bytes(FMT, D));
-  b.v_ = (uint64_t)(h.v + base * hist_row_bytes(FMT, D));
-  b.ks = (uint64_t)(h.ks + base * (D / 32));
-  b.vs = (uint64_t)(h.vs + base * (D / 32));
+  b.k = (gptr_t)h.k + base * hist_row_bytes(FMT, D);
+  b.v_ = (gptr_t)h.v + base * hist_row_bytes(FMT, D);
+  b.ks = (gptr_t)h.ks + base * (D / 32);
+  b.vs = (gptr_t)h.vs + base * (D / 32);
   b.rows = h.rows;
   b.pinned = h.ring ? h.pinned : 0;
   b.span = h.rows - b.pinned;
@@ -150,6 +155,13 @@ __device__ __forceinline__ int key_row(const Block &b, int j) {
   const int p = j < b.v.fold ? j : j - b.v.fold + b.v.low;
   int r = p < b.pinned ? p : p + b.delta;
   return r >= b.rows ? r - b.span : r;
+}
+// Whether keys j .. j + n − 1 are all there, in consecutive rows.
+__device__ __forceinline__ bool in_a_row(const Block &b, int j, int n) {
+  if (j + n > b.v.n || (j < b.v.fold && j + n > b.v.fold)) return false;
+  const int p = j < b.v.fold ? j : j - b.v.fold + b.v.low;
+  if (p < b.pinned) return p + n <= b.pinned;
+  return p + b.delta >= b.rows || p + b.delta + n <= b.rows;
 }
 // The first x of 32 keys.
 __device__ __forceinline__ uint32_t first_keys(int x) { return x >= 32 ? 0xFFFFFFFFu : x <= 0 ? 0u : (1u << x) - 1; }
@@ -217,20 +229,29 @@ template <int QT, bool BF, int NQ> __device__ __forceinline__ void query_terms(c
   }
 }
 
-// Two probabilities as NP terms: bf16 by cutting off, the last rounded.
-template <bool BF, int NP> __device__ __forceinline__ void split_terms(float p0, float p1, float minus1, uint32_t (&w)[NP]) {
+// Two probabilities as NP terms: bf16 by cutting off, the last rounded. What is left of a probability is exact, as the sum of it and −1
+// times its head, which the dot product takes from the packed heads: one instruction in place of a mask and a subtraction. The constants
+// are registers: as immediates, (−1, 0) and (0, −1) in bf16 come out alike.
+struct SplitConst {
+  float minus1;
+  uint32_t m0, m1;
+  __device__ __forceinline__ SplitConst() : minus1(-1.f), m0(0x0000BF80u), m1(0xBF800000u) { asm volatile("" : "+s"(minus1), "+s"(m0), "+s"(m1)); }
+};
+template <bool BF, int NP> __device__ __forceinline__ void split_terms(float p0, float p1, const SplitConst &k, uint32_t (&w)[NP]) {
   if constexpr (!BF) {
-    const u32x2 v = split_pair(p0, p1, minus1);
+    const u32x2 v = split_pair(p0, p1, k.minus1);
     w[0] = v[0], w[1] = v[1];
   } else {
-    if constexpr (NP == 3) {
-      const uint32_t u0 = __float_as_uint(p0), u1 = __float_as_uint(p1);
-      w[0] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
-      p0 -= __uint_as_float(u0 & 0xFFFF0000u);
-      p1 -= __uint_as_float(u1 & 0xFFFF0000u);
+    const bf16x2 m0 = __builtin_bit_cast(bf16x2, k.m0), m1 = __builtin_bit_cast(bf16x2, k.m1);
+#pragma unroll
+    for (int t = 0; t + 1 < NP; ++t) {
+      w[t] = __builtin_amdgcn_perm(__float_as_uint(p1), __float_as_uint(p0), 0x07060302u);
+      const bf16x2 h = __builtin_bit_cast(bf16x2, w[t]);
+      p0 = __builtin_amdgcn_fdot2_f32_bf16(h, m0, p0, false);
+      p1 = __builtin_amdgcn_fdot2_f32_bf16(h, m1, p1, false);
     }
-    const u32x2 v = split_pair_bf16(p0, p1);
-    w[NP - 2] = v[0], w[NP - 1] = v[1];
+    const bf16x2 l = {(__bf16)p0, (__bf16)p1};
+    w[NP - 1] = __builtin_bit_cast(uint32_t, l);
   }
 }
 
@@ -300,203 +321,250 @@ __device__ void put_odd(const Block &b, int first, int low, int high, int j0, in
   }
 }
 
-// The rows' state over a run of 32 keys at a time.
-template <int QT, int FMT, int D> struct RowState {
-  using T = HistTypes<QT, FMT>;
-  static constexpr int NB = D / 32;
-  float M = kNone, L = 0.f;
-  f32x16 acc[NB];
-  __device__ __forceinline__ void init() {
+// Logits of a run of keys to probabilities 2^(y − R), y = S·scale, and the sums on: N of them a lane, its row's shared with the lanes
+// that `top_of` exchanges with. R follows the row's maximum y, less kOff, by steps of at least kLag. The product and the difference
+// are one fma; where some R is so far from zero that the product's lost bits would matter, y is rounded first, as R was. After a step of R
+// the sums so far are off by what this returns (1: none).
+constexpr float kFar = 65536.f;
+template <int N, typename V, typename F>
+__device__ __forceinline__ float to_probabilities(V &S, float scale, float &R, float &L, bool &far, F top_of) {
+  auto relative = [&](float (&y)[N]) {
+    if (far) {
 #pragma unroll
-    for (int n = 0; n < NB; ++n) acc[n] = f32x16{};
+      for (int i = 0; i < N; ++i) y[i] = S[i] * scale - R;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) y[i] = fmaf(S[i], scale, -R);
+    }
+  };
+  auto largest = [&](const float (&y)[N]) {
+    float top = fmaxf(y[0], y[1]);
+#pragma unroll
+    for (int i = 2; i < N; i += 2) top = fmaxf(fmaxf(top, y[i]), y[i + 1]);
+    return top_of(top);
+  };
+  float y[N], corr = 1.f;
+  relative(y);
+  if (__any(largest(y) > kOff + kLag)) {
+    float r[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = S[i] * scale;
+    const float to = fmaxf(R, largest(r) - kOff);
+    corr = exp2_(R - to);
+    R = to;
+    L *= corr;
+    far = __any(fabsf(R) > kFar && R > kNone);
+    relative(y);
   }
-  // S, in element i the logit of key 8 (i / 4) + 4 hh + i % 4, to probabilities: `sees` has a bit a key, from this lane's first.
-  // `mem`: the values [32][D] in LDS, 16-byte pieces XORed by the row; vcol: this lane's part of reading them by columns.
-  __device__ __forceinline__ void softmax(f32x16 &S, bool part, uint32_t sees, float scale) {
-    if constexpr (QT != E_F32) S *= scale;                   // rounded to y once, before the maximum
-    if (part) {
+  float sum[2] = {0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 16; ++i) S[i] = sees >> (8 * (i >> 2) + (i & 3)) & 1 ? S[i] : -INFINITY;
-    }
-    float top = fmaxf(S[0], S[1]);
-#pragma unroll
-    for (int i = 2; i < 16; ++i) top = fmaxf(top, S[i]);
-    top = max_halves(top);
-    if (__any(top - M > kLag)) {
-      const float mn = fmaxf(M, top), corr = exp2_(M - mn);
-      M = mn;
-      L *= corr;
-#pragma unroll
-      for (int n = 0; n < NB; ++n) acc[n] *= corr;
-    }
-    const float sub = kOff - M;
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      S[i] = exp2_(S[i] + sub);
-      sum[i & 3] += S[i];
-    }
-    L += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  for (int i = 0; i < N; ++i) {
+    S[i] = exp2_(y[i]);
+    sum[i & 1] += S[i];
   }
-  __device__ __forceinline__ void values(const f32x16 &S, const uint8_t *vcol, int vpiece, float minus1) {
-#pragma unroll
-    for (int kc = 0; kc < 2; ++kc) {
-      u32x4 p[T::NP];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t w[T::NP];
-        split_terms<T::BF, T::NP>(S[8 * kc + 2 * e], S[8 * kc + 2 * e + 1], minus1, w);
-#pragma unroll
-        for (int t = 0; t < T::NP; ++t) p[t][e] = w[t];
-      }
-#pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        u32x4 vf;
-#pragma unroll
-        for (int x8 = 0; x8 < 2; ++x8) {
-          const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) s16x4 *)(vcol + (16 * kc + 8 * x8) * 2 * D + ((vpiece ^ (4 * n)) << 4)));
-          const u32x2 v = __builtin_bit_cast(u32x2, w);
-          vf[2 * x8] = v[0];
-          vf[2 * x8 + 1] = v[1];
-        }
-#pragma unroll
-        for (int t = 0; t < T::NP; ++t) acc[n] = mfma32<T::BF>(vf, p[t], acc[n]);
-      }
-    }
-  }
-};
-__device__ __forceinline__ int piece_xor(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+  L += sum[0] + sum[1];
+  return corr;
+}
 
-// Few rows: each wave has all of a kv head's (up to 32) and tiles of 32 keys of its own, W of them a workgroup; the next tile's bytes are
-// in flight under this one's products. Keys go from memory to the operands' registers: the order of a product's columns is free, so
-// that a lane's 16 bytes are its own; values pass through LDS to be read by columns. No barrier until the waves' states meet.
-template <int QT, int FMT, int D, int W, int OCC>
+__device__ __forceinline__ int piece_xor(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+template <bool BF> __device__ __forceinline__ f32x4 mfma16(const u32x4 &a, const u32x4 &b, const f32x4 &c) {
+  if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ u32x2 read_columns(const uint8_t *p) {   // transposing: four rows of the lane's column
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p));
+}
+
+// Few rows: each wave has all of a kv head's, 16·RT, and tiles of 32 keys of its own, W of them a workgroup; the next tile's bytes are
+// in flight under this one's products. On the 16x16 MFMA, S^T [16 keys × 16 rows] twice a tile: a head of 64 in 8 bits is 64 bytes, four
+// lanes of a key, so that a load is one stretch of memory, and goes to the operands' registers as it is, since the order of a product's
+// columns is free. Values pass through LDS to be read by columns. No barrier until the waves' states meet.
+template <int QT, int FMT, int D, int RT, int W, int OCC>
 __global__ __launch_bounds__(64 * W, OCC) void history_few_kernel(HistAttnArgs a) {
   using T = HistTypes<QT, FMT>;
-  constexpr int E = T::E, U = D / (2 * E), X = E / 8, RB = D * 16 / E, NB = D / 32, ROWS = 32;
-  __shared__ __align__(1024) uint8_t s_mem[W * ROWS * D * 4];
+  constexpr int E = T::E, RB = D * 16 / E, PB = RB / 4 < 16 ? RB / 4 : 16, U = RB / 4 / PB, EP = PB * E / 16, X = EP / 8;
+  constexpr int NF = D / 32, NB = D / 16, ROWS = 16 * RT;   // operands of a query or of 16 keys; blocks of 16 value columns
+  __shared__ __align__(1024) uint8_t s_mem[W * (ROWS * D * 4 > 64 * D ? ROWS * D * 4 : 64 * D)];
   __shared__ float s_m[W][ROWS], s_l[W][ROWS];
   __shared__ int s_lo[ROWS], s_hi[ROWS], s_odd;
   warm_kernargs<sizeof(HistAttnArgs)>();
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, hh = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, quad = lane >> 4;
   const int heads = a.shared ? a.kvh : a.S * a.kvh;
   Block b;
   if (!block_of<FMT, D>(a, (int)(blockIdx.x % heads), 0, (int)(blockIdx.x / heads), b)) return;
-  const Row row = row_of(a, b, l32);
-  u32x4 q[D / 16][T::NQ];                    // fragment u·X + x: columns 2E u + E hh + 8 x
-  {
-    const int64_t at = ((int64_t)row.s * a.N + row.i) * a.q_stride + (int64_t)row.head * D + E * hh;
+  u32x4 q[RT][NF][T::NQ];                    // operand u·X + x: columns EP (4 u + quad) + 8 x
+  int low[RT], high[RT];
 #pragma unroll
-    for (int f = 0; f < D / 16; ++f)
-      query_terms<QT, T::BF, T::NQ>(a.q, at + 2 * E * (f / X) + 8 * (f % X), a.scale * kLog2e, q[f]);
+  for (int r = 0; r < RT; ++r) {
+    const Row row = row_of(a, b, 16 * r + l16);
+    low[r] = row.low, high[r] = row.high;
+    if (wave == 0 && quad == 0) s_lo[16 * r + l16] = row.low, s_hi[16 * r + l16] = row.high;
+    const int64_t at = ((int64_t)row.s * a.N + row.i) * a.q_stride + (int64_t)row.head * D + EP * quad;
+#pragma unroll
+    for (int f = 0; f < NF; ++f) query_terms<QT, T::BF, T::NQ>(a.q, at + 4 * EP * (f / X) + 8 * (f % X), a.scale * kLog2e, q[r][f]);
   }
-  const float scale = a.scale * kLog2e;
-  if (wave == 0 && hh == 0) s_lo[l32] = row.low, s_hi[l32] = row.high;
+  const float scale = QT == E_F32 ? 1.f : a.scale * kLog2e;
   if (tid == 0) s_odd = 0;
   __syncthreads();
 
   const int tiles = (b.nc + 31) / 32;
-  struct Raw {
-    u32x4 k[U], v[U];
-    uint64_t ks, vs;
-  } raw;
   typedef typename std::conditional<D == 64, uint16_t, typename std::conditional<D == 128, uint32_t, uint64_t>::type>::type scales_t;
+  typedef typename std::conditional<PB == 16, u32x4, u32x2>::type piece_t;
+  piece_t raw[2][2][U];                      // keys and values, 16 keys, pieces
+  scales_t rs[2][2];
   auto fetch = [&](int t) {
-    const uint64_t r = key_row(b, b.c0 + 32 * t + l32);
-    const uint64_t at = r * RB + 16 * hh;
+    const int j = b.c0 + 32 * t;
+    gptr_t at[2][2], sc[2][2];
+    if (in_a_row(b, j, 32)) {
+      const int64_t r = key_row(b, j);
+      const uint32_t o = (uint32_t)(l16 * RB + quad * PB), so = (uint32_t)(l16 * (D / 32));
 #pragma unroll
-    for (int u = 0; u < U; ++u) raw.k[u] = *(const u32x4 *)(b.k + at + 32 * u);
-    if constexpr (T::MX) raw.ks = *(const scales_t *)(b.ks + r * (D / 32));
+      for (int kg = 0; kg < 2; ++kg) {
+        at[0][kg] = b.k + r * RB + 16 * kg * RB + o;
+        at[1][kg] = b.v_ + r * RB + 16 * kg * RB + o;
+        sc[0][kg] = b.ks + r * (D / 32) + 16 * kg * (D / 32) + so;
+        sc[1][kg] = b.vs + r * (D / 32) + 16 * kg * (D / 32) + so;
+      }
+    } else {
 #pragma unroll
-    for (int u = 0; u < U; ++u) raw.v[u] = *(const u32x4 *)(b.v_ + at + 32 * u);
-    if constexpr (T::MX) raw.vs = *(const scales_t *)(b.vs + r * (D / 32));
+      for (int kg = 0; kg < 2; ++kg) {
+        const int64_t r = key_row(b, j + 16 * kg + l16);
+        at[0][kg] = b.k + r * RB + quad * PB;
+        at[1][kg] = b.v_ + r * RB + quad * PB;
+        sc[0][kg] = b.ks + r * (D / 32);
+        sc[1][kg] = b.vs + r * (D / 32);
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+      for (int kg = 0; kg < 2; ++kg) {
+        if constexpr (T::MX) rs[v][kg] = load_global<scales_t>(sc[v][kg]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[v][kg][u] = load_global<piece_t>(at[v][kg] + 4 * PB * u);
+      }
   };
-  auto scale_of = [&](uint64_t s, int u) { return (uint32_t)(s >> (FMT == H_MXFP4 ? 8 * (2 * u + hh) : 8 * u)) & 0xFFu; };
+  // The scale byte of piece u: its 32 columns are EP (4 u + quad) / 32.
+  const int sshift = 8 * (EP * quad / 32);
+  auto scale_of = [&](scales_t s, int u) { return (uint32_t)(s >> sshift >> 8 * (4 * EP * u / 32)) & 0xFFu; };
+  auto operands = [&](int v, int kg, int u, u32x4 (&w)[X]) {
+    uint32_t x[PB / 4];
+#pragma unroll
+    for (int i = 0; i < PB / 4; ++i) x[i] = raw[v][kg][u][i];
+    const uint32_t sc = T::MX ? scale_of(rs[v][kg], u) : 0;
+    widen<FMT, PB>(x, sc, w);
+    if (T::MX && __any(sc == 255)) {
+      if (sc == 255)
+#pragma unroll
+        for (int i = 0; i < X; ++i) w[i] = u32x4{kNan2, kNan2, kNan2, kNan2};
+    }
+  };
   auto is_part = [&](int t) {
     const int j = b.c0 + 32 * t;
     return j + 31 > b.first_high || (j + 32 > a.first && j < b.last_low);
   };
-  RowState<QT, FMT, D> st;
-  st.init();
-  float minus1 = -1.f;
-  asm volatile("" : "+s"(minus1));
-  uint8_t *vmem = s_mem + wave * (32 * D * 2);
-  const int j16 = lane & 15;
-  const int vrow = 4 * hh + (j16 >> 2), vpiece = (2 * ((lane >> 4) & 1) + ((j16 & 3) >> 1)) ^ piece_xor(vrow);
+  float R[RT], L[RT];
+  bool far[RT];
+  f32x4 acc[RT][NB];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    R[r] = kNone, L[r] = 0.f, far[r] = false;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) acc[r][n] = f32x4{};
+  }
+  const SplitConst kSplit;
+  uint8_t *vmem = s_mem + wave * (64 * D);
+  const int j16 = lane & 15, vrow = 4 * quad + (j16 >> 2), vpiece = ((j16 & 3) >> 1) ^ piece_xor(vrow);
   const uint8_t *vcol = vmem + vrow * (2 * D) + (j16 & 1) * 8;
   if (wave < tiles) fetch(wave);
   for (int t = wave; t < tiles; t += W) {
     const bool part = is_part(t);
-    u32x4 kf[D / 16];
-    bool bad = false;
+    f32x4 S[RT][2];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      u32x4 w[X];
-      const uint32_t sc = T::MX ? scale_of(raw.ks, u) : 0;
-      widen<FMT>(raw.k[u], sc, w);
-      if constexpr (T::MX) bad |= sc == 255;
+    for (int r = 0; r < RT; ++r) S[r][0] = S[r][1] = f32x4{};
 #pragma unroll
-      for (int x = 0; x < X; ++x) kf[u * X + x] = w[x];
-    }
-    if (T::MX && __any(bad)) {
+    for (int kg = 0; kg < 2; ++kg)
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (scale_of(raw.ks, u) == 255)
+      for (int u = 0; u < U; ++u) {
+        u32x4 w[X];
+        operands(0, kg, u, w);
 #pragma unroll
-          for (int x = 0; x < X; ++x) kf[u * X + x] = u32x4{0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u};
-    }
-    f32x16 S = f32x16{};
+        for (int x = 0; x < X; ++x)
 #pragma unroll
-    for (int f = 0; f < D / 16; ++f)
+          for (int r = 0; r < RT; ++r)
 #pragma unroll
-      for (int n = 0; n < T::NQ; ++n) S = mfma32<T::BF>(kf[f], q[f][n], S);
+            for (int n = 0; n < T::NQ; ++n) S[r][kg] = mfma16<T::BF>(w[x], q[r][u * X + x][n], S[r][kg]);
+      }
     asm volatile("" ::: "memory");           // the wave's last tile has been read: LDS takes its accesses in their order
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      u32x4 w[X];
-      const uint32_t sc = T::MX ? scale_of(raw.vs, u) : 0;
-      widen<FMT>(raw.v[u], sc, w);
-      if (T::MX && __any(sc == 255)) {
-        if (sc == 255)
+    for (int kg = 0; kg < 2; ++kg)
 #pragma unroll
-          for (int x = 0; x < X; ++x) w[x] = u32x4{0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u};
+      for (int u = 0; u < U; ++u) {
+        u32x4 w[X];
+        operands(1, kg, u, w);
+        if (part) {
+          bool odd = false;
+#pragma unroll
+          for (int x = 0; x < X; ++x) odd |= take_odd<T::BF>(w[x]);
+          if (odd) s_odd = 1;
+        }
+        const int row = 16 * kg + l16;
+#pragma unroll
+        for (int x = 0; x < X; ++x)
+          *(u32x4 *)(vmem + row * (2 * D) + ((EP * (4 * u + quad) / 8 + x ^ piece_xor(row)) << 4)) = w[x];
       }
-      if (part) {
-        bool odd = false;
-#pragma unroll
-        for (int x = 0; x < X; ++x) odd |= take_odd<T::BF>(w[x]);
-        if (odd) s_odd = 1;
-      }
-#pragma unroll
-      for (int x = 0; x < X; ++x)
-        *(u32x4 *)(vmem + l32 * (2 * D) + (((2 * E * u + E * hh + 8 * x) / 8 ^ piece_xor(l32)) << 4)) = w[x];
-    }
     asm volatile("" ::: "memory");           // the rows are read by other lanes than wrote them, behind the writes
     if (t + W < tiles) fetch(t + W);
-    uint32_t sees = 0;
-    if (part) {
-      const int j = b.c0 + 32 * t;
-      sees = ((~first_keys(row.low - j) | first_keys(a.first - j)) & first_keys(row.high + 1 - j)) >> (4 * hh);
+    u32x4 p[RT][T::NP];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      // Element 4 kg + i is key 16 kg + 4 quad + i of the 32.
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = S[r][i >> 2][i & 3];
+      if (part) {
+        const int j = b.c0 + 32 * t;
+        const uint32_t sees = ((~first_keys(low[r] - j) | first_keys(a.first - j)) & first_keys(high[r] + 1 - j)) >> (4 * quad);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = sees >> (16 * (i >> 2) + (i & 3)) & 1 ? y[i] : scale < 0.f ? INFINITY : -INFINITY;
+      }
+      const float corr = to_probabilities<8>(y, scale, R[r], L[r], far[r], [](float v) { return max_lane_groups(v); });
+      if (__any(corr != 1.f))
+#pragma unroll
+        for (int n = 0; n < NB; ++n) acc[r][n] *= corr;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t w[T::NP];
+        split_terms<T::BF, T::NP>(y[2 * e], y[2 * e + 1], kSplit, w);
+#pragma unroll
+        for (int n = 0; n < T::NP; ++n) p[r][n][e] = w[n];
+      }
     }
-    st.softmax(S, part, sees, scale);
-    st.values(S, vcol, vpiece, minus1);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const u32x2 v0 = read_columns(vcol + ((vpiece ^ (2 * n)) << 4)), v1 = read_columns(vcol + 32 * D + ((vpiece ^ (2 * n)) << 4));
+      const u32x4 vf = {v0[0], v0[1], v1[0], v1[1]};
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int k = 0; k < T::NP; ++k) acc[r][n] = mfma16<T::BF>(vf, p[r][k], acc[r][n]);
+    }
   }
 
   // The waves' states meet in LDS, the sums of a row in 16-byte pieces XORed by the row.
-  st.L += other_half(st.L);
   __syncthreads();
-  float *so = (float *)s_mem + (size_t)(wave * ROWS + l32) * D;
-  if (hh == 0) {
-    s_m[wave][l32] = st.M - kOff;            // the exponent that L and O are relative to
-    s_l[wave][l32] = st.L;
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int row = 16 * r + l16;
+    const float l = sum_lane_groups(L[r]);
+    if (quad == 0) {
+      s_m[wave][row] = R[r];                 // the exponent that L and O are relative to
+      s_l[wave][row] = l;
+    }
+    float *so = (float *)s_mem + (size_t)(wave * ROWS + row) * D;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) *(f32x4 *)(so + 4 * ((4 * n + quad) ^ (row & 7))) = acc[r][n];
   }
-#pragma unroll
-  for (int n = 0; n < NB; ++n)
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      *(f32x4 *)(so + 4 * ((8 * n + 2 * e + hh) ^ (l32 & 7))) =
-          f32x4{st.acc[n][4 * e], st.acc[n][4 * e + 1], st.acc[n][4 * e + 2], st.acc[n][4 * e + 3]};
   __syncthreads();
 #pragma unroll 1
   for (int e = tid; e < ROWS * (D / 4); e += 64 * W) {
@@ -523,14 +591,31 @@ __global__ __launch_bounds__(64 * W, OCC) void history_few_kernel(HistAttnArgs a
   }
 }
 
-// Many rows: 128 a workgroup, 32 a wave; tiles of KT keys, whose 16-byte pieces the threads share, become operands in LDS, two tiles in
-// turn, read by every wave. The bytes of the tile after the next are in flight under a tile's products. A tile's one barrier keeps
-// the waves of a workgroup in step, so the workgroups are small: several a compute unit, each at its own place.
+// Which 16 bytes of a tile a thread takes: the row and its piece. Eight lanes one after the other write to eight different places of the
+// 128 bytes that LDS takes at a time (piece_xor of rows r and r + 4 is one apart, of r and r + 1 two), and 64 cover whole rows.
+template <int X, int PR> __device__ __forceinline__ void piece_place(int e, int &row, int &c) {
+  if constexpr (X == 1) {
+    c = e % PR, row = e / PR;
+  } else if constexpr (X == 2) {             // c0 c1 r2 c2.. r0 r1 r3..
+    const int r2 = e >> 2 & 1, rest = e >> 3, hi = rest % (PR / 4), rr = rest / (PR / 4);
+    c = (e & 3) + 4 * hi;
+    row = (rr & 3) + 4 * r2 + (rr >> 2 << 3);
+  } else {                                   // c0 r2 r0 c1.. r1 r3..
+    const int r2 = e >> 1 & 1, r0 = e >> 2 & 1, rest = e >> 3, hi = rest % (PR / 2), rr = rest / (PR / 2);
+    c = (e & 1) + 2 * hi;
+    row = r0 + 2 * (rr & 1) + 4 * r2 + (rr >> 1 << 3);
+  }
+}
+
+// Many rows: 128 a workgroup, 32 a wave, on the 32x32 MFMA; tiles of KT keys, whose 16-byte pieces the threads share, become operands in
+// LDS, two tiles in turn, read by every wave. The bytes of the tile after the next are in flight under a tile's products. A tile's one
+// barrier keeps the waves of a workgroup in step, so the workgroups are small: several a compute unit, each at its own place.
 template <int QT, int FMT, int D, int KT, int OCC>
 __global__ __launch_bounds__(256, OCC) void history_many_kernel(HistAttnArgs a) {
   using T = HistTypes<QT, FMT>;
   constexpr int E = T::E, X = E / 8, RB = D * 16 / E, PR = RB / 16, NB = D / 32, ROWS = 128;
   constexpr int ALL = 2 * KT * PR, NPC = (ALL + 255) / 256, STAGE = KT * D * 4;
+  static_assert(ALL % 256 == 0, "whole pieces a thread");
   constexpr int OUTS = ROWS * D * 4;
   __shared__ __align__(1024) uint8_t s_mem[2 * STAGE > OUTS ? 2 * STAGE : OUTS];
   __shared__ int s_odd;
@@ -555,7 +640,7 @@ __global__ __launch_bounds__(256, OCC) void history_many_kernel(HistAttnArgs a) 
 #pragma unroll
     for (int f = 0; f < D / 16; ++f) query_terms<QT, T::BF, T::NQ>(a.q, from + 16 * f, a.scale * kLog2e, q[f]);
   }
-  const float scale = a.scale * kLog2e;
+  const float scale = QT == E_F32 ? 1.f : a.scale * kLog2e;
   if (tid == 0) s_odd = 0;
   // The keys that any of the wave's rows sees.
   int wlow = row.low, whigh = row.high;
@@ -566,16 +651,39 @@ __global__ __launch_bounds__(256, OCC) void history_many_kernel(HistAttnArgs a) 
   __syncthreads();
 
   const int tiles = (b.nc + KT - 1) / KT;
+  // Piece u of a thread: of the keys in the first half of the pieces, of the values in the second (a thread's one piece, where it
+  // has one, by its wave).
+  const int half = NPC == 1 ? tid >> 7 : 0;
+  constexpr int HALF = NPC == 1 ? 1 : NPC / 2;
+  uint32_t off[HALF], soff[HALF];            // in a tile of consecutive rows
+  int prow[HALF], to[HALF];
+#pragma unroll
+  for (int u = 0; u < HALF; ++u) {
+    int c;
+    piece_place<X, PR>(NPC == 1 ? tid & 127 : u * 256 + tid, prow[u], c);
+    off[u] = prow[u] * RB + 16 * c;
+    soff[u] = prow[u] * (D / 32) + E * c / 32;
+    to[u] = prow[u] * (2 * D) + ((c * X ^ piece_xor(prow[u])) << 4);
+  }
   u32x4 raw[NPC];
   uint32_t rs[NPC];
   auto fetch = [&](int t) {
+    const int j = b.c0 + t * KT;
+    const bool plain = in_a_row(b, j, KT);
+    const int64_t r0 = key_row(b, j);
 #pragma unroll
     for (int u = 0; u < NPC; ++u) {
-      const int e = u * 256 + tid, v = e >= ALL / 2, p = e - v * (ALL / 2), c = p % PR;
-      if (ALL < 256 && e >= ALL) continue;
-      const uint64_t r = key_row(b, b.c0 + t * KT + p / PR);
-      raw[u] = *(const u32x4 *)((v ? b.v_ : b.k) + r * RB + 16 * c);
-      if constexpr (T::MX) rs[u] = *(const uint8_t *)((v ? b.vs : b.ks) + r * (D / 32) + (E * c) / 32);
+      const int h = u % HALF;
+      gptr_t base = b.k, sbase = b.ks;
+      if (NPC == 1 ? half != 0 : u >= HALF) base = b.v_, sbase = b.vs;
+      if (plain) {
+        raw[u] = load_global<u32x4>(base + r0 * RB + off[h]);
+        if constexpr (T::MX) rs[u] = load_global<uint8_t>(sbase + r0 * (D / 32) + soff[h]);
+      } else {
+        const int64_t r = key_row(b, j + prow[h]);
+        raw[u] = load_global<u32x4>(base + r * RB + (off[h] - prow[h] * RB));
+        if constexpr (T::MX) rs[u] = load_global<uint8_t>(sbase + r * (D / 32) + (soff[h] - prow[h] * (D / 32)));
+      }
     }
   };
   auto is_part = [&](int j, int n) { return j + n - 1 > b.first_high || (j + n > a.first && j < b.last_low); };
@@ -583,28 +691,32 @@ __global__ __launch_bounds__(256, OCC) void history_many_kernel(HistAttnArgs a) 
     const bool part = is_part(b.c0 + t * KT, KT);
 #pragma unroll
     for (int u = 0; u < NPC; ++u) {
-      const int e = u * 256 + tid, v = e >= ALL / 2, p = e - v * (ALL / 2), c = p % PR, r = p / PR;
-      if (ALL < 256 && e >= ALL) continue;
+      const bool v = NPC == 1 ? half != 0 : u >= HALF;
       u32x4 o[X];
-      widen<FMT>(raw[u], T::MX ? rs[u] : 0, o);
-      if (T::MX && rs[u] == 255)
+      uint32_t x[4] = {raw[u][0], raw[u][1], raw[u][2], raw[u][3]};
+      widen<FMT, 16>(x, T::MX ? rs[u] : 0, o);
+      if (T::MX && __any(rs[u] == 255)) {
+        if (rs[u] == 255)
 #pragma unroll
-        for (int x = 0; x < X; ++x) o[x] = u32x4{0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u};
+          for (int i = 0; i < X; ++i) o[i] = u32x4{kNan2, kNan2, kNan2, kNan2};
+      }
       if (part && v) {
         bool odd = false;
 #pragma unroll
-        for (int x = 0; x < X; ++x) odd |= take_odd<T::BF>(o[x]);
+        for (int i = 0; i < X; ++i) odd |= take_odd<T::BF>(o[i]);
         if (odd) s_odd = 1;
       }
-      uint8_t *to = s_mem + slot * STAGE + v * (KT * D * 2) + r * (2 * D);
+      uint8_t *dst = s_mem + slot * STAGE + (v ? KT * D * 2 : 0);
 #pragma unroll
-      for (int x = 0; x < X; ++x) *(u32x4 *)(to + ((c * X + x ^ piece_xor(r)) << 4)) = o[x];
+      for (int i = 0; i < X; ++i) *(u32x4 *)(dst + (to[u % HALF] ^ (i << 4))) = o[i];
     }
   };
-  RowState<QT, FMT, D> st;
-  st.init();
-  float minus1 = -1.f;
-  asm volatile("" : "+s"(minus1));
+  float R = kNone, L = 0.f;
+  const SplitConst kSplit;
+  bool far = false;
+  f32x16 acc[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) acc[n] = f32x16{};
   const int j16 = lane & 15;
   const int vrow = 4 * hh + (j16 >> 2), vpiece = (2 * ((lane >> 4) & 1) + ((j16 & 3) >> 1)) ^ piece_xor(vrow);
   if (tiles > 0) {
@@ -627,11 +739,37 @@ __global__ __launch_bounds__(256, OCC) void history_many_kernel(HistAttnArgs a) 
 #pragma unroll
         for (int n = 0; n < T::NQ; ++n) S = mfma32<T::BF>(kf, q[f][n], S);
       }
-      const bool part = is_part(j, 32);
-      uint32_t sees = 0;
-      if (part) sees = ((~first_keys(row.low - j) | first_keys(a.first - j)) & first_keys(row.high + 1 - j)) >> (4 * hh);
-      st.softmax(S, part, sees, scale);
-      st.values(S, stage + KT * D * 2 + (32 * k + vrow) * (2 * D) + (j16 & 1) * 8, vpiece, minus1);
+      if (is_part(j, 32)) {
+        // Element i is key 8 (i / 4) + 4 hh + i % 4 of the 32.
+        const uint32_t sees = ((~first_keys(row.low - j) | first_keys(a.first - j)) & first_keys(row.high + 1 - j)) >> (4 * hh);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) S[i] = sees >> (8 * (i >> 2) + (i & 3)) & 1 ? S[i] : scale < 0.f ? INFINITY : -INFINITY;
+      }
+      const float corr = to_probabilities<16>(S, scale, R, L, far, [](float v) { return max_halves(v); });
+      if (__any(corr != 1.f))
+#pragma unroll
+        for (int n = 0; n < NB; ++n) acc[n] *= corr;
+      // V^T: lane (l32, hh) takes dimension 32 n + l32 of keys 16 kc + 8 x + 4 hh .. + 3, the order of P^T.
+      const uint8_t *vcol = stage + KT * D * 2 + (32 * k + vrow) * (2 * D) + (j16 & 1) * 8;
+#pragma unroll
+      for (int kc = 0; kc < 2; ++kc) {
+        u32x4 p[T::NP];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t x[T::NP];
+          split_terms<T::BF, T::NP>(S[8 * kc + 2 * e], S[8 * kc + 2 * e + 1], kSplit, x);
+#pragma unroll
+          for (int n = 0; n < T::NP; ++n) p[n][e] = x[n];
+        }
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          const u32x2 v0 = read_columns(vcol + 16 * kc * 2 * D + ((vpiece ^ (4 * n)) << 4));
+          const u32x2 v1 = read_columns(vcol + (16 * kc + 8) * 2 * D + ((vpiece ^ (4 * n)) << 4));
+          const u32x4 vf = {v0[0], v0[1], v1[0], v1[1]};
+#pragma unroll
+          for (int k2 = 0; k2 < T::NP; ++k2) acc[n] = mfma32<T::BF>(vf, p[k2], acc[n]);
+        }
+      }
     }
     if (t + 1 < tiles) {
       place(t + 1, (t + 1) & 1);
@@ -641,20 +779,20 @@ __global__ __launch_bounds__(256, OCC) void history_many_kernel(HistAttnArgs a) 
   }
 
   // Rows to their columns' order through LDS: a wave's own 32 rows.
-  st.L += other_half(st.L);
+  L += other_half(L);
   float *so = (float *)s_mem + (size_t)(wave * 32) * D;
 #pragma unroll
   for (int n = 0; n < NB; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       *(f32x4 *)(so + l32 * D + 4 * ((8 * n + 2 * e + hh) ^ (l32 & 7))) =
-          f32x4{st.acc[n][4 * e], st.acc[n][4 * e + 1], st.acc[n][4 * e + 2], st.acc[n][4 * e + 3]};
+          f32x4{acc[n][4 * e], acc[n][4 * e + 1], acc[n][4 * e + 2], acc[n][4 * e + 3]};
   asm volatile("" ::: "memory");
 #pragma unroll 1
   for (int e = lane; e < 32 * (D / 4); e += 64) {
-    const int r = e / (D / 4), q4 = e % (D / 4);             // one row, or a few, for the whole wave
+    const int r = e / (D / 4), q4 = e % (D / 4);
     f32x4 o = *(const f32x4 *)(so + r * D + 4 * (q4 ^ (r & 7)));
-    const float m = __shfl(st.M, r) - kOff, den = __shfl(st.L, r);
+    const float m = __shfl(R, r), den = __shfl(L, r);
     const Row x = row_of(a, b, b.r0 + wave * 32 + r);
     if (!x.in) continue;
     if (s_odd)
@@ -711,9 +849,11 @@ template <int QT, int D> __global__ __launch_bounds__(256) void history_merge_ke
 template <int QT, int FMT, int D> static void launch_pass(const HistAttnArgs &a, hipStream_t s) {
   const HistAttnArgs::Pass &p = a.shared ? a.pre : a.own;
   const int64_t groups = (int64_t)(a.shared ? a.kvh : a.S * a.kvh) * p.chunks;
-  constexpr int KT = D == 256 ? 32 : 64, OCC_FEW = D == 64 ? 3 : D == 128 ? 2 : 1, OCC_MANY = D == 256 ? 1 : 2;
-  if (p.block_rows == kFewRows) {
-    hipLaunchKernelGGL((history_few_kernel<QT, FMT, D, 4, OCC_FEW>), dim3((uint32_t)groups), dim3(256), 0, s, a);
+  constexpr int KT = D == 256 ? 32 : 64, OCC = D == 64 ? 4 : D == 128 ? 3 : 2, OCC_MANY = D == 256 ? 1 : 2;
+  if (p.block_rows == 16) {
+    hipLaunchKernelGGL((history_few_kernel<QT, FMT, D, 1, 4, OCC>), dim3((uint32_t)groups), dim3(256), 0, s, a);
+  } else if (p.block_rows == 32) {
+    hipLaunchKernelGGL((history_few_kernel<QT, FMT, D, 2, 4, OCC - 1>), dim3((uint32_t)groups), dim3(256), 0, s, a);
   } else {
     const int parts = groups >= 8 ? 1 : (int)((8 + groups - 1) / groups), share = (p.row_blocks + parts - 1) / parts;
     const int64_t all = groups * share * parts;
