@@ -30,9 +30,8 @@ template <int QT, int FMT> struct HistTypes {
 typedef const uint8_t __attribute__((address_space(1))) *gptr_t;
 template <typename V> __device__ __forceinline__ V load_global(gptr_t p) { return *(const V __attribute__((address_space(1))) *)p; }
 
-// N bytes of a row (16, or 8 of MXFP4) and their scale byte as MFMA operands of eight numbers. Scale byte 0 gives 0 or 2^-127; 255 is
-// the caller's to see to.
-constexpr uint32_t kNan2 = 0x7FC07FC0u;
+// N bytes of a row (16, or 8 of MXFP4) and their scale byte as MFMA operands of eight numbers. The conversions take a
+// scale's exponent bits as e8m0: 255 makes every number NaN.
 template <int FMT, int N> __device__ __forceinline__ void widen(const uint32_t (&raw)[N / 4], uint32_t scale, u32x4 (&out)[HistTypes<0, FMT>::E * N / 128]) {
   if constexpr (FMT == H_F16 || FMT == H_BF16) {
     out[0] = u32x4{raw[0], raw[1], raw[2], raw[3]};
@@ -100,6 +99,7 @@ struct Block {
   int first_low, last_low, first_high;      // of the first and the last row
   gptr_t k, v_, ks, vs;                     // the head's rows
   int rows, span, pinned, delta;            // position -> row
+  int even, even_end, even_row;             // keys even .. even_end − 1 are in consecutive rows from even_row on: all but a few
 };
 __device__ __forceinline__ int row_low(const HistAttnArgs &a, const Visible &v, int i) {
   return a.window ? v.fold + max(v.length + i - a.window + 1, v.low) - v.low : 0;
@@ -147,6 +147,11 @@ template <int FMT, int D> __device__ __forceinline__ bool block_of(const HistAtt
     const int from = max(b.v.low, b.pinned);
     b.delta = (int)((uint32_t)(from - b.pinned) % (uint32_t)b.span) + b.pinned - from;
   }
+  // From the window's start, or behind the pinned rows, to the end, or to where a ring goes on at its first row.
+  const int from = max(b.v.low, b.pinned);
+  b.even = b.v.fold + from - b.v.low;
+  b.even_row = from + b.delta;
+  b.even_end = min(b.v.n, b.even + b.rows - b.even_row);
   return true;
 }
 // The row of key j, j clamped to those that there are (n > 0).
@@ -155,13 +160,6 @@ __device__ __forceinline__ int key_row(const Block &b, int j) {
   const int p = j < b.v.fold ? j : j - b.v.fold + b.v.low;
   int r = p < b.pinned ? p : p + b.delta;
   return r >= b.rows ? r - b.span : r;
-}
-// Whether keys j .. j + n − 1 are all there, in consecutive rows.
-__device__ __forceinline__ bool in_a_row(const Block &b, int j, int n) {
-  if (j + n > b.v.n || (j < b.v.fold && j + n > b.v.fold)) return false;
-  const int p = j < b.v.fold ? j : j - b.v.fold + b.v.low;
-  if (p < b.pinned) return p + n <= b.pinned;
-  return p + b.delta >= b.rows || p + b.delta + n <= b.rows;
 }
 // The first x of 32 keys.
 __device__ __forceinline__ uint32_t first_keys(int x) { return x >= 32 ? 0xFFFFFFFFu : x <= 0 ? 0u : (1u << x) - 1; }
@@ -321,49 +319,52 @@ __device__ void put_odd(const Block &b, int first, int low, int high, int j0, in
   }
 }
 
-// Logits of a run of keys to probabilities 2^(y − R), y = S·scale, and the sums on: N of them a lane, its row's shared with the lanes
-// that `top_of` exchanges with. R follows the row's maximum y, less kOff, by steps of at least kLag. The product and the difference
-// are one fma; where some R is so far from zero that the product's lost bits would matter, y is rounded first, as R was. After a step of R
-// the sums so far are off by what this returns (1: none).
+// Logits S of a run of keys, N of them a lane, its row's shared with the lanes that `top_of` exchanges with, to probabilities
+// 2^(y − R), y = S·scale, and their sum to L. R follows the row's maximum y, less kOff, by steps of at least kLag. Whether it has to
+// step is seen from the sum of what comes out with the R that there is, so that no maximum is formed but where it does. The product and
+// the difference are one fma; where some R is so far from zero that the product's lost bits would matter, y is rounded first, as R
+// was. Returns what the sums so far are to be multiplied with after a step of R (1: none); L is.
 constexpr float kFar = 65536.f;
-template <int N, typename V, typename F>
-__device__ __forceinline__ float to_probabilities(V &S, float scale, float &R, float &L, bool &far, F top_of) {
-  auto relative = [&](float (&y)[N]) {
-    if (far) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) y[i] = S[i] * scale - R;
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) y[i] = fmaf(S[i], scale, -R);
-    }
-  };
-  auto largest = [&](const float (&y)[N]) {
-    float top = fmaxf(y[0], y[1]);
-#pragma unroll
-    for (int i = 2; i < N; i += 2) top = fmaxf(fmaxf(top, y[i]), y[i + 1]);
-    return top_of(top);
-  };
+template <int N, typename F> __device__ __forceinline__ float to_probabilities(float (&S)[N], float scale, float &R, float &L, bool &far, F top_of) {
   float y[N], corr = 1.f;
-  relative(y);
-  if (__any(largest(y) > kOff + kLag)) {
-    float r[N];
+  auto sum_of = [&]() {
+    float sum[2] = {0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < N; ++i) r[i] = S[i] * scale;
-    const float to = fmaxf(R, largest(r) - kOff);
+    for (int i = 0; i < N; ++i) {
+      y[i] = exp2_(y[i]);
+      sum[i & 1] += y[i];
+    }
+    return sum[0] + sum[1];
+  };
+#pragma unroll
+  for (int i = 0; i < N; ++i) y[i] = fmaf(S[i], scale, -R);
+  float sum = sum_of();
+  if (far || __any(sum > 23170.475f)) {      // 2^(kOff + kLag)
+    // Nearly never: with a scale of its own, so that its products are not made ahead of the branch.
+    float own = scale;
+    asm volatile("" : "+v"(own));
+    float top = S[0] * own;
+#pragma unroll
+    for (int i = 1; i < N; ++i) top = fmaxf(top, S[i] * own);
+    top = top_of(top);
+    const float to = fmaxf(R, top - kOff);
     corr = exp2_(R - to);
     R = to;
     L *= corr;
     far = __any(fabsf(R) > kFar && R > kNone);
-    relative(y);
-  }
-  float sum[2] = {0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    S[i] = exp2_(y[i]);
-    sum[i & 1] += S[i];
+    for (int i = 0; i < N; ++i) y[i] = far ? S[i] * own - R : fmaf(S[i], own, -R);
+    sum = sum_of();
   }
-  L += sum[0] + sum[1];
+  L += sum;
+#pragma unroll
+  for (int i = 0; i < N; ++i) S[i] = y[i];
   return corr;
+}
+// Operands from memory, waited for here: a wait left to a loop's first use would there wait for the loop's own loads each time.
+template <int N> __device__ __forceinline__ void arrived(u32x4 (&q)[N]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) asm volatile("" : "+v"(q[n]));
 }
 
 __device__ __forceinline__ int piece_xor(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
@@ -415,8 +416,8 @@ __global__ __launch_bounds__(64 * W, OCC) void history_few_kernel(HistAttnArgs a
   auto fetch = [&](int t) {
     const int j = b.c0 + 32 * t;
     gptr_t at[2][2], sc[2][2];
-    if (in_a_row(b, j, 32)) {
-      const int64_t r = key_row(b, j);
+    if (j >= b.even && j + 32 <= b.even_end) {
+      const int64_t r = b.even_row + (j - b.even);
       const uint32_t o = (uint32_t)(l16 * RB + quad * PB), so = (uint32_t)(l16 * (D / 32));
 #pragma unroll
       for (int kg = 0; kg < 2; ++kg) {
@@ -453,11 +454,6 @@ __global__ __launch_bounds__(64 * W, OCC) void history_few_kernel(HistAttnArgs a
     for (int i = 0; i < PB / 4; ++i) x[i] = raw[v][kg][u][i];
     const uint32_t sc = T::MX ? scale_of(rs[v][kg], u) : 0;
     widen<FMT, PB>(x, sc, w);
-    if (T::MX && __any(sc == 255)) {
-      if (sc == 255)
-#pragma unroll
-        for (int i = 0; i < X; ++i) w[i] = u32x4{kNan2, kNan2, kNan2, kNan2};
-    }
   };
   auto is_part = [&](int t) {
     const int j = b.c0 + 32 * t;
@@ -477,6 +473,10 @@ __global__ __launch_bounds__(64 * W, OCC) void history_few_kernel(HistAttnArgs a
   const int j16 = lane & 15, vrow = 4 * quad + (j16 >> 2), vpiece = ((j16 & 3) >> 1) ^ piece_xor(vrow);
   const uint8_t *vcol = vmem + vrow * (2 * D) + (j16 & 1) * 8;
   if (wave < tiles) fetch(wave);
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int f = 0; f < NF; ++f) arrived(q[r][f]);
   for (int t = wave; t < tiles; t += W) {
     const bool part = is_part(t);
     f32x4 S[RT][2];
@@ -609,7 +609,10 @@ template <int X, int PR> __device__ __forceinline__ void piece_place(int e, int 
 
 // Many rows: 128 a workgroup, 32 a wave, on the 32x32 MFMA; tiles of KT keys, whose 16-byte pieces the threads share, become operands in
 // LDS, two tiles in turn, read by every wave. The bytes of the tile after the next are in flight under a tile's products. A tile's one
-// barrier keeps the waves of a workgroup in step, so the workgroups are small: several a compute unit, each at its own place.
+// barrier keeps the waves of a workgroup in step, so the workgroups are small: several a compute unit, each at its own place. Bound by the
+// VALU's instructions (four fifths of them the softmax: an fma, an exponential, a sum, the terms), so that what changes from tile to tile is
+// kept to scalars and immediate offsets. Scores of the next tile formed under the exponentials of one, with a third place for values,
+// took 7 to 10 percent longer.
 template <int QT, int FMT, int D, int KT, int OCC>
 __global__ __launch_bounds__(256, OCC) void history_many_kernel(HistAttnArgs a) {
   using T = HistTypes<QT, FMT>;
@@ -663,52 +666,53 @@ __global__ __launch_bounds__(256, OCC) void history_many_kernel(HistAttnArgs a) 
     piece_place<X, PR>(NPC == 1 ? tid & 127 : u * 256 + tid, prow[u], c);
     off[u] = prow[u] * RB + 16 * c;
     soff[u] = prow[u] * (D / 32) + E * c / 32;
-    to[u] = prow[u] * (2 * D) + ((c * X ^ piece_xor(prow[u])) << 4);
+    to[u] = prow[u] * (2 * D) + ((c * X ^ piece_xor(prow[u])) << 4) + (NPC == 1 ? half * (KT * D * 2) : 0);
   }
   u32x4 raw[NPC];
   uint32_t rs[NPC];
+  // Tiles from `even` to `even_end` are of consecutive rows; those from `high` on, and from `low` to `low_end`, are not seen whole by some row.
+  const int even = max(0, (b.even - b.c0 + KT - 1) / KT), even_end = (b.even_end - b.c0) / KT;
+  const int high = max(0, (b.first_high + 1 - b.c0) / KT);   // first_high >= −1
+  const int low = max(0, (min(a.first, b.last_low) - b.c0) / KT), low_end = b.last_low > b.c0 ? (b.last_low - b.c0 + KT - 1) / KT : 0;
+  const int row0 = b.even_row + b.c0 - b.even;
   auto fetch = [&](int t) {
-    const int j = b.c0 + t * KT;
-    const bool plain = in_a_row(b, j, KT);
-    const int64_t r0 = key_row(b, j);
+    int64_t at[HALF], sat[HALF];             // one load for both ways to its address, so that none waits where they meet
+    const int64_t r0 = row0 + t * KT;
 #pragma unroll
-    for (int u = 0; u < NPC; ++u) {
-      const int h = u % HALF;
-      gptr_t base = b.k, sbase = b.ks;
-      if (NPC == 1 ? half != 0 : u >= HALF) base = b.v_, sbase = b.vs;
-      if (plain) {
-        raw[u] = load_global<u32x4>(base + r0 * RB + off[h]);
-        if constexpr (T::MX) rs[u] = load_global<uint8_t>(sbase + r0 * (D / 32) + soff[h]);
-      } else {
-        const int64_t r = key_row(b, j + prow[h]);
-        raw[u] = load_global<u32x4>(base + r * RB + (off[h] - prow[h] * RB));
-        if constexpr (T::MX) rs[u] = load_global<uint8_t>(sbase + r * (D / 32) + (soff[h] - prow[h] * (D / 32)));
+    for (int h = 0; h < HALF; ++h) at[h] = r0 * RB + off[h], sat[h] = r0 * (D / 32) + soff[h];
+    if (t < even || t >= even_end) {
+#pragma unroll
+      for (int h = 0; h < HALF; ++h) {
+        const int64_t r = key_row(b, b.c0 + t * KT + prow[h]) - prow[h];
+        at[h] = r * RB + off[h], sat[h] = r * (D / 32) + soff[h];
       }
     }
-  };
-  auto is_part = [&](int j, int n) { return j + n - 1 > b.first_high || (j + n > a.first && j < b.last_low); };
-  auto place = [&](int t, int slot) {
-    const bool part = is_part(b.c0 + t * KT, KT);
 #pragma unroll
     for (int u = 0; u < NPC; ++u) {
       const bool v = NPC == 1 ? half != 0 : u >= HALF;
+      raw[u] = load_global<u32x4>((v ? b.v_ : b.k) + at[u % HALF]);
+      if constexpr (T::MX) rs[u] = load_global<uint8_t>((v ? b.vs : b.ks) + sat[u % HALF]);
+    }
+  };
+  auto is_part = [&](int t) { return t >= high || (t >= low && t < low_end); };
+  auto place = [&](int t, auto slot) {
+    const bool part = is_part(t);
+#pragma unroll
+    for (int u = 0; u < NPC; ++u) {
       u32x4 o[X];
       uint32_t x[4] = {raw[u][0], raw[u][1], raw[u][2], raw[u][3]};
       widen<FMT, 16>(x, T::MX ? rs[u] : 0, o);
-      if (T::MX && __any(rs[u] == 255)) {
-        if (rs[u] == 255)
+      if (part && (NPC == 1 || u >= HALF)) {
+        if (NPC > 1 || half) {
+          bool odd = false;
 #pragma unroll
-          for (int i = 0; i < X; ++i) o[i] = u32x4{kNan2, kNan2, kNan2, kNan2};
+          for (int i = 0; i < X; ++i) odd |= take_odd<T::BF>(o[i]);
+          if (odd) s_odd = 1;
+        }
       }
-      if (part && v) {
-        bool odd = false;
 #pragma unroll
-        for (int i = 0; i < X; ++i) odd |= take_odd<T::BF>(o[i]);
-        if (odd) s_odd = 1;
-      }
-      uint8_t *dst = s_mem + slot * STAGE + (v ? KT * D * 2 : 0);
-#pragma unroll
-      for (int i = 0; i < X; ++i) *(u32x4 *)(dst + (to[u % HALF] ^ (i << 4))) = o[i];
+      for (int i = 0; i < X; ++i)
+        *(u32x4 *)(s_mem + slot * STAGE + (NPC > 1 && u >= HALF ? KT * D * 2 : 0) + (to[u % HALF] ^ (i << 4))) = o[i];
     }
   };
   float R = kNone, L = 0.f;
@@ -719,63 +723,82 @@ __global__ __launch_bounds__(256, OCC) void history_many_kernel(HistAttnArgs a) 
   for (int n = 0; n < NB; ++n) acc[n] = f32x16{};
   const int j16 = lane & 15;
   const int vrow = 4 * hh + (j16 >> 2), vpiece = (2 * ((lane >> 4) & 1) + ((j16 & 3) >> 1)) ^ piece_xor(vrow);
-  if (tiles > 0) {
-    fetch(0);
-    place(0, 0);
-    if (tiles > 1) fetch(1);
-  }
-  __syncthreads();
-  for (int t = 0; t < tiles; ++t) {
-    const uint8_t *stage = s_mem + (t & 1) * STAGE;
-#pragma unroll 1
+  int kat[D / 16], vat[NB];                  // this lane's places in a tile of keys and of values
+#pragma unroll
+  for (int f = 0; f < D / 16; ++f) kat[f] = l32 * (2 * D) + (((2 * f + hh) ^ piece_xor(l32)) << 4);
+#pragma unroll
+  for (int n = 0; n < NB; ++n) vat[n] = vrow * (2 * D) + (j16 & 1) * 8 + ((vpiece ^ (4 * n)) << 4);
+  auto compute = [&](int t, auto slot) {
+    const bool part = is_part(t);
+#pragma unroll
     for (int k = 0; k < KT / 32; ++k) {
       const int j = b.c0 + t * KT + 32 * k;
-      if (j > whigh || (j >= a.first && j + 32 <= wlow)) continue;
-      const uint8_t *krow = stage + (32 * k + l32) * (2 * D);
+      if (part && (j > whigh || (j >= a.first && j + 32 <= wlow))) continue;
+      const uint8_t *keys = s_mem + slot * STAGE + 64 * D * k, *values = keys + KT * D * 2;
       f32x16 S = f32x16{};
 #pragma unroll
       for (int f = 0; f < D / 16; ++f) {
-        const u32x4 kf = *(const u32x4 *)(krow + (((2 * f + hh) ^ piece_xor(l32)) << 4));
+        const u32x4 kf = *(const u32x4 *)(keys + kat[f]);
 #pragma unroll
         for (int n = 0; n < T::NQ; ++n) S = mfma32<T::BF>(kf, q[f][n], S);
       }
-      if (is_part(j, 32)) {
+      float y[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) y[i] = S[i];
+      if (part) {
         // Element i is key 8 (i / 4) + 4 hh + i % 4 of the 32.
         const uint32_t sees = ((~first_keys(row.low - j) | first_keys(a.first - j)) & first_keys(row.high + 1 - j)) >> (4 * hh);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) S[i] = sees >> (8 * (i >> 2) + (i & 3)) & 1 ? S[i] : scale < 0.f ? INFINITY : -INFINITY;
+        for (int i = 0; i < 16; ++i) y[i] = sees >> (8 * (i >> 2) + (i & 3)) & 1 ? y[i] : scale < 0.f ? INFINITY : -INFINITY;
       }
-      const float corr = to_probabilities<16>(S, scale, R, L, far, [](float v) { return max_halves(v); });
+      const float corr = to_probabilities<16>(y, scale, R, L, far, [](float v) { return max_halves(v); });
       if (__any(corr != 1.f))
 #pragma unroll
         for (int n = 0; n < NB; ++n) acc[n] *= corr;
       // V^T: lane (l32, hh) takes dimension 32 n + l32 of keys 16 kc + 8 x + 4 hh .. + 3, the order of P^T.
-      const uint8_t *vcol = stage + KT * D * 2 + (32 * k + vrow) * (2 * D) + (j16 & 1) * 8;
 #pragma unroll
       for (int kc = 0; kc < 2; ++kc) {
         u32x4 p[T::NP];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           uint32_t x[T::NP];
-          split_terms<T::BF, T::NP>(S[8 * kc + 2 * e], S[8 * kc + 2 * e + 1], kSplit, x);
+          split_terms<T::BF, T::NP>(y[8 * kc + 2 * e], y[8 * kc + 2 * e + 1], kSplit, x);
 #pragma unroll
           for (int n = 0; n < T::NP; ++n) p[n][e] = x[n];
         }
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-          const u32x2 v0 = read_columns(vcol + 16 * kc * 2 * D + ((vpiece ^ (4 * n)) << 4));
-          const u32x2 v1 = read_columns(vcol + (16 * kc + 8) * 2 * D + ((vpiece ^ (4 * n)) << 4));
+          const u32x2 v0 = read_columns(values + vat[n] + 16 * kc * 2 * D), v1 = read_columns(values + vat[n] + (16 * kc + 8) * 2 * D);
           const u32x4 vf = {v0[0], v0[1], v1[0], v1[1]};
 #pragma unroll
           for (int k2 = 0; k2 < T::NP; ++k2) acc[n] = mfma32<T::BF>(vf, p[k2], acc[n]);
         }
       }
     }
+  };
+  typedef std::integral_constant<int, 0> zero_t;
+  typedef std::integral_constant<int, 1> one_t;
+  auto step = [&](int t, auto slot, auto next) {
+    compute(t, slot);
     if (t + 1 < tiles) {
-      place(t + 1, (t + 1) & 1);
+      place(t + 1, next);
       if (t + 2 < tiles) fetch(t + 2);
     }
     __syncthreads();
+  };
+  if (tiles > 0) fetch(0);
+#pragma unroll
+  for (int f = 0; f < D / 16; ++f) arrived(q[f]);
+  if (tiles > 0) {
+    place(0, zero_t{});
+    if (tiles > 1) fetch(1);
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int t = 0; t < tiles; ++t) {
+    step(t, zero_t{}, one_t{});
+    if (++t >= tiles) break;
+    step(t, one_t{}, zero_t{});
   }
 
   // Rows to their columns' order through LDS: a wave's own 32 rows.
@@ -797,7 +820,7 @@ __global__ __launch_bounds__(256, OCC) void history_many_kernel(HistAttnArgs a) 
     if (!x.in) continue;
     if (s_odd)
       for (int t = 0; t < tiles; ++t)
-        if (is_part(b.c0 + t * KT, KT))
+        if (is_part(t))
           put_odd<FMT, D>(b, a.first, x.low, x.high, b.c0 + t * KT, min(b.c0 + t * KT + KT, b.c0 + b.nc), q4, o);
     leave_row<QT, D>(a, b, x, q4, m, den, o);
   }
@@ -849,7 +872,7 @@ template <int QT, int D> __global__ __launch_bounds__(256) void history_merge_ke
 template <int QT, int FMT, int D> static void launch_pass(const HistAttnArgs &a, hipStream_t s) {
   const HistAttnArgs::Pass &p = a.shared ? a.pre : a.own;
   const int64_t groups = (int64_t)(a.shared ? a.kvh : a.S * a.kvh) * p.chunks;
-  constexpr int KT = D == 256 ? 32 : 64, OCC = D == 64 ? 4 : D == 128 ? 3 : 2, OCC_MANY = D == 256 ? 1 : 2;
+  constexpr int KT = D == 256 ? 32 : 64, OCC = D == 64 ? 4 : D == 128 ? 3 : 2, OCC_MANY = D == 256 ? 1 : D == 128 ? 2 : HistTypes<QT, FMT>::NQ == 1 ? 4 : 3;
   if (p.block_rows == 16) {
     hipLaunchKernelGGL((history_few_kernel<QT, FMT, D, 1, 4, OCC>), dim3((uint32_t)groups), dim3(256), 0, s, a);
   } else if (p.block_rows == 32) {
