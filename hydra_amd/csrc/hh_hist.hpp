@@ -41,10 +41,9 @@ struct HistAttnArgs {
   // How the work is split (history_plan). A pass is over the sequences' own histories or over the prefix, whose rows are those of
   // all sequences' tokens; its keys are cut into chunks of `per` keys, whole tiles.
   struct Pass {
-    int chunks, per, tile, block_rows, row_blocks;
+    int chunks, per, tile, block_rows, row_blocks, blocks;
   } own, pre;
   int chunks;                          // of a row, the prefix's first
-  int shared;                          // the kernel's pass
   float *pm, *pl, *po;                 // chunk states [S][N][qh][chunks], their sums [..][chunks][d]
 };
 

@@ -3,18 +3,18 @@
 
 namespace hh {
 
-// Workgroups that a pass's keys are split for: those that the chip holds at once.
-static int wanted_groups(int d) { return d == 64 ? 768 : d == 128 ? 512 : 256; }
-constexpr int kHistChunks = 256;             // most chunks of a pass
+// Workgroups that a pass's keys are split for: those that the chip holds at once, by the kernels' registers.
+static int wanted_groups(int d, bool few) { return few ? (d == 64 ? 768 : 512) : d == 64 ? 768 : d == 128 ? 512 : 256; }
 
 static HistAttnArgs::Pass plan_pass(const HistAttnArgs &a, int64_t rows, int64_t heads, int64_t keys) {
   HistAttnArgs::Pass p{};
-  const bool few = rows <= kFewRows;
+  // With a prefix both passes are one launch, of workgroups for 16 rows and for 128.
+  const bool few = rows <= (a.p.k ? 16 : kFewRows);
   p.block_rows = rows <= 16 ? 16 : few ? kFewRows : 128;
   p.row_blocks = (int)((rows + p.block_rows - 1) / p.block_rows);
   p.tile = few ? 128 : a.d == 256 ? 32 : 64;
   const int64_t most = (keys + p.tile - 1) / p.tile;
-  int64_t chunks = wanted_groups(a.d) / (heads * p.row_blocks);
+  int64_t chunks = wanted_groups(a.d, few) / (heads * p.row_blocks);
   // A few tiles one after the other take less than a launch that joins them.
   if (chunks > most / 2) chunks = most / 2;
   if (chunks > kHistChunks) chunks = kHistChunks;
@@ -24,6 +24,9 @@ static HistAttnArgs::Pass plan_pass(const HistAttnArgs &a, int64_t rows, int64_t
   p.per = (int)per;
   p.chunks = (int)((keys + per - 1) / per);
   if (p.chunks < 1) p.chunks = 1;
+  // The workgroups of many rows are dealt to the eight XCDs (history_many).
+  const int64_t groups = heads * p.chunks, parts = groups >= 8 ? 1 : (8 + groups - 1) / groups, share = (p.row_blocks + parts - 1) / parts;
+  p.blocks = (int)(few ? groups : 8 * ((groups * share * parts + 7) / 8));
   return p;
 }
 
@@ -54,7 +57,7 @@ size_t history_reserve(const HistAttnArgs &a, int64_t length, int64_t prefix_row
     int64_t chunks = (keys + 31) / 32 / 2;
     if (chunks > kHistChunks) chunks = kHistChunks;
     if (chunks < 2) return (int64_t)0;
-    const int64_t groups = (int64_t)wanted_groups(a.d) * 128;
+    const int64_t groups = (int64_t)wanted_groups(a.d, true) * 128;
     return rows * chunks < groups ? rows * chunks : groups;
   };
   if (!a.h.ring && length > a.h.rows) length = a.h.rows;

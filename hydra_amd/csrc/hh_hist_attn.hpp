@@ -19,6 +19,8 @@ namespace hh {
 
 constexpr int kFewRows = 32;                 // rows of a kv head up to which a wave takes all of them, 16 or 32
 
+constexpr int kHistChunks = 256;             // most chunks of a pass
+
 template <int QT, int FMT> struct HistTypes {
   static constexpr bool BF = FMT != H_F16, MX = FMT >= H_MXFP8;
   static constexpr int E = FMT == H_MXFP8 ? 16 : FMT == H_MXFP4 ? 32 : 8;                       // numbers of 16 bytes
@@ -94,6 +96,7 @@ __device__ __forceinline__ int used_chunks(int n, int per) { return n <= per ? 1
 
 // A block of rows of a pass: whose rows, what they see, and which keys of it are this workgroup's.
 struct Block {
+  bool shared;
   int s, g, r0, count, chunk, c0, nc;       // keys c0 .. c0 + nc − 1
   Visible v;
   int first_low, last_low, first_high;      // of the first and the last row
@@ -106,15 +109,16 @@ __device__ __forceinline__ int row_low(const HistAttnArgs &a, const Visible &v, 
 }
 __device__ __forceinline__ int row_high(const Visible &v, int i) { return v.fold + max(0, min(v.length + i, v.last) - v.low + 1) - 1; }
 
-template <int FMT, int D> __device__ __forceinline__ bool block_of(const HistAttnArgs &a, int sg, int rb, int chunk, Block &b) {
-  const HistAttnArgs::Pass &p = a.shared ? a.pre : a.own;
-  const HistView &h = a.shared ? a.p : a.h;
-  b.s = a.shared ? 0 : sg / a.kvh;
+template <int FMT, int D> __device__ __forceinline__ bool block_of(const HistAttnArgs &a, bool shared, int sg, int rb, int chunk, Block &b) {
+  const HistAttnArgs::Pass &p = shared ? a.pre : a.own;
+  const HistView &h = shared ? a.p : a.h;
+  b.shared = shared;
+  b.s = shared ? 0 : sg / a.kvh;
   b.g = sg - b.s * a.kvh;
   b.r0 = rb * p.block_rows;
   b.chunk = chunk;
   int i0 = 0;
-  if (a.shared) {
+  if (shared) {
     b.count = a.S * a.N;
     b.v = visible_prefix(a);
     b.first_low = b.last_low = 0;
@@ -175,7 +179,7 @@ __device__ __forceinline__ Row row_of(const HistAttnArgs &a, const Block &b, int
   x.in = t < b.count;
   const int tt = x.in ? t : b.r0 / a.qm;                     // rows past the last stand for the block's first
   x.head = b.g * a.qm + (x.in ? r - t * a.qm : 0);
-  if (a.shared) {
+  if (b.shared) {
     x.s = tt / a.N;
     x.i = tt - x.s * a.N;
     x.in = x.in && x.i < step_count(a.counts, x.s, a.N);
@@ -280,7 +284,7 @@ template <int QT, int D>
 __device__ __forceinline__ void leave_row(const HistAttnArgs &a, const Block &b, const Row &x, int q4, float m, float den, f32x4 o) {
   const int64_t row = ((int64_t)x.s * a.N + x.i) * a.qh + x.head;
   if (a.chunks > 1) {
-    const int64_t slot = row * a.chunks + (a.shared ? 0 : a.pre.chunks) + b.chunk;
+    const int64_t slot = row * a.chunks + (b.shared ? 0 : a.pre.chunks) + b.chunk;
     *(f32x4 *)(a.po + slot * D + 4 * q4) = o;
     if (q4 == 0) {
       a.pm[slot] = m;
@@ -380,19 +384,18 @@ __device__ __forceinline__ u32x2 read_columns(const uint8_t *p) {   // transposi
 // in flight under this one's products. On the 16x16 MFMA, S^T [16 keys × 16 rows] twice a tile: a head of 64 in 8 bits is 64 bytes, four
 // lanes of a key, so that a load is one stretch of memory, and goes to the operands' registers as it is, since the order of a product's
 // columns is free. Values pass through LDS to be read by columns. No barrier until the waves' states meet.
-template <int QT, int FMT, int D, int RT, int W, int OCC>
-__global__ __launch_bounds__(64 * W, OCC) void history_few_kernel(HistAttnArgs a) {
+template <int D, int RT, int W> constexpr int few_lds() { return W * (16 * RT * D * 4 > 64 * D ? 16 * RT * D * 4 : 64 * D); }
+template <int QT, int FMT, int D, int RT, int W>
+__device__ __forceinline__ void history_few(const HistAttnArgs &a, bool shared, int block, uint8_t *s_mem) {
   using T = HistTypes<QT, FMT>;
   constexpr int E = T::E, RB = D * 16 / E, PB = RB / 4 < 16 ? RB / 4 : 16, U = RB / 4 / PB, EP = PB * E / 16, X = EP / 8;
   constexpr int NF = D / 32, NB = D / 16, ROWS = 16 * RT;   // operands of a query or of 16 keys; blocks of 16 value columns
-  __shared__ __align__(1024) uint8_t s_mem[W * (ROWS * D * 4 > 64 * D ? ROWS * D * 4 : 64 * D)];
   __shared__ float s_m[W][ROWS], s_l[W][ROWS];
   __shared__ int s_lo[ROWS], s_hi[ROWS], s_odd;
-  warm_kernargs<sizeof(HistAttnArgs)>();
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, quad = lane >> 4;
-  const int heads = a.shared ? a.kvh : a.S * a.kvh;
+  const int heads = shared ? a.kvh : a.S * a.kvh;
   Block b;
-  if (!block_of<FMT, D>(a, (int)(blockIdx.x % heads), 0, (int)(blockIdx.x / heads), b)) return;
+  if (!block_of<FMT, D>(a, shared, block % heads, 0, block / heads, b)) return;
   u32x4 q[RT][NF][T::NQ];                    // operand u·X + x: columns EP (4 u + quad) + 8 x
   int low[RT], high[RT];
 #pragma unroll
@@ -613,29 +616,27 @@ template <int X, int PR> __device__ __forceinline__ void piece_place(int e, int 
 // VALU's instructions (four fifths of them the softmax: an fma, an exponential, a sum, the terms), so that what changes from tile to tile is
 // kept to scalars and immediate offsets. Scores of the next tile formed under the exponentials of one, with a third place for values,
 // took 7 to 10 percent longer.
-template <int QT, int FMT, int D, int KT, int OCC>
-__global__ __launch_bounds__(256, OCC) void history_many_kernel(HistAttnArgs a) {
+template <int D> constexpr int many_keys() { return D == 256 ? 32 : 64; }
+template <int D> constexpr int many_lds() { return 2 * many_keys<D>() * D * 4 > 128 * D * 4 ? 2 * many_keys<D>() * D * 4 : 128 * D * 4; }
+template <int QT, int FMT, int D> __device__ __forceinline__ void history_many(const HistAttnArgs &a, bool shared, uint32_t block, uint8_t *s_mem) {
   using T = HistTypes<QT, FMT>;
-  constexpr int E = T::E, X = E / 8, RB = D * 16 / E, PR = RB / 16, NB = D / 32, ROWS = 128;
+  constexpr int KT = many_keys<D>(), E = T::E, X = E / 8, RB = D * 16 / E, PR = RB / 16, NB = D / 32;
   constexpr int ALL = 2 * KT * PR, NPC = (ALL + 255) / 256, STAGE = KT * D * 4;
   static_assert(ALL % 256 == 0, "whole pieces a thread");
-  constexpr int OUTS = ROWS * D * 4;
-  __shared__ __align__(1024) uint8_t s_mem[2 * STAGE > OUTS ? 2 * STAGE : OUTS];
   __shared__ int s_odd;
-  warm_kernargs<sizeof(HistAttnArgs)>();
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, hh = lane >> 5;
   // Each XCD takes a stretch of the list (head and chunk, block of rows), so that what it reads again is in its L2; a block's share of
   // a head that several XCDs have is spread over its rows, the ones that see most first.
-  const HistAttnArgs::Pass &pass = a.shared ? a.pre : a.own;
-  const int heads = a.shared ? a.kvh : a.S * a.kvh, groups = heads * pass.chunks;
+  const HistAttnArgs::Pass &pass = shared ? a.pre : a.own;
+  const int heads = shared ? a.kvh : a.S * a.kvh, groups = heads * pass.chunks;
   const int parts = groups >= 8 ? 1 : (8 + groups - 1) / groups, share = (pass.row_blocks + parts - 1) / parts;
-  const uint32_t all = (uint32_t)groups * (uint32_t)(share * parts), each = (all + 7) / 8, w = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
-  if ((blockIdx.x >> 3) >= each || w >= all) return;
+  const uint32_t all = (uint32_t)groups * (uint32_t)(share * parts), each = (all + 7) / 8, w = (block & 7) * each + (block >> 3);
+  if ((block >> 3) >= each || w >= all) return;
   const int grp = (int)(w / (uint32_t)(share * parts)), at = (int)(w - (uint32_t)grp * (uint32_t)(share * parts));
   const int rb = pass.row_blocks - 1 - (at % share * parts + at / share);
   if (rb < 0) return;
   Block b;
-  if (!block_of<FMT, D>(a, grp % heads, rb, grp / heads, b)) return;
+  if (!block_of<FMT, D>(a, shared, grp % heads, rb, grp / heads, b)) return;
   const Row row = row_of(a, b, b.r0 + wave * 32 + l32);
   u32x4 q[D / 16][T::NQ];
   {
@@ -826,6 +827,47 @@ __global__ __launch_bounds__(256, OCC) void history_many_kernel(HistAttnArgs a) 
   }
 }
 
+template <int QT, int FMT, int D, int RT, int OCC> __global__ __launch_bounds__(256, OCC) void history_few_kernel(HistAttnArgs a) {
+  __shared__ __align__(1024) uint8_t s_mem[few_lds<D, RT, 4>()];
+  warm_kernargs<sizeof(HistAttnArgs)>();
+  history_few<QT, FMT, D, RT, 4>(a, false, (int)blockIdx.x, s_mem);
+}
+template <int QT, int FMT, int D, int OCC> __global__ __launch_bounds__(256, OCC) void history_many_kernel(HistAttnArgs a) {
+  __shared__ __align__(1024) uint8_t s_mem[many_lds<D>()];
+  warm_kernargs<sizeof(HistAttnArgs)>();
+  history_many<QT, FMT, D>(a, false, blockIdx.x, s_mem);
+}
+// The prefix's pass and behind it the own histories', which fill the chip under its last workgroups.
+template <int QT, int FMT, int D, int OCC> __global__ __launch_bounds__(256, OCC) void history_prefix_kernel(HistAttnArgs a) {
+  constexpr int few = few_lds<D, 1, 4>();
+  __shared__ __align__(1024) uint8_t s_mem[many_lds<D>() > few ? many_lds<D>() : few];
+  warm_kernargs<sizeof(HistAttnArgs)>();
+  const bool shared = blockIdx.x < (uint32_t)a.pre.blocks;
+  const uint32_t block = shared ? blockIdx.x : blockIdx.x - a.pre.blocks;
+  if ((shared ? a.pre.block_rows : a.own.block_rows) == 16) history_few<QT, FMT, D, 1, 4>(a, shared, (int)block, s_mem);
+  else history_many<QT, FMT, D>(a, shared, block, s_mem);
+}
+
+// The chunks that a row has states of: of the prefix, then its own; none for a token that is not there.
+struct RowChunks {
+  int head, pre, own;
+  __device__ __forceinline__ int64_t slot(const HistAttnArgs &a, int64_t row, int c) const { return row * a.chunks + (c < pre ? c : a.pre.chunks + c - pre); }
+};
+__device__ __forceinline__ RowChunks row_chunks(const HistAttnArgs &a, int64_t row) {
+  RowChunks x{};
+  x.head = (int)(row % a.qh);
+  const int i = (int)(row / a.qh % a.N), s = (int)(row / ((int64_t)a.qh * a.N)), count = step_count(a.counts, s, a.N);
+  if (i >= count) return x;
+  const int r0 = (i * a.qm + x.head % a.qm) / a.own.block_rows * a.own.block_rows;
+  const Visible v = visible_of(a, s, r0 / a.qm, min(count, (r0 + a.own.block_rows - 1) / a.qm + 1) - 1);
+  x.own = used_chunks(v.n, chunk_keys(a.own, v.n));
+  if (a.p.k) {
+    const int n = visible_prefix(a).n;
+    x.pre = used_chunks(n, chunk_keys(a.pre, n));
+  }
+  return x;
+}
+
 // Joins a row's chunks, in order: a wave per row, D / 4 lanes a chunk.
 template <int QT, int D> __global__ __launch_bounds__(256) void history_merge_kernel(HistAttnArgs a) {
   warm_kernargs<sizeof(HistAttnArgs)>();
@@ -833,27 +875,16 @@ template <int QT, int D> __global__ __launch_bounds__(256) void history_merge_ke
   const int lane = threadIdx.x & 63, q4 = lane % LR, cg = lane / LR;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= (int64_t)a.S * a.N * a.qh) return;
-  const int hd = (int)(row % a.qh), i = (int)(row / a.qh % a.N), s = (int)(row / ((int64_t)a.qh * a.N));
-  const int count = step_count(a.counts, s, a.N);
-  if (i >= count) return;
-  const int r0 = (i * a.qm + hd % a.qm) / a.own.block_rows * a.own.block_rows;
-  const Visible v = visible_of(a, s, r0 / a.qm, min(count, (r0 + a.own.block_rows - 1) / a.qm + 1) - 1);
-  const int own = used_chunks(v.n, chunk_keys(a.own, v.n));
-  int pre = 0;
-  if (a.p.k) {
-    const int n = visible_prefix(a).n;
-    pre = used_chunks(n, chunk_keys(a.pre, n));
-  }
-  const int used = pre + own;
-  auto slot = [&](int c) { return row * a.chunks + (c < pre ? c : a.pre.chunks + c - pre); };
+  const RowChunks rc = row_chunks(a, row);
+  const int used = rc.pre + rc.own;
   float m = kNone;
-  for (int c = lane; c < used; c += 64) m = fmaxf(m, a.pm[slot(c)]);
+  for (int c = lane; c < used; c += 64) m = fmaxf(m, a.pm[rc.slot(a, row, c)]);
   for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
   float den = 0.f;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int c = cg; c < used; c += GR) {
-    const int64_t at = slot(c);
+    const int64_t at = rc.slot(a, row, c);
     const float f = exp2_(a.pm[at] - m);
     den = fmaf(a.pl[at], f, den);
     const f32x4 w = *(const f32x4 *)(a.po + at * D + 4 * q4);
@@ -866,35 +897,79 @@ template <int QT, int D> __global__ __launch_bounds__(256) void history_merge_ke
 #pragma unroll
     for (int k = 0; k < 4; ++k) sum[k] += __shfl_xor(sum[k], o);
   }
-  if (cg == 0) finish_history_row<QT, D>(a, row, hd, q4, m, den, sum);
+  if (cg == 0 && used) finish_history_row<QT, D>(a, row, rc.head, q4, m, den, sum);
 }
 
-template <int QT, int FMT, int D> static void launch_pass(const HistAttnArgs &a, hipStream_t s) {
-  const HistAttnArgs::Pass &p = a.shared ? a.pre : a.own;
-  const int64_t groups = (int64_t)(a.shared ? a.kvh : a.S * a.kvh) * p.chunks;
-  constexpr int KT = D == 256 ? 32 : 64, OCC = D == 64 ? 4 : D == 128 ? 3 : 2, OCC_MANY = D == 256 ? 1 : D == 128 ? 2 : HistTypes<QT, FMT>::NQ == 1 ? 4 : 3;
-  if (p.block_rows == 16) {
-    hipLaunchKernelGGL((history_few_kernel<QT, FMT, D, 1, 4, OCC>), dim3((uint32_t)groups), dim3(256), 0, s, a);
-  } else if (p.block_rows == 32) {
-    hipLaunchKernelGGL((history_few_kernel<QT, FMT, D, 2, 4, OCC - 1>), dim3((uint32_t)groups), dim3(256), 0, s, a);
-  } else {
-    const int parts = groups >= 8 ? 1 : (int)((8 + groups - 1) / groups), share = (p.row_blocks + parts - 1) / parts;
-    const int64_t all = groups * share * parts;
-    hipLaunchKernelGGL((history_many_kernel<QT, FMT, D, KT, OCC_MANY>), dim3((uint32_t)(8 * ((all + 7) / 8))), dim3(256), 0, s, a);
+// The same for few rows, of many chunks: a workgroup for 64 of a row's columns. Every chunk's factor into LDS first; then sixteen lanes a chunk and sixteen
+// chunks at a time, whose sums meet in LDS, in order. (16 rows of 128 chunks: 5.4 us, a wave a row 16; 4096 rows
+// of 34 chunks 14, a wave a row 8.)
+constexpr int kMergeChunks = 2 * kHistChunks, kWideRows = 256;
+template <int QT, int D> __global__ __launch_bounds__(256) void history_merge_wide_kernel(HistAttnArgs a) {
+  __shared__ float s_f[kMergeChunks], s_red[8];
+  __shared__ __align__(16) f32x4 s_o[16][16];
+  warm_kernargs<sizeof(HistAttnArgs)>();
+  constexpr int PARTS = D / 64;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t row = (int64_t)(blockIdx.x / PARTS);
+  const int part = blockIdx.x % PARTS;
+  const RowChunks rc = row_chunks(a, row);
+  const int used = rc.pre + rc.own;          // at most kMergeChunks
+  if (!used) return;
+  float m2[2] = {kNone, kNone}, l2[2] = {0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (tid + 256 * k < used) m2[k] = a.pm[rc.slot(a, row, tid + 256 * k)], l2[k] = a.pl[rc.slot(a, row, tid + 256 * k)];
+  float m = fmaxf(m2[0], m2[1]);
+  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  if (lane == 0) s_red[wave] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+  float den = 0.f;
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (tid + 256 * k < used) {
+      const float f = exp2_(m2[k] - m);
+      s_f[tid + 256 * k] = f;
+      den = fmaf(l2[k], f, den);
+    }
+  for (int o = 32; o; o >>= 1) den += __shfl_xor(den, o);
+  if (lane == 0) s_red[4 + wave] = den;
+  __syncthreads();
+  den = (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]);
+  const int q4 = tid & 15, cg = tid >> 4;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int c = cg; c < used; c += 16) {
+    const f32x4 w = *(const f32x4 *)(a.po + rc.slot(a, row, c) * D + 64 * part + 4 * q4);
+    const float f = s_f[c];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sum[k] = fmaf(w[k], f, sum[k]);
   }
+  s_o[cg][q4] = sum;
+  __syncthreads();
+  if (tid >= 16) return;
+  sum = s_o[0][tid];
+  for (int c = 1; c < min(used, 16); ++c) {
+    const f32x4 w = s_o[c][tid];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sum[k] += w[k];
+  }
+  finish_history_row<QT, D>(a, row, rc.head, 16 * part + tid, m, den, sum);
 }
 
 template <int QT, int FMT, int D> static hipError_t launch_types(HistAttnArgs a, hipStream_t s, int *launches) {
-  *launches = 0;
-  for (int shared = a.p.k ? 1 : 0; shared >= 0; --shared) {
-    a.shared = shared;
-    launch_pass<QT, FMT, D>(a, s);
-    ++*launches;
-  }
+  constexpr int OCC = D == 64 ? 4 : D == 128 ? 3 : 2, OCC_MANY = D == 256 ? 1 : D == 128 ? 2 : HistTypes<QT, FMT>::NQ == 1 ? 4 : 3;
+  const dim3 grid((uint32_t)(a.pre.blocks + a.own.blocks)), block(256);
+  if (a.p.k) hipLaunchKernelGGL((history_prefix_kernel<QT, FMT, D, OCC_MANY>), grid, block, 0, s, a);
+  else if (a.own.block_rows == 16) hipLaunchKernelGGL((history_few_kernel<QT, FMT, D, 1, OCC>), grid, block, 0, s, a);
+  else if (a.own.block_rows == 32) hipLaunchKernelGGL((history_few_kernel<QT, FMT, D, 2, OCC - 1>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((history_many_kernel<QT, FMT, D, OCC_MANY>), grid, block, 0, s, a);
+  *launches = 1;
   if (a.chunks > 1) {
     const int64_t rows = (int64_t)a.S * a.N * a.qh;
-    hipLaunchKernelGGL((history_merge_kernel<QT, D>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, s, a);
-    ++*launches;
+    if (rows < kWideRows) hipLaunchKernelGGL((history_merge_wide_kernel<QT, D>), dim3((uint32_t)(rows * (D / 64))), block, 0, s, a);
+    else hipLaunchKernelGGL((history_merge_kernel<QT, D>), dim3((uint32_t)((rows + 3) / 4)), block, 0, s, a);
+    *launches = 2;
   }
   return hipGetLastError();
 }
