@@ -59,7 +59,7 @@ struct RotaryArgs {
   const int32_t *positions;
   float magnitude;
   int tokens, count, d, rotated, span, interleaved, type;
-  int per_block, parts;                // tokens a workgroup, workgroups that share them
+  int per_block, parts, lanes;         // tokens a workgroup, workgroups that share them, log2 of a row's lanes
 };
 
 __device__ __forceinline__ int hist_length(const int32_t *lengths, int s) { return min(max(lengths[s], 0), kHistLength); }

@@ -99,60 +99,81 @@ template <int FMT> __device__ __forceinline__ void decode8(const uint8_t *row, c
   }
 }
 
-// A piece of eight columns: items run over columns, tokens, heads, sequences, then keys and values.
-struct Piece {
-  int s, g, i, c, v;
+// A workgroup's rows: of one sequence's keys or values, heads outermost, U of 256·8 / d at a time each lane.
+template <int U> struct RowItems {
+  int s, v, c;
+  int g[U], i[U];              // head, token; token −1: none
+  __device__ __forceinline__ RowItems(const HistRowsArgs &a) {
+    const int lanes = a.d / 8, each = 256 / lanes, r0 = (int)blockIdx.x * each * U + (int)threadIdx.x / lanes;
+    s = blockIdx.y >> 1, v = blockIdx.y & 1, c = (int)threadIdx.x % lanes * 8;
+    const int count = step_count(a.counts, s, a.N), rows = a.kvh * a.N;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = r0 + u * each;
+      g[u] = (int)((uint32_t)r / (uint32_t)a.N);
+      i[u] = r - g[u] * a.N;
+      if (r >= rows || i[u] >= count) i[u] = -1;
+    }
+  }
 };
-__device__ __forceinline__ bool piece_of(const HistRowsArgs &a, int64_t e, Piece &p) {
-  const int pieces = a.d / 8;
-  p.c = (int)(e % pieces) * 8;
-  e /= pieces;
-  p.i = (int)(e % a.N);
-  e /= a.N;
-  p.g = (int)(e % a.kvh);
-  e /= a.kvh;
-  p.s = (int)(e % a.S);
-  p.v = (int)(e / a.S);
-  return p.v < 2;
-}
 
-template <int T, int FMT> __global__ __launch_bounds__(256) void history_write_kernel(HistRowsArgs a) {
-  Piece p;
-  if (!piece_of(a, (int64_t)blockIdx.x * 256 + threadIdx.x, p)) return;   // a group's lanes together
-  const int count = step_count(a.counts, p.s, a.N);
-  if (p.i >= count) return;
-  const int length = hist_length(a.h.lengths, p.s), at = length + p.i, row = hist_row(a.h, at);
-  // Of a step longer than the ring the last.
-  if (row < 0 || (a.h.ring && at >= a.h.pinned && at < length + count - (a.h.rows - a.h.pinned))) return;
-  float x[8];
-  load8<T>(p.v ? a.v : a.k, ((int64_t)p.s * a.N + p.i) * a.kv_stride + (int64_t)p.g * a.d + p.c, x);
-  const int64_t r = ((int64_t)p.s * a.kvh + p.g) * a.h.rows + row;
-  uint8_t *to = (p.v ? a.h.v : a.h.k) + r * hist_row_bytes(FMT, a.d);
-  if constexpr (FMT == H_F16) {
-    store8<E_F16>(to, p.c, x);
-  } else if constexpr (FMT == H_BF16) {
-    store8<E_BF16>(to, p.c, x);
-  } else {
-    uint32_t w[2], scale;
-    encode8<FMT>(x, w, scale);
-    if constexpr (FMT == H_MXFP8) *(u32x2 *)(to + p.c) = u32x2{w[0], w[1]};
-    else *(uint32_t *)(to + p.c / 2) = w[0];
-    if ((p.c & 31) == 0) ((p.v ? a.h.vs : a.h.ks) + r * (a.d / 32))[p.c >> 5] = (uint8_t)scale;
+template <int T, int FMT, int U> __global__ __launch_bounds__(256) void history_write_kernel(HistRowsArgs a) {
+  warm_kernargs<sizeof(HistRowsArgs)>();
+  const RowItems<U> p(a);      // a group's four lanes together
+  const int count = step_count(a.counts, p.s, a.N), length = hist_length(a.h.lengths, p.s);
+  const void *from = p.v ? a.v : a.k;
+  uint8_t *codes = p.v ? a.h.v : a.h.k, *scales = p.v ? a.h.vs : a.h.ks;
+  float x[U][8];
+  int row[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    row[u] = -1;
+    if (p.i[u] < 0) continue;
+    const int at = length + p.i[u];
+    // Of a step longer than the ring the last.
+    if (a.h.ring && at >= a.h.pinned && at < length + count - (a.h.rows - a.h.pinned)) continue;
+    row[u] = hist_row(a.h, at);
+    if (row[u] >= 0) load8<T>(from, ((int64_t)p.s * a.N + p.i[u]) * a.kv_stride + (int64_t)p.g[u] * a.d + p.c, x[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (row[u] < 0) continue;
+    const int64_t r = ((int64_t)p.s * a.kvh + p.g[u]) * a.h.rows + row[u];
+    uint8_t *to = codes + r * hist_row_bytes(FMT, a.d);
+    if constexpr (FMT == H_F16) {
+      store8<E_F16>(to, p.c, x[u]);
+    } else if constexpr (FMT == H_BF16) {
+      store8<E_BF16>(to, p.c, x[u]);
+    } else {
+      uint32_t w[2], scale;
+      encode8<FMT>(x[u], w, scale);
+      if constexpr (FMT == H_MXFP8) *(u32x2 *)(to + p.c) = u32x2{w[0], w[1]};
+      else *(uint32_t *)(to + p.c / 2) = w[0];
+      if ((p.c & 31) == 0) (scales + r * (a.d / 32))[p.c >> 5] = (uint8_t)scale;
+    }
   }
 }
 
-template <int T, int FMT> __global__ __launch_bounds__(256) void history_read_kernel(HistRowsArgs a) {
-  Piece p;
-  if (!piece_of(a, (int64_t)blockIdx.x * 256 + threadIdx.x, p)) return;
-  if (p.i >= step_count(a.counts, p.s, a.N)) return;
-  const int64_t at = (int64_t)a.starts[p.s] + p.i;
-  if (at < 0 || at > INT32_MAX) return;
-  const int row = hist_row(a.h, (int)at);
-  if (row < 0) return;
-  const int64_t r = ((int64_t)p.s * a.kvh + p.g) * a.h.rows + row;
-  float x[8];
-  decode8<FMT>((p.v ? a.h.v : a.h.k) + r * hist_row_bytes(FMT, a.d), (p.v ? a.h.vs : a.h.ks) + r * (a.d / 32), p.c, x);
-  store8<T>(p.v ? a.vo : a.ko, (((int64_t)p.s * a.N + p.i) * a.kvh + p.g) * a.d + p.c, x);
+template <int T, int FMT, int U> __global__ __launch_bounds__(256) void history_read_kernel(HistRowsArgs a) {
+  warm_kernargs<sizeof(HistRowsArgs)>();
+  const RowItems<U> p(a);
+  const uint8_t *codes = p.v ? a.h.v : a.h.k, *scales = p.v ? a.h.vs : a.h.ks;
+  void *to = p.v ? a.vo : a.ko;
+  float x[U][8];
+  int row[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    row[u] = -1;
+    const int64_t at = (int64_t)a.starts[p.s] + p.i[u];
+    if (p.i[u] < 0 || at < 0 || at > INT32_MAX) continue;
+    row[u] = hist_row(a.h, (int)at);
+    if (row[u] < 0) continue;
+    const int64_t r = ((int64_t)p.s * a.kvh + p.g[u]) * a.h.rows + row[u];
+    decode8<FMT>(codes + r * hist_row_bytes(FMT, a.d), scales + r * (a.d / 32), p.c, x[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (row[u] >= 0) store8<T>(to, (((int64_t)p.s * a.N + p.i[u]) * a.kvh + p.g[u]) * a.d + p.c, x[u]);
 }
 
 __global__ __launch_bounds__(64) void history_advance_kernel(int32_t *lengths, const int32_t *counts, int S, int N) {
@@ -160,11 +181,19 @@ __global__ __launch_bounds__(64) void history_advance_kernel(int32_t *lengths, c
   if (s < S) lengths[s] = min(hist_length(lengths, s) + step_count(counts, s, N), kHistLength);
 }
 
+constexpr int kRowsAhead = 4;  // rows that a lane has in flight, where there are enough to fill the chip
 template <int T, int FMT> static void launch_rows_tf(const HistRowsArgs &a, bool write, hipStream_t s) {
-  const int64_t items = 2 * (int64_t)a.S * a.N * a.kvh * (a.d / 8);
-  const dim3 grid((uint32_t)((items + 255) / 256));
-  if (write) hipLaunchKernelGGL((history_write_kernel<T, FMT>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((history_read_kernel<T, FMT>), grid, dim3(256), 0, s, a);
+  const int64_t rows = (int64_t)a.kvh * a.N, each = 256 / (a.d / 8);
+  const bool ahead = 2 * rows * a.S >= 1024 * kRowsAhead * each;
+  const int64_t per = ahead ? kRowsAhead * each : each;
+  const dim3 grid((uint32_t)((rows + per - 1) / per), 2 * a.S), block(256);
+  if (write) {
+    if (ahead) hipLaunchKernelGGL((history_write_kernel<T, FMT, kRowsAhead>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((history_write_kernel<T, FMT, 1>), grid, block, 0, s, a);
+  } else {
+    if (ahead) hipLaunchKernelGGL((history_read_kernel<T, FMT, kRowsAhead>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((history_read_kernel<T, FMT, 1>), grid, block, 0, s, a);
+  }
 }
 template <int T> static void launch_rows_t(const HistRowsArgs &a, bool write, hipStream_t s) {
   if (a.format == H_F16) launch_rows_tf<T, H_F16>(a, write, s);
