@@ -9,7 +9,6 @@
 namespace hh {
 
 constexpr int kRotaryPairs = 2048;   // of a workgroup's tokens: 16 KB of LDS
-constexpr int kRotaryAhead = 4;      // rows that a thread has in flight
 
 // T: float, _Float16 or __bf16. MODE 0: pairs of neighbours, 1: halves whose distance is whole pieces, 2: any halves. A row (token, head) has
 // 2^lanes lanes, a piece each: of MODE 1 those of the first half, which write the second's too, and those behind the pairs' span.
@@ -33,64 +32,51 @@ template <typename T, int MODE> __global__ __launch_bounds__(256) void rotary_ke
   const int piece = tid & ((1 << a.lanes) - 1);
   const int c = (MODE == 1 && piece >= half / V ? piece + half / V : piece) * V;
   if (c >= a.d) return;
-  for (int r0 = part * each + (tid >> a.lanes); r0 < rows; r0 += kRotaryAhead * stride) {
-    const T *x[kRotaryAhead];
-    T *y[kRotaryAhead];
-    vec v[kRotaryAhead], w[kRotaryAhead];
-    int at[kRotaryAhead];            // the token's sines, −1: no row
+  // One row at a time: with two in flight a lane 78 us, with four 103, 67 with one (16384 tokens of 18 heads of 256, bf16, 302 MB).
+  for (int r = part * each + (tid >> a.lanes); r < rows; r += stride) {
+    const int t = (int)((uint32_t)r / (uint32_t)heads), h = r - t * heads;
+    const bool second = h >= a.r[0].heads;
+    const RotaryRows &z = a.r[second];
+    const int64_t o = (int64_t)(h - (second ? a.r[0].heads : 0)) * a.d;
+    const T *x = (const T *)z.x + (int64_t)(t0 + t) * z.x_stride + o;
+    T *y = (T *)z.y + (int64_t)(t0 + t) * z.y_stride + o;
+    const float *cs = s_cos + t * pairs, *sn = s_sin + t * pairs;
+    if constexpr (MODE == 0) {
+      vec v = *(const vec *)(x + c);
 #pragma unroll
-    for (int u = 0; u < kRotaryAhead; ++u) {
-      const int r = r0 + u * stride;
-      at[u] = -1;
-      if (r >= rows) continue;
-      const int t = (int)((uint32_t)r / (uint32_t)heads), h = r - t * heads;
-      const bool second = h >= a.r[0].heads;
-      const RotaryRows &z = a.r[second];
-      const int64_t o = (int64_t)(h - (second ? a.r[0].heads : 0)) * a.d;
-      at[u] = t * pairs;
-      x[u] = (const T *)z.x + (int64_t)(t0 + t) * z.x_stride + o;
-      y[u] = (T *)z.y + (int64_t)(t0 + t) * z.y_stride + o;
-      if constexpr (MODE < 2) v[u] = *(const vec *)(x[u] + c);
-      if (MODE == 1 && c < half) w[u] = *(const vec *)(x[u] + c + half);
-    }
+      for (int j = 0; j < V; j += 2) {
+        const int i = (c + j) / 2;
+        if (i >= pairs) break;
+        const float x1 = (float)v[j], x2 = (float)v[j + 1];
+        v[j] = (T)fmaf(x1, cs[i], -(x2 * sn[i]));
+        v[j + 1] = (T)fmaf(x2, cs[i], x1 * sn[i]);
+      }
+      *(vec *)(y + c) = v;
+    } else if constexpr (MODE == 1) {
+      vec v = *(const vec *)(x + c);
+      if (c < half) {
+        vec w = *(const vec *)(x + c + half);
 #pragma unroll
-    for (int u = 0; u < kRotaryAhead; ++u) {
-      if (at[u] < 0) continue;
-      const float *cs = s_cos + at[u], *sn = s_sin + at[u];
-      if constexpr (MODE == 0) {
-#pragma unroll
-        for (int j = 0; j < V; j += 2) {
-          const int i = (c + j) / 2;
-          if (i >= pairs) break;
-          const float x1 = (float)v[u][j], x2 = (float)v[u][j + 1];
-          v[u][j] = (T)fmaf(x1, cs[i], -(x2 * sn[i]));
-          v[u][j + 1] = (T)fmaf(x2, cs[i], x1 * sn[i]);
-        }
-        *(vec *)(y[u] + c) = v[u];
-      } else if constexpr (MODE == 1) {
-        if (c < half) {
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const int i = c + j;
-            if (i >= pairs) break;
-            const float x1 = (float)v[u][j], x2 = (float)w[u][j];
-            v[u][j] = (T)fmaf(x1, cs[i], -(x2 * sn[i]));
-            w[u][j] = (T)fmaf(x2, cs[i], x1 * sn[i]);
-          }
-          *(vec *)(y[u] + c + half) = w[u];
-        }
-        *(vec *)(y[u] + c) = v[u];
-      } else {
-        // Column by column: a pair by the thread of its first column, and columns of no pair.
         for (int j = 0; j < V; ++j) {
-          const int k = c + j;
-          if (k < pairs) {
-            const float x1 = (float)x[u][k], x2 = (float)x[u][k + half];
-            y[u][k] = (T)fmaf(x1, cs[k], -(x2 * sn[k]));
-            y[u][k + half] = (T)fmaf(x2, cs[k], x1 * sn[k]);
-          } else if (k < half || k >= half + pairs) {
-            y[u][k] = x[u][k];
-          }
+          const int i = c + j;
+          if (i >= pairs) break;
+          const float x1 = (float)v[j], x2 = (float)w[j];
+          v[j] = (T)fmaf(x1, cs[i], -(x2 * sn[i]));
+          w[j] = (T)fmaf(x2, cs[i], x1 * sn[i]);
+        }
+        *(vec *)(y + c + half) = w;
+      }
+      *(vec *)(y + c) = v;
+    } else {
+      // Column by column: a pair by the thread of its first column, and columns of no pair.
+      for (int j = 0; j < V; ++j) {
+        const int k = c + j;
+        if (k < pairs) {
+          const float x1 = (float)x[k], x2 = (float)x[k + half];
+          y[k] = (T)fmaf(x1, cs[k], -(x2 * sn[k]));
+          y[k + half] = (T)fmaf(x2, cs[k], x1 * sn[k]);
+        } else if (k < half || k >= half + pairs) {
+          y[k] = x[k];
         }
       }
     }
@@ -110,9 +96,9 @@ hipError_t launch_rotary(RotaryArgs a, hipStream_t s) {
   if (!a.interleaved && a.span / 2 % V == 0) pieces -= a.span / 2 / V;
   while (1 << a.lanes < pieces) ++a.lanes;
   const int each = 256 >> a.lanes;
-  // Sixteen tokens a workgroup, fewer where they fill LDS or there are few: then several share a token's heads.
+  // Four tokens a workgroup (one: 74 us, sixteen: 94), fewer where they fill LDS or there are few: then several share a token's heads.
   a.per_block = kRotaryPairs / (a.rotated / 2);
-  const int fill = a.tokens / 1024 < 16 ? a.tokens / 1024 : 16;
+  const int fill = a.tokens / 1024 < 4 ? a.tokens / 1024 : 4;
   if (a.per_block > fill) a.per_block = fill;
   if (a.per_block < 1) a.per_block = 1;
   const int blocks = (a.tokens + a.per_block - 1) / a.per_block;
