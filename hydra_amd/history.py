@@ -45,12 +45,19 @@ class Rotary:
         self.turns = torch.tensor(list(table), dtype=torch.float64, device=device)
 
 
+_ROWS = {n: RotaryRowsC * n for n in (1, 2)}
+
+
 def _tokens(t, name, shape, dtype, device):
     """The elements between tokens of a [..][heads][d] tensor with packed heads and equally spaced tokens."""
-    s, lead = t.stride(), t.shape[:-2]
-    if t.shape != shape or t.dtype is not dtype or t.device != device or s[-1] != 1 or (s[-2] != shape[-1] and shape[-2] > 1):
-        raise ValueError(f"{name} must be a {dtype} tensor {tuple(shape)} on {device} with packed heads, not {t.dtype} "
-                         f"{tuple(t.shape)} on {t.device} with strides {s}")
+    if t.shape != shape or t.dtype is not dtype or t.device != device:
+        raise ValueError(f"{name} must be a {dtype} tensor {tuple(shape)} on {device}, not {t.dtype} {tuple(t.shape)} on {t.device}")
+    row = shape[-1] * shape[-2]
+    if t.is_contiguous():
+        return row
+    s, lead = t.stride(), shape[:-2]
+    if s[-1] != 1 or (s[-2] != shape[-1] and shape[-2] > 1):
+        raise ValueError(f"{name} must have packed heads, not strides {s}")
     step, over = None, 1
     for n, st in zip(reversed(lead), reversed(s[:-2])):
         if n == 1:
@@ -60,9 +67,8 @@ def _tokens(t, name, shape, dtype, device):
         elif st != step * over:
             raise ValueError(f"{name}: the tokens must be equally spaced, not with strides {s}")
         over *= n
-    row = shape[-1] * shape[-2]
     if step is None:
-        step = row
+        return row
     if step < row:
         raise ValueError(f"{name}: tokens {step} elements apart overlap")
     return step
@@ -77,21 +83,20 @@ def rotary_into(ctx: Context, rotary: Rotary, positions, q, q_out, k=None, k_out
         raise ValueError(f"q must be fp32, fp16 or bf16 [..][heads][{rotary.head_dim}], not {dtype} {tuple(q.shape)}")
     if rotary.turns.device != dev:
         raise ValueError(f"the frequencies are on {rotary.turns.device}, q on {dev}")
-    _same(positions, "positions", q.shape[:-2], _I32, dev)
-    pairs = [("q", q, q_out)]
+    shape = q.shape
+    _same(positions, "positions", shape[:-2], _I32, dev)
+    rows = [(q.data_ptr(), q_out.data_ptr(), shape[-2], _tokens(q, "q", shape, dtype, dev), _tokens(q_out, "q_out", shape, dtype, dev))]
     if k is not None:
         if k_out is None:
             raise ValueError("k needs k_out")
-        if k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]:
-            raise ValueError(f"k {tuple(k.shape)} must have the tokens and head_dim of q {tuple(q.shape)}")
-        pairs.append(("k", k, k_out))
-    rows = (RotaryRowsC * len(pairs))(*[
-        RotaryRowsC(x.data_ptr(), y.data_ptr(), x.shape[-2], _tokens(x, name, x.shape, dtype, dev),
-                    _tokens(y, name + "_out", x.shape, dtype, dev)) for name, x, y in pairs])
-    if positions.numel() == 0:   # tensors of nothing have no address
-        return (q_out, k_out) if k is not None else q_out
-    check(lib().hh_rotary(ctx.handle, C.byref(rotary.c), rotary.turns.data_ptr(), rotary.magnitude, ELEM[dtype],
-                          positions.numel(), positions.data_ptr(), rows, len(pairs)))
+        other = k.shape
+        if other[:-2] != shape[:-2] or other[-1] != shape[-1]:
+            raise ValueError(f"k {tuple(other)} must have the tokens and head_dim of q {tuple(shape)}")
+        rows.append((k.data_ptr(), k_out.data_ptr(), other[-2], _tokens(k, "k", other, dtype, dev), _tokens(k_out, "k_out", other, dtype, dev)))
+    n = positions.numel()
+    if n:   # tensors of nothing have no address
+        check(lib().hh_rotary(ctx.handle, C.byref(rotary.c), rotary.turns.data_ptr(), rotary.magnitude, ELEM[dtype], n,
+                              positions.data_ptr(), _ROWS[len(rows)](*rows), len(rows)))
     return (q_out, k_out) if k is not None else q_out
 
 
