@@ -633,7 +633,11 @@ template <int QT, int FMT, int D> __device__ __forceinline__ void history_many(c
   const uint32_t all = (uint32_t)groups * (uint32_t)(share * parts), each = (all + 7) / 8, w = (block & 7) * each + (block >> 3);
   if ((block >> 3) >= each || w >= all) return;
   const int grp = (int)(w / (uint32_t)(share * parts)), at = (int)(w - (uint32_t)grp * (uint32_t)(share * parts));
-  const int rb = pass.row_blocks - 1 - (at % share * parts + at / share);
+  // An XCD's 32 compute units take them in turn: where it holds all at once, forth and back, so that those that see most do not meet on one
+  // (a prompt of 2048, 64 / 8 heads of 64: 74 us, 79 without); more are dealt as units come free (4096 tokens: 246, 251 forth and back).
+  int turn = at % share;
+  if (share <= 128 && turn >> 5 & 1) turn = (turn & ~31) + min(32, share - (turn & ~31)) - 1 - (turn & 31);
+  const int rb = pass.row_blocks - 1 - (turn * parts + at / share);
   if (rb < 0) return;
   Block b;
   if (!block_of<FMT, D>(a, shared, grp % heads, rb, grp / heads, b)) return;
@@ -957,12 +961,17 @@ template <int QT, int D> __global__ __launch_bounds__(256) void history_merge_wi
   finish_history_row<QT, D>(a, row, rc.head, 16 * part + tid, m, den, sum);
 }
 
+// Waves a SIMD of the kernels of few rows, by the registers that a tile's bytes, the queries' terms and the sums take.
+template <int QT, int FMT, int D> constexpr int few_waves() {
+  if (D == 256) return HistTypes<QT, FMT>::E == 8 || (FMT == H_MXFP8 && HistTypes<QT, FMT>::NQ == 3) ? 1 : 2;
+  return D == 64 ? 4 : 3;
+}
 template <int QT, int FMT, int D> static hipError_t launch_types(HistAttnArgs a, hipStream_t s, int *launches) {
-  constexpr int OCC = D == 64 ? 4 : D == 128 ? 3 : 2, OCC_MANY = D == 256 ? 1 : D == 128 ? 2 : HistTypes<QT, FMT>::NQ == 1 ? 4 : 3;
+  constexpr int OCC = few_waves<QT, FMT, D>(), OCC_MANY = D == 256 ? 1 : D == 128 ? 2 : HistTypes<QT, FMT>::NQ == 1 ? 4 : 3;
   const dim3 grid((uint32_t)(a.pre.blocks + a.own.blocks)), block(256);
   if (a.p.k) hipLaunchKernelGGL((history_prefix_kernel<QT, FMT, D, OCC_MANY>), grid, block, 0, s, a);
   else if (a.own.block_rows == 16) hipLaunchKernelGGL((history_few_kernel<QT, FMT, D, 1, OCC>), grid, block, 0, s, a);
-  else if (a.own.block_rows == 32) hipLaunchKernelGGL((history_few_kernel<QT, FMT, D, 2, OCC - 1>), grid, block, 0, s, a);
+  else if (a.own.block_rows == 32) hipLaunchKernelGGL((history_few_kernel<QT, FMT, D, 2, (OCC > 1 ? OCC - 1 : 1)>), grid, block, 0, s, a);
   else hipLaunchKernelGGL((history_many_kernel<QT, FMT, D, OCC_MANY>), grid, block, 0, s, a);
   *launches = 1;
   if (a.chunks > 1) {
