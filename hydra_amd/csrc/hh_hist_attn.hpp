@@ -11,6 +11,7 @@
 // probabilities as two (outputs of 16 bits: to 2^-15 of each) or three (F32: as exact as the sums) of bf16, or two of fp16.
 #pragma once
 #include <type_traits>
+#include <utility>
 
 #include "hh_attn_mfma.hpp"
 #include "hh_hist.hpp"
@@ -257,26 +258,33 @@ template <bool BF, int NP> __device__ __forceinline__ void split_terms(float p0,
   }
 }
 
-// A row's four outputs from its joined state: the sink's share of the denominator, the quotient, its rounding.
-template <int QT, int D>
-__device__ __forceinline__ void finish_history_row(const HistAttnArgs &a, int64_t row, int head, int q4, float m, float den, f32x4 o) {
-  if (a.sinks) {
-    const float y = bf16_bits_to_f32(a.sinks[head]) * kLog2e, mn = fmaxf(m, y), f = exp2_(m - mn);
-    den = fmaf(den, f, exp2_(y - mn));
-    o *= f;
-    m = mn;
-  }
-  const float inv = den == 0.f ? 0.f : 1.f / den;            // of nothing: 0
+// The sink into a row's denominator; returns the factor of what was summed before. The log of a denominator: of nothing −inf.
+__device__ __forceinline__ float sink_share(const HistAttnArgs &a, int head, float &m, float &den) {
+  if (!a.sinks) return 1.f;
+  const float y = bf16_bits_to_f32(a.sinks[head]) * kLog2e, mn = fmaxf(m, y), f = exp2_(m - mn);
+  den = fmaf(den, f, exp2_(y - mn));
+  m = mn;
+  return f;
+}
+__device__ __forceinline__ float lse_of(float m, float den) { return den == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(den)) * kLn2; }
+// Four outputs, rounded once.
+template <int QT> __device__ __forceinline__ void store_out(const HistAttnArgs &a, int64_t at, f32x4 o) {
   if constexpr (QT == E_F32) {
-    *(f32x4 *)((float *)a.out + row * D + 4 * q4) = o * inv;
+    *(f32x4 *)((float *)a.out + at) = o;
   } else if constexpr (QT == E_F16) {
     typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-    *(f16x4 *)((_Float16 *)a.out + row * D + 4 * q4) = f16x4{(_Float16)(o[0] * inv), (_Float16)(o[1] * inv), (_Float16)(o[2] * inv), (_Float16)(o[3] * inv)};
+    *(f16x4 *)((_Float16 *)a.out + at) = f16x4{(_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3]};
   } else {
     typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-    *(bf16x4 *)((__bf16 *)a.out + row * D + 4 * q4) = bf16x4{(__bf16)(o[0] * inv), (__bf16)(o[1] * inv), (__bf16)(o[2] * inv), (__bf16)(o[3] * inv)};
+    *(bf16x4 *)((__bf16 *)a.out + at) = bf16x4{(__bf16)o[0], (__bf16)o[1], (__bf16)o[2], (__bf16)o[3]};
   }
-  if (q4 == 0 && a.lse) a.lse[row] = den == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(den)) * kLn2;
+}
+// A row's four outputs from its joined state.
+template <int QT, int D>
+__device__ __forceinline__ void finish_history_row(const HistAttnArgs &a, int64_t row, int head, int q4, float m, float den, f32x4 o) {
+  const float f = sink_share(a, head, m, den) * (den == 0.f ? 0.f : 1.f / den);   // of nothing: 0
+  store_out<QT>(a, row * D + 4 * q4, o * f);
+  if (q4 == 0 && a.lse) a.lse[row] = lse_of(m, den);
 }
 
 // A row's state of one chunk, or its outputs where there is no other.
@@ -296,17 +304,29 @@ __device__ __forceinline__ void leave_row(const HistAttnArgs &a, const Block &b,
 }
 
 // Infinities and NaN of an operand's eight numbers taken out: 0·NaN would carry them to rows that do not see them. They are put back
-// into the rows that do behind the loop.
+// into the rows that do behind the loop. An exponent of all ones carries into the sign's place when one is added to it.
 template <bool BF> __device__ __forceinline__ bool take_odd(u32x4 &x) {
-  bool odd = false;
+  constexpr uint32_t em = BF ? 0x7F80u : 0x7C00u, both = em | em << 16, one = BF ? 0x00800080u : 0x04000400u;
+  uint32_t any = 0;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const uint32_t em = BF ? 0x7F80u : 0x7C00u;
-    const bool l = (x[e] & em) == em, h = (x[e] >> 16 & em) == em;
-    x[e] &= (l ? 0u : 0xFFFFu) | (h ? 0u : 0xFFFF0000u);
-    odd |= l || h;
-  }
+  for (int e = 0; e < 4; ++e) any |= (x[e] & both) + one;
+  const bool odd = any & 0x80008000u;
+  if (!__any(odd)) return false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] &= ((x[e] & em) == em ? 0u : 0xFFFFu) | ((x[e] >> 16 & em) == em ? 0u : 0xFFFF0000u);
   return odd;
+}
+// A logit, or where bit BIT of `hidden` is set `none`'s bits: two instructions (the bit's extraction in assembly, or the compiler makes a
+// comparison and a selection of it, with waits between).
+template <int BIT> __device__ __forceinline__ float seen_or(float s, uint32_t hidden, uint32_t none) {
+  uint32_t m;
+  asm("v_bfe_i32 %0, %1, %2, 1" : "=v"(m) : "v"(hidden), "n"(BIT));
+  return __uint_as_float((none & m) | (__float_as_uint(s) & ~m));
+}
+// The same of N logits: element G k + i is key PER k + i from the lane's first.
+template <int G, int PER, int N, int... I>
+__device__ __forceinline__ void hide(float (&y)[N], uint32_t hidden, uint32_t none, std::integer_sequence<int, I...>) {
+  ((y[I] = seen_or<PER * (I / G) + I % G>(y[I], hidden, none)), ...);
 }
 // What take_odd took out of keys j0 .. j1 − 1, for one row's four columns.
 template <int FMT, int D>
@@ -408,6 +428,7 @@ __device__ __forceinline__ void history_few(const HistAttnArgs &a, bool shared, 
     for (int f = 0; f < NF; ++f) query_terms<QT, T::BF, T::NQ>(a.q, at + 4 * EP * (f / X) + 8 * (f % X), a.scale * kLog2e, q[r][f]);
   }
   const float scale = QT == E_F32 ? 1.f : a.scale * kLog2e;
+  const uint32_t none = scale < 0.f ? 0x7F800000u : 0xFF800000u;   // the logit of a key that is not seen: y is −inf
   if (tid == 0) s_odd = 0;
   __syncthreads();
 
@@ -527,9 +548,8 @@ __device__ __forceinline__ void history_few(const HistAttnArgs &a, bool shared, 
       for (int i = 0; i < 8; ++i) y[i] = S[r][i >> 2][i & 3];
       if (part) {
         const int j = b.c0 + 32 * t;
-        const uint32_t sees = ((~first_keys(low[r] - j) | first_keys(a.first - j)) & first_keys(high[r] + 1 - j)) >> (4 * quad);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = sees >> (16 * (i >> 2) + (i & 3)) & 1 ? y[i] : scale < 0.f ? INFINITY : -INFINITY;
+        const uint32_t hidden = ~((~first_keys(low[r] - j) | first_keys(a.first - j)) & first_keys(high[r] + 1 - j)) >> (4 * quad);
+        hide<4, 16>(y, hidden, none, std::make_integer_sequence<int, 8>{});
       }
       const float corr = to_probabilities<8>(y, scale, R[r], L[r], far[r], [](float v) { return max_lane_groups(v); });
       if (__any(corr != 1.f))
@@ -649,6 +669,7 @@ template <int QT, int FMT, int D> __device__ __forceinline__ void history_many(c
     for (int f = 0; f < D / 16; ++f) query_terms<QT, T::BF, T::NQ>(a.q, from + 16 * f, a.scale * kLog2e, q[f]);
   }
   const float scale = QT == E_F32 ? 1.f : a.scale * kLog2e;
+  const uint32_t none = scale < 0.f ? 0x7F800000u : 0xFF800000u;   // the logit of a key that is not seen: y is −inf
   if (tid == 0) s_odd = 0;
   // The keys that any of the wave's rows sees.
   int wlow = row.low, whigh = row.high;
@@ -752,9 +773,8 @@ template <int QT, int FMT, int D> __device__ __forceinline__ void history_many(c
       for (int i = 0; i < 16; ++i) y[i] = S[i];
       if (part) {
         // Element i is key 8 (i / 4) + 4 hh + i % 4 of the 32.
-        const uint32_t sees = ((~first_keys(row.low - j) | first_keys(a.first - j)) & first_keys(row.high + 1 - j)) >> (4 * hh);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) y[i] = sees >> (8 * (i >> 2) + (i & 3)) & 1 ? y[i] : scale < 0.f ? INFINITY : -INFINITY;
+        const uint32_t hidden = ~((~first_keys(row.low - j) | first_keys(a.first - j)) & first_keys(row.high + 1 - j)) >> (4 * hh);
+        hide<4, 8>(y, hidden, none, std::make_integer_sequence<int, 16>{});
       }
       const float corr = to_probabilities<16>(y, scale, R, L, far, [](float v) { return max_halves(v); });
       if (__any(corr != 1.f))
@@ -806,8 +826,24 @@ template <int QT, int FMT, int D> __device__ __forceinline__ void history_many(c
     step(t, one_t{}, zero_t{});
   }
 
-  // Rows to their columns' order through LDS: a wave's own 32 rows.
+  // What a lane's row leaves besides its sums: its state, or its denominator with the sink's share, lse, and the sums' factor.
   L += other_half(L);
+  int64_t to_row = -1;                       // where its sums go
+  float by = 1.f;
+  if (row.in) {
+    const int64_t out = ((int64_t)row.s * a.N + row.i) * a.qh + row.head;
+    if (a.chunks > 1) {
+      to_row = out * a.chunks + (shared ? 0 : a.pre.chunks) + b.chunk;
+      if (hh == 0) a.pm[to_row] = R, a.pl[to_row] = L;
+    } else {
+      to_row = out;
+      float m = R, den = L;
+      by = sink_share(a, row.head, m, den);
+      by *= den == 0.f ? 0.f : 1.f / den;
+      if (hh == 0 && a.lse) a.lse[out] = lse_of(m, den);
+    }
+  }
+  // Rows to their columns' order through LDS: a wave's own 32 rows.
   float *so = (float *)s_mem + (size_t)(wave * 32) * D;
 #pragma unroll
   for (int n = 0; n < NB; ++n)
@@ -820,14 +856,16 @@ template <int QT, int FMT, int D> __device__ __forceinline__ void history_many(c
   for (int e = lane; e < 32 * (D / 4); e += 64) {
     const int r = e / (D / 4), q4 = e % (D / 4);
     f32x4 o = *(const f32x4 *)(so + r * D + 4 * (q4 ^ (r & 7)));
-    const float m = __shfl(R, r), den = __shfl(L, r);
-    const Row x = row_of(a, b, b.r0 + wave * 32 + r);
-    if (!x.in) continue;
-    if (s_odd)
+    const int64_t at = (int64_t)(((uint64_t)(uint32_t)__shfl((int)(to_row >> 32), r) << 32) | (uint32_t)__shfl((int)to_row, r));
+    const float f = __shfl(by, r);
+    if (s_odd) {
+      const int rlow = __shfl(row.low, r), rhigh = __shfl(row.high, r);
       for (int t = 0; t < tiles; ++t)
-        if (is_part(t))
-          put_odd<FMT, D>(b, a.first, x.low, x.high, b.c0 + t * KT, min(b.c0 + t * KT + KT, b.c0 + b.nc), q4, o);
-    leave_row<QT, D>(a, b, x, q4, m, den, o);
+        if (is_part(t)) put_odd<FMT, D>(b, a.first, rlow, rhigh, b.c0 + t * KT, min(b.c0 + t * KT + KT, b.c0 + b.nc), q4, o);
+    }
+    if (at < 0) continue;
+    if (a.chunks > 1) *(f32x4 *)(a.po + at * D + 4 * q4) = o;
+    else store_out<QT>(a, at * D + 4 * q4, o * f);
   }
 }
 
@@ -967,7 +1005,7 @@ template <int QT, int FMT, int D> constexpr int few_waves() {
   return D == 64 ? 4 : 3;
 }
 template <int QT, int FMT, int D> static hipError_t launch_types(HistAttnArgs a, hipStream_t s, int *launches) {
-  constexpr int OCC = few_waves<QT, FMT, D>(), OCC_MANY = D == 256 ? 1 : D == 128 ? 2 : HistTypes<QT, FMT>::NQ == 1 ? 4 : 3;
+  constexpr int OCC = few_waves<QT, FMT, D>(), OCC_MANY = D == 256 ? 1 : D == 128 ? 2 : HistTypes<QT, FMT>::NQ == 1 && HistTypes<QT, FMT>::MX ? 4 : 3;
   const dim3 grid((uint32_t)(a.pre.blocks + a.own.blocks)), block(256);
   if (a.p.k) hipLaunchKernelGGL((history_prefix_kernel<QT, FMT, D, OCC_MANY>), grid, block, 0, s, a);
   else if (a.own.block_rows == 16) hipLaunchKernelGGL((history_few_kernel<QT, FMT, D, 1, OCC>), grid, block, 0, s, a);
