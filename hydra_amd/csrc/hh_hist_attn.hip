@@ -60,7 +60,9 @@ size_t history_reserve(const HistAttnArgs &a, int64_t length, int64_t prefix_row
     const int64_t groups = (int64_t)wanted_groups(a.d, true) * 128;
     return rows * chunks < groups ? rows * chunks : groups;
   };
-  if (!a.h.ring && length > a.h.rows) length = a.h.rows;
+  // A block of rows over a ring sees its window and no more than 130 tokens beside it, whatever the length.
+  if (a.h.ring) length = (int64_t)a.h.rows + 130;
+  else if (length > a.h.rows) length = a.h.rows;
   int64_t n = states(length);
   if (a.p.k) n = (n > rows ? n : rows) + (states(prefix_rows) > rows ? states(prefix_rows) : rows);
   return sizeof(float) * (size_t)n * (a.d + 2);

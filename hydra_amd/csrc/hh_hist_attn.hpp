@@ -195,8 +195,8 @@ __device__ __forceinline__ Row row_of(const HistAttnArgs &a, const Block &b, int
   return x;
 }
 
-// Eight columns of a query as NQ operands.
-template <int QT, bool BF, int NQ> __device__ __forceinline__ void query_terms(const void *q, int64_t at, float scale, u32x4 (&out)[NQ]) {
+// Eight columns of a query as NQ operands. Logits are scaled as fp32 sums: scaled first, a query's terms would be no short numbers any more.
+template <int QT, bool BF, int NQ> __device__ __forceinline__ void query_terms(const void *q, int64_t at, u32x4 (&out)[NQ]) {
   if constexpr (NQ == 1) {
     out[0] = *(const u32x4 *)((const uint16_t *)q + at);
   } else {
@@ -205,11 +205,7 @@ template <int QT, bool BF, int NQ> __device__ __forceinline__ void query_terms(c
       const f32x4 *p = (const f32x4 *)((const float *)q + at);
       const f32x4 l = p[0], h = p[1];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = (e < 4 ? l[e & 3] : h[e & 3]) * scale;
-        // Rounded to fp32 before it is split: a head from the product by one mixed-precision instruction differs near ties.
-        asm volatile("" : "+v"(x[e]));
-      }
+      for (int e = 0; e < 8; ++e) x[e] = e < 4 ? l[e & 3] : h[e & 3];
     } else {
       const f16x8 v = *(const f16x8 *)((const _Float16 *)q + at);
 #pragma unroll
@@ -425,9 +421,9 @@ __device__ __forceinline__ void history_few(const HistAttnArgs &a, bool shared, 
     if (wave == 0 && quad == 0) s_lo[16 * r + l16] = row.low, s_hi[16 * r + l16] = row.high;
     const int64_t at = ((int64_t)row.s * a.N + row.i) * a.q_stride + (int64_t)row.head * D + EP * quad;
 #pragma unroll
-    for (int f = 0; f < NF; ++f) query_terms<QT, T::BF, T::NQ>(a.q, at + 4 * EP * (f / X) + 8 * (f % X), a.scale * kLog2e, q[r][f]);
+    for (int f = 0; f < NF; ++f) query_terms<QT, T::BF, T::NQ>(a.q, at + 4 * EP * (f / X) + 8 * (f % X), q[r][f]);
   }
-  const float scale = QT == E_F32 ? 1.f : a.scale * kLog2e;
+  const float scale = a.scale * kLog2e;
   const uint32_t none = scale < 0.f ? 0x7F800000u : 0xFF800000u;   // the logit of a key that is not seen: y is −inf
   if (tid == 0) s_odd = 0;
   __syncthreads();
@@ -666,9 +662,9 @@ template <int QT, int FMT, int D> __device__ __forceinline__ void history_many(c
   {
     const int64_t from = ((int64_t)row.s * a.N + row.i) * a.q_stride + (int64_t)row.head * D + 8 * hh;
 #pragma unroll
-    for (int f = 0; f < D / 16; ++f) query_terms<QT, T::BF, T::NQ>(a.q, from + 16 * f, a.scale * kLog2e, q[f]);
+    for (int f = 0; f < D / 16; ++f) query_terms<QT, T::BF, T::NQ>(a.q, from + 16 * f, q[f]);
   }
-  const float scale = QT == E_F32 ? 1.f : a.scale * kLog2e;
+  const float scale = a.scale * kLog2e;
   const uint32_t none = scale < 0.f ? 0x7F800000u : 0xFF800000u;   // the logit of a key that is not seen: y is −inf
   if (tid == 0) s_odd = 0;
   // The keys that any of the wave's rows sees.

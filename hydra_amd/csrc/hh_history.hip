@@ -8,7 +8,7 @@ namespace {
 
 using hh::fail;
 
-constexpr int kMaxSequences = 4096, kMaxTokens = 65536, kMaxRows = 1 << 28, kMaxStep = 1 << 22;
+constexpr int kMaxSequences = 4096, kMaxTokens = 65536, kMaxRows = 1 << 28, kMaxStep = 1 << 22, kMaxHeadRows = 1 << 25;
 
 bool aligned(const void *p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 bool elem(int32_t type) { return type >= HH_F32 && type <= HH_BF16; }
@@ -56,6 +56,7 @@ int check_history(const hh_history *h) {
   if (!h) return fail(HH_EINVAL, "history is NULL");
   if (h->sequences < 1 || h->sequences > kMaxSequences) return fail(HH_EINVAL, "sequences outside 1..4096");
   if (h->kv_heads < 1 || h->kv_heads > 256) return fail(HH_ESHAPE, "kv_heads outside 1..256");
+  if ((int64_t)h->sequences * h->kv_heads > 1 << 18) return fail(HH_EINVAL, "sequences x kv_heads above 2^18");
   if (h->head_dim != 64 && h->head_dim != 128 && h->head_dim != 256) return fail(HH_ESHAPE, "head_dim must be 64, 128 or 256");
   if (h->format < HH_HISTORY_F16 || h->format > HH_HISTORY_MXFP4) return fail(HH_EINVAL, "unknown history format");
   if (h->rows < 1 || h->rows > kMaxRows) return fail(HH_EINVAL, "a history's rows outside 1..2^28");
@@ -110,6 +111,7 @@ int check_attention(const hh_history_desc *d, const hh_history *h, const hh_hist
   if (int rc = check_step(h, d->tokens)) return rc;
   if (d->q_heads < 1 || d->q_heads % h->kv_heads || d->q_heads / h->kv_heads > hh::kTreeQM)
     return fail(HH_ESHAPE, "q_heads must be kv_heads x 1..16");
+  if ((int64_t)h->sequences * d->tokens * d->q_heads > kMaxHeadRows) return fail(HH_EINVAL, "more than 2^25 heads of tokens: split the batch");
   const bool mx = h->format >= HH_HISTORY_MXFP8;
   if (!elem(d->type) || !(mx || h->format == (d->type == HH_BF16 ? HH_HISTORY_BF16 : HH_HISTORY_F16)))
     return fail(HH_EINVAL, "types must be F32 or F16 over F16, BF16 over BF16, or any over MXFP8 or MXFP4");

@@ -595,7 +595,7 @@ typedef struct hh_history {
   void    *k, *v;              /* 16-byte aligned                                               */
   uint8_t *k_scales, *v_scales;/* MXFP8 and MXFP4, 8-byte aligned; NULL otherwise               */
   const int32_t *lengths;      /* [S]                                                           */
-  int32_t sequences, kv_heads; /* 1..4096, 1..256                                               */
+  int32_t sequences, kv_heads; /* 1..4096, 1..256; S x kv_heads at most 2^18                     */
   int32_t head_dim;            /* 64, 128, 256                                                  */
   int32_t format;              /* hh_history_format                                             */
   int32_t rows;                /* 1..2^28                                                       */
@@ -620,7 +620,7 @@ int hh_history_advance(hh_ctx *ctx, const hh_history *h, int32_t tokens, const i
 
 typedef struct hh_history_desc {
   int32_t tokens;              /* N of the step: 1..65536; S·N at most 2^22                      */
-  int32_t q_heads;             /* kv_heads x 1..16                                              */
+  int32_t q_heads;             /* kv_heads x 1..16; S·N·q_heads at most 2^25                     */
   int32_t type;                /* hh_elem of q and out: F32 and F16 over F16, MXFP8, MXFP4; BF16 over BF16, MXFP8, MXFP4 */
   int32_t window, first;       /* 0: every position up to the token's own. Otherwise those above its own − window, and those below
                                   `first`                                                       */
@@ -639,13 +639,15 @@ typedef struct hh_history_desc {
  *   prefix  NULL, or a history of one sequence (same heads, head_dim and format; no ring; window 0): its lengths[0] rows come before
  *           every sequence's own and are seen by each token. They are read once for the batch.
  * Tokens from counts[s] on are not written. A token that sees nothing (its own position not held) gets 0 and lse −inf, or with a sink the
- * sink. Keys that a token does not see, infinities and NaN among them, have no part in its output. Logits may be of any size that
- * fp32 holds, times log2(e).                                                                      */
+ * sink. Keys that a token does not see, infinities and NaN among them, have no part in its output. Logits, and the products before
+ * sm_scale, may be of any size that fp32 holds, times log2(e). F32 queries over an F16 history are held to 2^-22, or 2^-25 where that
+ * is more, and up to 65504.                                                                       */
 int hh_history_attention(hh_ctx *ctx, const hh_history_desc *desc, const hh_history *h, const hh_history *prefix,
                          const void *q, const int32_t *counts, const uint16_t *sinks, void *out, float *lse);
 
 /* Pre-sizes the context's workspace of hh_history_attention for every call with these heads, head_dim, type and format, and with
- * sequences, tokens, rows, max_length and prefix rows up to these, any window. It grows by itself in eager calls, but not while a graph is
+ * sequences, tokens, rows, max_length and prefix rows up to these, any window (over a ring any max_length). It grows by itself in
+ * eager calls, but not while a graph is
  * recorded or lives: then this succeeds where a call of just these sizes fits.                    */
 int hh_history_reserve(hh_ctx *ctx, const hh_history_desc *desc, const hh_history *h, const hh_history *prefix);
 

@@ -66,6 +66,13 @@ def test_writes(kw, code):
     assert write(history(), **kw) == code
 
 
+def test_too_many_heads():
+    h = history(sequences=4096, kv_heads=65)
+    assert write(h) == -1 and attend(h, q_heads=65) == -1
+    assert attend(history(sequences=4096, kv_heads=64), tokens=129, q_heads=64) == -1
+    assert attend(history(sequences=4096, kv_heads=64), tokens=128, q_heads=64, q=72) == -2
+
+
 def test_too_many_tokens():
     assert write(history(sequences=4096), tokens=1025) == -1
     assert attend(history(sequences=4096), tokens=1025) == -1
