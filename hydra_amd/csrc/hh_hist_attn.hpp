@@ -673,6 +673,9 @@ template <int QT, int FMT, int D> __device__ __forceinline__ void history_many(c
   for (int o = 1; o < 32; o <<= 1) wlow = min(wlow, __shfl_xor(wlow, o)), whigh = max(whigh, __shfl_xor(whigh, o));
   wlow = __builtin_amdgcn_readfirstlane(wlow);
   whigh = __builtin_amdgcn_readfirstlane(whigh);
+  // A wave without rows only loads, and leaves its SIMD to other workgroups' (40 rows of 16384 keys, heads of 64: 24 us, 30 with its
+  // products; of 128: 33 and 39). Heads of 256 have one wave a SIMD: nothing to leave it to, and prompts 3% longer.
+  const bool idle = D < 256 && b.r0 + wave * 32 >= b.count * a.qm;
   __syncthreads();
 
   const int tiles = (b.nc + KT - 1) / KT;
@@ -751,6 +754,7 @@ template <int QT, int FMT, int D> __device__ __forceinline__ void history_many(c
 #pragma unroll
   for (int n = 0; n < NB; ++n) vat[n] = vrow * (2 * D) + (j16 & 1) * 8 + ((vpiece ^ (4 * n)) << 4);
   auto compute = [&](int t, auto slot) {
+    if (idle) return;
     const bool part = is_part(t);
 #pragma unroll
     for (int k = 0; k < KT / 32; ++k) {

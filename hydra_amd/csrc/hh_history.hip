@@ -117,7 +117,7 @@ int check_attention(const hh_history_desc *d, const hh_history *h, const hh_hist
     return fail(HH_EINVAL, "types must be F32 or F16 over F16, BF16 over BF16, or any over MXFP8 or MXFP4");
   if (d->window < 0 || d->first < 0 || d->max_length < 0) return fail(HH_EINVAL, "window, first and max_length must be >= 0");
   if (d->first && !d->window) return fail(HH_EINVAL, "first tokens are a window's");
-  if (!std::isfinite(d->sm_scale) || d->sm_scale == 0.f) return fail(HH_EINVAL, "sm_scale must be finite and not 0");
+  if (!std::isfinite(1.5f * d->sm_scale) || d->sm_scale == 0.f) return fail(HH_EINVAL, "sm_scale must be finite, log2(e) times too, and not 0");
   if (h->ring) {
     if (!d->window || (int64_t)d->window + d->tokens - 1 > h->rows - h->pinned)
       return fail(HH_EINVAL, "a ring needs a window, and rows for window + tokens - 1 positions besides the pinned ones");

@@ -626,7 +626,7 @@ typedef struct hh_history_desc {
                                   `first`                                                       */
   int32_t max_length;          /* the longest expected history with the step's tokens, 0 = the history's rows: it sizes the
                                   launch; every length is handled                                */
-  float   sm_scale;            /* finite, not 0                                                 */
+  float   sm_scale;            /* finite, log2(e) times too, not 0                              */
   int64_t q_stride;            /* elements between tokens of q, 0 = packed; a multiple of 16 bytes */
 } hh_history_desc;
 

@@ -96,7 +96,7 @@ def test_advances():
 @pytest.mark.parametrize("kw,code", [
     (dict(q_heads=0), -6), (dict(q_heads=5), -6), (dict(q_heads=34), -6), (dict(type=3), -1), (dict(window=-1), -1), (dict(first=-1, window=3), -1),
     (dict(first=2), -1), (dict(max_length=-1), -1), (dict(sm_scale=0.0), -1), (dict(sm_scale=float("nan")), -1),
-    (dict(sm_scale=float("inf")), -1), (dict(q_stride=255), -6), (dict(q_stride=257), -2), (dict(q_stride=260, type=2), -2),
+    (dict(sm_scale=float("inf")), -1), (dict(sm_scale=3e38), -1), (dict(q_stride=255), -6), (dict(q_stride=257), -2), (dict(q_stride=260, type=2), -2),
     (dict(q_stride=1 << 31), -6), (dict(tokens=0), -1), (dict(tokens=65537), -1),
 ])
 def test_attention_descriptions(kw, code):
