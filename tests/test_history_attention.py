@@ -2,7 +2,10 @@
 
 Tolerances, rel-L2 of a row (one token's head). fp32 sums of up to 256 products (terms of a logit sum to ~10 in magnitude:
 sqrt(256)·10·2^-24 = 1e-5 of a probability), probabilities and their sums alike: 2e-5. F16 and BF16 outputs are rounded once, half
-a step of each number; probabilities of BF16's products are pairs, to 2^-15 each (3e-5). lse, absolute: 1e-5 of a logit's
+a step of each number; probabilities of BF16's products are pairs, to 2^-15 each (3e-5). Of more than 32 rows of a kv head (16 of a
+prefix's) probabilities of the output's own type are rounded once too, and normalised by their rounded sum: an error of Σ d_j p_j (v_j − o)
+besides, |d_j| up to half a step, for independent d_j a fraction sqrt(Σ p_j^2) |v − o| / |o| of d's 0.42 half steps (rms), as the output's own 0.42:
+0.6 of the half step with values as large as their spread. lse, absolute: 1e-5 of a logit's
 error, its sum's and its logarithm's with it 4e-5."""
 import math
 
