@@ -420,7 +420,11 @@ __device__ __forceinline__ u32x2 read_columns(const uint8_t *p) {   // transposi
 // Few rows: each wave has all of a kv head's, 16·RT, and tiles of 32 keys of its own, W of them a workgroup; the next tile's bytes are
 // in flight under this one's products. On the 16x16 MFMA, S^T [16 keys × 16 rows] twice a tile: a head of 64 in 8 bits is 64 bytes, four
 // lanes of a key, so that a load is one stretch of memory, and goes to the operands' registers as it is, since the order of a product's
-// columns is free. Values pass through LDS to be read by columns. No barrier until the waves' states meet.
+// columns is free. Values pass through LDS to be read by columns. No barrier until the waves' states meet. Bound by the bytes where
+// there are enough: eight streams of up to 32768 keys in 8 bits, fp32, 64 / 8 heads of 64, 208 MB in 39 us (5.3 TB/s; the joining launch 5
+// more); 131071 keys in 4 bits, 16 / 2 heads of 256, 71 MB in 17.5 us (4.1 TB/s). By the chain of latencies where
+// there are few: 16 windows of 132 keys 6.7 us. With 64 rows a wave (four of these tiles of 16) 64 rows of 32768 keys took 26 us of heads of 64 in
+// bf16, the kernel of many rows 29; but of fp32 42 and 35, and of 1000 keys 14.7 and 13.6: the sums and the queries' terms fill the registers.
 template <int D, int RT, int W> constexpr int few_lds() { return W * (16 * RT * D * 4 > 64 * D ? 16 * RT * D * 4 : 64 * D); }
 template <int QT, int FMT, int D, int RT, int W>
 __device__ __forceinline__ void history_few(const HistAttnArgs &a, bool shared, int block, uint8_t *s_mem) {
@@ -650,9 +654,13 @@ template <int X, int PR> __device__ __forceinline__ void piece_place(int e, int 
 // Many rows: 128 a workgroup, 32 a wave, on the 32x32 MFMA; tiles of KT keys, whose 16-byte pieces the threads share, become operands in
 // LDS, two tiles in turn, read by every wave. The bytes of the tile after the next are in flight under a tile's products. A tile's one
 // barrier keeps the waves of a workgroup in step, so the workgroups are small: several a compute unit, each at its own place. Bound by the
-// VALU's instructions (four fifths of them the softmax: an fma, an exponential, a sum, the terms), so that what changes from tile to tile is
-// kept to scalars and immediate offsets. Scores of the next tile formed under the exponentials of one, with a third place for values,
-// took 7 to 10 percent longer.
+// VALU's instructions and the matrix unit's cycles, one after the other on a SIMD (a prompt of 4096, 64 / 8 heads of 64, bf16 over 8 bits: 67%
+// and 35% of the time, 105 instructions for a wave's 32 keys, 64 of them the softmax: an fma, an exponential, two sums, the rounding), so what
+// changes from tile to tile is kept to scalars and immediate offsets. That prompt takes 168 us (820 TFLOP/s; at a large
+// library product's rate it would be 110); two prompts of 6001, 32 / 8 heads of 128 in fp16 under a window of 1024, 242 us (630); 256 tokens
+// behind 16384, 16 / 2 heads of 256, 138 us (500: one wave a SIMD); a prompt of 2048 of those heads 123 us (280: one workgroup a unit, and the first see
+// little). Tried and slower: scores of the next tile formed under the exponentials of one, with a third place for values (7 to 10%); rounded
+// probabilities packed where they are summed (12%: they spill at four waves a SIMD).
 template <int D> constexpr int many_keys() { return D == 256 ? 32 : 64; }
 template <int D> constexpr int many_lds() { return 2 * many_keys<D>() * D * 4 > 128 * D * 4 ? 2 * many_keys<D>() * D * 4 : 128 * D * 4; }
 template <int QT, int FMT, int D> __device__ __forceinline__ void history_many(const HistAttnArgs &a, bool shared, uint32_t block, uint8_t *s_mem) {
@@ -908,7 +916,9 @@ template <int QT, int FMT, int D, int OCC> __global__ __launch_bounds__(256, OCC
   warm_kernargs<sizeof(HistAttnArgs)>();
   history_many<QT, FMT, D>(a, false, blockIdx.x, s_mem);
 }
-// The prefix's pass and behind it the own histories', which fill the chip under its last workgroups.
+// The prefix's pass and behind it the own histories', which fill the chip under its last workgroups: 64 streams of 500 over 24576 shared keys
+// 47 us; four streams of 50 over 1000, fp32 in fp16, 9.2 (latencies). The prefix's rows of all streams are in one workgroup's tiles, so
+// that its keys are read once for 128 rows.
 template <int QT, int FMT, int D, int OCC> __global__ __launch_bounds__(256, OCC) void history_prefix_kernel(HistAttnArgs a) {
   constexpr int few = few_lds<D, 1, 4>();
   __shared__ __align__(1024) uint8_t s_mem[many_lds<D>() > few ? many_lds<D>() : few];
@@ -939,7 +949,7 @@ __device__ __forceinline__ RowChunks row_chunks(const HistAttnArgs &a, int64_t r
   return x;
 }
 
-// Joins a row's chunks, in order: a wave per row, D / 4 lanes a chunk.
+// Joins a row's chunks, in order: a wave per row, D / 4 lanes a chunk. 4096 rows of 34 chunks of 64: 8 us (4.5 TB/s); 512 of up to 12: 5.
 template <int QT, int D> __global__ __launch_bounds__(256) void history_merge_kernel(HistAttnArgs a) {
   warm_kernargs<sizeof(HistAttnArgs)>();
   constexpr int LR = D / 4, GR = 64 / LR;    // lanes per chunk, chunks at a time

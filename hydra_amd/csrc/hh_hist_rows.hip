@@ -2,7 +2,9 @@
 //
 // Eight columns a lane, four lanes a scale: the largest magnitude of 32 columns by two exchanges, the scale's exponent from
 // its bits, and x·2^-e, exact, through the conversion to e4m3 or e2m1, to nearest even. Lanes run over a head's columns, then over
-// the tokens, so that both sides move whole stretches: [token][head] on one, [head][row] on the other. Bound by the bytes.
+// the tokens, so that both sides move whole stretches: [token][head] on one, [head][row] on the other. Bound by the bytes: two prompts of up to
+// 8000 tokens, 8 heads of 128, bf16 into 4 bits 16.4 us and back 14.4 (62 MB in and out each way: 3.8 and 4.3 TB/s, a copy 5.2); a step of 32 tokens
+// 3 us each, its latencies.
 #include "hh_hist.hpp"
 
 namespace hh {
@@ -181,7 +183,7 @@ __global__ __launch_bounds__(64) void history_advance_kernel(int32_t *lengths, c
   if (s < S) lengths[s] = min(hist_length(lengths, s) + step_count(counts, s, N), kHistLength);
 }
 
-constexpr int kRowsAhead = 4;  // rows that a lane has in flight, where there are enough to fill the chip
+constexpr int kRowsAhead = 4;  // rows that a lane has in flight, where there are enough to fill the chip (two prompts of 8000: 34 us, 47 with one)
 template <int T, int FMT> static void launch_rows_tf(const HistRowsArgs &a, bool write, hipStream_t s) {
   const int64_t rows = (int64_t)a.kvh * a.N, each = 256 / (a.d / 8);
   const bool ahead = 2 * rows * a.S >= 1024 * kRowsAhead * each;
