@@ -209,6 +209,7 @@ int hh_rotary(hh_ctx *ctx, const hh_rotary_desc *d, const double *turns, float m
     a.r[i] = {r.x, r.y, r.heads, xs, ys};
   }
   if (count == 2 && a.r[0].y == a.r[1].y) return fail(HH_EINVAL, "both outputs are the same memory");
+  if (count == 2 && (a.r[0].y == a.r[1].x || a.r[1].y == a.r[0].x)) return fail(HH_EINVAL, "an output is the other's input");
   if (tokens == 0) return HH_OK;
   a.turns = turns;
   a.positions = positions;

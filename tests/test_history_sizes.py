@@ -219,3 +219,43 @@ def test_another_context_and_torch_streams_beside_it():
     a.synchronize()
     b.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.parametrize("kind,fmt", [("bf16", "mxfp8"), ("f16", "f16"), ("f32", "mxfp4")])
+@pytest.mark.parametrize("S,N,rows,shared", [(2, 3, 900, None), (2, 50, 300, None), (3, 40, 80, 500)])
+def test_outputs_in_place_strided_queries_and_no_lse(kind, fmt, S, N, rows, shared):
+    """The same bits as into memory of their own with lse, whatever few or many rows, chunks or a prefix do with them."""
+    import torch
+    from hydra_amd import history as hi
+    from hydra_amd.layer import Context
+    ctx = Context(0)
+    H, G, D = 8, 2, 64
+    t = make(torch, S, N, H, G, D, kind, fmt, rows, [rows - N, 5, 0][:S], sinks=True, shared=shared, seed=3)
+    want, _ = call(torch, ctx, t)
+    h, p = histories(torch, t)
+    q, c, sinks = t["q"].cuda(), t["counts"].cuda(), t["sinks"].cuda()
+    wide = torch.full((S, N, (H + 2 * G) * D), float("nan"), dtype=q.dtype, device="cuda:0")
+    wide[..., :H * D] = q.reshape(S, N, -1)
+    out = torch.zeros_like(q)
+    torch.cuda.synchronize()
+    hi.history_attention_into(ctx, h, wide[..., :H * D].unflatten(-1, (H, D)), c, out, sinks=sinks, prefix=p)
+    hi.history_attention_into(ctx, h, q, c, q, sinks=sinks, prefix=p)
+    ctx.synchronize()
+    assert torch.equal(out, want) and torch.equal(q, want)
+
+
+@pytest.mark.parametrize("kind,fmt", [("bf16", "mxfp8"), ("f16", "f16"), ("f32", "mxfp8")])
+@pytest.mark.parametrize("N,shared", [(2, None), (40, None), (40, 300)])
+def test_a_query_of_nan_or_infinities_stays_alone(kind, fmt, N, shared):
+    import torch
+    from hydra_amd.layer import Context
+    ctx = Context(0)
+    t = make(torch, 2, N, 8, 2, 64, kind, fmt, 400, [300, 7], shared=shared, seed=4)
+    want, wl = call(torch, ctx, t)
+    t["q"][0, 1, 3, 5] = float("nan")
+    t["q"][1, 0, 2] = float("inf")
+    out, lse = call(torch, ctx, t)
+    touched = torch.zeros(out.shape[:3], dtype=torch.bool, device="cuda:0")
+    touched[0, 1, 3] = touched[1, 0, 2] = True
+    assert torch.equal(out[~touched], want[~touched]) and torch.equal(lse[~touched], wl[~touched])
+    assert torch.isnan(out[touched]).all()

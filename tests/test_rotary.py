@@ -182,7 +182,7 @@ def call(rows=None, count=1, tokens=4, type_=0, ctx=1 << 20, positions=64, turns
     (dict(rows={0: dict(x_stride=128)}), -6), (dict(rows={0: dict(y_stride=255)}), -6), (dict(rows={0: dict(x_stride=257)}), -2),
     (dict(rows={0: dict(x_stride=260)}, type_=1), -2), (dict(rows={0: dict(y=64, y_stride=512)}), -1),
     (dict(rows={0: dict(x_stride=1 << 31)}), -6), (dict(rows={1: dict(y=1024)}, count=2), -1), (dict(rows={1: dict(x=None)}, count=2), -1),
-    (dict(rotated=65), -6),
+    (dict(rotated=65), -6), (dict(rows={1: dict(y=64)}, count=2), -1), (dict(rows={0: dict(y=4096)}, count=2), -1),
 ])
 def test_calls_that_are_refused(kw, code):
     assert call(**kw) == code
