@@ -183,12 +183,12 @@ def lib() -> C.CDLL:
     L.hh_draft_reserve.argtypes = [vp, C.POINTER(TreeDescC), C.POINTER(KVCacheC), i32,
                                    C.POINTER(VerifyDescC)]
     L.hh_rotary_table.argtypes = [C.POINTER(RotaryDescC), C.POINTER(C.c_double), C.POINTER(C.c_float)]
-    L.hh_rotary.argtypes = [vp, C.POINTER(RotaryDescC), vp, C.c_float, i32, i32, vp, C.POINTER(RotaryRowsC), i32]
+    L.hh_rotary.argtypes = [vp, C.POINTER(RotaryDescC), vp, C.c_float, i32, i32, vp, vp, i32]     # rows: an array of RotaryRowsC, or its bytes
     L.hh_history_write.argtypes = [vp, C.POINTER(HistoryC), i32, vp, vp, i64, i32, vp]
     L.hh_history_read.argtypes = [vp, C.POINTER(HistoryC), i32, vp, i32, vp, vp, vp]
     L.hh_history_advance.argtypes = [vp, C.POINTER(HistoryC), i32, vp]
-    L.hh_history_attention.argtypes = [vp, C.POINTER(HistoryDescC), C.POINTER(HistoryC), C.POINTER(HistoryC)] + [vp] * 5
-    L.hh_history_reserve.argtypes = [vp, C.POINTER(HistoryDescC), C.POINTER(HistoryC), C.POINTER(HistoryC)]
+    L.hh_history_attention.argtypes = [vp, vp, C.POINTER(HistoryC), C.POINTER(HistoryC)] + [vp] * 5    # a HistoryDescC, or its bytes
+    L.hh_history_reserve.argtypes = [vp, vp, C.POINTER(HistoryC), C.POINTER(HistoryC)]
     L.hh_ctx_profile_read.argtypes = [vp, C.POINTER(C.c_double), C.POINTER(C.c_int64)]
     for name in EXPORTS:
         if name not in ("hh_last_error", "hh_ctx_stream", "hh_dispatch_count"):

@@ -15,10 +15,11 @@ recorded with `Context.capture` follows them. The conventions of formats, positi
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
-from ._lib import HistoryC, HistoryDescC, RotaryDescC, RotaryRowsC, check, lib
+from ._lib import HistoryC, RotaryDescC, check, lib
 from .layer import Context
 from .speculative import ELEM, _cuda, _ptr, _same, _spaced
 
@@ -45,7 +46,7 @@ class Rotary:
         self.turns = torch.tensor(list(table), dtype=torch.float64, device=device)
 
 
-_ROWS = {n: RotaryRowsC * n for n in (1, 2)}
+_ROWS = (struct.Struct("PPiqq"), struct.Struct("PPiqqPPiqq"))      # one and two RotaryRowsC: an array of structures takes five times as long to make
 
 
 def _tokens(t, name, shape, dtype, device):
@@ -85,18 +86,21 @@ def rotary_into(ctx: Context, rotary: Rotary, positions, q, q_out, k=None, k_out
         raise ValueError(f"the frequencies are on {rotary.turns.device}, q on {dev}")
     shape = q.shape
     _same(positions, "positions", shape[:-2], _I32, dev)
-    rows = [(q.data_ptr(), q_out.data_ptr(), shape[-2], _tokens(q, "q", shape, dtype, dev), _tokens(q_out, "q_out", shape, dtype, dev))]
+    x = _tokens(q, "q", shape, dtype, dev)
+    rows = (q.data_ptr(), q_out.data_ptr(), shape[-2], x, x if q_out is q else _tokens(q_out, "q_out", shape, dtype, dev))
     if k is not None:
         if k_out is None:
             raise ValueError("k needs k_out")
         other = k.shape
         if other[:-2] != shape[:-2] or other[-1] != shape[-1]:
             raise ValueError(f"k {tuple(other)} must have the tokens and head_dim of q {tuple(shape)}")
-        rows.append((k.data_ptr(), k_out.data_ptr(), other[-2], _tokens(k, "k", other, dtype, dev), _tokens(k_out, "k_out", other, dtype, dev)))
+        x = _tokens(k, "k", other, dtype, dev)
+        rows += (k.data_ptr(), k_out.data_ptr(), other[-2], x, x if k_out is k else _tokens(k_out, "k_out", other, dtype, dev))
     n = positions.numel()
     if n:   # tensors of nothing have no address
+        count = len(rows) // 5
         check(lib().hh_rotary(ctx.handle, C.byref(rotary.c), rotary.turns.data_ptr(), rotary.magnitude, ELEM[dtype], n,
-                              positions.data_ptr(), _ROWS[len(rows)](*rows), len(rows)))
+                              positions.data_ptr(), _ROWS[count - 1].pack(*rows), count))
     return (q_out, k_out) if k is not None else q_out
 
 
@@ -192,9 +196,15 @@ def history_advance(ctx: Context, history: History, counts, tokens: int):
     check(lib().hh_history_advance(ctx.handle, C.byref(history.c), tokens, counts.data_ptr()))
 
 
+_DESC = struct.Struct("iiiiiifq")            # a HistoryDescC
+
+
 def _desc(history, tokens, q_heads, dtype, window, first, max_length, sm_scale, q_stride):
-    return HistoryDescC(tokens, q_heads, ELEM[dtype], window, first, max_length,
-                        history.head_dim ** -0.5 if sm_scale is None else sm_scale, q_stride)
+    try:
+        return _DESC.pack(tokens, q_heads, ELEM[dtype], window, first, max_length,
+                          history.head_dim ** -0.5 if sm_scale is None else sm_scale, q_stride)
+    except struct.error as e:
+        raise ValueError(f"tokens, window, first and max_length must be 32-bit whole numbers, sm_scale a number: {e}") from None
 
 
 def history_attention_into(ctx: Context, history: History, q, counts, out, lse=None, sinks=None, window: int = 0, first: int = 0,
@@ -219,7 +229,7 @@ def history_attention_into(ctx: Context, history: History, q, counts, out, lse=N
     if prefix is not None and prefix.device != dev:
         raise ValueError(f"the prefix is on {prefix.device}, the history on {dev}")
     d = _desc(history, N, H, q.dtype, window, first, max_length, sm_scale, stride)
-    check(lib().hh_history_attention(ctx.handle, C.byref(d), C.byref(history.c), None if prefix is None else C.byref(prefix.c),
+    check(lib().hh_history_attention(ctx.handle, d, C.byref(history.c), None if prefix is None else C.byref(prefix.c),
                                      q.data_ptr(), counts.data_ptr(), _ptr(sinks), out.data_ptr(), _ptr(lse)))
     return out
 
@@ -231,4 +241,4 @@ def history_reserve(ctx: Context, history: History, tokens: int, q_heads: int, d
     if dtype not in ELEM:
         raise ValueError(f"dtype must be fp32, fp16 or bf16, not {dtype}")
     d = _desc(history, tokens, q_heads, dtype, window, first, max_length, None, 0)
-    check(lib().hh_history_reserve(ctx.handle, C.byref(d), C.byref(history.c), None if prefix is None else C.byref(prefix.c)))
+    check(lib().hh_history_reserve(ctx.handle, d, C.byref(history.c), None if prefix is None else C.byref(prefix.c)))

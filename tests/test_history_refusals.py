@@ -171,3 +171,25 @@ def test_python():
     for t in (q[:, ::2].expand(2, 3, 4, 64)[:, :, :, ::2], q.transpose(2, 3), q[:, :3], q[:1, :1].expand(2, 5, 4, 64)):
         with pytest.raises(ValueError):
             hi._tokens(t, "q", t.shape, torch.float32, q.device)
+
+
+def test_python_describes_calls_as_the_header_does():
+    """What is packed for the C entries is the structures', and what does not fit them is refused."""
+    import torch
+    from hydra_amd import history as hi
+    for n in (1, 2):
+        v = (64, 128, 3, 1 << 33, 5, 4096, 8192, 7, 9, 1 << 34)[:5 * n]
+        a = (L.RotaryRowsC * n).from_buffer_copy(hi._ROWS[n - 1].pack(*v))
+        assert tuple(getattr(a[i], f) for i in range(n) for f, _ in L.RotaryRowsC._fields_) == v
+        assert hi._ROWS[n - 1].size == C.sizeof(a)
+    h = hi.History.empty(2, 3, 10, 64, device="cpu")
+    d = L.HistoryDescC.from_buffer_copy(hi._desc(h, 1, 2, torch.float16, 3, 4, 5, 0.25, 1 << 33))
+    assert hi._DESC.size == C.sizeof(d)
+    assert [getattr(d, f) for f, _ in L.HistoryDescC._fields_] == [1, 2, 1, 3, 4, 5, 0.25, 1 << 33]
+    for kw in (dict(window=1 << 31), dict(first=-(1 << 31) - 1), dict(max_length=1 << 40), dict(sm_scale="1"), dict(tokens=1.5)):
+        a = dict(tokens=1, window=0, first=0, max_length=0, sm_scale=1.0)
+        a.update(kw)
+        with pytest.raises(ValueError):
+            hi._desc(h, a["tokens"], 6, torch.float32, a["window"], a["first"], a["max_length"], a["sm_scale"], 0)
+    d = L.HistoryDescC.from_buffer_copy(hi._desc(h, 1, 2, torch.float16, 0, 0, 0, 1e39, 0))
+    assert d.sm_scale == float("inf")        # which the entry refuses
