@@ -44,7 +44,7 @@ struct HistAttnArgs {
     int chunks, per, tile, block_rows, row_blocks, blocks;
   } own, pre;
   int chunks;                          // of a row, the prefix's first
-  float *pm, *pl, *pu, *po;            // chunk states [S][N][qh][chunks] (pu: of the rounded weights), their sums [..][chunks][d]
+  float *pm, *pl, *po;                 // chunk states [S][N][qh][chunks], their sums [..][chunks][d]
 };
 
 struct RotaryRows {

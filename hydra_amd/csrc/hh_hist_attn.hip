@@ -47,7 +47,7 @@ void history_plan(HistAttnArgs &a, int64_t length, int64_t prefix_rows) {
 }
 
 size_t history_workspace(const HistAttnArgs &a) {
-  return a.chunks > 1 ? sizeof(float) * (size_t)a.S * a.N * a.qh * a.chunks * (a.d + 3) : 0;
+  return a.chunks > 1 ? sizeof(float) * (size_t)a.S * a.N * a.qh * a.chunks * (a.d + 2) : 0;
 }
 
 // A pass that is cut has at most wanted_groups workgroups of at most 128 rows each, and a row at most as many chunks as half its tiles, of
@@ -66,7 +66,7 @@ size_t history_reserve(const HistAttnArgs &a, int64_t length, int64_t prefix_row
   else if (length > a.h.rows) length = a.h.rows;
   int64_t n = states(length);
   if (a.p.k) n = (n > rows ? n : rows) + (states(prefix_rows) > rows ? states(prefix_rows) : rows);
-  return sizeof(float) * (size_t)n * (a.d + 3);
+  return sizeof(float) * (size_t)n * (a.d + 2);
 }
 
 hipError_t launch_history_attention(HistAttnArgs a, int type, hipStream_t s, int *launches) {

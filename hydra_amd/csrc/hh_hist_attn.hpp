@@ -9,10 +9,8 @@
 // Numbers in 8 and 4 bits become bf16 as they are loaded, exactly (4 and 2 bits of mantissa, any power of two), so products are those
 // of the numbers held. Queries enter as the terms of bf16 that hold them (F16: two, F32: three; over F16 histories F32 as two of fp16),
 // probabilities as two (outputs of 16 bits: to 2^-15 of each) or three (F32: as exact as the sums) of bf16, or two of fp16: outputs of 16 bits
-// are rounded once. Of many rows, where the products and terms are what takes the time and not the bytes, probabilities are rounded once
-// where the operand's type is the output's, to half a step as the output then is (a prompt of 4096, bf16: 168 us and 2.2e-3 from 64 bits, two
-// terms 214 us and 1.7e-3). Their sum is then taken of the rounded ones too, so that a row's weights come to one: a row with one key is that
-// key's value; the log of the denominator is of the sum before rounding.
+// are rounded once, and a token's weights are held alike whether few or many share its call. (One term of many rows would take a fifth off
+// a prompt's time, and a fourth onto its error.)
 #pragma once
 #include <type_traits>
 #include <utility>
@@ -31,11 +29,7 @@ template <int QT, int FMT> struct HistTypes {
   static constexpr int E = FMT == H_MXFP8 ? 16 : FMT == H_MXFP4 ? 32 : 8;                       // numbers of 16 bytes
   static constexpr int NQ = QT == E_F32 ? (BF ? 3 : 2) : QT == E_F16 && BF ? 2 : 1;             // terms of a query
   static constexpr int NP = QT == E_F32 && BF ? 3 : 2;                                          // of a probability
-  static constexpr int NPM = QT == E_BF16 || (QT == E_F16 && !BF) ? 1 : NP;                     // of many rows
 };
-
-// Whether a row has a denominator of its own for the weights used.
-constexpr bool two_sums(int qt) { return qt != E_F32; }
 
 // Memory that is read as the device's own: a load that could be of LDS too would wait with LDS's.
 typedef const uint8_t __attribute__((address_space(1))) *gptr_t;
@@ -245,10 +239,7 @@ struct SplitConst {
   __device__ __forceinline__ SplitConst() : minus1(-1.f), m0(0x0000BF80u), m1(0xBF800000u) { asm volatile("" : "+s"(minus1), "+s"(m0), "+s"(m1)); }
 };
 template <bool BF, int NP> __device__ __forceinline__ void split_terms(float p0, float p1, const SplitConst &k, uint32_t (&w)[NP]) {
-  if constexpr (!BF && NP == 1) {
-    const f16x2 l = {(_Float16)p0, (_Float16)p1};
-    w[0] = __builtin_bit_cast(uint32_t, l);
-  } else if constexpr (!BF) {
+  if constexpr (!BF) {
     const u32x2 v = split_pair(p0, p1, k.minus1);
     w[0] = v[0], w[1] = v[1];
   } else {
@@ -265,19 +256,11 @@ template <bool BF, int NP> __device__ __forceinline__ void split_terms(float p0,
   }
 }
 
-// A packed pair's sum to `sum`.
-template <bool BF> __device__ __forceinline__ float add_pair(uint32_t w, float sum) {
-  if constexpr (BF) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), bf16x2{(__bf16)1.f, (__bf16)1.f}, sum, false);
-  else return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), f16x2{(_Float16)1.f, (_Float16)1.f}, sum, false);
-}
-
-// The sink into a row's denominator, and into that of the weights used; returns the factor of what was summed before. The log of a
-// denominator: of nothing −inf.
-__device__ __forceinline__ float sink_share(const HistAttnArgs &a, int head, float &m, float &den, float &used) {
+// The sink into a row's denominator; returns the factor of what was summed before. The log of a denominator: of nothing −inf.
+__device__ __forceinline__ float sink_share(const HistAttnArgs &a, int head, float &m, float &den) {
   if (!a.sinks) return 1.f;
-  const float y = bf16_bits_to_f32(a.sinks[head]) * kLog2e, mn = fmaxf(m, y), f = exp2_(m - mn), e = exp2_(y - mn);
-  den = fmaf(den, f, e);
-  used = fmaf(used, f, e);
+  const float y = bf16_bits_to_f32(a.sinks[head]) * kLog2e, mn = fmaxf(m, y), f = exp2_(m - mn);
+  den = fmaf(den, f, exp2_(y - mn));
   m = mn;
   return f;
 }
@@ -294,11 +277,10 @@ template <int QT> __device__ __forceinline__ void store_out(const HistAttnArgs &
     *(bf16x4 *)((__bf16 *)a.out + at) = bf16x4{(__bf16)o[0], (__bf16)o[1], (__bf16)o[2], (__bf16)o[3]};
   }
 }
-// A row's four outputs from its joined state: its maximum, its denominator, that of the weights used, and the sums.
+// A row's four outputs from its joined state.
 template <int QT, int D>
-__device__ __forceinline__ void finish_history_row(const HistAttnArgs &a, int64_t row, int head, int q4, float m, float den, float used, f32x4 o) {
-  float f = sink_share(a, head, m, den, used);
-  f *= used == 0.f ? 0.f : 1.f / used;       // of nothing: 0
+__device__ __forceinline__ void finish_history_row(const HistAttnArgs &a, int64_t row, int head, int q4, float m, float den, f32x4 o) {
+  const float f = sink_share(a, head, m, den) * (den == 0.f ? 0.f : 1.f / den);   // of nothing: 0
   store_out<QT>(a, row * D + 4 * q4, o * f);
   if (q4 == 0 && a.lse) a.lse[row] = lse_of(m, den);
 }
@@ -313,10 +295,9 @@ __device__ __forceinline__ void leave_row(const HistAttnArgs &a, const Block &b,
     if (q4 == 0) {
       a.pm[slot] = m;
       a.pl[slot] = den;
-      if constexpr (two_sums(QT)) a.pu[slot] = den;
     }
   } else {
-    finish_history_row<QT, D>(a, row, x.head, q4, m, den, den, o);
+    finish_history_row<QT, D>(a, row, x.head, q4, m, den, o);
   }
 }
 
@@ -769,8 +750,7 @@ template <int QT, int FMT, int D> __device__ __forceinline__ void history_many(c
         *(u32x4 *)(s_mem + slot * STAGE + (NPC > 1 && u >= HALF ? KT * D * 2 : 0) + (to[u % HALF] ^ (i << 4))) = o[i];
     }
   };
-  constexpr int NP = T::NPM;
-  float R = kNone, L = 0.f, LU = 0.f;        // LU: of the rounded probabilities
+  float R = kNone, L = 0.f;
   const SplitConst kSplit;
   bool far = false;
   f32x16 acc[NB];
@@ -807,29 +787,26 @@ template <int QT, int FMT, int D> __device__ __forceinline__ void history_many(c
         hide<4, 8>(y, hidden, none, std::make_integer_sequence<int, 16>{});
       }
       const float corr = to_probabilities<16>(y, scale, R, L, far, [](float v) { return max_halves(v); });
-      if (__any(corr != 1.f)) {
-        LU *= corr;
+      if (__any(corr != 1.f))
 #pragma unroll
         for (int n = 0; n < NB; ++n) acc[n] *= corr;
-      }
       // V^T: lane (l32, hh) takes dimension 32 n + l32 of keys 16 kc + 8 x + 4 hh .. + 3, the order of P^T.
 #pragma unroll
       for (int kc = 0; kc < 2; ++kc) {
-        u32x4 p[NP];
+        u32x4 p[T::NP];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          uint32_t x[NP];
-          split_terms<T::BF, NP>(y[8 * kc + 2 * e], y[8 * kc + 2 * e + 1], kSplit, x);
+          uint32_t x[T::NP];
+          split_terms<T::BF, T::NP>(y[8 * kc + 2 * e], y[8 * kc + 2 * e + 1], kSplit, x);
 #pragma unroll
-          for (int n = 0; n < NP; ++n) p[n][e] = x[n];
-          if constexpr (NP == 1) LU = add_pair<T::BF>(x[0], LU);
+          for (int n = 0; n < T::NP; ++n) p[n][e] = x[n];
         }
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
           const u32x2 v0 = read_columns(values + vat[n] + 16 * kc * 2 * D), v1 = read_columns(values + vat[n] + (16 * kc + 8) * 2 * D);
           const u32x4 vf = {v0[0], v0[1], v1[0], v1[1]};
 #pragma unroll
-          for (int k2 = 0; k2 < NP; ++k2) acc[n] = mfma32<T::BF>(vf, p[k2], acc[n]);
+          for (int k2 = 0; k2 < T::NP; ++k2) acc[n] = mfma32<T::BF>(vf, p[k2], acc[n]);
         }
       }
     }
@@ -861,22 +838,18 @@ template <int QT, int FMT, int D> __device__ __forceinline__ void history_many(c
 
   // What a lane's row leaves besides its sums: its state, or its denominator with the sink's share, lse, and the sums' factor.
   L += other_half(L);
-  LU = NP == 1 ? LU + other_half(LU) : L;
   int64_t to_row = -1;                       // where its sums go
   float by = 1.f;
   if (row.in) {
     const int64_t out = ((int64_t)row.s * a.N + row.i) * a.qh + row.head;
     if (a.chunks > 1) {
       to_row = out * a.chunks + (shared ? 0 : a.pre.chunks) + b.chunk;
-      if (hh == 0) {
-        a.pm[to_row] = R, a.pl[to_row] = L;
-        if constexpr (two_sums(QT)) a.pu[to_row] = LU;
-      }
+      if (hh == 0) a.pm[to_row] = R, a.pl[to_row] = L;
     } else {
       to_row = out;
-      float m = R, den = L, used = LU;
-      by = sink_share(a, row.head, m, den, used);
-      by *= used == 0.f ? 0.f : 1.f / used;
+      float m = R, den = L;
+      by = sink_share(a, row.head, m, den);
+      by *= den == 0.f ? 0.f : 1.f / den;
       if (hh == 0 && a.lse) a.lse[out] = lse_of(m, den);
     }
   }
@@ -961,14 +934,13 @@ template <int QT, int D> __global__ __launch_bounds__(256) void history_merge_ke
   float m = kNone;
   for (int c = lane; c < used; c += 64) m = fmaxf(m, a.pm[rc.slot(a, row, c)]);
   for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  float den = 0.f, weights = 0.f;
+  float den = 0.f;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int c = cg; c < used; c += GR) {
     const int64_t at = rc.slot(a, row, c);
     const float f = exp2_(a.pm[at] - m);
     den = fmaf(a.pl[at], f, den);
-    if constexpr (two_sums(QT)) weights = fmaf(a.pu[at], f, weights);
     const f32x4 w = *(const f32x4 *)(a.po + at * D + 4 * q4);
 #pragma unroll
     for (int k = 0; k < 4; ++k) sum[k] = fmaf(w[k], f, sum[k]);
@@ -976,11 +948,10 @@ template <int QT, int D> __global__ __launch_bounds__(256) void history_merge_ke
 #pragma unroll
   for (int o = LR; o < 64; o <<= 1) {
     den += __shfl_xor(den, o);
-    if constexpr (two_sums(QT)) weights += __shfl_xor(weights, o);
 #pragma unroll
     for (int k = 0; k < 4; ++k) sum[k] += __shfl_xor(sum[k], o);
   }
-  if (cg == 0 && used) finish_history_row<QT, D>(a, row, rc.head, q4, m, den, two_sums(QT) ? weights : den, sum);
+  if (cg == 0 && used) finish_history_row<QT, D>(a, row, rc.head, q4, m, den, sum);
 }
 
 // The same for few rows, of many chunks: a workgroup for 64 of a row's columns. Every chunk's factor into LDS first; then sixteen lanes a chunk and sixteen
@@ -988,7 +959,7 @@ template <int QT, int D> __global__ __launch_bounds__(256) void history_merge_ke
 // of 34 chunks 14, a wave a row 8.)
 constexpr int kMergeChunks = 2 * kHistChunks, kWideRows = 256;
 template <int QT, int D> __global__ __launch_bounds__(256) void history_merge_wide_kernel(HistAttnArgs a) {
-  __shared__ float s_f[kMergeChunks], s_red[12];
+  __shared__ float s_f[kMergeChunks], s_red[8];
   __shared__ __align__(16) f32x4 s_o[16][16];
   warm_kernargs<sizeof(HistAttnArgs)>();
   constexpr int PARTS = D / 64;
@@ -998,36 +969,27 @@ template <int QT, int D> __global__ __launch_bounds__(256) void history_merge_wi
   const RowChunks rc = row_chunks(a, row);
   const int used = rc.pre + rc.own;          // at most kMergeChunks
   if (!used) return;
-  float m2[2] = {kNone, kNone}, l2[2] = {0.f, 0.f}, u2[2] = {0.f, 0.f};
+  float m2[2] = {kNone, kNone}, l2[2] = {0.f, 0.f};
 #pragma unroll
   for (int k = 0; k < 2; ++k)
-    if (tid + 256 * k < used) {
-      const int64_t at = rc.slot(a, row, tid + 256 * k);
-      m2[k] = a.pm[at], l2[k] = a.pl[at];
-      if constexpr (two_sums(QT)) u2[k] = a.pu[at];
-    }
+    if (tid + 256 * k < used) m2[k] = a.pm[rc.slot(a, row, tid + 256 * k)], l2[k] = a.pl[rc.slot(a, row, tid + 256 * k)];
   float m = fmaxf(m2[0], m2[1]);
   for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
   if (lane == 0) s_red[wave] = m;
   __syncthreads();
   m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-  float den = 0.f, weights = 0.f;
+  float den = 0.f;
 #pragma unroll
   for (int k = 0; k < 2; ++k)
     if (tid + 256 * k < used) {
       const float f = exp2_(m2[k] - m);
       s_f[tid + 256 * k] = f;
       den = fmaf(l2[k], f, den);
-      weights = fmaf(u2[k], f, weights);
     }
-  for (int o = 32; o; o >>= 1) {
-    den += __shfl_xor(den, o);
-    if constexpr (two_sums(QT)) weights += __shfl_xor(weights, o);
-  }
-  if (lane == 0) s_red[4 + wave] = den, s_red[8 + wave] = weights;
+  for (int o = 32; o; o >>= 1) den += __shfl_xor(den, o);
+  if (lane == 0) s_red[4 + wave] = den;
   __syncthreads();
   den = (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]);
-  weights = two_sums(QT) ? (s_red[8] + s_red[9]) + (s_red[10] + s_red[11]) : den;
   const int q4 = tid & 15, cg = tid >> 4;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
@@ -1046,7 +1008,7 @@ template <int QT, int D> __global__ __launch_bounds__(256) void history_merge_wi
 #pragma unroll
     for (int k = 0; k < 4; ++k) sum[k] += w[k];
   }
-  finish_history_row<QT, D>(a, row, rc.head, 16 * part + tid, m, den, weights, sum);
+  finish_history_row<QT, D>(a, row, rc.head, 16 * part + tid, m, den, sum);
 }
 
 // Waves a SIMD of the kernels of few rows, by the registers that a tile's bytes, the queries' terms and the sums take.

@@ -299,7 +299,6 @@ int hh_history_attention(hh_ctx *ctx, const hh_history_desc *d, const hh_history
   a.po = (float *)ctx->hist;
   a.pm = a.po + slots * a.d;
   a.pl = a.pm + slots;
-  a.pu = a.pl + slots;
   int launches = 0;
   HH_HIP(hh::launch_history_attention(a, d->type, ctx->stream, &launches));
   ctx->dispatches += launches;
