@@ -141,7 +141,7 @@ class History:
     @classmethod
     def empty(cls, sequences: int, kv_heads: int, rows: int, head_dim: int, format: str = "mxfp8", ring: bool = False,
               pinned: int = 0, lengths=None, device="cuda:0"):
-        """A history of its own tensors; its lengths are 0, or `lengths`, which layers may share."""
+        """A history of its own tensors, zeros, which are complete when this returns; its lengths are 0, or `lengths`, which layers may share."""
         if format not in FORMATS:
             raise ValueError(f"format must be one of {sorted(FORMATS)}, not {format!r}")
         if lengths is None:
@@ -149,10 +149,14 @@ class History:
         shape = (sequences, kv_heads, rows)
         if format in ("f16", "bf16"):
             new = lambda: torch.zeros(shape + (head_dim,), dtype=torch.float16 if format == "f16" else torch.bfloat16, device=device)
-            return cls(new(), new(), lengths, ring=ring, pinned=pinned)
-        code = lambda: torch.zeros(shape + (head_dim if format == "mxfp8" else head_dim // 2,), dtype=torch.uint8, device=device)
-        scale = lambda: torch.zeros(shape + (head_dim // 32,), dtype=torch.uint8, device=device)
-        return cls(code(), code(), lengths, scale(), scale(), ring=ring, pinned=pinned)
+            h = cls(new(), new(), lengths, ring=ring, pinned=pinned)
+        else:
+            code = lambda: torch.zeros(shape + (head_dim if format == "mxfp8" else head_dim // 2,), dtype=torch.uint8, device=device)
+            scale = lambda: torch.zeros(shape + (head_dim // 32,), dtype=torch.uint8, device=device)
+            h = cls(code(), code(), lengths, scale(), scale(), ring=ring, pinned=pinned)
+        if h.device.type == "cuda":   # a context's stream does not wait for torch's, which fills them
+            torch.cuda.current_stream(h.device).synchronize()
+        return h
 
 
 def history_write(ctx: Context, history: History, k, v, counts):
