@@ -344,10 +344,12 @@ __device__ void put_odd(const Block &b, int first, int low, int high, int j0, in
 // Logits S of a run of keys, N of them a lane, its row's shared with the lanes that `top_of` exchanges with, to probabilities
 // 2^(y − R), y = S·scale, and their sum to L. R follows the row's maximum y, less kOff, by steps of at least kLag. Whether it has to
 // step is seen from the sum of what comes out with the R that there is, so that no maximum is formed but where it does. The product and
-// the difference are one fma; where some R is so far from zero that the product's lost bits would matter, y is rounded first, as R
-// was. Returns what the sums so far are to be multiplied with after a step of R (1: none); L is.
+// the difference are one fma; where R is so far from zero that the product's lost bits would matter (`far`), y is rounded first, as R
+// was, and R follows every new maximum. The wave goes into the branch as one, but each row steps and rounds by its own logits alone, so that
+// its bits do not depend on the rows beside it. Returns what the sums so far are to be multiplied with after a step of R (1: none); L is.
 constexpr float kFar = 65536.f;
 template <int N, typename F> __device__ __forceinline__ float to_probabilities(float (&S)[N], float scale, float &R, float &L, bool &far, F top_of) {
+  constexpr float kMost = 23170.475f;        // 2^(kOff + kLag)
   float y[N], corr = 1.f;
   auto sum_of = [&]() {
     float sum[2] = {0.f, 0.f};
@@ -361,7 +363,7 @@ template <int N, typename F> __device__ __forceinline__ float to_probabilities(f
 #pragma unroll
   for (int i = 0; i < N; ++i) y[i] = fmaf(S[i], scale, -R);
   float sum = sum_of();
-  if (far || __any(sum > 23170.475f)) {      // 2^(kOff + kLag)
+  if (__any(far || sum > kMost)) {
     // Nearly never: with a scale of its own, so that its products are not made ahead of the branch.
     float own = scale;
     asm volatile("" : "+v"(own));
@@ -369,11 +371,12 @@ template <int N, typename F> __device__ __forceinline__ float to_probabilities(f
 #pragma unroll
     for (int i = 1; i < N; ++i) top = fmaxf(top, S[i] * own);
     top = top_of(top);
-    const float to = fmaxf(R, top - kOff);
-    corr = exp2_(R - to);
+    const bool moves = far || top_of(sum > kMost ? 1.f : 0.f) > 0.f;
+    const float to = moves ? fmaxf(R, top - kOff) : R;
+    corr = moves ? exp2_(R - to) : 1.f;
     R = to;
     L *= corr;
-    far = __any(fabsf(R) > kFar && R > kNone);
+    far = fabsf(R) > kFar && R > kNone;
 #pragma unroll
     for (int i = 0; i < N; ++i) y[i] = far ? S[i] * own - R : fmaf(S[i], own, -R);
     sum = sum_of();
