@@ -180,7 +180,7 @@ __device__ __forceinline__ Row row_of(const HistAttnArgs &a, const Block &b, int
   Row x;
   const int t = r / a.qm;
   x.in = t < b.count;
-  const int tt = x.in ? t : b.r0 / a.qm;                     // rows past the last stand for the block's first
+  const int tt = x.in ? t : b.r0 / a.qm;                     // rows past the last see what the block's first sees
   x.head = b.g * a.qm + (x.in ? r - t * a.qm : 0);
   if (b.shared) {
     x.s = tt / a.N;
@@ -430,7 +430,12 @@ __device__ __forceinline__ void history_few(const HistAttnArgs &a, bool shared, 
     if (wave == 0 && quad == 0) s_lo[16 * r + l16] = row.low, s_hi[16 * r + l16] = row.high;
     const int64_t at = ((int64_t)row.s * a.N + row.i) * a.q_stride + (int64_t)row.head * D + EP * quad;
 #pragma unroll
-    for (int f = 0; f < NF; ++f) query_terms<QT, T::BF, T::NQ>(a.q, at + 4 * EP * (f / X) + 8 * (f % X), q[r][f]);
+    for (int f = 0; f < NF; ++f)
+#pragma unroll
+      for (int n = 0; n < T::NQ; ++n) q[r][f][n] = u32x4{};
+    if (row.in)                              // queries of tokens that are not there are not read
+#pragma unroll
+      for (int f = 0; f < NF; ++f) query_terms<QT, T::BF, T::NQ>(a.q, at + 4 * EP * (f / X) + 8 * (f % X), q[r][f]);
   }
   const float scale = a.scale * kLog2e;
   const uint32_t none = scale < 0.f ? 0x7F800000u : 0xFF800000u;   // the logit of a key that is not seen: y is −inf
@@ -675,7 +680,12 @@ template <int QT, int FMT, int D> __device__ __forceinline__ void history_many(c
   {
     const int64_t from = ((int64_t)row.s * a.N + row.i) * a.q_stride + (int64_t)row.head * D + 8 * hh;
 #pragma unroll
-    for (int f = 0; f < D / 16; ++f) query_terms<QT, T::BF, T::NQ>(a.q, from + 16 * f, q[f]);
+    for (int f = 0; f < D / 16; ++f)
+#pragma unroll
+      for (int n = 0; n < T::NQ; ++n) q[f][n] = u32x4{};
+    if (row.in)                              // queries of tokens that are not there are not read
+#pragma unroll
+      for (int f = 0; f < D / 16; ++f) query_terms<QT, T::BF, T::NQ>(a.q, from + 16 * f, q[f]);
   }
   const float scale = a.scale * kLog2e;
   const uint32_t none = scale < 0.f ? 0x7F800000u : 0xFF800000u;   // the logit of a key that is not seen: y is −inf

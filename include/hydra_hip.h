@@ -638,7 +638,7 @@ typedef struct hh_history_desc {
  *   lse     fp32 [S][N][q_heads] or NULL: the log of the denominator
  *   prefix  NULL, or a history of one sequence (same heads, head_dim and format; no ring; window 0): its lengths[0] rows come before
  *           every sequence's own and are seen by each token. They are read once for the batch.
- * Tokens from counts[s] on are not written. A token that sees nothing (its own position not held) gets 0 and lse −inf, or with a sink the
+ * Tokens from counts[s] on are neither read nor written. A token that sees nothing (its own position not held) gets 0 and lse −inf, or with a sink the
  * sink. Keys that a token does not see, infinities and NaN among them, have no part in its output. Logits, and the products before
  * sm_scale, may be of any size that fp32 holds, times log2(e). F32 queries over an F16 history are held to 2^-22, or 2^-25 where that
  * is more, and up to 65504.                                                                       */

@@ -48,3 +48,23 @@ def test_other_queries_do_not_change_a_row(kind, fmt, N, D, shared, size):
     touched[:, :, 1::2] = True
     t["q"][:, :, 1::2] *= size
     others(torch, want, call(torch, ctx, t, scale=8.0), touched)
+
+
+@pytest.mark.parametrize("kind,fmt", TYPES)
+@pytest.mark.parametrize("S,N,D,shared", [(3, 2, 64, 300), (9, 3, 128, 1300), (20, 5, 256, 40), (3, 40, 64, None), (3, 2, 64, None)])
+def test_tokens_that_are_not_there_are_not_read(kind, fmt, S, N, D, shared):
+    """Whatever stands behind counts[s], tokens of a sequence that has none among them."""
+    import torch
+    from hydra_amd.layer import Context
+    print(f"[gpu] padding {kind} {fmt} S={S} N={N} D={D} shared={shared}", flush=True)
+    ctx = Context(0)
+    counts = [N, 0, 1] + [(i % (N + 1)) for i in range(S - 3)]
+    t = make(torch, S, N, 8, 2, D, kind, fmt, 90, [50 - i for i in range(S)], counts=counts, shared=shared, seed=6)
+    there = torch.arange(N)[None] < torch.tensor(counts)[:, None]
+    t["q"][~there] = 0.0
+    want, wl = call(torch, ctx, t)
+    assert (want[~there] == 7.0).all() and (wl[~there] == 7.0).all()
+    for x in (float("nan"), float("inf"), 60000.0):
+        t["q"][~there] = x
+        out, lse = call(torch, ctx, t)
+        assert torch.equal(out, want) and torch.equal(lse, wl)
