@@ -342,14 +342,17 @@ __device__ void put_odd(const Block &b, int first, int low, int high, int j0, in
 }
 
 // Logits S of a run of keys, N of them a lane, its row's shared with the lanes that `top_of` exchanges with, to probabilities
-// 2^(y − R), y = S·scale, and their sum to L. R follows the row's maximum y, less kOff, by steps of at least kLag. Whether it has to
+// 2^(y − R), y = S·scale, and their sum to L. R follows the row's maximum y, less `off`, by steps of at least kLag. Whether it has to
 // step is seen from the sum of what comes out with the R that there is, so that no maximum is formed but where it does. The product and
 // the difference are one fma; where R is so far from zero that the product's lost bits would matter (`far`), y is rounded first, as R
 // was, and R follows every new maximum. The wave goes into the branch as one, but each row steps and rounds by its own logits alone, so that
 // its bits do not depend on the rows beside it. Returns what the sums so far are to be multiplied with after a step of R (1: none); L is.
+//
+// The largest probability of fp16 operands is 2^7 to 2^14.5 (kOff, for fp16's smallest steps); bf16 reaches as far down as fp32, and there none is above 1, so that
+// the sums of values stay within fp32 wherever the values times the keys do.
 constexpr float kFar = 65536.f;
-template <int N, typename F> __device__ __forceinline__ float to_probabilities(float (&S)[N], float scale, float &R, float &L, bool &far, F top_of) {
-  constexpr float kMost = 23170.475f;        // 2^(kOff + kLag)
+template <bool BF, int N, typename F> __device__ __forceinline__ float to_probabilities(float (&S)[N], float scale, float &R, float &L, bool &far, F top_of) {
+  constexpr float off = BF ? -kLag : kOff, kMost = BF ? 1.f : 23170.475f;    // 2^(off + kLag)
   float y[N], corr = 1.f;
   auto sum_of = [&]() {
     float sum[2] = {0.f, 0.f};
@@ -372,7 +375,7 @@ template <int N, typename F> __device__ __forceinline__ float to_probabilities(f
     for (int i = 1; i < N; ++i) top = fmaxf(top, S[i] * own);
     top = top_of(top);
     const bool moves = far || top_of(sum > kMost ? 1.f : 0.f) > 0.f;
-    const float to = moves ? fmaxf(R, top - kOff) : R;
+    const float to = moves ? fmaxf(R, top - off) : R;
     corr = moves ? exp2_(R - to) : 1.f;
     R = to;
     L *= corr;
@@ -561,7 +564,7 @@ __device__ __forceinline__ void history_few(const HistAttnArgs &a, bool shared, 
         const uint32_t hidden = ~((~first_keys(low[r] - j) | first_keys(a.first - j)) & first_keys(high[r] + 1 - j)) >> (4 * quad);
         hide<4, 16>(y, hidden, none, std::make_integer_sequence<int, 8>{});
       }
-      const float corr = to_probabilities<8>(y, scale, R[r], L[r], far[r], [](float v) { return max_lane_groups(v); });
+      const float corr = to_probabilities<T::BF, 8>(y, scale, R[r], L[r], far[r], [](float v) { return max_lane_groups(v); });
       if (__any(corr != 1.f))
 #pragma unroll
         for (int n = 0; n < NB; ++n) acc[r][n] *= corr;
@@ -799,7 +802,7 @@ template <int QT, int FMT, int D> __device__ __forceinline__ void history_many(c
         const uint32_t hidden = ~((~first_keys(row.low - j) | first_keys(a.first - j)) & first_keys(row.high + 1 - j)) >> (4 * hh);
         hide<4, 8>(y, hidden, none, std::make_integer_sequence<int, 16>{});
       }
-      const float corr = to_probabilities<16>(y, scale, R, L, far, [](float v) { return max_halves(v); });
+      const float corr = to_probabilities<T::BF, 16>(y, scale, R, L, far, [](float v) { return max_halves(v); });
       if (__any(corr != 1.f))
 #pragma unroll
         for (int n = 0; n < NB; ++n) acc[n] *= corr;

@@ -640,7 +640,8 @@ typedef struct hh_history_desc {
  *           every sequence's own and are seen by each token. They are read once for the batch.
  * Tokens from counts[s] on are neither read nor written. A token that sees nothing (its own position not held) gets 0 and lse −inf, or with a sink the
  * sink. Keys that a token does not see, infinities and NaN among them, have no part in its output. Logits, and the products before
- * sm_scale, may be of any size that fp32 holds, times log2(e). F32 queries over an F16 history are held to 2^-22, or 2^-25 where that
+ * sm_scale, may be of any size that fp32 holds, times log2(e). So may values over F16 histories; over the others the values that a
+ * token sees, times their number, have to be within it. F32 queries over an F16 history are held to 2^-22, or 2^-25 where that
  * is more, and up to 65504.                                                                       */
 int hh_history_attention(hh_ctx *ctx, const hh_history_desc *desc, const hh_history *h, const hh_history *prefix,
                          const void *q, const int32_t *counts, const uint16_t *sinks, void *out, float *lse);
