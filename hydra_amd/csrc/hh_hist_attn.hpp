@@ -57,13 +57,24 @@ template <int FMT, int N> __device__ __forceinline__ void widen(const uint32_t (
   }
 }
 
-template <int FMT> __device__ __forceinline__ float number_at(const uint8_t *row, const uint8_t *scales, int c) {
-  if constexpr (FMT == H_F16) return (float)((const _Float16 *)row)[c];
-  else if constexpr (FMT == H_BF16) return bf16_bits_to_f32(((const uint16_t *)row)[c]);
-  else if constexpr (FMT == H_MXFP8) return __builtin_amdgcn_cvt_f32_fp8((int)row[c], 0) * hist_scale(scales[c >> 5]);
-  else {
-    const bf16x2 v = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(row[c >> 1] >> 4 * (c & 1) & 15u, 1.f, 0);
-    return (float)v[0] * hist_scale(scales[c >> 5]);
+// Columns 4 q4 .. 4 q4 + 3 of a row.
+template <int FMT> __device__ __forceinline__ f32x4 numbers_at(gptr_t row, gptr_t scales, int q4) {
+  if constexpr (FMT == H_F16) {
+    const f16x2 l = __builtin_bit_cast(f16x2, load_global<uint32_t>(row + 8 * q4)), h = __builtin_bit_cast(f16x2, load_global<uint32_t>(row + 8 * q4 + 4));
+    return f32x4{(float)l[0], (float)l[1], (float)h[0], (float)h[1]};
+  } else if constexpr (FMT == H_BF16) {
+    const u32x2 w = load_global<u32x2>(row + 8 * q4);
+    return f32x4{__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xFFFF0000u), __uint_as_float(w[1] << 16), __uint_as_float(w[1] & 0xFFFF0000u)};
+  } else if constexpr (FMT == H_MXFP8) {
+    const int w = (int)load_global<uint32_t>(row + 4 * q4);
+    const float by = hist_scale(load_global<uint8_t>(scales + (q4 >> 3)));
+    return f32x4{__builtin_amdgcn_cvt_f32_fp8(w, 0) * by, __builtin_amdgcn_cvt_f32_fp8(w, 1) * by, __builtin_amdgcn_cvt_f32_fp8(w, 2) * by,
+                 __builtin_amdgcn_cvt_f32_fp8(w, 3) * by};
+  } else {
+    const uint32_t w = load_global<uint16_t>(row + 2 * q4);
+    const float by = hist_scale(load_global<uint8_t>(scales + (q4 >> 3)));
+    const bf16x2 l = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.f, 0), h = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.f, 1);
+    return f32x4{(float)l[0] * by, (float)l[1] * by, (float)h[0] * by, (float)h[1] * by};
   }
 }
 
@@ -326,19 +337,46 @@ template <int G, int PER, int N, int... I>
 __device__ __forceinline__ void hide(float (&y)[N], uint32_t hidden, uint32_t none, std::integer_sequence<int, I...>) {
   ((y[I] = seen_or<PER * (I / G) + I % G>(y[I], hidden, none)), ...);
 }
-// What take_odd took out of keys j0 .. j1 − 1, for one row's four columns.
+// The infinities and NaN among the values of keys j0 .. j1 − 1 (j0 < j1) that a row sees, in four columns, added to `odd`.
 template <int FMT, int D>
-__device__ void put_odd(const Block &b, int first, int low, int high, int j0, int j1, int q4, f32x4 &o) {
+__device__ __forceinline__ void add_odd(const Block &b, int first, int low, int high, int j0, int j1, int q4, f32x4 &odd) {
 #pragma unroll 1
-  for (int j = j0; j < j1; ++j) {
-    if (j > high || (j >= first && j < low)) continue;
-    const int64_t r = key_row(b, j);
+  for (int j = j0; j < j1; j += 4) {
+    f32x4 v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float v = number_at<FMT>((const uint8_t *)b.v_ + r * hist_row_bytes(FMT, D), (const uint8_t *)b.vs + r * (D / 32), 4 * q4 + i);
-      if (!(fabsf(v) < INFINITY)) o[i] += v;
+    for (int u = 0; u < 4; ++u) {
+      const int64_t r = key_row(b, j + u);
+      v[u] = numbers_at<FMT>(b.v_ + r * hist_row_bytes(FMT, D), b.vs + r * (D / 32), q4);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int k = j + u;
+      const bool seen = k < j1 && k <= high && (k < first || k >= low);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (seen && !(fabsf(v[u][i]) < INFINITY)) odd[i] += v[u][i];
     }
   }
+}
+// A row's four sums with the infinities and NaN of the values that it sees: those that take_odd took out (`taken`) of the tiles that some
+// row does not see whole, and, where a sum is NaN though the row's logits are numbers, those of all tiles, since a zero among an
+// infinity's probability terms has made it NaN there. KT keys a tile.
+template <int FMT, int D, int KT, typename P>
+__device__ __forceinline__ void put_odd(const Block &b, int first, int low, int high, int tiles, bool taken, P is_part, float den, int q4, f32x4 &o) {
+  const bool lost = den == den && !(o[0] == o[0] && o[1] == o[1] && o[2] == o[2] && o[3] == o[3]);
+  if (!taken && !lost) return;
+  f32x4 odd = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int t = 0; t < tiles; ++t) {
+    if (!lost && !is_part(t)) continue;
+    add_odd<FMT, D>(b, first, low, high, b.c0 + KT * t, min(b.c0 + KT * t + KT, b.c0 + b.nc), q4, odd);
+    bool all = !taken;                       // every sum is a number or NaN for good
+#pragma unroll
+    for (int i = 0; i < 4; ++i) all = all && (o[i] == o[i] || odd[i] != odd[i]);
+    if (all) break;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = o[i] == o[i] ? o[i] + odd[i] : odd[i] != 0.f ? odd[i] : o[i];
 }
 
 // Logits S of a run of keys, N of them a lane, its row's shared with the lanes that `top_of` exchanges with, to probabilities
@@ -620,9 +658,7 @@ __device__ __forceinline__ void history_few(const HistAttnArgs &a, bool shared, 
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[i] = fmaf(w[i], f, o[i]);
     }
-    if (s_odd)
-      for (int t = 0; t < tiles; ++t)
-        if (is_part(t)) put_odd<FMT, D>(b, a.first, s_lo[r], s_hi[r], b.c0 + 32 * t, min(b.c0 + 32 * t + 32, b.c0 + b.nc), q4, o);
+    put_odd<FMT, D, 32>(b, a.first, s_lo[r], s_hi[r], tiles, s_odd, is_part, den, q4, o);
     leave_row<QT, D>(a, b, x, q4, m, den, o);
   }
 }
@@ -884,11 +920,8 @@ template <int QT, int FMT, int D> __device__ __forceinline__ void history_many(c
     f32x4 o = *(const f32x4 *)(so + r * D + 4 * (q4 ^ (r & 7)));
     const int64_t at = (int64_t)(((uint64_t)(uint32_t)__shfl((int)(to_row >> 32), r) << 32) | (uint32_t)__shfl((int)to_row, r));
     const float f = __shfl(by, r);
-    if (s_odd) {
-      const int rlow = __shfl(row.low, r), rhigh = __shfl(row.high, r);
-      for (int t = 0; t < tiles; ++t)
-        if (is_part(t)) put_odd<FMT, D>(b, a.first, rlow, rhigh, b.c0 + t * KT, min(b.c0 + t * KT + KT, b.c0 + b.nc), q4, o);
-    }
+    const int rlow = __shfl(row.low, r), rhigh = __shfl(row.high, r);
+    put_odd<FMT, D, KT>(b, a.first, rlow, rhigh, tiles, s_odd, is_part, __shfl(L, r), q4, o);
     if (at < 0) continue;
     if (a.chunks > 1) *(f32x4 *)(a.po + at * D + 4 * q4) = o;
     else store_out<QT>(a, at * D + 4 * q4, o * f);

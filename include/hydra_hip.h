@@ -639,7 +639,8 @@ typedef struct hh_history_desc {
  *   prefix  NULL, or a history of one sequence (same heads, head_dim and format; no ring; window 0): its lengths[0] rows come before
  *           every sequence's own and are seen by each token. They are read once for the batch.
  * Tokens from counts[s] on are neither read nor written. A token that sees nothing (its own position not held) gets 0 and lse −inf, or with a sink the
- * sink. Keys that a token does not see, infinities and NaN among them, have no part in its output. Logits, and the products before
+ * sink. Keys that a token does not see, infinities and NaN among them, have no part in its output. An infinity
+ * among the values that it sees is its output's in that column, wherever it stands, as long as fp32 holds its weight. Logits, and the products before
  * sm_scale, may be of any size that fp32 holds, times log2(e). So may values over F16 histories; over the others the values that a
  * token sees, times their number, have to be within it. F32 queries over an F16 history are held to 2^-22, or 2^-25 where that
  * is more, and up to 65504.                                                                       */
