@@ -13,6 +13,29 @@ constexpr int kMaxSequences = 4096, kMaxTokens = 65536, kMaxRows = 1 << 28, kMax
 bool aligned(const void *p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 bool elem(int32_t type) { return type >= HH_F32 && type <= HH_BF16; }
 
+// n rows of `bytes`, `step` (at least that) apart.
+struct Rows {
+  const void *at;
+  int64_t step, bytes, n;
+};
+// Whether some byte is in rows of both.
+bool meet(const Rows &a, const Rows &b) {
+  const int64_t d = (int64_t)((intptr_t)b.at - (intptr_t)a.at);
+  if (d >= (a.n - 1) * a.step + a.bytes || -d >= (b.n - 1) * b.step + b.bytes) return false;
+  // Row j of b meets row i of a where d + j·b.step − i·a.step is above −b.bytes and below a.bytes: the first j above, for each i.
+  auto above = [](int64_t x, int64_t step) { return x < 0 ? -((-x + step - 1) / step) + 1 : x / step + 1; };   // least k: k·step > x
+  if (a.step == b.step) {                  // k = j − i
+    const int64_t k = above(-b.bytes - d, a.step), least = 1 - a.n;
+    const int64_t from = k > least ? k : least;
+    return from < b.n && d + from * a.step < a.bytes;
+  }
+  for (int64_t i = 0; i < a.n; ++i) {
+    const int64_t e = d - i * a.step, k = above(-b.bytes - e, b.step), j = k > 0 ? k : 0;
+    if (j < b.n && e + j * b.step < a.bytes) return true;
+  }
+  return false;
+}
+
 // The workspace grows in eager calls; recorded graphs hold its address.
 int ensure_history(hh_ctx *ctx, size_t bytes) {
   if (ctx->hist_bytes >= bytes) return HH_OK;
@@ -211,6 +234,15 @@ int hh_rotary(hh_ctx *ctx, const hh_rotary_desc *d, const double *turns, float m
   if (count == 2 && a.r[0].y == a.r[1].y) return fail(HH_EINVAL, "both outputs are the same memory");
   if (count == 2 && (a.r[0].y == a.r[1].x || a.r[1].y == a.r[0].x)) return fail(HH_EINVAL, "an output is the other's input");
   if (tokens == 0) return HH_OK;
+  const int64_t size = type == HH_F32 ? 4 : 2;
+  auto rows_of = [&](const void *p, int64_t stride, int heads) { return Rows{p, size * stride, size * heads * d->head_dim, tokens}; };
+  for (int i = 0; i < count; ++i)
+    for (int j = 0; j < count; ++j) {
+      const Rows y = rows_of(a.r[i].y, a.r[i].y_stride, a.r[i].heads);
+      if ((i != j || a.r[i].x != a.r[i].y) && meet(y, rows_of(a.r[j].x, a.r[j].x_stride, a.r[j].heads)))
+        return fail(HH_EINVAL, "an output overlaps an input: y is its x, with the same stride, or apart from every x");
+      if (i < j && meet(y, rows_of(a.r[j].y, a.r[j].y_stride, a.r[j].heads))) return fail(HH_EINVAL, "the outputs overlap");
+    }
   a.turns = turns;
   a.positions = positions;
   a.magnitude = magnitude;

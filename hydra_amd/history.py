@@ -77,7 +77,7 @@ def _tokens(t, name, shape, dtype, device):
 
 def rotary_into(ctx: Context, rotary: Rotary, positions, q, q_out, k=None, k_out=None):
     """Turns q, and k, by their tokens' positions (hh_rotary). q, q_out [..][q_heads][d], k, k_out [..][kv_heads][d], of one type, with
-    equally spaced tokens; positions int32 [..]. An output is its input or apart from it. Returns the outputs."""
+    equally spaced tokens; positions int32 [..]. An output is its input or apart from every tensor of the call. Returns the outputs."""
     dev, dtype = q.device, q.dtype
     _cuda(ctx, dev)
     if dtype not in ELEM or q.dim() < 2 or q.shape[-1] != rotary.head_dim:

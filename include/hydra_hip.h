@@ -558,7 +558,7 @@ typedef struct hh_rotary_desc {
 } hh_rotary_desc;
 
 /* One tensor of a call: [tokens][heads][head_dim] with its heads packed and equally spaced tokens. `y` is x, with the
- * same stride, or does not overlap it. 16-byte aligned; strides in elements, 0 = packed, multiples of 16 bytes. */
+ * same stride, or overlaps no tensor of the call (other calls are refused). 16-byte aligned; strides in elements, 0 = packed, multiples of 16 bytes. */
 typedef struct hh_rotary_rows {
   const void *x;
   void   *y;
