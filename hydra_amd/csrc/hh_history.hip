@@ -271,6 +271,13 @@ int hh_history_write(hh_ctx *ctx, const hh_history *h, int32_t type, const void 
   if (kv_stride && kv_stride < row) return fail(HH_ESHAPE, "kv_stride is smaller than a token's rows");
   if (kv_stride > 1 << 30) return fail(HH_ESHAPE, "kv_stride above 2^30");
   if (kv_stride % (type == HH_F32 ? 4 : 8)) return fail(HH_EALIGN, "kv_stride must be a multiple of 16 bytes");
+  const int64_t held = (int64_t)h->sequences * h->kv_heads * h->rows, codes = held * hh::hist_row_bytes(h->format, h->head_dim);
+  const int64_t scales = h->format >= HH_HISTORY_MXFP8 ? held * (h->head_dim / 32) : 0;
+  const Rows own[5] = {{h->k, codes, codes, 1}, {h->v, codes, codes, 1}, {h->lengths, 4 * h->sequences, 4 * h->sequences, 1},
+                       {h->k_scales, scales, scales, 1}, {h->v_scales, scales, scales, 1}};
+  for (int i = 0; i < (scales ? 5 : 3); ++i)
+    for (int j = 0; j < i; ++j)
+      if (meet(own[i], own[j])) return fail(HH_EINVAL, "tensors of the history overlap");
   hh::HistRowsArgs a = rows_args(h, type, tokens, counts);
   a.k = k;
   a.v = v;
@@ -289,7 +296,8 @@ int hh_history_read(hh_ctx *ctx, const hh_history *h, int32_t type, const int32_
   if (!elem(type)) return fail(HH_EINVAL, "unknown type");
   if (!starts || !counts || !k || !v) return fail(HH_EINVAL, "NULL argument");
   if (!aligned(k, 16) || !aligned(v, 16)) return fail(HH_EALIGN, "k and v must be 16-byte aligned");
-  if (k == v) return fail(HH_EINVAL, "k and v are the same memory");
+  const int64_t out = (int64_t)h->sequences * tokens * h->kv_heads * h->head_dim * (type == HH_F32 ? 4 : 2);
+  if (meet({k, out, out, 1}, {v, out, out, 1})) return fail(HH_EINVAL, "k and v overlap");
   hh::HistRowsArgs a = rows_args(h, type, tokens, counts);
   a.ko = k;
   a.vo = v;
@@ -305,7 +313,8 @@ int hh_history_advance(hh_ctx *ctx, const hh_history *h, int32_t tokens, const i
   if (int rc = check_history(h)) return rc;
   if (int rc = check_step(h, tokens)) return rc;
   if (!counts) return fail(HH_EINVAL, "NULL argument");
-  if (counts == h->lengths) return fail(HH_EINVAL, "lengths and counts are the same memory");
+  const int64_t bytes = 4 * h->sequences;
+  if (meet({h->lengths, bytes, bytes, 1}, {counts, bytes, bytes, 1})) return fail(HH_EINVAL, "lengths and counts overlap");
   HH_HIP(hipSetDevice(ctx->device));
   HH_HIP(hh::launch_history_advance(const_cast<int32_t *>(h->lengths), counts, h->sequences, tokens, ctx->stream));
   ctx->dispatches += 1;
@@ -324,6 +333,11 @@ int hh_history_attention(hh_ctx *ctx, const hh_history_desc *d, const hh_history
   a.sinks = sinks;
   a.out = out;
   a.lse = lse;
+  const int64_t n = (int64_t)a.S * a.N, size = d->type == HH_F32 ? 4 : 2, row = (int64_t)a.qh * a.d;
+  const Rows to = {out, size * row, size * row, n}, from = {q, size * a.q_stride, size * row, n}, sums = {lse, 4 * a.qh, 4 * a.qh, n};
+  // In place a workgroup reads its rows' queries before it writes them, and reads no others'.
+  if ((out != q || (a.q_stride != row && n > 1)) && meet(to, from)) return fail(HH_EINVAL, "out overlaps q: it is q, packed, or apart from it");
+  if (lse && (meet(sums, to) || meet(sums, from))) return fail(HH_EINVAL, "lse overlaps q or out");
   HH_HIP(hipSetDevice(ctx->device));
   hh::history_plan(a, d->max_length ? d->max_length : h->rows, prefix ? prefix->rows : 0);
   if (int rc = ensure_history(ctx, hh::history_workspace(a))) return rc;

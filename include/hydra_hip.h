@@ -610,7 +610,7 @@ int hh_history_write(hh_ctx *ctx, const hh_history *h, int32_t type, const void 
                      int32_t tokens, const int32_t *counts);
 
 /* Rows back as numbers: positions starts[s] + i, i < counts[s], of sequence s to k and v (type, [S][tokens][kv_heads][head_dim],
- * packed). Which position a ring's row holds is the caller's to know; positions below 0 and, without ring, from `rows` on
+ * packed, apart from each other). Which position a ring's row holds is the caller's to know; positions below 0 and, without ring, from `rows` on
  * leave their places as they were, as do tokens from counts[s] on.                                */
 int hh_history_read(hh_ctx *ctx, const hh_history *h, int32_t type, const int32_t *starts, int32_t tokens,
                     const int32_t *counts, void *k, void *v);
@@ -633,7 +633,7 @@ typedef struct hh_history_desc {
 /* Attention of a step's tokens, one a sequence or a whole prompt, over the history that they have been written to
  * (hh_history_write before this): token i of sequence s sees positions up to its own, by window and first. A ring needs
  * a window of its own: window + tokens − 1 <= rows − pinned, first <= pinned.
- *   q, out  type [S][N][q_heads][head_dim] (q with q_stride), 16-byte aligned
+ *   q, out  type [S][N][q_heads][head_dim] (q with q_stride), 16-byte aligned; out may be q, packed, but overlaps it in no other way
  *   sinks   bf16 [q_heads] or NULL: a logit in the denominator only
  *   lse     fp32 [S][N][q_heads] or NULL: the log of the denominator
  *   prefix  NULL, or a history of one sequence (same heads, head_dim and format; no ring; window 0): its lengths[0] rows come before
