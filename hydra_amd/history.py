@@ -15,6 +15,7 @@ recorded with `Context.capture` follows them. The conventions of formats, positi
 from __future__ import annotations
 
 import ctypes as C
+import operator
 import struct
 
 import torch
@@ -29,6 +30,13 @@ SCALINGS = {"none": 0, "linear": 1, "yarn": 2}
 _I32, _F32 = torch.int32, torch.float32
 
 
+def _i32(**values):
+    """Raises unless the values are 32-bit whole numbers: ctypes would cut off what does not fit."""
+    for name, v in values.items():
+        if not hasattr(v, "__index__") or not -(1 << 31) <= operator.index(v) < 1 << 31:
+            raise ValueError(f"{name} must be a 32-bit whole number, not {v!r}")
+
+
 class Rotary:
     """A model's rotary frequencies (hh_rotary_desc, hh_rotary_table), kept on the device. `rotated` columns of each head turn (0: all),
     as pairs over the first `span` columns (0: rotated)."""
@@ -38,8 +46,9 @@ class Rotary:
                  beta_slow: float = 1.0, truncate: bool = True, device="cuda:0"):
         if scaling not in SCALINGS:
             raise ValueError(f"scaling must be one of {sorted(SCALINGS)}, not {scaling!r}")
-        self.c = RotaryDescC(head_dim, rotated or head_dim, span, int(interleaved), SCALINGS[scaling], original_length,
-                             int(truncate), factor, beta_fast, beta_slow, base)
+        _i32(head_dim=head_dim, rotated=rotated, span=span, original_length=original_length)
+        self.c = RotaryDescC(head_dim, rotated or head_dim, span, int(bool(interleaved)), SCALINGS[scaling], original_length,
+                             int(bool(truncate)), factor, beta_fast, beta_slow, base)
         table, magnitude = (C.c_double * max(1, self.c.rotated // 2))(), C.c_float()
         check(lib().hh_rotary_table(C.byref(self.c), table, C.byref(magnitude)))
         self.head_dim, self.magnitude = head_dim, magnitude.value
@@ -132,6 +141,7 @@ class History:
         else:
             raise ValueError(f"k must be fp16, bf16 or uint8 codes, not {k.dtype}")
         _same(lengths, "lengths", (S,), _I32, dev)
+        _i32(rows=rows, pinned=pinned)
         self.k, self.v, self.k_scales, self.v_scales, self.lengths = k, v, k_scales, v_scales, lengths
         self.sequences, self.kv_heads, self.rows, self.head_dim, self.format = S, G, rows, D, format_
         self.ring, self.pinned, self.device = bool(ring), pinned, dev
@@ -197,6 +207,7 @@ def history_advance(ctx: Context, history: History, counts, tokens: int):
     """history.lengths += counts (each 0..tokens), the end of a step (hh_history_advance)."""
     _cuda(ctx, history.device)
     _same(counts, "counts", (history.sequences,), _I32, history.device)
+    _i32(tokens=tokens)
     check(lib().hh_history_advance(ctx.handle, C.byref(history.c), tokens, counts.data_ptr()))
 
 
