@@ -364,7 +364,7 @@ __device__ __forceinline__ void add_odd(const Block &b, int first, int low, int 
 template <int FMT, int D, int KT, typename P>
 __device__ __forceinline__ void put_odd(const Block &b, int first, int low, int high, int tiles, bool taken, P is_part, float den, int q4, f32x4 &o) {
   const bool lost = den == den && !(o[0] == o[0] && o[1] == o[1] && o[2] == o[2] && o[3] == o[3]);
-  if (!taken && !lost) return;
+  if (__builtin_expect(!taken && !lost, 1)) return;   // expected, or the loop before it spills registers for this one
   f32x4 odd = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
   for (int t = 0; t < tiles; ++t) {
@@ -920,8 +920,11 @@ template <int QT, int FMT, int D> __device__ __forceinline__ void history_many(c
     f32x4 o = *(const f32x4 *)(so + r * D + 4 * (q4 ^ (r & 7)));
     const int64_t at = (int64_t)(((uint64_t)(uint32_t)__shfl((int)(to_row >> 32), r) << 32) | (uint32_t)__shfl((int)to_row, r));
     const float f = __shfl(by, r);
-    const int rlow = __shfl(row.low, r), rhigh = __shfl(row.high, r);
-    put_odd<FMT, D, KT>(b, a.first, rlow, rhigh, tiles, s_odd, is_part, __shfl(L, r), q4, o);
+    const float all = o[0] + o[1] + (o[2] + o[3]);
+    if (__any(s_odd || all != all)) {
+      const int rlow = __shfl(row.low, r), rhigh = __shfl(row.high, r);
+      put_odd<FMT, D, KT>(b, a.first, rlow, rhigh, tiles, s_odd, is_part, __shfl(L, r), q4, o);
+    }
     if (at < 0) continue;
     if (a.chunks > 1) *(f32x4 *)(a.po + at * D + 4 * q4) = o;
     else store_out<QT>(a, at * D + 4 * q4, o * f);
