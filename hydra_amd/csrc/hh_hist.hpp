@@ -11,6 +11,8 @@ namespace hh {
 
 enum HistFormat { H_F16 = 1, H_BF16 = 2, H_MXFP8 = 3, H_MXFP4 = 4 };
 constexpr int kHistLength = 1 << 30;   // lengths count as at most this
+constexpr int kFewRows = 32;           // rows of a kv head up to which a wave takes all of them, 16 or 32
+constexpr int kHistChunks = 256;       // most chunks of an attention pass
 
 // A history as kernels take it: [S][kvh][rows][d].
 struct HistView {

@@ -1,5 +1,5 @@
 // hh_hist_attn.hip — how an attention call over histories is split, and its launch.
-#include "hh_hist_attn.hpp"
+#include "hh_hist.hpp"
 
 namespace hh {
 

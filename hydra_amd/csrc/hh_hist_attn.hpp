@@ -20,10 +20,6 @@
 
 namespace hh {
 
-constexpr int kFewRows = 32;                 // rows of a kv head up to which a wave takes all of them, 16 or 32
-
-constexpr int kHistChunks = 256;             // most chunks of a pass
-
 template <int QT, int FMT> struct HistTypes {
   static constexpr bool BF = FMT != H_F16, MX = FMT >= H_MXFP8;
   static constexpr int E = FMT == H_MXFP8 ? 16 : FMT == H_MXFP4 ? 32 : 8;                       // numbers of 16 bytes
@@ -113,7 +109,7 @@ struct Block {
   bool shared;
   int s, g, r0, count, chunk, c0, nc;       // keys c0 .. c0 + nc − 1
   Visible v;
-  int first_low, last_low, first_high;      // of the first and the last row
+  int last_low, first_high;                 // of the last and the first row
   gptr_t k, v_, ks, vs;                     // the head's rows
   int rows, span, pinned, delta;            // position -> row
   int even, even_end, even_row;             // keys even .. even_end − 1 are in consecutive rows from even_row on: all but a few
@@ -135,7 +131,7 @@ template <int FMT, int D> __device__ __forceinline__ bool block_of(const HistAtt
   if (shared) {
     b.count = a.S * a.N;
     b.v = visible_prefix(a);
-    b.first_low = b.last_low = 0;
+    b.last_low = 0;
     b.first_high = b.v.n - 1;
   } else {
     b.count = step_count(a.counts, b.s, a.N);
@@ -143,7 +139,6 @@ template <int FMT, int D> __device__ __forceinline__ bool block_of(const HistAtt
     i0 = b.r0 / a.qm;
     const int i1 = min(b.count, (b.r0 + p.block_rows - 1) / a.qm + 1) - 1;
     b.v = visible_of(a, b.s, i0, i1);
-    b.first_low = row_low(a, b.v, i0);
     b.last_low = row_low(a, b.v, i1);
     b.first_high = row_high(b.v, i0);
   }
