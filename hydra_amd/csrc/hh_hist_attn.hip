@@ -4,7 +4,7 @@
 namespace hh {
 
 // Workgroups that a pass's keys are split for: those that the chip holds at once, by the kernels' registers (256 tokens behind 16384, bf16 over
-// 8 bits: heads of 64 122 us, with 512 workgroups 133, with 1024 123; heads of 128 96 us, with 384 or 768 110).
+// 8 bits: heads of 64 162 us, with 512 workgroups 163, with 1024 158; heads of 128 115 us, with 384 133, with 768 127; of 256 161, with 128 289, with 512 180).
 static int wanted_groups(int d, bool few) { return few ? (d == 64 ? 768 : 512) : d == 64 ? 768 : d == 128 ? 512 : 256; }
 
 static HistAttnArgs::Pass plan_pass(const HistAttnArgs &a, int64_t rows, int64_t heads, int64_t keys) {

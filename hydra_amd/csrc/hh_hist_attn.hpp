@@ -10,7 +10,7 @@
 // of the numbers held. Queries enter as the terms of bf16 that hold them (F16: two, F32: three; over F16 histories F32 as two of fp16),
 // probabilities as two (outputs of 16 bits: to 2^-15 of each) or three (F32: as exact as the sums) of bf16, or two of fp16: outputs of 16 bits
 // are rounded once, and a token's weights are held alike whether few or many share its call. (One term of many rows would take a fifth off
-// a prompt's time, and a fourth onto its error.)
+// a prompt's time: 168 us for 215, but 2.2e-3 from 64 bits for 1.7e-3, the output's own rounding.)
 #pragma once
 #include <type_traits>
 #include <utility>
@@ -442,9 +442,12 @@ __device__ __forceinline__ u32x2 read_columns(const uint8_t *p) {   // transposi
 // lanes of a key, so that a load is one stretch of memory, and goes to the operands' registers as it is, since the order of a product's
 // columns is free. Values pass through LDS to be read by columns. No barrier until the waves' states meet. Bound by the bytes where
 // there are enough: eight streams of up to 32768 keys in 8 bits, fp32, 64 / 8 heads of 64, 208 MB in 39 us (5.3 TB/s; the joining launch 5
-// more); 131071 keys in 4 bits, 16 / 2 heads of 256, 71 MB in 17.5 us (4.1 TB/s). By the chain of latencies where
-// there are few: 16 windows of 132 keys 6.7 us. With 64 rows a wave (four of these tiles of 16) 64 rows of 32768 keys took 26 us of heads of 64 in
-// bf16, the kernel of many rows 29; but of fp32 42 and 35, and of 1000 keys 14.7 and 13.6: the sums and the queries' terms fill the registers.
+// more), in fp16 403 MB in 83 (4.9); 131071 keys in 4 bits, 16 / 2 heads of 256, 71 MB in 17.5 us (4.1 TB/s: the LDS that the waves' states meet in
+// lets two workgroups onto a unit). By the chain of latencies where
+// there are few: 16 windows of 132 keys 6.9 us. Of 32 rows with heads of 256 the sums leave one wave a SIMD, and other types than bf16 over
+// codes spill 11 to 129 registers: four streams of 16384 keys over 8 bits 43 us in bf16 and 83 in fp32 (16 rows: 28 and 38). With 64 rows a wave (four of these tiles of 16)
+// 64 rows of 32768 keys took 26 us of heads of 64 in bf16, the kernel of many rows 30; but of fp32 42 and 35, and of 1000 keys 14.7 and 13.6: the
+// sums and the queries' terms fill the registers.
 template <int D, int RT, int W> constexpr int few_lds() { return W * (16 * RT * D * 4 > 64 * D ? 16 * RT * D * 4 : 64 * D); }
 template <int QT, int FMT, int D, int RT, int W>
 __device__ __forceinline__ void history_few(const HistAttnArgs &a, bool shared, int block, uint8_t *s_mem) {
@@ -677,13 +680,14 @@ template <int X, int PR> __device__ __forceinline__ void piece_place(int e, int 
 // Many rows: 128 a workgroup, 32 a wave, on the 32x32 MFMA; tiles of KT keys, whose 16-byte pieces the threads share, become operands in
 // LDS, two tiles in turn, read by every wave. The bytes of the tile after the next are in flight under a tile's products. A tile's one
 // barrier keeps the waves of a workgroup in step, so the workgroups are small: several a compute unit, each at its own place. Bound by the
-// VALU's instructions and the matrix unit's cycles, one after the other on a SIMD (a prompt of 4096, 64 / 8 heads of 64, bf16 over 8 bits: 67%
-// and 35% of the time, 105 instructions for a wave's 32 keys, 64 of them the softmax: an fma, an exponential, two sums, the rounding), so what
-// changes from tile to tile is kept to scalars and immediate offsets. That prompt takes 168 us (820 TFLOP/s; at a large
-// library product's rate it would be 110); two prompts of 6001, 32 / 8 heads of 128 in fp16 under a window of 1024, 242 us (630); 256 tokens
-// behind 16384, 16 / 2 heads of 256, 138 us (500: one wave a SIMD); a prompt of 2048 of those heads 123 us (280: one workgroup a unit, and the first see
-// little). Tried and slower: scores of the next tile formed under the exponentials of one, with a third place for values (7 to 10%); rounded
-// probabilities packed where they are summed (12%: they spill at four waves a SIMD).
+// VALU's instructions and the matrix unit's cycles, one after the other on a SIMD (a prompt of 4096, 64 / 8 heads of 64, bf16 over 8 bits: 64%
+// and 43% of the time, LDS 30%; 127 instructions for a wave's 32 keys: the softmax, and the probabilities' two terms), so what
+// changes from tile to tile is kept to scalars and immediate offsets. That prompt takes 215 us (640 TFLOP/s; at a large
+// library product's rate it would be 110). Two prompts of 6001, 32 / 8 heads of 128 in fp16 under a window of 1024, take 271 us (560): VALU, matrix unit and
+// LDS 37, 37 and 34%, which two waves a SIMD hardly put beside each other. 256 tokens
+// behind 16384, 16 / 2 heads of 256, 160 us (430: one wave a SIMD); a prompt of 2048 of those heads 145 us (240: one workgroup a unit, and the first see
+// little). In fp32, three terms a query and a probability: a prompt of 2048, heads of 64 over 8 bits, 110 us (310; bf16 72), of 256 300 (115; 61 to 81 registers
+// spilled). Tried and slower: scores of the next tile formed under the exponentials of one, with a third place for values (7 to 10%).
 template <int D> constexpr int many_keys() { return D == 256 ? 32 : 64; }
 template <int D> constexpr int many_lds() { return 2 * many_keys<D>() * D * 4 > 128 * D * 4 ? 2 * many_keys<D>() * D * 4 : 128 * D * 4; }
 template <int QT, int FMT, int D> __device__ __forceinline__ void history_many(const HistAttnArgs &a, bool shared, uint32_t block, uint8_t *s_mem) {
@@ -702,7 +706,7 @@ template <int QT, int FMT, int D> __device__ __forceinline__ void history_many(c
   if ((block >> 3) >= each || w >= all) return;
   const int grp = (int)(w / (uint32_t)(share * parts)), at = (int)(w - (uint32_t)grp * (uint32_t)(share * parts));
   // An XCD's 32 compute units take them in turn: where it holds all at once, forth and back, so that those that see most do not meet on one
-  // (a prompt of 2048, 64 / 8 heads of 64: 74 us, 79 without); more are dealt as units come free (4096 tokens: 246, 251 forth and back).
+  // (a prompt of 2048, 64 / 8 heads of 64: 73 us, 74 without); more are dealt as units come free (4096 tokens: 234, 240 forth and back).
   int turn = at % share;
   if (share <= 128 && turn >> 5 & 1) turn = (turn & ~31) + min(32, share - (turn & ~31)) - 1 - (turn & 31);
   const int rb = pass.row_blocks - 1 - (turn * parts + at / share);
@@ -730,8 +734,8 @@ template <int QT, int FMT, int D> __device__ __forceinline__ void history_many(c
   for (int o = 1; o < 32; o <<= 1) wlow = min(wlow, __shfl_xor(wlow, o)), whigh = max(whigh, __shfl_xor(whigh, o));
   wlow = __builtin_amdgcn_readfirstlane(wlow);
   whigh = __builtin_amdgcn_readfirstlane(whigh);
-  // A wave without rows only loads, and leaves its SIMD to other workgroups' (40 rows of 16384 keys, heads of 64: 24 us, 30 with its
-  // products; of 128: 33 and 39). Heads of 256 have one wave a SIMD: nothing to leave it to, and prompts 3% longer.
+  // A wave without rows only loads, and leaves its SIMD to other workgroups' (40 rows of 16384 keys in bf16, heads of 64: 25 us, 31 with its
+  // products; of 128: 33 and 41). Heads of 256 have one wave a SIMD: nothing to leave it to, and prompts 3% longer.
   const bool idle = D < 256 && b.r0 + wave * 32 >= b.count * a.qm;
   __syncthreads();
 
@@ -937,7 +941,7 @@ template <int QT, int FMT, int D, int OCC> __global__ __launch_bounds__(256, OCC
   history_many<QT, FMT, D>(a, false, blockIdx.x, s_mem);
 }
 // The prefix's pass and behind it the own histories', which fill the chip under its last workgroups: 64 streams of 500 over 24576 shared keys
-// 47 us; four streams of 50 over 1000, fp32 in fp16, 9.2 (latencies). The prefix's rows of all streams are in one workgroup's tiles, so
+// 56 us (fp32 85); four streams of 50 over 1000, fp32 in fp16, 10.4 (latencies). The prefix's rows of all streams are in one workgroup's tiles, so
 // that its keys are read once for 128 rows.
 template <int QT, int FMT, int D, int OCC> __global__ __launch_bounds__(256, OCC) void history_prefix_kernel(HistAttnArgs a) {
   constexpr int few = few_lds<D, 1, 4>();
@@ -969,7 +973,7 @@ __device__ __forceinline__ RowChunks row_chunks(const HistAttnArgs &a, int64_t r
   return x;
 }
 
-// Joins a row's chunks, in order: a wave per row, D / 4 lanes a chunk. 4096 rows of 34 chunks of 64: 8 us (4.5 TB/s); 512 of up to 12: 5.
+// Joins a row's chunks, in order: a wave per row, D / 4 lanes a chunk. 4096 rows of 25 chunks of 64: 7.7 us (3.5 TB/s); 512 of up to 12: 5.
 template <int QT, int D> __global__ __launch_bounds__(256) void history_merge_kernel(HistAttnArgs a) {
   warm_kernargs<sizeof(HistAttnArgs)>();
   constexpr int LR = D / 4, GR = 64 / LR;    // lanes per chunk, chunks at a time
@@ -1002,8 +1006,8 @@ template <int QT, int D> __global__ __launch_bounds__(256) void history_merge_ke
 }
 
 // The same for few rows, of many chunks: a workgroup for 64 of a row's columns. Every chunk's factor into LDS first; then sixteen lanes a chunk and sixteen
-// chunks at a time, whose sums meet in LDS, in order. (16 rows of 128 chunks: 5.4 us, a wave a row 16; 4096 rows
-// of 34 chunks 14, a wave a row 8.)
+// chunks at a time, whose sums meet in LDS, in order. (16 rows of 256 chunks of 256: 6.0 us, a wave a row 30; 4096 rows
+// of 25 chunks of 64 13, a wave a row 7.7.)
 constexpr int kMergeChunks = 2 * kHistChunks, kWideRows = 256;
 template <int QT, int D> __global__ __launch_bounds__(256) void history_merge_wide_kernel(HistAttnArgs a) {
   __shared__ float s_f[kMergeChunks], s_red[8];

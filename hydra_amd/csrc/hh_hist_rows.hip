@@ -3,7 +3,7 @@
 // Eight columns a lane, four lanes a scale: the largest magnitude of 32 columns by two exchanges, the scale's exponent from
 // its bits, and x·2^-e, exact, through the conversion to e4m3 or e2m1, to nearest even. Lanes run over a head's columns, then over
 // the tokens, so that both sides move whole stretches: [token][head] on one, [head][row] on the other. Bound by the bytes: two prompts of up to
-// 8000 tokens, 8 heads of 128, bf16 into 4 bits 16.4 us and back 14.4 (62 MB in and out each way: 3.8 and 4.3 TB/s, a copy 5.2); a step of 32 tokens
+// 8000 tokens, 8 heads of 128, bf16 into 4 bits 16.5 us and back 14.6 (62 MB in and out each way: 3.8 and 4.3 TB/s, a copy 5.2); a step of 32 tokens
 // 3 us each, its latencies.
 #include "hh_hist.hpp"
 

@@ -4,7 +4,8 @@
 // fp64 product of position and frequency loses its whole turns exactly, and what is left, within half a turn, is rounded to
 // fp32 (2^-25 of a turn) for sine and cosine. A workgroup takes some tokens, puts the sines and cosines of their pairs
 // into LDS once for all heads, and passes over the heads' columns in 16-byte pieces; both tensors are read and written once. Bound by the
-// bytes: 16384 tokens of 18 heads of 256, 64 columns turned, bf16, 302 MB in 55 us (5.5 TB/s); one token of 72 heads 2.7 us, its latencies.
+// bytes: 16384 tokens of 18 heads of 256, 64 columns turned, bf16, 302 MB in 55 us (5.5 TB/s); one token of 72 heads 2.7 us, its latencies. Halves whose
+// distance is no whole pieces go column by column: 18 heads of 96, 24 columns turned, 113 MB in 96 us (1.2 TB/s).
 #include "hh_hist.hpp"
 
 namespace hh {
@@ -33,7 +34,7 @@ template <typename T, int MODE> __global__ __launch_bounds__(256) void rotary_ke
   const int piece = tid & ((1 << a.lanes) - 1);
   const int c = (MODE == 1 && piece >= half / V ? piece + half / V : piece) * V;
   if (c >= a.d) return;
-  // One row at a time: with two in flight a lane 78 us, with four 103, 67 with one (16384 tokens of 18 heads of 256, bf16, 302 MB).
+  // One row at a time: two in flight a lane took 1.2 times as long, four 1.5 times (16384 tokens of 18 heads of 256, bf16).
   for (int r = part * each + (tid >> a.lanes); r < rows; r += stride) {
     const int t = (int)((uint32_t)r / (uint32_t)heads), h = r - t * heads;
     const bool second = h >= a.r[0].heads;
@@ -97,7 +98,7 @@ hipError_t launch_rotary(RotaryArgs a, hipStream_t s) {
   if (!a.interleaved && a.span / 2 % V == 0) pieces -= a.span / 2 / V;
   while (1 << a.lanes < pieces) ++a.lanes;
   const int each = 256 >> a.lanes;
-  // Four tokens a workgroup (one: 74 us, sixteen: 94), fewer where they fill LDS or there are few: then several share a token's heads.
+  // Four tokens a workgroup (54 us; one: 62, sixteen: 84), fewer where they fill LDS or there are few: then several share a token's heads.
   a.per_block = kRotaryPairs / (a.rotated / 2);
   const int fill = a.tokens / 1024 < 4 ? a.tokens / 1024 : 4;
   if (a.per_block > fill) a.per_block = fill;

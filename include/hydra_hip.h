@@ -581,7 +581,7 @@ int hh_rotary(hh_ctx *ctx, const hh_rotary_desc *desc, const double *turns, floa
  * Keys and values of S sequences, heads outermost: [S][kv_heads][rows][head_dim], so that a head's rows are one
  * stretch of memory. MXFP8 (e4m3 codes) and MXFP4 (e2m1, low nibble = even column) hold 32 columns with one e8m0 scale byte,
  * [S][kv_heads][rows][head_dim / 32]: the least power of two, 2^-126 or more, under which no number passes the format's largest (448, 6). Numbers
- * are rounded to the nearest, ties to even; 32 columns that hold an infinity or a NaN have scale byte 255 and are NaN.
+ * are rounded to the nearest, ties to even (from 3.3e38 in MXFP8 and 3.0e38 in MXFP4 on to 2^128, which reads as an infinity); 32 columns that hold an infinity or a NaN have scale byte 255 and are NaN.
  *
  * A step brings up to `tokens` new tokens a sequence, counts[s] of them real; token i has position lengths[s] + i. Lengths
  * are what was held before the step: the calls of every layer of a step take the same, and hh_history_advance moves them on
@@ -637,7 +637,7 @@ typedef struct hh_history_desc {
  *   sinks   bf16 [q_heads] or NULL: a logit in the denominator only
  *   lse     fp32 [S][N][q_heads] or NULL: the log of the denominator
  *   prefix  NULL, or a history of one sequence (same heads, head_dim and format; no ring; window 0): its lengths[0] rows come before
- *           every sequence's own and are seen by each token. They are read once for the batch.
+ *           every sequence's own and are seen by each token. They are read once for 128 rows (tokens x query heads) of a kv head in the batch.
  * Tokens from counts[s] on are neither read nor written. A token that sees nothing (its own position not held) gets 0 and lse −inf, or with a sink the
  * sink. Keys that a token does not see, infinities and NaN among them, have no part in its output. An infinity
  * among the values that it sees is its output's in that column, wherever it stands, as long as fp32 holds its weight. Logits, and the products before
