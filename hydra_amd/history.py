@@ -226,7 +226,7 @@ def history_attention_into(ctx: Context, history: History, q, counts, out, lse=N
                            sm_scale: float | None = None, max_length: int = 0, prefix: History | None = None):
     """Attention of a step's tokens over the history that they have been written to, and a shared `prefix` before it
     (hh_history_attention). q, out fp32, fp16 or bf16 [S][N][q_heads][d] (q may be a slice with equally spaced tokens); counts int32 [S];
-    sinks bf16 (or int16 bits) [q_heads]; lse fp32 [S][N][q_heads]. Returns `out`."""
+    sinks bf16 (or int16 bits) [q_heads]; lse fp32 [S][N][q_heads]. `out` may be a packed q. Returns `out`."""
     dev = history.device
     _cuda(ctx, dev)
     if q.dtype not in ELEM or q.dim() != 4:
